@@ -14,6 +14,7 @@
 #include <mutex>
 
 #include "fp8ops.h"
+#include "host.h"
 #include "gemm_kmajor.cuh"
 #include "gemm_wgrad.cuh"
 #include "quantize.cuh"
@@ -38,16 +39,25 @@ __device__ int g_fp8_device_error = 0;
 constexpr int kFoldCounters = 8192;
 __device__ unsigned int g_fold_counters[kFoldCounters];
 
+namespace fp8host {
+
 namespace {
 
 constexpr int kMaxDevices = 64;
 
-// Kernels launched through this library since load (graph replays not included).
 std::atomic<unsigned long long> g_launches{0};
-inline void count_launches(unsigned n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
 thread_local int t_last_status = FP8_OK;
 thread_local char t_last_msg[512] = {0};
+
+DeviceState g_dev[kMaxDevices];
+std::mutex g_dev_mu;
+
+}  // namespace
+
+int g_pdl = 0;
+
+void count_launches(unsigned n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
 int set_error(int status, const char* fmt, ...) {
   t_last_status = status;
@@ -63,32 +73,6 @@ int ok() {
   t_last_msg[0] = 0;
   return FP8_OK;
 }
-
-#define FP8_CUDA_TRY(expr)                                                                       \
-  do {                                                                                           \
-    cudaError_t e_ = (expr);                                                                     \
-    if (e_ != cudaSuccess)                                                                       \
-      return set_error(FP8_ERR_CUDA, "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(e_),     \
-                       __FILE__, __LINE__);                                                      \
-  } while (0)
-
-#define FP8_REQUIRE(cond, status, ...)         \
-  do {                                         \
-    if (!(cond)) return set_error(status, __VA_ARGS__); \
-  } while (0)
-
-// ------------------------------------------------------------------ per-device state
-struct DeviceState {
-  int sm_count = 0;
-  int* err_ptr = nullptr;
-  unsigned int* fold_base = nullptr;  // g_fold_counters on this device
-  std::atomic<unsigned int> fold_next{0};
-  // Set (release) after the fields above are written; a reader that sees it
-  // (acquire) sees them too.
-  std::atomic<bool> init{false};
-};
-DeviceState g_dev[kMaxDevices];
-std::mutex g_dev_mu;
 
 int device_state(DeviceState** out) {
   int dev = 0;
@@ -111,16 +95,6 @@ int device_state(DeviceState** out) {
   return FP8_OK;
 }
 
-// The counter of the next launch that folds a scale in its last CTA.
-unsigned int* fold_counter(DeviceState* st) {
-  return st->fold_base + st->fold_next.fetch_add(1, std::memory_order_relaxed) % kFoldCounters;
-}
-
-// ------------------------------------------------------------------ TMA tensor maps
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 int get_encode_fn(EncodeTiledFn* out) {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
@@ -136,6 +110,18 @@ int get_encode_fn(EncodeTiledFn* out) {
   return FP8_OK;
 }
 
+}  // namespace fp8host
+
+using namespace fp8host;
+
+namespace {
+
+// The counter of the next launch that folds a scale in its last CTA.
+unsigned int* fold_counter(DeviceState* st) {
+  return st->fold_base + st->fold_next.fetch_add(1, std::memory_order_relaxed) % kFoldCounters;
+}
+
+// ------------------------------------------------------------------ TMA tensor maps
 // 2-D byte matrix [rows][cols] (cols contiguous), box = 128 bytes x box_rows, 128B swizzle.
 int make_map_2d(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int box_rows) {
   EncodeTiledFn enc = nullptr;
@@ -215,17 +201,6 @@ int make_map_conv(CUtensorMap* map, const void* ptr, int batch, int height, int 
   return FP8_OK;
 }
 
-bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
-
-// Programmatic dependent launch: 0 = plain stream order (the default), 1 = the
-// tensor-core kernels, 2 = every kernel.  Each kernel waits for its predecessor
-// (pdl_sync / pdl_wait) before touching global memory, so the attribute only
-// lets its CTAs start, and run their prologue, while the previous kernel's CTAs
-// drain.  Measured on B200: a conv kernel following another conv kernel gains
-// 0.5-1 us, but the quantize -> conv chains of a training step gain nothing
-// (their streaming kernels leave no SM free early), so it is off by default.
-int g_pdl = 0;
-
 // History entry of an all-zero tensor in the delayed-scaling windows:
 // 0 = the reference's (its scale, 1.0), 1 = 0.0 (fp8_set_empty_tensor_history).
 int g_empty_zero = 0;
@@ -239,37 +214,6 @@ int g_quant_resident = 1;
 // measured on config 2, the cooperative launch and grid barrier cost more than the
 // conversion launch they replace, 25.8 vs 24.6 us for the whole dW).
 int g_wgrad_fused = 0;
-
-enum KernelClass { kStreamingKernel = 0, kTensorKernel = 1 };
-
-// Launch `kern` on `stream`, with programmatic stream serialization when enabled
-// for its class, optionally as clusters of `cluster_x` CTAs.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                          int cluster_x, KernelClass cls, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  unsigned n = 0;
-  if (g_pdl == 2 || (g_pdl == 1 && cls == kTensorKernel)) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  if (cluster_x > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = static_cast<unsigned>(cluster_x);
-    attr[n].val.clusterDim.y = 1;
-    attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
-}
 
 // Batched byte transpose dst[b][c][r] = src[b][r][c]; whole 16-byte-aligned
 // 64x64 tiles take the vectorised kernel.

@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -18,6 +19,7 @@ SRC_DIR = PKG_DIR.parent / "csrc"
 INCLUDE_DIR = PKG_DIR.parent.parent / "include"
 LIB_NAME = "libfp8ops.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+OBJ_DIR = PKG_DIR / "_build"
 
 NVCC_FLAGS = [
     "-gencode",
@@ -27,7 +29,6 @@ NVCC_FLAGS = [
     "-std=c++17",
     "-Xcompiler",
     "-fPIC",
-    "-shared",
 ]
 
 
@@ -43,7 +44,11 @@ def _nvcc() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted(SRC_DIR.glob("*.cu")) + sorted(SRC_DIR.glob("*.cuh")) + [INCLUDE_DIR / "fp8ops.h"]
+    return sorted(SRC_DIR.glob("*.cu")) + headers()
+
+
+def headers() -> list[Path]:
+    return sorted(SRC_DIR.glob("*.cuh")) + sorted(SRC_DIR.glob("*.h")) + [INCLUDE_DIR / "fp8ops.h"]
 
 
 def needs_rebuild() -> bool:
@@ -53,16 +58,33 @@ def needs_rebuild() -> bool:
     return any(p.stat().st_mtime > mtime for p in sources())
 
 
-def build_library(force: bool = False, verbose: bool = False) -> Path:
-    """Compile csrc/fp8ops.cu into libfp8ops.so for sm_100a; returns its path."""
-    if not force and not needs_rebuild():
-        return LIB_PATH
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [_nvcc(), *NVCC_FLAGS, f"-I{INCLUDE_DIR}", "-o", str(tmp), str(SRC_DIR / "fp8ops.cu")]
+def _compile(src: Path, obj: Path, verbose: bool) -> None:
+    cmd = [_nvcc(), *NVCC_FLAGS, f"-I{INCLUDE_DIR}", "-c", "-o", str(obj), str(src)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
+    """Compile every csrc/*.cu (side by side) and link libfp8ops.so for sm_100a; returns its path.
+
+    An object file in ``_build/`` is kept while it is newer than its source and every header."""
+    if not force and not needs_rebuild():
+        return LIB_PATH
+    OBJ_DIR.mkdir(exist_ok=True)
+    newest_header = max(p.stat().st_mtime for p in headers())
+    jobs = []
+    for src in sorted(SRC_DIR.glob("*.cu")):
+        obj = OBJ_DIR / (src.stem + ".o")
+        if force or not obj.exists() or obj.stat().st_mtime <= max(newest_header, src.stat().st_mtime):
+            jobs.append((src, obj))
+    with ThreadPoolExecutor() as pool:
+        for done in [pool.submit(_compile, src, obj, verbose) for src, obj in jobs]:
+            done.result()
+    tmp = LIB_PATH.with_suffix(".so.tmp")
+    objs = [str(OBJ_DIR / (src.stem + ".o")) for src in sorted(SRC_DIR.glob("*.cu"))]
+    subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", str(tmp), *objs], check=True)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 
