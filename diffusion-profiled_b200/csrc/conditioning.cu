@@ -1,0 +1,282 @@
+// conditioning.cu — C ABI of the text-conditioning operators (include/fp8ops.h): the
+// token embedding, the counter-based dropout and the attention over an encoder's
+// states.  Host code validates, lays out workspaces and launches; it allocates nothing.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "cross_attention.cuh"
+#include "dropout.cuh"
+#include "embedding.cuh"
+#include "fp8ops.h"
+#include "host.h"
+
+using namespace fp8b;
+using namespace fp8host;
+
+namespace {
+
+cudaStream_t cuda_stream(fp8_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
+
+int dtype_size(int dtype) { return dtype == FP8_DTYPE_FP32 ? 4 : 2; }
+bool known_dtype(int dtype) { return dtype >= FP8_DTYPE_BF16 && dtype <= FP8_DTYPE_FP16; }
+
+// Calls f with a value of the C++ type of `dtype`.
+template <typename F>
+int with_dtype(int dtype, F&& f) {
+  switch (dtype) {
+    case FP8_DTYPE_BF16: return f(__nv_bfloat16{});
+    case FP8_DTYPE_FP32: return f(float{});
+    default: return f(__half{});
+  }
+}
+
+unsigned grid_for(int64_t items, int64_t per_block, int sm_count, int blocks_per_sm) {
+  const int64_t blocks = (items + per_block - 1) / per_block;
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(blocks, int64_t(sm_count) * blocks_per_sm)));
+}
+
+// ------------------------------------------------------------------ cross attention
+bool strides_fit(const fp8_head_strides& s, int batch, int tokens, int heads) {
+  return (batch == 1 || s.batch % 8 == 0) && (tokens == 1 || s.token % 8 == 0) && (heads == 1 || s.head % 8 == 0);
+}
+XStrides strides_of(const fp8_head_strides& s) { return {s.batch, s.token, s.head}; }
+
+int x_check(const fp8_cross_attention_args* a, bool backward) {
+  FP8_REQUIRE(a != nullptr, FP8_ERR_INVALID_ARGUMENT, "cross attention: args is NULL");
+  FP8_REQUIRE(a->batch > 0 && a->q_len > 0 && a->k_len > 0 && a->heads > 0 && a->kv_heads > 0,
+              FP8_ERR_INVALID_ARGUMENT, "cross attention: sizes must be positive (batch %d, q_len %d, k_len %d, heads %d, "
+              "kv_heads %d)", a->batch, a->q_len, a->k_len, a->heads, a->kv_heads);
+  FP8_REQUIRE(a->heads % a->kv_heads == 0, FP8_ERR_INVALID_ARGUMENT,
+              "cross attention: %d heads are not a multiple of %d key heads", a->heads, a->kv_heads);
+  FP8_REQUIRE(a->head_dim >= 8 && a->head_dim <= 128 && a->head_dim % 8 == 0, FP8_ERR_UNSUPPORTED,
+              "cross attention: head_dim must be a multiple of 8 up to 128, got %d", a->head_dim);
+  FP8_REQUIRE(a->dtype == FP8_DTYPE_BF16 || a->dtype == FP8_DTYPE_FP16, FP8_ERR_UNSUPPORTED,
+              "cross attention: dtype must be bf16 or fp16, got code %d", a->dtype);
+  FP8_REQUIRE(std::isfinite(a->scale), FP8_ERR_INVALID_ARGUMENT, "cross attention: scale is not finite");
+  FP8_REQUIRE(a->q && a->k && a->v && a->o && aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) &&
+                  aligned(a->o, 16) && aligned(a->lse, 4) && aligned(a->key_lengths, 4),
+              FP8_ERR_INVALID_ARGUMENT, "cross attention: q, k, v and o must be 16-byte aligned, lse and key_lengths 4-byte");
+  FP8_REQUIRE(strides_fit(a->q_stride, a->batch, a->q_len, a->heads) &&
+                  strides_fit(a->o_stride, a->batch, a->q_len, a->heads) &&
+                  strides_fit(a->k_stride, a->batch, a->k_len, a->kv_heads) &&
+                  strides_fit(a->v_stride, a->batch, a->k_len, a->kv_heads),
+              FP8_ERR_INVALID_ARGUMENT, "cross attention: strides must be multiples of 8 elements");
+  if (backward) {
+    FP8_REQUIRE(a->lse && a->dout && a->dq && a->dk && a->dv && aligned(a->dout, 16) && aligned(a->dq, 16) &&
+                    aligned(a->dk, 16) && aligned(a->dv, 16),
+                FP8_ERR_INVALID_ARGUMENT,
+                "cross attention backward: needs lse, and dout, dq, dk and dv 16-byte aligned");
+    FP8_REQUIRE(strides_fit(a->dout_stride, a->batch, a->q_len, a->heads) &&
+                    strides_fit(a->dq_stride, a->batch, a->q_len, a->heads) &&
+                    strides_fit(a->dk_stride, a->batch, a->k_len, a->kv_heads) &&
+                    strides_fit(a->dv_stride, a->batch, a->k_len, a->kv_heads),
+                FP8_ERR_INVALID_ARGUMENT, "cross attention backward: strides must be multiples of 8 elements");
+  }
+  return FP8_OK;
+}
+
+XAttnParams x_params(const fp8_cross_attention_args* a, DeviceState* st) {
+  XAttnParams p{};
+  p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
+  p.o = a->o;
+  p.o_in = a->o;
+  p.lse = a->lse;
+  p.dout = a->dout;
+  p.dq = a->dq;
+  p.dk = a->dk;
+  p.dv = a->dv;
+  p.sq = strides_of(a->q_stride);
+  p.sk = strides_of(a->k_stride);
+  p.sv = strides_of(a->v_stride);
+  p.so = strides_of(a->o_stride);
+  p.sdo = strides_of(a->dout_stride);
+  p.sdq = strides_of(a->dq_stride);
+  p.sdk = strides_of(a->dk_stride);
+  p.sdv = strides_of(a->dv_stride);
+  p.key_lengths = a->key_lengths;
+  p.key_mask = a->key_mask;
+  p.mask_stride = a->mask_stride;
+  p.batch = a->batch;
+  p.q_len = a->q_len;
+  p.k_len = a->k_len;
+  p.heads = a->heads;
+  p.kv_heads = a->kv_heads;
+  p.head_dim = a->head_dim;
+  p.scale = a->scale;
+  p.err = st->err_ptr;
+  return p;
+}
+
+template <typename T>
+int x_fwd(const XAttnParams& p, DeviceState* st, cudaStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.q_len;
+  FP8_CUDA_TRY(launch_kernel(x_fwd_simple_kernel<T>, dim3(grid_for(rows, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,
+                             kStreamingKernel, p));
+  count_launches(1);
+  return ok();
+}
+
+template <typename T>
+int x_bwd(const XAttnParams& p, DeviceState* st, cudaStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.q_len;
+  const int64_t keys = static_cast<int64_t>(p.batch) * p.kv_heads * p.k_len;
+  FP8_CUDA_TRY(launch_kernel(x_dq_simple_kernel<T>, dim3(grid_for(rows, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,
+                             kStreamingKernel, p));
+  FP8_CUDA_TRY(launch_kernel(x_dkv_simple_kernel<T>, dim3(grid_for(keys, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,
+                             kStreamingKernel, p));
+  count_launches(2);
+  return ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fp8_cross_attention_workspace_bytes(const fp8_cross_attention_args* a, int backward) {
+  if (a == nullptr || a->batch <= 0 || a->q_len <= 0 || a->heads <= 0 || !backward) return 0;
+  return sizeof(float) * static_cast<size_t>(a->batch) * a->heads * a->q_len;  // delta
+}
+
+int fp8_cross_attention_fwd(const fp8_cross_attention_args* a, void* workspace, size_t workspace_bytes,
+                            fp8_stream_t stream) {
+  if (int s = x_check(a, false)) return s;
+  FP8_REQUIRE(workspace_bytes >= fp8_cross_attention_workspace_bytes(a, 0), FP8_ERR_WORKSPACE,
+              "cross attention: workspace too small");
+  DeviceState* st = nullptr;
+  if (int s = device_state(&st)) return s;
+  const XAttnParams p = x_params(a, st);
+  (void)workspace;
+  return a->dtype == FP8_DTYPE_BF16 ? x_fwd<__nv_bfloat16>(p, st, cuda_stream(stream))
+                                    : x_fwd<__half>(p, st, cuda_stream(stream));
+}
+
+int fp8_cross_attention_bwd(const fp8_cross_attention_args* a, void* workspace, size_t workspace_bytes,
+                            fp8_stream_t stream) {
+  if (int s = x_check(a, true)) return s;
+  FP8_REQUIRE(workspace != nullptr && aligned(workspace, 16) &&
+                  workspace_bytes >= fp8_cross_attention_workspace_bytes(a, 1),
+              FP8_ERR_WORKSPACE, "cross attention backward: workspace too small or not 16-byte aligned");
+  DeviceState* st = nullptr;
+  if (int s = device_state(&st)) return s;
+  XAttnParams p = x_params(a, st);
+  p.delta = static_cast<float*>(workspace);
+  return a->dtype == FP8_DTYPE_BF16 ? x_bwd<__nv_bfloat16>(p, st, cuda_stream(stream))
+                                    : x_bwd<__half>(p, st, cuda_stream(stream));
+}
+
+// ------------------------------------------------------------------ token embedding
+static int embed_check(const void* ids, int ids64, int64_t tokens, int64_t vocab, int width, int weight_dtype,
+                       int out_dtype) {
+  FP8_REQUIRE(tokens >= 0 && vocab > 0 && width > 0, FP8_ERR_INVALID_ARGUMENT,
+              "embedding: bad sizes (tokens %lld, vocab %lld, width %d)", (long long)tokens, (long long)vocab, width);
+  FP8_REQUIRE(known_dtype(weight_dtype) && known_dtype(out_dtype), FP8_ERR_UNSUPPORTED,
+              "embedding: unknown dtype code %d / %d", weight_dtype, out_dtype);
+  FP8_REQUIRE(tokens == 0 || (ids != nullptr && aligned(ids, ids64 ? 8 : 4)), FP8_ERR_INVALID_ARGUMENT,
+              "embedding: ids is NULL or misaligned");
+  return FP8_OK;
+}
+
+int fp8_embedding_fwd(const void* ids, int ids64, int64_t tokens, const void* weight, int weight_dtype, int64_t vocab,
+                      int width, int64_t weight_stride, float scale, void* out, int out_dtype, fp8_stream_t stream) {
+  if (int s = embed_check(ids, ids64, tokens, vocab, width, weight_dtype, out_dtype)) return s;
+  if (tokens == 0) return ok();
+  FP8_REQUIRE(weight && out && aligned(weight, dtype_size(weight_dtype)) && aligned(out, dtype_size(out_dtype)),
+              FP8_ERR_INVALID_ARGUMENT, "embedding: weight or out is NULL or misaligned");
+  DeviceState* st = nullptr;
+  if (int s = device_state(&st)) return s;
+  EmbedParams p{};
+  p.ids = ids;
+  p.ids64 = ids64;
+  p.weight = weight;
+  p.weight_stride = weight_stride;
+  p.out = out;
+  p.tokens = tokens;
+  p.vocab = vocab;
+  p.width = width;
+  p.scale = scale;
+  p.err = st->err_ptr;
+  const int status = with_dtype(weight_dtype, [&](auto w) {
+    return with_dtype(out_dtype, [&](auto o) {
+      FP8_CUDA_TRY(launch_kernel(embed_fwd_kernel<decltype(w), decltype(o)>, dim3(grid_for(tokens, 8, st->sm_count, 8)),
+                                 dim3(256), 0, cuda_stream(stream), 1, kStreamingKernel, p));
+      return FP8_OK;
+    });
+  });
+  if (status) return status;
+  count_launches(1);
+  return ok();
+}
+
+size_t fp8_embedding_bwd_workspace_bytes(int64_t, int64_t, int) { return 0; }
+
+int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* dout, int out_dtype, void* dweight,
+                      int weight_dtype, int64_t vocab, int width, float scale, int64_t padding_idx, void* workspace,
+                      size_t workspace_bytes, fp8_stream_t stream) {
+  if (int s = embed_check(ids, ids64, tokens, vocab, width, weight_dtype, out_dtype)) return s;
+  FP8_REQUIRE((tokens == 0 || dout) && dweight && aligned(dweight, dtype_size(weight_dtype)) &&
+                  aligned(dout, dtype_size(out_dtype)),
+              FP8_ERR_INVALID_ARGUMENT, "embedding backward: dout or dweight is NULL or misaligned");
+  FP8_REQUIRE(workspace_bytes >= fp8_embedding_bwd_workspace_bytes(tokens, vocab, width), FP8_ERR_WORKSPACE,
+              "embedding backward: workspace too small");
+  (void)workspace;
+  DeviceState* st = nullptr;
+  if (int s = device_state(&st)) return s;
+  EmbedParams p{};
+  p.ids = ids;
+  p.ids64 = ids64;
+  p.dout = dout;
+  p.dweight = dweight;
+  p.tokens = tokens;
+  p.vocab = vocab;
+  p.padding_idx = padding_idx;
+  p.width = width;
+  p.scale = scale;
+  p.err = st->err_ptr;
+  const int status = with_dtype(weight_dtype, [&](auto w) {
+    return with_dtype(out_dtype, [&](auto o) {
+      FP8_CUDA_TRY(launch_kernel(embed_bwd_simple_kernel<decltype(w), decltype(o)>,
+                                 dim3(grid_for(vocab, 8, st->sm_count, 8)), dim3(256), 0, cuda_stream(stream), 1,
+                                 kStreamingKernel, p));
+      return FP8_OK;
+    });
+  });
+  if (status) return status;
+  count_launches(1);
+  return ok();
+}
+
+// ------------------------------------------------------------------ dropout
+int fp8_dropout(const void* x, const void* residual, void* y, int dtype, int64_t n, double p, const int64_t* seed,
+                fp8_stream_t stream) {
+  FP8_REQUIRE(n >= 0, FP8_ERR_INVALID_ARGUMENT, "dropout: negative size");
+  FP8_REQUIRE(known_dtype(dtype), FP8_ERR_UNSUPPORTED, "dropout: unknown dtype code %d", dtype);
+  FP8_REQUIRE(p >= 0.0 && p <= 1.0, FP8_ERR_INVALID_ARGUMENT, "dropout: p must be in [0, 1], got %g", p);
+  if (n == 0) return ok();
+  const size_t size = dtype_size(dtype);
+  FP8_REQUIRE(x && y && seed && aligned(x, size) && aligned(y, size) && aligned(residual, size) && aligned(seed, 8),
+              FP8_ERR_INVALID_ARGUMENT, "dropout: x, y or seed is NULL, or a pointer is misaligned");
+  DeviceState* st = nullptr;
+  if (int s = device_state(&st)) return s;
+  DropoutParams d{};
+  d.x = x;
+  d.residual = residual;
+  d.y = y;
+  d.seed = seed;
+  d.n = n;
+  d.thresh = static_cast<uint32_t>(std::lrint(p * 65536.0));
+  d.scale = p < 1.0 ? static_cast<float>(1.0 / (1.0 - p)) : 0.0f;
+  const int status = with_dtype(dtype, [&](auto t) {
+    FP8_CUDA_TRY(launch_kernel(dropout_kernel<decltype(t)>, dim3(grid_for(n, 8 * kDropoutThreads, st->sm_count, 8)),
+                               dim3(kDropoutThreads), 0, cuda_stream(stream), 1, kStreamingKernel, d));
+    return FP8_OK;
+  });
+  if (status) return status;
+  count_launches(1);
+  return ok();
+}
+
+}  // extern "C"

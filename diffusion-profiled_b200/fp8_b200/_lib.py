@@ -24,6 +24,29 @@ EPILOGUE_NONE = 0
 EPILOGUE_BIAS = 1
 EPILOGUE_BIAS_SILU = 2
 
+DTYPE_BF16 = 0
+DTYPE_FP32 = 1
+DTYPE_FP16 = 2
+
+
+class HeadStrides(ctypes.Structure):
+    """fp8_head_strides."""
+
+    _fields_ = [("batch", c_int64), ("token", c_int64), ("head", c_int64)]
+
+
+class CrossAttentionArgs(ctypes.Structure):
+    """fp8_cross_attention_args."""
+
+    _fields_ = (
+        [(n, c_void_p) for n in ("q", "k", "v", "o", "lse", "dout", "dq", "dk", "dv")]
+        + [(n + "_stride", HeadStrides) for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv")]
+        + [("key_lengths", c_void_p), ("key_mask", c_void_p), ("mask_stride", c_int64)]
+        + [(n, ctypes.c_int32) for n in ("batch", "q_len", "k_len", "heads", "kv_heads", "head_dim", "dtype")]
+        + [("scale", c_float)]
+    )
+
+
 # name -> (restype, argtypes); mirrors include/fp8ops.h one to one.
 _SIGNATURES: dict[str, tuple] = {
     "fp8_abi_version": (c_int, []),
@@ -167,6 +190,17 @@ _SIGNATURES: dict[str, tuple] = {
     "fp8_gn_act_bwd": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_float,
                                c_float, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                                c_size_t, c_void_p]),
+    "fp8_cross_attention_workspace_bytes": (c_size_t, [POINTER(CrossAttentionArgs), c_int]),
+    "fp8_cross_attention_fwd": (c_int, [POINTER(CrossAttentionArgs), c_void_p, c_size_t, c_void_p]),
+    "fp8_cross_attention_bwd": (c_int, [POINTER(CrossAttentionArgs), c_void_p, c_size_t, c_void_p]),
+    "fp8_embedding_fwd": (
+        c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int, c_int64, c_float, c_void_p, c_int,
+                c_void_p]),
+    "fp8_embedding_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "fp8_embedding_bwd": (
+        c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_float, c_int64,
+                c_void_p, c_size_t, c_void_p]),
+    "fp8_dropout": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, ctypes.c_double, c_void_p, c_void_p]),
     "fp8_set_conv_algo": (c_int, [c_int]),
     "fp8_set_pdl": (c_int, [c_int]),
     "fp8_set_empty_tensor_history": (c_int, [c_int]),

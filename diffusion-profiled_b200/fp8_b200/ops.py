@@ -45,6 +45,21 @@ def _require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
+DTYPE_CODES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_FP32, torch.float16: _lib.DTYPE_FP16}
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """Call the C entry ``name`` with ``args`` and ``dev``'s current stream (switching device only if needed)."""
+    fn = getattr(_lib.load(), name)
+    if dev.index == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if status:
+        _lib.check(status, name)
+
+
 def _nhwc_dims(t: torch.Tensor) -> tuple[int, int, int, int]:
     b, c, h, w = t.shape
     return b, c, h, w

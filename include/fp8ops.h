@@ -518,6 +518,79 @@ int fp8_attention_bwd(const void* qkv, const void* o, const void* dout, const fl
                       void* dqkv, int batch, int seq, int heads, int head_dim, int ld_qkv, int ld_o,
                       fp8_stream_t stream);
 
+/* ------------------------------------------------------------ text conditioning */
+
+/* Element types of the operators below. */
+#define FP8_DTYPE_BF16 0
+#define FP8_DTYPE_FP32 1
+#define FP8_DTYPE_FP16 2
+
+/* Attention of queries over an encoder's states of another length.
+ *   s_ij = scale * q_i . k_j over the kept keys j, p_i = softmax(s_i), o_i = sum_j p_ij v_j
+ * q, o, dout, dq: [batch][q_len][heads][head_dim]; k, v, dk, dv:
+ * [batch][k_len][kv_heads][head_dim], of dtype FP8_DTYPE_BF16 or FP8_DTYPE_FP16.
+ * Head channels are contiguous; the other strides (in elements) are free:
+ * multiples of 8, pointers 16-byte aligned, gradients not overlapping themselves.
+ * heads is a multiple of kv_heads: query head h reads key head h / (heads /
+ * kv_heads).  head_dim: a multiple of 8 up to 128.  A key j of sequence b is kept
+ * when j < key_lengths[b] (NULL: k_len; values outside [0, k_len] are clamped) and
+ * key_mask[b * mask_stride + j] != 0 (NULL: all).  A query without kept keys gets
+ * o = 0, lse = -inf and adds nothing to any gradient.  Values at keys that are not
+ * kept are never used, so they may be infinite or NaN.
+ * lse: fp32 [batch][heads][q_len], log-sum-exp of each query's kept scores, written
+ * by the forward (NULL: not wanted) and read by the backward.
+ * q_len and k_len are at least 1. */
+typedef struct {
+  int64_t batch, token, head;
+} fp8_head_strides;
+
+typedef struct {
+  const void *q, *k, *v;
+  void* o; /* written by the forward, read by the backward */
+  float* lse;
+  const void* dout;   /* backward only, as dq, dk and dv */
+  void *dq, *dk, *dv;
+  fp8_head_strides q_stride, k_stride, v_stride, o_stride, dout_stride, dq_stride, dk_stride, dv_stride;
+  const int32_t* key_lengths;
+  const uint8_t* key_mask;
+  int64_t mask_stride;
+  int32_t batch, q_len, k_len, heads, kv_heads, head_dim, dtype;
+  float scale;
+} fp8_cross_attention_args;
+
+/* Bytes of workspace (16-byte aligned) the call needs on the current device. */
+size_t fp8_cross_attention_workspace_bytes(const fp8_cross_attention_args* args, int backward);
+int fp8_cross_attention_fwd(const fp8_cross_attention_args* args, void* workspace, size_t workspace_bytes,
+                            fp8_stream_t stream);
+int fp8_cross_attention_bwd(const fp8_cross_attention_args* args, void* workspace, size_t workspace_bytes,
+                            fp8_stream_t stream);
+
+/* Token embedding with scaling: out[i][c] = scale * weight[ids[i]][c] in fp32,
+ * rounded once to out_dtype.  ids: int64 (ids64 != 0) or int32 [tokens]; weight:
+ * [vocab] rows of `width` values, weight_stride elements apart.  An id outside
+ * [0, vocab) gives a row of zeros and device error 201 (fp8_device_error). */
+int fp8_embedding_fwd(const void* ids, int ids64, int64_t tokens, const void* weight, int weight_dtype,
+                      int64_t vocab, int width, int64_t weight_stride, float scale, void* out, int out_dtype,
+                      fp8_stream_t stream);
+
+/* Its gradient: dweight[v][c] = scale * sum of dout[i][c] over the tokens i with
+ * ids[i] = v, zero for tokens that do not occur and for padding_idx (< 0: none).
+ * Every element of the dense [vocab][width] dweight is written.  The sums are fp32,
+ * in an order that the ids alone fix: the same call gives the same bits. */
+size_t fp8_embedding_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int width);
+int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* dout, int out_dtype, void* dweight,
+                      int weight_dtype, int64_t vocab, int width, float scale, int64_t padding_idx, void* workspace,
+                      size_t workspace_bytes, fp8_stream_t stream);
+
+/* Dropout with a mask made from a counter: y[e] = keep(e) ? x[e] / (1 - p) : 0, plus
+ * residual[e] where residual is not NULL, in fp32, rounded once to dtype.  keep(e):
+ * the (e mod 4)-th 16 bits of splitmix64(*seed ^ (e / 4) * 0xD1B54A32D192ED03) are
+ * at least p * 65536 rounded to an integer (the group norm's dropout draws from the
+ * same generator).  The gradient of x is the same call on dy without a residual.
+ * seed: device int64; 0 <= p <= 1.  y may be x. */
+int fp8_dropout(const void* x, const void* residual, void* y, int dtype, int64_t n, double p, const int64_t* seed,
+                fp8_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
