@@ -39,7 +39,8 @@ unsigned grid_for(int64_t items, int64_t per_block, int sm_count, int blocks_per
 
 // ------------------------------------------------------------------ cross attention
 bool strides_fit(const fp8_head_strides& s, int batch, int tokens, int heads) {
-  return (batch == 1 || s.batch % 8 == 0) && (tokens == 1 || s.token % 8 == 0) && (heads == 1 || s.head % 8 == 0);
+  const auto fits = [](int n, int64_t stride) { return n == 1 || (stride > 0 && stride % 8 == 0); };
+  return fits(batch, s.batch) && fits(tokens, s.token) && fits(heads, s.head);
 }
 XStrides strides_of(const fp8_head_strides& s) { return {s.batch, s.token, s.head}; }
 
@@ -62,7 +63,7 @@ int x_check(const fp8_cross_attention_args* a, bool backward) {
                   strides_fit(a->o_stride, a->batch, a->q_len, a->heads) &&
                   strides_fit(a->k_stride, a->batch, a->k_len, a->kv_heads) &&
                   strides_fit(a->v_stride, a->batch, a->k_len, a->kv_heads),
-              FP8_ERR_INVALID_ARGUMENT, "cross attention: strides must be multiples of 8 elements");
+              FP8_ERR_INVALID_ARGUMENT, "cross attention: strides must be positive multiples of 8 elements");
   if (backward) {
     FP8_REQUIRE(a->lse && a->dout && a->dq && a->dk && a->dv && aligned(a->dout, 16) && aligned(a->dq, 16) &&
                     aligned(a->dk, 16) && aligned(a->dv, 16),
@@ -72,7 +73,7 @@ int x_check(const fp8_cross_attention_args* a, bool backward) {
                     strides_fit(a->dq_stride, a->batch, a->q_len, a->heads) &&
                     strides_fit(a->dk_stride, a->batch, a->k_len, a->kv_heads) &&
                     strides_fit(a->dv_stride, a->batch, a->k_len, a->kv_heads),
-                FP8_ERR_INVALID_ARGUMENT, "cross attention backward: strides must be multiples of 8 elements");
+                FP8_ERR_INVALID_ARGUMENT, "cross attention backward: strides must be positive multiples of 8 elements");
   }
   return FP8_OK;
 }
@@ -106,17 +107,113 @@ XAttnParams x_params(const fp8_cross_attention_args* a, DeviceState* st) {
   p.heads = a->heads;
   p.kv_heads = a->kv_heads;
   p.head_dim = a->head_dim;
+  p.group = a->heads / a->kv_heads;
+  p.pack = p.group <= kXTile ? p.group : 1;
+  p.tile_tokens = kXTile / p.pack;
   p.scale = a->scale;
   p.err = st->err_ptr;
   return p;
 }
 
-template <typename T>
-int x_fwd(const XAttnParams& p, DeviceState* st, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.q_len;
-  FP8_CUDA_TRY(launch_kernel(x_fwd_simple_kernel<T>, dim3(grid_for(rows, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,
-                             kStreamingKernel, p));
+// [batch][tokens][heads][channels] of 16-bit values with 64-channel, 128-byte-swizzled
+// rows: box {64 channels, box_heads, box_tokens, 1}.  What lies outside reads as zero.
+int x_map(CUtensorMap* map, const void* ptr, int dtype, const XStrides& st, int batch, int tokens, int heads,
+          int channels, int box_heads, int box_tokens) {
+  EncodeTiledFn enc = nullptr;
+  if (int s = get_encode_fn(&enc)) return s;
+  // the stride of a dimension of one is never used, but has to be a legal one
+  const auto bytes = [](int n, int64_t stride) { return static_cast<cuuint64_t>(n == 1 ? 16 : stride * 2); };
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(heads),
+                        static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(batch)};
+  cuuint64_t strides[3] = {bytes(heads, st.head), bytes(tokens, st.token), bytes(batch, st.batch)};
+  cuuint32_t box[4] = {64u, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens), 1u};
+  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = enc(map, dtype == FP8_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  FP8_REQUIRE(r == CUDA_SUCCESS, FP8_ERR_CUDA, "cuTensorMapEncodeTiled(attention [%d][%d][%d][%d]) failed: %d", batch,
+              tokens, heads, channels, (int)r);
+  return FP8_OK;
+}
+
+constexpr int kXMaxSplits = 128;
+
+// How a forward call divides its work.
+struct XPlan {
+  int row_tiles, hv, n_tiles, nt, splits, key_chunk;
+  int64_t rows, items, slots;
+};
+XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
+  XPlan w{};
+  const int group = a->heads / a->kv_heads, pack = group <= kXTile ? group : 1, tokens = kXTile / pack;
+  w.row_tiles = (a->q_len + tokens - 1) / tokens;
+  w.hv = a->heads / pack;
+  w.n_tiles = (a->k_len + kXTile - 1) / kXTile;
+  w.nt = w.row_tiles > 1 ? 2 : 1;
+  w.rows = static_cast<int64_t>(a->batch) * a->heads * a->q_len;
+  w.slots = static_cast<int64_t>(sm_count) * (w.nt == 1 ? 2 : 1);
+  const int64_t base = static_cast<int64_t>(a->batch) * w.hv * ((w.row_tiles + w.nt - 1) / w.nt);
+  w.splits = 1;
+  w.key_chunk = w.n_tiles;
+  // A split writes its rows' partial outputs in fp32.  With a few rows a tile that is nothing, and pieces that
+  // are a quarter of an even share even out sequences of different lengths; with whole tiles of rows the keys
+  // are split only to reach SMs that would have no work at all.
+  const bool few_rows = w.row_tiles == 1 && a->q_len * pack <= 16;
+  const int64_t pieces = few_rows ? 4 * w.slots : w.slots;
+  if (w.n_tiles > 1 && 2 * base <= pieces) {
+    w.key_chunk = static_cast<int>(std::max<int64_t>((w.n_tiles * base + pieces - 1) / pieces,
+                                                     (w.n_tiles + kXMaxSplits - 1) / kXMaxSplits));
+    w.splits = (w.n_tiles + w.key_chunk - 1) / w.key_chunk;
+  }
+  w.items = base * w.splits;
+  return w;
+}
+size_t x_fwd_workspace(const fp8_cross_attention_args* a, const XPlan& w) {
+  return w.splits == 1 ? 0 : sizeof(float) * static_cast<size_t>(w.splits) * w.rows * (a->head_dim + 1);
+}
+
+template <typename T, int HALVES, int NT>
+int x_fwd_launch(const XFwdParams& f, const CUtensorMap (&maps)[4], int64_t slots, cudaStream_t stream) {
+  using Ly = XFwdLayout<HALVES, NT>;
+  FP8_CUDA_TRY(cudaFuncSetAttribute(x_fwd_kernel<T, HALVES, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    Ly::kSmemBytes));
+  FP8_CUDA_TRY(launch_kernel(x_fwd_kernel<T, HALVES, NT>, dim3(static_cast<unsigned>(std::min(f.items, slots))),
+                             dim3(Ly::kThreads), Ly::kSmemBytes, stream, 1, kTensorKernel, f, maps[0], maps[1], maps[2],
+                             maps[3]));
   count_launches(1);
+  return FP8_OK;
+}
+
+template <typename T>
+int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPlan& w, void* workspace, DeviceState* st,
+          cudaStream_t stream) {
+  XFwdParams f{};
+  f.a = a;
+  f.row_tiles = w.row_tiles;
+  f.key_chunk = w.key_chunk;
+  f.splits = w.splits;
+  f.part_o = static_cast<float*>(workspace);
+  f.part_lse = f.part_o == nullptr ? nullptr : f.part_o + static_cast<int64_t>(w.splits) * w.rows * a.head_dim;
+  f.rows = w.rows;
+  f.items = w.items;
+  CUtensorMap maps[4];
+  const int dt = args->dtype;
+  if (int s = x_map(&maps[0], a.q, dt, a.sq, a.batch, a.q_len, a.heads, a.head_dim, a.pack, a.tile_tokens)) return s;
+  if (int s = x_map(&maps[1], a.k, dt, a.sk, a.batch, a.k_len, a.kv_heads, a.head_dim, 1, kXTile)) return s;
+  if (int s = x_map(&maps[2], a.v, dt, a.sv, a.batch, a.k_len, a.kv_heads, a.head_dim, 1, kXTile)) return s;
+  if (int s = x_map(&maps[3], a.o, dt, a.so, a.batch, a.q_len, a.heads, a.head_dim, a.pack, a.tile_tokens)) return s;
+  int status;
+  if (a.head_dim <= 64)
+    status = w.nt == 1 ? x_fwd_launch<T, 1, 1>(f, maps, w.slots, stream) : x_fwd_launch<T, 1, 2>(f, maps, w.slots, stream);
+  else
+    status = w.nt == 1 ? x_fwd_launch<T, 2, 1>(f, maps, w.slots, stream) : x_fwd_launch<T, 2, 2>(f, maps, w.slots, stream);
+  if (status) return status;
+  if (w.splits > 1) {
+    FP8_CUDA_TRY(launch_kernel(x_combine_kernel<T>, dim3(grid_for(w.rows, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,
+                               kStreamingKernel, f));
+    count_launches(1);
+  }
   return ok();
 }
 
@@ -137,21 +234,28 @@ int x_bwd(const XAttnParams& p, DeviceState* st, cudaStream_t stream) {
 extern "C" {
 
 size_t fp8_cross_attention_workspace_bytes(const fp8_cross_attention_args* a, int backward) {
-  if (a == nullptr || a->batch <= 0 || a->q_len <= 0 || a->heads <= 0 || !backward) return 0;
-  return sizeof(float) * static_cast<size_t>(a->batch) * a->heads * a->q_len;  // delta
+  DeviceState* st = nullptr;
+  if (a == nullptr || a->batch <= 0 || a->q_len <= 0 || a->k_len <= 0 || a->heads <= 0 || a->kv_heads <= 0 ||
+      a->heads % a->kv_heads != 0)
+    return 0;
+  if (backward) return sizeof(float) * static_cast<size_t>(a->batch) * a->heads * a->q_len;  // delta
+  if (device_state(&st)) return 0;
+  return x_fwd_workspace(a, x_plan(a, st->sm_count));
 }
 
 int fp8_cross_attention_fwd(const fp8_cross_attention_args* a, void* workspace, size_t workspace_bytes,
                             fp8_stream_t stream) {
   if (int s = x_check(a, false)) return s;
-  FP8_REQUIRE(workspace_bytes >= fp8_cross_attention_workspace_bytes(a, 0), FP8_ERR_WORKSPACE,
-              "cross attention: workspace too small");
   DeviceState* st = nullptr;
   if (int s = device_state(&st)) return s;
+  const XPlan w = x_plan(a, st->sm_count);
+  const size_t need = x_fwd_workspace(a, w);
+  FP8_REQUIRE(need == 0 || (workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= need),
+              FP8_ERR_WORKSPACE, "cross attention: workspace too small or not 16-byte aligned (%zu bytes, needs %zu)",
+              workspace_bytes, need);
   const XAttnParams p = x_params(a, st);
-  (void)workspace;
-  return a->dtype == FP8_DTYPE_BF16 ? x_fwd<__nv_bfloat16>(p, st, cuda_stream(stream))
-                                    : x_fwd<__half>(p, st, cuda_stream(stream));
+  return a->dtype == FP8_DTYPE_BF16 ? x_fwd<__nv_bfloat16>(a, p, w, workspace, st, cuda_stream(stream))
+                                    : x_fwd<__half>(a, p, w, workspace, st, cuda_stream(stream));
 }
 
 int fp8_cross_attention_bwd(const fp8_cross_attention_args* a, void* workspace, size_t workspace_bytes,

@@ -9,6 +9,28 @@
 // with the sums over i running over the queries of every head that shares the keys.
 // A query without kept keys has o = 0, lse = -inf and adds nothing to any gradient;
 // what is stored at a key that is not kept (infinities and NaN too) is never used.
+//
+// Rows.  The `pack` query heads that share a key head are rows of one tile: row
+// r = token * pack + head-in-group, floor(128 / pack) tokens a tile, so that keys and
+// values are read once for all of them and their gradients need no second sum.
+//
+// Forward (x_fwd_kernel): one pass over the keys with a running maximum and sum.
+//   * S = Q K^T of a 128-row, 128-key tile on tcgen05 kind::f16 into TMEM (fp32); one
+//     thread owns one row, reads it, and writes P (rounded to the tensors' type, the
+//     tensor cores' operand) over S in TMEM, where the second product O += P V takes
+//     it from;
+//   * the exponent's reference is the row's maximum so far, raised only when a score
+//     passes it by more than 2^8: then O and the sum are rescaled.  Scores that stay
+//     within that factor need no rescaling pass, and P <= 2^8 keeps its relative
+//     precision in bf16 and fp16;
+//   * with two row tiles a CTA, one's softmax runs while the other's products do;
+//   * tiles with keys that are not kept: their rows of K and V are zeroed in shared
+//     memory before the products, and their scores are -inf.
+// The sums and statistics are fp32; P is the one value rounded before a sum (it is a
+// matrix operand).
+//
+// Every mbarrier wait is bounded (mbar_wait); on a timeout the kernel records the error
+// code, skips the remaining work and frees its tensor memory.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -17,6 +39,8 @@
 #include "sm100_common.cuh"
 
 namespace fp8b {
+
+constexpr int kXTile = 128;  // rows of a query tile and keys of a key tile
 
 struct XStrides {
   int64_t batch, token, head;  // elements
@@ -32,6 +56,9 @@ struct XAttnParams {
   const uint8_t* key_mask;
   int64_t mask_stride;
   int batch, q_len, k_len, heads, kv_heads, head_dim;
+  int group;       // query heads per key head
+  int pack;        // query heads side by side in a row tile (group, or 1 where group > 128)
+  int tile_tokens; // tokens of a row tile: 128 / pack
   float scale;
   int* err;
 };
@@ -41,6 +68,649 @@ __device__ __forceinline__ int x_key_count(const XAttnParams& p, int b) {
 }
 __device__ __forceinline__ bool x_key_kept(const XAttnParams& p, int b, int j) {
   return p.key_mask == nullptr || p.key_mask[b * p.mask_stride + j] != 0;
+}
+
+// ---------------------------------------------------------------- tcgen05, 16-bit operands
+template <typename T>
+struct XType;
+template <>
+struct XType<__nv_bfloat16> {
+  static constexpr uint32_t kFormat = 1u;
+  static __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+template <>
+struct XType<__half> {
+  static constexpr uint32_t kFormat = 0u;
+  static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+// kind::f16 instruction descriptor for operands of type T, f32 accumulator, M = 128.
+template <typename T>
+__device__ __forceinline__ uint32_t x_idesc(int n, int a_mn_major, int b_mn_major) {
+  return (1u << 4) | (XType<T>::kFormat << 7) | (XType<T>::kFormat << 10) |
+         (static_cast<uint32_t>(a_mn_major) << 15) | (static_cast<uint32_t>(b_mn_major) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kXTile >> 4) << 24);
+}
+
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]: A's 16-bit elements lie two to a column, row r in lane r
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 lanes x 16 columns, register -> TMEM.
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Makes the uses of r come after the asm statements before it (a tcgen05.wait::ld).
+__device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31]));
+}
+
+// Tiled TMA store of a {channels, heads, tokens, batch} box.
+__device__ __forceinline__ void tma_store_4d(const void* tmap, const void* src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A wait whose outcome the whole warp shares (the loads of tensor memory are warp-wide).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
+                                          int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
+}
+
+// The 128 keep bits of the keys [j0, j0 + 128) of sequence b (whole warp).
+__device__ __forceinline__ uint4 x_keep_words(const XAttnParams& p, int b, int j0, int count, int lane) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = j0 + 32 * i + lane;
+    w[i] = __ballot_sync(0xffffffffu, j < count && x_key_kept(p, b, j));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Zeroes the rows of a [128][64 * HALVES] tile (128-byte swizzled rows, halves 16 KB apart) whose keep bit is 0
+// (whole warp): a weight of zero times an infinity or NaN stored there would not be zero.
+template <int HALVES>
+__device__ __forceinline__ void x_zero_rows(uint8_t* tile, const uint4& keep, int lane) {
+  const uint32_t w[4] = {keep.x, keep.y, keep.z, keep.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] >> lane) & 1u) continue;
+    uint8_t* row = tile + (32 * i + lane) * 128;
+    for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(row + hf * 16384 + c * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// ============================================================================ forward
+constexpr int kXMaskSlots = 8;  // key tiles whose keep bits are held: more than are ever between load and use
+
+struct XFwdParams {
+  XAttnParams a;
+  int row_tiles;    // row tiles of a (sequence, head group)
+  int key_chunk;    // key tiles of a split; splits == 1: all of them
+  int splits;
+  float* part_o;    // [splits][batch * heads * q_len][head_dim], with splits > 1
+  float* part_lse;  // [splits][batch * heads * q_len], base-2 logarithm
+  int64_t rows;     // batch * heads * q_len
+  int64_t items;    // (sequence, head group, row tile group, split)
+};
+
+// NT row tiles of HALVES * 64 channels a CTA.
+template <int HALVES, int NT>
+struct XFwdLayout {
+  static constexpr int kTileBytes = HALVES * 16384;
+  static constexpr int kQStages = HALVES == 1 ? 2 : 1;
+  // key / value entries: as many as fit the CTA's share of the SM (two CTAs with NT = 1)
+  static constexpr int kEntries = NT == 2 ? (HALVES == 1 ? 6 : 4) : (HALVES == 1 ? 4 : 2);
+  static constexpr int kKV = NT * kTileBytes * kQStages;
+  static constexpr int kWords = kKV + kEntries * kTileBytes;
+  static constexpr int kBar = kWords + kXMaskSlots * 16;
+  static constexpr int kNumBars = 2 * kQStages + 2 * kEntries + 5 * NT + 1;
+  static constexpr int kTail = kBar + kNumBars * 8;
+  static constexpr int kSmemBytes = kTail + 16 + 1024;  // + alignment slack
+  static constexpr int kThreads = NT * 128 + 64;
+  static constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
+  static constexpr int kCtasPerSm = NT == 2 ? 1 : 2;
+};
+static_assert(XFwdLayout<2, 2>::kSmemBytes <= 232448 && XFwdLayout<1, 2>::kSmemBytes <= 232448, "one CTA per SM");
+static_assert(2 * XFwdLayout<2, 1>::kSmemBytes <= 232448 && 2 * XFwdLayout<1, 1>::kSmemBytes <= 232448,
+              "two CTAs per SM");
+
+// One unit of work: the row tiles [tile0, tile0 + tiles) of a head group against the key tiles [j0, j1).
+struct XItem {
+  int b, hv, tile0, tiles, split, keys, j0, j1;
+};
+template <int NT>
+__device__ __forceinline__ XItem x_item(const XFwdParams& p, int64_t i) {
+  XItem t;
+  const int groups = (p.row_tiles + NT - 1) / NT;
+  t.tile0 = static_cast<int>(i % groups) * NT;
+  i /= groups;
+  t.split = static_cast<int>(i % p.splits);
+  i /= p.splits;
+  const int hv = p.a.heads / p.a.pack;
+  t.hv = static_cast<int>(i % hv);
+  t.b = static_cast<int>(i / hv);
+  t.tiles = min(NT, p.row_tiles - t.tile0);
+  t.keys = x_key_count(p.a, t.b);
+  const int n = (t.keys + kXTile - 1) / kXTile;
+  t.j0 = min(n, t.split * p.key_chunk);
+  t.j1 = min(n, t.j0 + p.key_chunk);
+  return t;
+}
+// 32-key chunks of key tile j that hold keys.
+__device__ __forceinline__ int x_chunks(int keys, int j) { return (min(kXTile, keys - j * kXTile) + 31) >> 5; }
+
+template <typename T, int HALVES, int NT>
+__global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<HALVES, NT>::kCtasPerSm)
+    x_fwd_kernel(const XFwdParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap o_map) {
+  using Ly = XFwdLayout<HALVES, NT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint4* words = reinterpret_cast<uint4*>(smem + Ly::kWords);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + Ly::kBar);
+  uint64_t* q_empty = q_full + Ly::kQStages;
+  uint64_t* kv_full = q_empty + Ly::kQStages;
+  uint64_t* kv_empty = kv_full + Ly::kEntries;
+  uint64_t* s_full = kv_empty + Ly::kEntries;
+  uint64_t* p_full = s_full + NT;
+  uint64_t* o_full = p_full + NT;
+  uint64_t* o_free = o_full + NT;
+  uint64_t* staged = o_free + NT;
+  uint64_t* drained = staged + NT;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::kTail);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < Ly::kQStages; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, NT);
+    }
+    for (int i = 0; i < Ly::kEntries; ++i) {
+      mbar_init(kv_full + i, 1);
+      mbar_init(kv_empty + i, 1);
+    }
+    for (int i = 0; i < NT; ++i) {
+      mbar_init(s_full + i, 2);  // the products' commit, and the issuing thread (keep bits)
+      mbar_init(p_full + i, 4);
+      mbar_init(o_full + i, 1);
+      mbar_init(o_free + i, 4);
+      mbar_init(staged + i, 4);
+    }
+    mbar_init(drained, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 4 * NT) {
+    tmem_alloc(tmem_slot, Ly::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  const XAttnParams& a = p.a;
+  const bool masked = a.key_mask != nullptr;
+  const int ksteps = (a.head_dim + 15) >> 4;  // 16-channel steps of Q K^T, and 16-column steps of P V's width
+
+  if (warp == 4 * NT) {
+    // ------------------------------------------------------------ loads
+    if (lane == 0) {
+      tma_prefetch_desc(&q_map);
+      tma_prefetch_desc(&k_map);
+      tma_prefetch_desc(&v_map);
+    }
+    const uint32_t q_bytes = static_cast<uint32_t>(a.tile_tokens * a.pack) * 128u * HALVES;
+    uint32_t e = 0, loaded = 0, n_item = 0, g = 0;  // `loaded`: entries whose copy was started
+    bool ok = true;
+    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+      const XItem t = x_item<NT>(p, i);
+      if (t.j0 >= t.j1) continue;
+      const int qs = n_item % Ly::kQStages;
+      ok = warp_wait(q_empty + qs, ((n_item / Ly::kQStages) & 1) ^ 1, abort_flag, a.err, kErrTimeoutProducer);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full + qs, q_bytes * t.tiles);
+        for (int r = 0; r < t.tiles; ++r)
+          for (int hf = 0; hf < HALVES; ++hf)
+            tma_load_4d(smem + (qs * NT + r) * Ly::kTileBytes + hf * 16384, &q_map, q_full + qs, hf * 64, t.hv * a.pack,
+                        (t.tile0 + r) * a.tile_tokens, t.b);
+      }
+      ++n_item;
+      const int hk = t.hv * a.pack / a.group;
+      for (int j = t.j0; j < t.j1 && ok; ++j, ++g) {
+        const bool bits = masked || (j + 1) * kXTile > t.keys;
+        if (bits) {
+          const uint4 w = x_keep_words(a, t.b, j * kXTile, t.keys, lane);
+          if (lane == 0) words[g % kXMaskSlots] = w;
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2 && ok; ++kv, ++e) {
+          const int slot = e % Ly::kEntries;
+          ok = warp_wait(kv_empty + slot, ((e / Ly::kEntries) & 1) ^ 1, abort_flag, a.err, kErrTimeoutProducer);
+          if (!ok) break;
+          loaded = e + 1;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(kv_full + slot, Ly::kTileBytes);
+            for (int hf = 0; hf < HALVES; ++hf)
+              tma_load_4d(smem + Ly::kKV + slot * Ly::kTileBytes + hf * 16384, kv ? &v_map : &k_map, kv_full + slot,
+                          hf * 64, hk, j * kXTile, t.b);
+          }
+        }
+      }
+    }
+    if (!ok && lane == 0) {  // copies still in flight land before the CTA leaves
+      volatile int never = 0;
+      for (uint32_t k = loaded > Ly::kEntries ? loaded - Ly::kEntries : 0; k < loaded; ++k)
+        mbar_wait(kv_full + k % Ly::kEntries, (k / Ly::kEntries) & 1, &never, a.err, kErrTimeoutDrain);
+      if (n_item > 0)
+        mbar_wait(q_full + (n_item - 1) % Ly::kQStages, ((n_item - 1) / Ly::kQStages) & 1, &never, a.err,
+                  kErrTimeoutDrain);
+    }
+  } else if (warp == 4 * NT + 1) {
+    // ------------------------------------------------------------ products
+    struct Cursor {
+      int64_t i;
+      XItem t;
+      int j;
+      uint32_t g;       // key tiles before this one
+      uint32_t n_item;  // items with keys before this one
+    };
+    // moves to the next key tile; false when there is none
+    const auto seek = [&](Cursor& c) {
+      while (c.j >= c.t.j1) {
+        c.i += gridDim.x;
+        if (c.i >= p.items) return false;
+        if (c.t.j1 > c.t.j0) ++c.n_item;
+        c.t = x_item<NT>(p, c.i);
+        c.j = c.t.j0;
+      }
+      return true;
+    };
+    uint32_t n_p[NT] = {}, n_o[NT] = {};  // weights taken, items begun, by row tile
+    const uint32_t s_base = smem_u32(smem);
+    bool ok = true;
+    const auto wait_entry = [&](uint32_t entry, const Cursor& c) {
+      const int slot = entry % Ly::kEntries;
+      if (!warp_wait(kv_full + slot, (entry / Ly::kEntries) & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
+      if (masked || (c.j + 1) * kXTile > c.t.keys) {
+        const uint4 w = words[c.g % kXMaskSlots];
+        if ((w.x & w.y & w.z & w.w) != 0xffffffffu) x_zero_rows<HALVES>(smem + Ly::kKV + slot * Ly::kTileBytes, w, lane);
+      }
+      return true;
+    };
+    const auto issue_s = [&](const Cursor& c, int r) {
+      if (lane == 0) {
+        const int n = x_chunks(c.t.keys, c.j) * 32;
+        const uint32_t idesc = x_idesc<T>(n, 0, 0);
+        const uint32_t sq = s_base + ((c.n_item % Ly::kQStages) * NT + r) * Ly::kTileBytes;
+        const uint32_t sk = s_base + Ly::kKV + (2 * c.g % Ly::kEntries) * Ly::kTileBytes;
+        tc_fence_after();
+        for (int k = 0; k < ksteps; ++k) {
+          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+          umma_f16_ss(tmem + r * 128, make_smem_desc(sq + off, 16, 1024), make_smem_desc(sk + off, 16, 1024), idesc,
+                      k > 0 ? 1u : 0u);
+        }
+        umma_commit(s_full + r);
+        mbar_arrive(s_full + r);
+        if (r == c.t.tiles - 1) umma_commit(kv_empty + 2 * c.g % Ly::kEntries);
+      }
+    };
+    const auto issue_pv = [&](const Cursor& c, int r) {
+      if (!warp_wait(p_full + r, n_p[r] & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
+      ++n_p[r];
+      if (c.j == c.t.j0) {  // the last item's output has been read
+        if (n_o[r] > 0 && !warp_wait(o_free + r, (n_o[r] - 1) & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
+        ++n_o[r];
+      }
+      if (lane == 0) {
+        const uint32_t idesc = x_idesc<T>(ksteps * 16, 0, 1);
+        const uint32_t entry = 2 * c.g + 1;
+        const uint32_t sv = s_base + Ly::kKV + (entry % Ly::kEntries) * Ly::kTileBytes;
+        tc_fence_after();
+        const int steps = 2 * x_chunks(c.t.keys, c.j);
+        for (int k = 0; k < steps; ++k)
+          umma_f16_ts(tmem + NT * 128 + r * HALVES * 64, tmem + r * 128 + k * 8, make_smem_desc(sv + k * 2048, 16384, 1024),
+                      idesc, (c.j > c.t.j0 || k > 0) ? 1u : 0u);
+        if (c.j == c.t.j1 - 1) umma_commit(o_full + r);
+        if (r == c.t.tiles - 1) umma_commit(kv_empty + entry % Ly::kEntries);
+      }
+      __syncwarp();
+      return true;
+    };
+    const auto begin_tile = [&](const Cursor& c) {  // Q (with an item's first tile) and K are there
+      if (c.j == c.t.j0 && !warp_wait(q_full + c.n_item % Ly::kQStages, (c.n_item / Ly::kQStages) & 1, abort_flag, a.err,
+                                      kErrTimeoutMma))
+        return false;
+      return wait_entry(2 * c.g, c);
+    };
+
+    Cursor cur{};
+    cur.i = blockIdx.x;
+    bool more = cur.i < p.items;
+    if (more) {
+      cur.t = x_item<NT>(p, cur.i);
+      cur.j = cur.t.j0;
+      more = seek(cur);
+    }
+    if (more) {
+      ok = begin_tile(cur);
+      for (int r = 0; ok && r < cur.t.tiles; ++r) issue_s(cur, r);
+    }
+    while (more && ok) {
+      Cursor nxt = cur;
+      ++nxt.j;
+      ++nxt.g;
+      more = seek(nxt);
+      ok = wait_entry(2 * cur.g + 1, cur);
+      // with one Q stage the next item's Q waits for this item's output: every row tile's P V goes first
+      const bool apart = Ly::kQStages == 1 && more && nxt.j == nxt.t.j0;
+      bool begun = false;
+#pragma unroll
+      for (int r = 0; r < NT; ++r) {
+        if (ok && r < cur.t.tiles) ok = issue_pv(cur, r);
+        if (ok && more && !apart && r < nxt.t.tiles) {
+          if (!begun) ok = begin_tile(nxt);
+          begun = true;
+          if (ok) issue_s(nxt, r);
+        }
+      }
+      if (ok && more && apart) {
+        ok = begin_tile(nxt);
+        for (int r = 0; ok && r < nxt.t.tiles; ++r) issue_s(nxt, r);
+      }
+      cur = nxt;
+    }
+    if (!ok && lane == 0) {  // the products in flight end before the tensor memory is freed
+      volatile int never = 0;
+      umma_commit(drained);
+      mbar_wait(drained, 0, &never, a.err, kErrTimeoutDrain);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax: thread = row of row tile rt
+    const int rt = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t t_s = t_lane + rt * 128, t_o = t_lane + NT * 128 + rt * HALVES * 64;
+    const bool flip = a.scale < 0.0f;  // the largest score is the smallest product
+    // log2 units; a zero scale keeps a factor that leaves -inf at -inf
+    const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
+    const int rows = a.tile_tokens * a.pack;
+    uint32_t n_s = 0, n_out = 0, n_item = 0, g = 0;
+    bool ok = true;
+    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+      const XItem t = x_item<NT>(p, i);
+      const int token = (t.tile0 + rt) * a.tile_tokens + row / a.pack;
+      const bool live = rt < t.tiles && row < rows && token < a.q_len;
+      const int head = t.hv * a.pack + row % a.pack;
+      const int64_t r_index = (static_cast<int64_t>(t.b) * a.heads + head) * a.q_len + token;
+      if (t.j0 >= t.j1) {  // no keys
+        if (live) {
+          if (p.splits > 1) {
+            p.part_lse[t.split * p.rows + r_index] = -INFINITY;
+          } else {
+            T* o = static_cast<T*>(a.o) + t.b * a.so.batch + token * a.so.token + head * a.so.head;
+            for (int c = 0; c < a.head_dim; c += 8) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
+            if (a.lse != nullptr) a.lse[r_index] = -INFINITY;
+          }
+        }
+        continue;
+      }
+      const int qs = n_item % Ly::kQStages;
+      if (rt >= t.tiles) {  // this row tile has no rows in the item
+        if (quad == 0) {
+          ok = warp_wait(q_full + qs, (n_item / Ly::kQStages) & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+          if (ok && lane == 0) mbar_arrive(q_empty + qs);
+        }
+        ++n_item;
+        g += t.j1 - t.j0;
+        continue;
+      }
+      // rows of this warp that exist: a warp without any keeps only the barriers
+      const bool any_row = __any_sync(0xffffffffu, live);
+      float m = -INFINITY, l = 0.0f;
+      for (int j = t.j0; j < t.j1; ++j, ++g, ++n_s) {
+        ok = warp_wait(s_full + rt, n_s & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+        if (!ok) break;
+        tc_fence_after();
+        if (any_row) {
+          const int chunks = x_chunks(t.keys, j);
+          uint32_t v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c < chunks) tmem_ld_32x32b_x32(t_s + c * 32, v[c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) after_wait(v[c]);
+          if (flip) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[c][k] ^= 0x80000000u;
+          }
+          if (masked || (j + 1) * kXTile > t.keys) {
+            const uint4 w4 = words[g % kXMaskSlots];
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (c < chunks && w[c] != 0xffffffffu) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) v[c][k] = (w[c] >> k) & 1u ? v[c][k] : 0xff800000u;
+              }
+          }
+          float mt = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c < chunks) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 2)
+                mt = fmaxf(mt, fmaxf(__uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1])));
+            }
+          if (__any_sync(0xffffffffu, live && ((mt - m) * c2 > 8.0f || m == -INFINITY))) {
+            const float mn = fmaxf(m, mt);
+            const float f = m == -INFINITY ? 0.0f : ex2((m - mn) * c2);
+            l *= f;
+            m = mn;
+            if (j > t.j0) {
+#pragma unroll 1
+              for (int c = 0; c < 2 * HALVES; ++c) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(t_o + c * 32, o);
+                tmem_ld_wait();
+                after_wait(o);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                tmem_st_32x32b_x32(t_o + c * 32, o);
+              }
+            }
+          }
+          const float mc = m == -INFINITY ? 0.0f : m * c2;
+          float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c < chunks) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                const float p0 = ex2(fmaf(__uint_as_float(v[c][k]), c2, -mc));
+                const float p1 = ex2(fmaf(__uint_as_float(v[c][k + 1]), c2, -mc));
+                sum[0] += p0;
+                sum[1] += p1;
+                pk[k >> 1] = XType<T>::pack2(p0, p1);
+              }
+              tmem_st_32x32b_x16(t_s + c * 16, pk);
+            }
+          l += sum[0] + sum[1];
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + rt);
+      }
+      if (ok) ok = warp_wait(o_full + rt, n_out & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+      if (!ok) break;
+      ++n_out;
+      tc_fence_after();
+      const float inv = l > 0.0f ? __fdividef(1.0f, l) : (l == l ? 0.0f : l);
+      uint8_t* stage = smem + (qs * NT + rt) * Ly::kTileBytes;  // Q's tile, read by every product of the item by now
+#pragma unroll
+      for (int c = 0; c < 2 * HALVES; ++c) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(t_o + c * 32, o);
+        tmem_ld_wait();
+        after_wait(o);
+        if (p.splits > 1) {
+          if (live) {
+            float* dst = p.part_o + (t.split * p.rows + r_index) * a.head_dim + c * 32;
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              if (c * 32 + k < a.head_dim)
+                *reinterpret_cast<float4*>(dst + k) =
+                    make_float4(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv,
+                                __uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
+          }
+        } else {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 2)
+            pk[k >> 1] = XType<T>::pack2(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
+          uint8_t* half = stage + (c >> 1) * 16384;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            st_shared_v4(half + swizzle128_offset(row, (c & 1) * 4 + u), pk[4 * u], pk[4 * u + 1], pk[4 * u + 2],
+                         pk[4 * u + 3]);
+        }
+      }
+      tc_fence_before();
+      if (live) {
+        // lse in base 2; the natural one is log(2) times it
+        const float lse2 = l > 0.0f ? m * c2 + __log2f(l) : (l == l ? -INFINITY : l);
+        if (p.splits > 1) p.part_lse[t.split * p.rows + r_index] = lse2;
+        else if (a.lse != nullptr) a.lse[r_index] = lse2 * 0.6931471805599453f;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(o_free + rt);
+        mbar_arrive(staged + rt);
+      }
+      if (quad == 0 && lane == 0) {
+        ok = mbar_wait(staged + rt, (n_out - 1) & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+        if (ok && p.splits == 1) {
+          for (int hf = 0; hf < HALVES; ++hf)
+            tma_store_4d(&o_map, stage + hf * 16384, hf * 64, t.hv * a.pack, (t.tile0 + rt) * a.tile_tokens, t.b);
+          bulk_commit_group();
+          bulk_wait_group_read<0>();
+        }
+        if (ok) mbar_arrive(q_empty + qs);
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      ++n_item;
+    }
+    if (quad == 0 && lane == 0) bulk_wait_group<0>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4 * NT) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Ly::kTmemCols);
+  }
+}
+
+// Joins the splits of a row: o = sum_s 2^(lse_s - lse) o_s, in the order of the splits.  One warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) x_combine_kernel(const XFwdParams p) {
+  pdl_sync();
+  const XAttnParams& a = p.a;
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; r < p.rows;
+       r += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
+    const int token = static_cast<int>(r % a.q_len), head = static_cast<int>(r / a.q_len % a.heads),
+              b = static_cast<int>(r / a.q_len / a.heads);
+    float m = -INFINITY;
+    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_lse[s * p.rows + r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float total = 0.0f, o[4] = {};
+    for (int s = 0; s < p.splits; ++s) {
+      const float lse = p.part_lse[s * p.rows + r];
+      if (lse == -INFINITY) continue;  // a split without keys wrote no output
+      const float w = ex2(lse - ref);
+      total += w;
+      if (lane * 4 < a.head_dim) {
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * p.rows + r) * a.head_dim + lane * 4);
+        o[0] = fmaf(w, v.x, o[0]);
+        o[1] = fmaf(w, v.y, o[1]);
+        o[2] = fmaf(w, v.z, o[2]);
+        o[3] = fmaf(w, v.w, o[3]);
+      }
+    }
+    const float inv = total > 0.0f ? __fdividef(1.0f, total) : (total == total ? 0.0f : total);
+    if (lane * 4 < a.head_dim)
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + b * a.so.batch + token * a.so.token + head * a.so.head + lane * 4) =
+          make_uint2(XType<T>::pack2(o[0] * inv, o[1] * inv), XType<T>::pack2(o[2] * inv, o[3] * inv));
+    if (a.lse != nullptr && lane == 0)
+      a.lse[r] = total > 0.0f ? (ref + __log2f(total)) * 0.6931471805599453f : (total == total ? -INFINITY : total);
+  }
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -63,38 +733,6 @@ __device__ __forceinline__ void x_store4(T* row, int lane, int d, const float (&
 }
 __device__ __forceinline__ float dot4(const float (&a)[4], const float (&b)[4]) {
   return a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3];
-}
-
-// One warp per query row.
-template <typename T>
-__global__ void __launch_bounds__(256) x_fwd_simple_kernel(const XAttnParams p) {
-  pdl_sync();
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.q_len;
-  const int group = p.heads / p.kv_heads;
-  for (int64_t r = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; r < rows;
-       r += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
-    const int i = static_cast<int>(r % p.q_len), h = static_cast<int>(r / p.q_len % p.heads),
-              b = static_cast<int>(r / p.q_len / p.heads), hk = h / group;
-    float q[4], o[4] = {}, m = -INFINITY, l = 0.0f;
-    x_load4(static_cast<const T*>(p.q) + b * p.sq.batch + i * p.sq.token + h * p.sq.head, lane, p.head_dim, q);
-    const int n = x_key_count(p, b);
-    for (int j = 0; j < n; ++j) {
-      if (!x_key_kept(p, b, j)) continue;
-      float k[4], v[4];
-      x_load4(static_cast<const T*>(p.k) + b * p.sk.batch + j * p.sk.token + hk * p.sk.head, lane, p.head_dim, k);
-      x_load4(static_cast<const T*>(p.v) + b * p.sv.batch + j * p.sv.token + hk * p.sv.head, lane, p.head_dim, v);
-      const float s = warp_sum(dot4(q, k)) * p.scale;
-      const float mn = fmaxf(m, s), f = m == -INFINITY ? 0.0f : expf(m - mn), w = expf(s - mn);
-      l = l * f + w;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] = o[c] * f + w * v[c];
-      m = mn;
-    }
-    x_store4(static_cast<T*>(p.o) + b * p.so.batch + i * p.so.token + h * p.so.head, lane, p.head_dim, o,
-             l > 0.0f ? 1.0f / l : 0.0f);
-    if (p.lse != nullptr && lane == 0) p.lse[r] = l > 0.0f ? m + logf(l) : -INFINITY;
-  }
 }
 
 // One warp per query row: delta and dq.
