@@ -7,6 +7,7 @@
 #include <cmath>
 
 #include "cross_attention.cuh"
+#include "cross_attention_bwd.cuh"
 #include "dropout.cuh"
 #include "embedding.cuh"
 #include "fp8ops.h"
@@ -137,6 +138,15 @@ int x_map(CUtensorMap* map, const void* ptr, int dtype, const XStrides& st, int 
   return FP8_OK;
 }
 
+// Makes the current device's context current to the driver on this thread too (a thread that has made no runtime
+// call yet, such as autograd's, has none, and the tensor-map encoder needs one).
+int bind_context() {
+  int dev = 0;
+  FP8_CUDA_TRY(cudaGetDevice(&dev));
+  FP8_CUDA_TRY(cudaSetDevice(dev));
+  return FP8_OK;
+}
+
 constexpr int kXMaxSplits = 128;
 
 // How a forward call divides its work.
@@ -197,6 +207,7 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
   f.part_lse = f.part_o == nullptr ? nullptr : f.part_o + static_cast<int64_t>(w.splits) * w.rows * a.head_dim;
   f.rows = w.rows;
   f.items = w.items;
+  if (int s = bind_context()) return s;
   CUtensorMap maps[4];
   const int dt = args->dtype;
   if (int s = x_map(&maps[0], a.q, dt, a.sq, a.batch, a.q_len, a.heads, a.head_dim, a.pack, a.tile_tokens)) return s;
@@ -217,15 +228,85 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
   return ok();
 }
 
-template <typename T>
-int x_bwd(const XAttnParams& p, DeviceState* st, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.q_len;
-  const int64_t keys = static_cast<int64_t>(p.batch) * p.kv_heads * p.k_len;
-  FP8_CUDA_TRY(launch_kernel(x_dq_simple_kernel<T>, dim3(grid_for(rows, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,
-                             kStreamingKernel, p));
-  FP8_CUDA_TRY(launch_kernel(x_dkv_simple_kernel<T>, dim3(grid_for(keys, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,
-                             kStreamingKernel, p));
+// How a backward call divides the dK / dV work, and what it keeps in the workspace.
+struct XBwdPlan {
+  int row_tiles, q_tiles, q_chunk, splits;
+  int64_t dq_items, dkv_items;
+  size_t stats_bytes, part_bytes;
+};
+XBwdPlan x_bwd_plan(const fp8_cross_attention_args* a, int sm_count) {
+  const XPlan f = x_plan(a, sm_count);
+  XBwdPlan w{};
+  const int group = a->heads / a->kv_heads, pack = a->heads / f.hv;
+  w.row_tiles = f.row_tiles;
+  w.q_tiles = group / pack * f.row_tiles;
+  w.dq_items = static_cast<int64_t>(a->batch) * f.hv * f.row_tiles;
+  const int64_t base = static_cast<int64_t>(a->batch) * a->kv_heads * f.n_tiles;
+  // queries are split (and the partial sums joined) only where key tiles alone leave half the SMs without work
+  w.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(w.q_tiles, sm_count / base)));
+  w.q_chunk = (w.q_tiles + w.splits - 1) / w.splits;
+  w.splits = (w.q_tiles + w.q_chunk - 1) / w.q_chunk;
+  w.dkv_items = base * w.splits;
+  w.stats_bytes = static_cast<size_t>(w.dq_items) * kXTile * sizeof(float2);
+  w.part_bytes = w.splits == 1 ? 0 : sizeof(float) * 2 * w.splits * a->batch * a->k_len * static_cast<size_t>(a->kv_heads) * a->head_dim;
+  return w;
+}
+
+template <typename T, int HALVES>
+int x_bwd_launch(const XBwdParams& dq, const XBwdParams& dkv, const CUtensorMap (&m)[7], DeviceState* st,
+                 cudaStream_t stream) {
+  FP8_CUDA_TRY(cudaFuncSetAttribute(x_dq_kernel<T, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    XDqLayout<HALVES>::kSmemBytes));
+  FP8_CUDA_TRY(cudaFuncSetAttribute(x_dkv_kernel<T, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    XDkvLayout<HALVES>::kSmemBytes));
+  const auto grid = [&](int64_t items) { return dim3(static_cast<unsigned>(std::min<int64_t>(items, st->sm_count))); };
+  FP8_CUDA_TRY(launch_kernel(x_dq_kernel<T, HALVES>, grid(dq.items), dim3(XDqLayout<HALVES>::kThreads),
+                             XDqLayout<HALVES>::kSmemBytes, stream, 1, kTensorKernel, dq, m[0], m[1], m[2], m[3], m[4]));
+  FP8_CUDA_TRY(launch_kernel(x_dkv_kernel<T, HALVES>, grid(dkv.items), dim3(XDkvLayout<HALVES>::kThreads),
+                             XDkvLayout<HALVES>::kSmemBytes, stream, 1, kTensorKernel, dkv, m[0], m[1], m[2], m[3], m[5],
+                             m[6]));
   count_launches(2);
+  return FP8_OK;
+}
+
+template <typename T>
+int x_bwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XBwdPlan& w, void* workspace,
+          DeviceState* st, cudaStream_t stream) {
+  XBwdParams p{};
+  p.a = a;
+  p.row_tiles = w.row_tiles;
+  p.stats = static_cast<float2*>(workspace);
+  p.items = w.dq_items;
+  XBwdParams kv = p;
+  kv.items = w.dkv_items;
+  kv.q_tiles = w.q_tiles;
+  kv.q_chunk = w.q_chunk;
+  kv.splits = w.splits;
+  kv.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.stats_bytes);
+  if (int s = bind_context()) return s;
+  CUtensorMap m[7];
+  const int dt = args->dtype;
+  const auto q_side = [&](CUtensorMap* map, const void* ptr, const XStrides& s) {
+    return x_map(map, ptr, dt, s, a.batch, a.q_len, a.heads, a.head_dim, a.pack, a.tile_tokens);
+  };
+  const auto k_side = [&](CUtensorMap* map, const void* ptr, const XStrides& s) {
+    return x_map(map, ptr, dt, s, a.batch, a.k_len, a.kv_heads, a.head_dim, 1, kXTile);
+  };
+  if (int s = q_side(&m[0], a.q, a.sq)) return s;
+  if (int s = k_side(&m[1], a.k, a.sk)) return s;
+  if (int s = k_side(&m[2], a.v, a.sv)) return s;
+  if (int s = q_side(&m[3], a.dout, a.sdo)) return s;
+  if (int s = q_side(&m[4], a.dq, a.sdq)) return s;
+  if (int s = k_side(&m[5], a.dk, a.sdk)) return s;
+  if (int s = k_side(&m[6], a.dv, a.sdv)) return s;
+  if (int s = a.head_dim <= 64 ? x_bwd_launch<T, 1>(p, kv, m, st, stream) : x_bwd_launch<T, 2>(p, kv, m, st, stream))
+    return s;
+  if (w.splits > 1) {
+    const int64_t quads = 2ll * a.batch * a.k_len * a.kv_heads * (a.head_dim / 4);
+    FP8_CUDA_TRY(launch_kernel(x_dkv_join_kernel<T>, dim3(grid_for(quads, 256, st->sm_count, 8)), dim3(256), 0, stream, 1,
+                               kStreamingKernel, kv));
+    count_launches(1);
+  }
   return ok();
 }
 
@@ -238,8 +319,11 @@ size_t fp8_cross_attention_workspace_bytes(const fp8_cross_attention_args* a, in
   if (a == nullptr || a->batch <= 0 || a->q_len <= 0 || a->k_len <= 0 || a->heads <= 0 || a->kv_heads <= 0 ||
       a->heads % a->kv_heads != 0)
     return 0;
-  if (backward) return sizeof(float) * static_cast<size_t>(a->batch) * a->heads * a->q_len;  // delta
   if (device_state(&st)) return 0;
+  if (backward) {
+    const XBwdPlan w = x_bwd_plan(a, st->sm_count);
+    return w.stats_bytes + w.part_bytes;
+  }
   return x_fwd_workspace(a, x_plan(a, st->sm_count));
 }
 
@@ -261,15 +345,16 @@ int fp8_cross_attention_fwd(const fp8_cross_attention_args* a, void* workspace, 
 int fp8_cross_attention_bwd(const fp8_cross_attention_args* a, void* workspace, size_t workspace_bytes,
                             fp8_stream_t stream) {
   if (int s = x_check(a, true)) return s;
-  FP8_REQUIRE(workspace != nullptr && aligned(workspace, 16) &&
-                  workspace_bytes >= fp8_cross_attention_workspace_bytes(a, 1),
-              FP8_ERR_WORKSPACE, "cross attention backward: workspace too small or not 16-byte aligned");
   DeviceState* st = nullptr;
   if (int s = device_state(&st)) return s;
-  XAttnParams p = x_params(a, st);
-  p.delta = static_cast<float*>(workspace);
-  return a->dtype == FP8_DTYPE_BF16 ? x_bwd<__nv_bfloat16>(p, st, cuda_stream(stream))
-                                    : x_bwd<__half>(p, st, cuda_stream(stream));
+  const XBwdPlan w = x_bwd_plan(a, st->sm_count);
+  const size_t need = w.stats_bytes + w.part_bytes;
+  FP8_REQUIRE(workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= need, FP8_ERR_WORKSPACE,
+              "cross attention backward: workspace too small or not 16-byte aligned (%zu bytes, needs %zu)",
+              workspace_bytes, need);
+  const XAttnParams p = x_params(a, st);
+  return a->dtype == FP8_DTYPE_BF16 ? x_bwd<__nv_bfloat16>(a, p, w, workspace, st, cuda_stream(stream))
+                                    : x_bwd<__half>(a, p, w, workspace, st, cuda_stream(stream));
 }
 
 // ------------------------------------------------------------------ token embedding
