@@ -247,7 +247,7 @@ XBwdPlan x_bwd_plan(const fp8_cross_attention_args* a, int sm_count) {
   w.q_chunk = (w.q_tiles + w.splits - 1) / w.splits;
   w.splits = (w.q_tiles + w.q_chunk - 1) / w.q_chunk;
   w.dkv_items = base * w.splits;
-  w.stats_bytes = static_cast<size_t>(w.dq_items) * kXTile * sizeof(float2);
+  w.stats_bytes = static_cast<size_t>(w.dq_items) * 2 * kXTile * sizeof(float);
   w.part_bytes = w.splits == 1 ? 0 : sizeof(float) * 2 * w.splits * a->batch * a->k_len * static_cast<size_t>(a->kv_heads) * a->head_dim;
   return w;
 }
@@ -275,7 +275,7 @@ int x_bwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XBwd
   XBwdParams p{};
   p.a = a;
   p.row_tiles = w.row_tiles;
-  p.stats = static_cast<float2*>(workspace);
+  p.stats = static_cast<float*>(workspace);
   p.items = w.dq_items;
   XBwdParams kv = p;
   kv.items = w.dkv_items;

@@ -23,7 +23,10 @@
 //     passes it by more than 2^8: then O and the sum are rescaled.  Scores that stay
 //     within that factor need no rescaling pass, and P <= 2^8 keeps its relative
 //     precision in bf16 and fp16;
-//   * with two row tiles a CTA, one's softmax runs while the other's products do;
+//   * with two row tiles a CTA, one's softmax runs while the other's products do; each
+//     has a warp of its own that issues its products (a product's issue takes about as
+//     long as the product, so one warp that waits for two softmaxes in turn leaves the
+//     tensor cores idle meanwhile);
 //   * tiles with keys that are not kept: their rows of K and V are zeroed in shared
 //     memory before the products, and their scores are -inf.
 // The sums and statistics are fp32; P is the one value rounded before a sum (it is a
@@ -35,12 +38,21 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "dropout.cuh"
 #include "sm100_common.cuh"
 
 namespace fp8b {
 
 constexpr int kXTile = 128;  // rows of a query tile and keys of a key tile
+
+// Device error codes of the bounded waits: kernel base + the barrier that was waited for.
+enum XError : int { kErrXForward = 300, kErrXDq = 320, kErrXDkv = 340 };
+enum XWait : int {
+  kWaitQFree = 1, kWaitKFree, kWaitVFree, kWaitQ, kWaitK, kWaitV, kWaitS, kWaitSFree, kWaitDP, kWaitDPFree, kWaitP,
+  kWaitPRest, kWaitAcc, kWaitAccFree, kWaitStaged, kWaitDelta, kWaitDrain
+};
 
 struct XStrides {
   int64_t batch, token, head;  // elements
@@ -115,6 +127,36 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
+// The warp index as a value the compiler knows to be the same in the whole warp, so that a role's branch and what
+// its loops count stay in uniform registers, where the operands of tcgen05.mma have to be.
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0); }
+
+// True in one lane of a converged warp, the same lane every time.  (With `lane == 0` in its place the operands of
+// every product are moved to uniform registers one by one: 120 cycles a product of 64 cycles.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is != 0;
+}
+
+// Descriptor of a 128-byte-swizzled operand tile of [128 rows][64 channels] halves 16 KB apart; read along its rows
+// (K-major: 16-channel steps) or across them (MN-major: 16-row steps).
+__device__ __forceinline__ uint64_t k_major_desc(uint32_t saddr) { return make_smem_desc(saddr, 16, 1024); }
+__device__ __forceinline__ uint64_t mn_major_desc(uint32_t saddr) { return make_smem_desc(saddr, 16384, 1024); }
+
+// D[128][n] = A B^T over `steps` 16-channel steps of two K-major tiles (one elected thread).
+__device__ __forceinline__ void products_k_major(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, int steps) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+    if (k < steps) umma_f16_ss(d_tmem, a + off, b + off, idesc, k > 0 ? 1u : 0u);
+  }
+}
+
 // 32 lanes x 16 columns, register -> TMEM.
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -161,6 +203,83 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 2^x for two values in fp32 arithmetic, for a share of the exponentials: the special-function unit makes 16 a cycle
+// and SM, which for heads of 64 is half of what the two products of a score take.  x = n + f with n the nearest
+// integer (read from the low bits of x + 1.5 * 2^23) and f in [-1/2, 1/2]; 2^f by the polynomial of least largest
+// relative error (fitted for this kernel: 7.5e-5 in degree 3, for weights rounded to bf16's 2^-9; 2.6e-6 in degree 4,
+// for fp16's 2^-12), and n added to its exponent.  x below -125 gives 2^-125; NaN stays NaN.
+template <int DEGREE>
+__device__ __forceinline__ void exp2_fma(float& x0, float& x1);
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Two fp32 values in one 64-bit register, for the packed fp32 instructions.
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t p, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+template <int DEGREE>
+__device__ __forceinline__ void exp2_fma(float& x0, float& x1) {
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(x0), "f"(-125.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(x1), "f"(-125.0f));
+  const uint64_t x = pair2(x0, x1);
+  const uint64_t t = add2(x, pair2(12582912.0f, 12582912.0f));
+  const uint64_t n = add2(t, pair2(-12582912.0f, -12582912.0f));
+  const uint64_t f = fma2(n, pair2(-1.0f, -1.0f), x);
+  const auto c = [](float v) { return pair2(v, v); };
+  uint64_t r;
+  if constexpr (DEGREE == 3) {
+    r = fma2(c(0.05517166853f), f, c(0.24261112511f));
+    r = fma2(r, f, c(0.69326096773f));
+    r = fma2(r, f, c(0.99992805719f));
+  } else {
+    r = fma2(c(0.00957010220f), f, c(0.05591785908f));
+    r = fma2(r, f, c(0.24024744332f));
+    r = fma2(r, f, c(0.69312179089f));
+    r = fma2(r, f, c(0.99999928474f));
+  }
+  float t0, t1, r0, r1;
+  unpair2(t, t0, t1);
+  unpair2(r, r0, r1);
+  x0 = __uint_as_float(__float_as_uint(r0) + (__float_as_uint(t0) << 23));
+  x1 = __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t1) << 23));
+}
+
+// 2^x of the pair-th pair of a row, in place; one pair of every EVERY goes by exp2_fma (0: none).
+template <typename T, int EVERY>
+__device__ __forceinline__ void exp2_pair(float& x0, float& x1, int pair) {
+  if (EVERY > 0 && pair % (EVERY > 0 ? EVERY : 1) == EVERY - 1) {
+    exp2_fma<XType<T>::kFormat == 1u ? 3 : 4>(x0, x1);
+  } else {
+    x0 = ex2(x0);
+    x1 = ex2(x1);
+  }
+}
+
 // A wait whose outcome the whole warp shares (the loads of tensor memory are warp-wide).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
                                           int code) {
@@ -196,6 +315,7 @@ __device__ __forceinline__ void x_zero_rows(uint8_t* tile, const uint4& keep, in
 }
 
 // ============================================================================ forward
+constexpr int kXExpEvery = 4;  // one pair of exponentials in so many goes by exp2_fma
 constexpr int kXMaskSlots = 8;  // key tiles whose keep bits are held: more than are ever between load and use
 
 struct XFwdParams {
@@ -213,22 +333,21 @@ struct XFwdParams {
 template <int HALVES, int NT>
 struct XFwdLayout {
   static constexpr int kTileBytes = HALVES * 16384;
-  static constexpr int kQStages = HALVES == 1 ? 2 : 1;
+  static constexpr int kQStages = HALVES == 2 ? 1 : NT == 2 ? 3 : 2;
   // key / value entries: as many as fit the CTA's share of the SM (two CTAs with NT = 1)
   static constexpr int kEntries = NT == 2 ? (HALVES == 1 ? 6 : 4) : (HALVES == 1 ? 4 : 2);
   static constexpr int kKV = NT * kTileBytes * kQStages;
   static constexpr int kWords = kKV + kEntries * kTileBytes;
   static constexpr int kBar = kWords + kXMaskSlots * 16;
-  static constexpr int kNumBars = 2 * kQStages + 2 * kEntries + 5 * NT + 1;
+  static constexpr int kNumBars = 2 * kQStages + 2 * kEntries + 7 * NT;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;  // + alignment slack
-  static constexpr int kThreads = NT * 128 + 64;
+  static constexpr int kThreads = NT * 128 + 32 + NT * 32;  // softmax, loads, products of each row tile
   static constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
   static constexpr int kCtasPerSm = NT == 2 ? 1 : 2;
 };
 static_assert(XFwdLayout<2, 2>::kSmemBytes <= 232448 && XFwdLayout<1, 2>::kSmemBytes <= 232448, "one CTA per SM");
-static_assert(2 * XFwdLayout<2, 1>::kSmemBytes <= 232448 && 2 * XFwdLayout<1, 1>::kSmemBytes <= 232448,
-              "two CTAs per SM");
+static_assert(XFwdLayout<2, 1>::kSmemBytes <= 115712 && XFwdLayout<1, 1>::kSmemBytes <= 115712, "two CTAs per SM");
 
 // One unit of work: the row tiles [tile0, tile0 + tiles) of a head group against the key tiles [j0, j1).
 struct XItem {
@@ -272,11 +391,12 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
   uint64_t* o_full = p_full + NT;
   uint64_t* o_free = o_full + NT;
   uint64_t* staged = o_free + NT;
-  uint64_t* drained = staged + NT;
+  uint64_t* p_rest = staged + NT;
+  uint64_t* drained = p_rest + NT;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::kTail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < Ly::kQStages; ++i) {
       mbar_init(q_full + i, 1);
@@ -284,7 +404,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
     }
     for (int i = 0; i < Ly::kEntries; ++i) {
       mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, 1);
+      mbar_init(kv_empty + i, NT);
     }
     for (int i = 0; i < NT; ++i) {
       mbar_init(s_full + i, 2);  // the products' commit, and the issuing thread (keep bits)
@@ -292,8 +412,9 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       mbar_init(o_full + i, 1);
       mbar_init(o_free + i, 4);
       mbar_init(staged + i, 4);
+      mbar_init(p_rest + i, 4);
+      mbar_init(drained + i, 1);
     }
-    mbar_init(drained, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -325,7 +446,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       const XItem t = x_item<NT>(p, i);
       if (t.j0 >= t.j1) continue;
       const int qs = n_item % Ly::kQStages;
-      ok = warp_wait(q_empty + qs, ((n_item / Ly::kQStages) & 1) ^ 1, abort_flag, a.err, kErrTimeoutProducer);
+      ok = warp_wait(q_empty + qs, ((n_item / Ly::kQStages) & 1) ^ 1, abort_flag, a.err, kErrXForward + kWaitQFree);
       if (!ok) break;
       if (lane == 0) {
         mbar_arrive_expect_tx(q_full + qs, q_bytes * t.tiles);
@@ -345,7 +466,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
 #pragma unroll
         for (int kv = 0; kv < 2 && ok; ++kv, ++e) {
           const int slot = e % Ly::kEntries;
-          ok = warp_wait(kv_empty + slot, ((e / Ly::kEntries) & 1) ^ 1, abort_flag, a.err, kErrTimeoutProducer);
+          ok = warp_wait(kv_empty + slot, ((e / Ly::kEntries) & 1) ^ 1, abort_flag, a.err, kErrXForward + kWaitKFree + kv);
           if (!ok) break;
           loaded = e + 1;
           if (lane == 0) {
@@ -360,129 +481,95 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
     if (!ok && lane == 0) {  // copies still in flight land before the CTA leaves
       volatile int never = 0;
       for (uint32_t k = loaded > Ly::kEntries ? loaded - Ly::kEntries : 0; k < loaded; ++k)
-        mbar_wait(kv_full + k % Ly::kEntries, (k / Ly::kEntries) & 1, &never, a.err, kErrTimeoutDrain);
+        mbar_wait(kv_full + k % Ly::kEntries, (k / Ly::kEntries) & 1, &never, a.err, kErrXForward + kWaitDrain);
       if (n_item > 0)
         mbar_wait(q_full + (n_item - 1) % Ly::kQStages, ((n_item - 1) / Ly::kQStages) & 1, &never, a.err,
-                  kErrTimeoutDrain);
+                  kErrXForward + kWaitDrain);
     }
-  } else if (warp == 4 * NT + 1) {
-    // ------------------------------------------------------------ products
-    struct Cursor {
-      int64_t i;
-      XItem t;
-      int j;
-      uint32_t g;       // key tiles before this one
-      uint32_t n_item;  // items with keys before this one
-    };
-    // moves to the next key tile; false when there is none
-    const auto seek = [&](Cursor& c) {
-      while (c.j >= c.t.j1) {
-        c.i += gridDim.x;
-        if (c.i >= p.items) return false;
-        if (c.t.j1 > c.t.j0) ++c.n_item;
-        c.t = x_item<NT>(p, c.i);
-        c.j = c.t.j0;
-      }
-      return true;
-    };
-    uint32_t n_p[NT] = {}, n_o[NT] = {};  // weights taken, items begun, by row tile
+  } else if (warp > 4 * NT) {
+    // ------------------------------------------------------------ products of row tile r
+    const int r = warp - 4 * NT - 1;
     const uint32_t s_base = smem_u32(smem);
+    const uint32_t idesc_o = x_idesc<T>(ksteps * 16, 0, 1);
+    const uint32_t t_s = tmem + r * 128, t_o = tmem + NT * 128 + r * HALVES * 64;
+    uint32_t n_item = 0, g = 0, n_s = 0, n_out = 0;  // items and key tiles of the CTA; key tiles and items of this row tile
     bool ok = true;
-    const auto wait_entry = [&](uint32_t entry, const Cursor& c) {
-      const int slot = entry % Ly::kEntries;
-      if (!warp_wait(kv_full + slot, (entry / Ly::kEntries) & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
-      if (masked || (c.j + 1) * kXTile > c.t.keys) {
-        const uint4 w = words[c.g % kXMaskSlots];
+    // Entry e (K of key tile e / 2, or its V) has arrived, with zeros in the rows that are not kept.  (Each row tile's
+    // warp writes them: the same zeros.)
+    const auto entry = [&](uint32_t e, bool bits) {
+      const int slot = e % Ly::kEntries;
+      if (!warp_wait(kv_full + slot, (e / Ly::kEntries) & 1, abort_flag, a.err, kErrXForward + kWaitK + (e & 1)))
+        return false;
+      if (bits) {
+        const uint4 w = words[(e >> 1) % kXMaskSlots];
         if ((w.x & w.y & w.z & w.w) != 0xffffffffu) x_zero_rows<HALVES>(smem + Ly::kKV + slot * Ly::kTileBytes, w, lane);
       }
       return true;
     };
-    const auto issue_s = [&](const Cursor& c, int r) {
-      if (lane == 0) {
-        const int n = x_chunks(c.t.keys, c.j) * 32;
-        const uint32_t idesc = x_idesc<T>(n, 0, 0);
-        const uint32_t sq = s_base + ((c.n_item % Ly::kQStages) * NT + r) * Ly::kTileBytes;
-        const uint32_t sk = s_base + Ly::kKV + (2 * c.g % Ly::kEntries) * Ly::kTileBytes;
-        tc_fence_after();
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          umma_f16_ss(tmem + r * 128, make_smem_desc(sq + off, 16, 1024), make_smem_desc(sk + off, 16, 1024), idesc,
-                      k > 0 ? 1u : 0u);
-        }
-        umma_commit(s_full + r);
-        mbar_arrive(s_full + r);
-        if (r == c.t.tiles - 1) umma_commit(kv_empty + 2 * c.g % Ly::kEntries);
-      }
-    };
-    const auto issue_pv = [&](const Cursor& c, int r) {
-      if (!warp_wait(p_full + r, n_p[r] & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
-      ++n_p[r];
-      if (c.j == c.t.j0) {  // the last item's output has been read
-        if (n_o[r] > 0 && !warp_wait(o_free + r, (n_o[r] - 1) & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
-        ++n_o[r];
-      }
-      if (lane == 0) {
-        const uint32_t idesc = x_idesc<T>(ksteps * 16, 0, 1);
-        const uint32_t entry = 2 * c.g + 1;
-        const uint32_t sv = s_base + Ly::kKV + (entry % Ly::kEntries) * Ly::kTileBytes;
-        tc_fence_after();
-        const int steps = 2 * x_chunks(c.t.keys, c.j);
-        for (int k = 0; k < steps; ++k)
-          umma_f16_ts(tmem + NT * 128 + r * HALVES * 64, tmem + r * 128 + k * 8, make_smem_desc(sv + k * 2048, 16384, 1024),
-                      idesc, (c.j > c.t.j0 || k > 0) ? 1u : 0u);
-        if (c.j == c.t.j1 - 1) umma_commit(o_full + r);
-        if (r == c.t.tiles - 1) umma_commit(kv_empty + entry % Ly::kEntries);
-      }
-      __syncwarp();
-      return true;
-    };
-    const auto begin_tile = [&](const Cursor& c) {  // Q (with an item's first tile) and K are there
-      if (c.j == c.t.j0 && !warp_wait(q_full + c.n_item % Ly::kQStages, (c.n_item / Ly::kQStages) & 1, abort_flag, a.err,
-                                      kErrTimeoutMma))
-        return false;
-      return wait_entry(2 * c.g, c);
-    };
-
-    Cursor cur{};
-    cur.i = blockIdx.x;
-    bool more = cur.i < p.items;
-    if (more) {
-      cur.t = x_item<NT>(p, cur.i);
-      cur.j = cur.t.j0;
-      more = seek(cur);
-    }
-    if (more) {
-      ok = begin_tile(cur);
-      for (int r = 0; ok && r < cur.t.tiles; ++r) issue_s(cur, r);
-    }
-    while (more && ok) {
-      Cursor nxt = cur;
-      ++nxt.j;
-      ++nxt.g;
-      more = seek(nxt);
-      ok = wait_entry(2 * cur.g + 1, cur);
-      // with one Q stage the next item's Q waits for this item's output: every row tile's P V goes first
-      const bool apart = Ly::kQStages == 1 && more && nxt.j == nxt.t.j0;
-      bool begun = false;
+    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+      const XItem t = x_item<NT>(p, i);
+      if (t.j0 >= t.j1) continue;
+      const int qs = n_item % Ly::kQStages;
+      if (r >= t.tiles) {  // no rows: the entries are only passed on
+        for (int j = t.j0; j < t.j1 && ok; ++j, ++g)
 #pragma unroll
-      for (int r = 0; r < NT; ++r) {
-        if (ok && r < cur.t.tiles) ok = issue_pv(cur, r);
-        if (ok && more && !apart && r < nxt.t.tiles) {
-          if (!begun) ok = begin_tile(nxt);
-          begun = true;
-          if (ok) issue_s(nxt, r);
+          for (uint32_t e = 2 * g; e < 2 * g + 2; ++e) {
+            const int slot = e % Ly::kEntries;
+            ok = ok && warp_wait(kv_full + slot, (e / Ly::kEntries) & 1, abort_flag, a.err, kErrXForward + kWaitK + (e & 1));
+            if (ok && lane == 0) mbar_arrive(kv_empty + slot);
+          }
+        ++n_item;
+        continue;
+      }
+      ok = warp_wait(q_full + qs, (n_item / Ly::kQStages) & 1, abort_flag, a.err, kErrXForward + kWaitQ);
+      const uint64_t sq = k_major_desc(s_base + (qs * NT + r) * Ly::kTileBytes);
+      for (int j = t.j0; j < t.j1 && ok; ++j, ++g, ++n_s) {
+        const int chunks = x_chunks(t.keys, j);
+        const bool bits = masked || (j + 1) * kXTile > t.keys;
+        // S over the last tile's P, whose product was issued before it (products run in their order)
+        if (!(ok = entry(2 * g, bits))) break;
+        tc_fence_after();
+        if (elect_one()) {
+          products_k_major(t_s, sq, k_major_desc(s_base + Ly::kKV + (2 * g % Ly::kEntries) * Ly::kTileBytes),
+                           x_idesc<T>(chunks * 32, 0, 0), ksteps);
+          umma_commit(s_full + r);
+          mbar_arrive(s_full + r);
+          umma_commit(kv_empty + 2 * g % Ly::kEntries);
         }
+        __syncwarp();
+        // O += P V, its first half as soon as the first 64 weights are there
+        ok = entry(2 * g + 1, bits) && warp_wait(p_full + r, n_s & 1, abort_flag, a.err, kErrXForward + kWaitP);
+        if (ok && j == t.j0 && n_out > 0)  // the last item's output has been read
+          ok = warp_wait(o_free + r, (n_out - 1) & 1, abort_flag, a.err, kErrXForward + kWaitAccFree);
+        if (!ok) break;
+        const uint64_t sv = mn_major_desc(s_base + Ly::kKV + ((2 * g + 1) % Ly::kEntries) * Ly::kTileBytes);
+        const uint32_t later = j > t.j0 ? 1u : 0u;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < 2 * chunks) umma_f16_ts(t_o, t_s + k * 8, sv + k * 128, idesc_o, k > 0 ? 1u : later);
+        }
+        __syncwarp();
+        ok = warp_wait(p_rest + r, n_s & 1, abort_flag, a.err, kErrXForward + kWaitPRest);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 4; k < 8; ++k)
+            if (k < 2 * chunks) umma_f16_ts(t_o, t_s + k * 8, sv + k * 128, idesc_o, 1u);
+          umma_commit(kv_empty + (2 * g + 1) % Ly::kEntries);
+          if (j == t.j1 - 1) umma_commit(o_full + r);
+        }
+        __syncwarp();
       }
-      if (ok && more && apart) {
-        ok = begin_tile(nxt);
-        for (int r = 0; ok && r < nxt.t.tiles; ++r) issue_s(nxt, r);
-      }
-      cur = nxt;
+      ++n_out;
+      ++n_item;
     }
-    if (!ok && lane == 0) {  // the products in flight end before the tensor memory is freed
+    if (!ok && elect_one()) {  // the products in flight end before the tensor memory is freed
       volatile int never = 0;
-      umma_commit(drained);
-      mbar_wait(drained, 0, &never, a.err, kErrTimeoutDrain);
+      umma_commit(drained + r);
+      mbar_wait(drained + r, 0, &never, a.err, kErrXForward + kWaitDrain);
     }
   } else {
     // ------------------------------------------------------------ softmax: thread = row of row tile rt
@@ -494,6 +581,15 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
     const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
     const int rows = a.tile_tokens * a.pack;
     uint32_t n_s = 0, n_out = 0, n_item = 0, g = 0;
+    int stored = -1;  // Q stage whose output is on its way out
+    // The stage is free for a new Q once the output has been read from it; asked for as late as can be.
+    const auto release_stored = [&]() {
+      if (Ly::kQStages > 1 && stored >= 0 && quad == 0 && lane == 0) {
+        bulk_wait_group_read<0>();
+        mbar_arrive(q_empty + stored);
+      }
+      stored = -1;
+    };
     bool ok = true;
     for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
       const XItem t = x_item<NT>(p, i);
@@ -515,8 +611,9 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       }
       const int qs = n_item % Ly::kQStages;
       if (rt >= t.tiles) {  // this row tile has no rows in the item
+        release_stored();
         if (quad == 0) {
-          ok = warp_wait(q_full + qs, (n_item / Ly::kQStages) & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+          ok = warp_wait(q_full + qs, (n_item / Ly::kQStages) & 1, abort_flag, a.err, kErrXForward + kWaitQ);
           if (ok && lane == 0) mbar_arrive(q_empty + qs);
         }
         ++n_item;
@@ -526,85 +623,139 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       // rows of this warp that exist: a warp without any keeps only the barriers
       const bool any_row = __any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.0f;
-      for (int j = t.j0; j < t.j1; ++j, ++g, ++n_s) {
-        ok = warp_wait(s_full + rt, n_s & 1, abort_flag, a.err, kErrTimeoutEpilogue);
-        if (!ok) break;
-        tc_fence_after();
-        if (any_row) {
-          const int chunks = x_chunks(t.keys, j);
-          uint32_t v[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c < chunks) tmem_ld_32x32b_x32(t_s + c * 32, v[c]);
-          tmem_ld_wait();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) after_wait(v[c]);
-          if (flip) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int k = 0; k < 32; ++k) v[c][k] ^= 0x80000000u;
-          }
-          if (masked || (j + 1) * kXTile > t.keys) {
-            const uint4 w4 = words[g % kXMaskSlots];
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (c < chunks && w[c] != 0xffffffffu) {
-#pragma unroll
-                for (int k = 0; k < 32; ++k) v[c][k] = (w[c] >> k) & 1u ? v[c][k] : 0xff800000u;
-              }
-          }
-          float mt = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c < chunks) {
-#pragma unroll
-              for (int k = 0; k < 32; k += 2)
-                mt = fmaxf(mt, fmaxf(__uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1])));
-            }
-          if (__any_sync(0xffffffffu, live && ((mt - m) * c2 > 8.0f || m == -INFINITY))) {
-            const float mn = fmaxf(m, mt);
-            const float f = m == -INFINITY ? 0.0f : ex2((m - mn) * c2);
-            l *= f;
-            m = mn;
-            if (j > t.j0) {
+      uint64_t sum[2];  // of the tile's weights, four partial sums
+      // Raises the exponent's reference to at least the row's maximum mt over 2^8, with what was summed so far.
+      const auto raise = [&](float mt, int j) {
+        if (__any_sync(0xffffffffu, live && ((mt - m) * c2 > 8.0f || m == -INFINITY))) {
+          const float mn = fmaxf(m, mt);
+          const float f = m == -INFINITY ? 0.0f : ex2((m - mn) * c2);
+          l *= f;
+          m = mn;
+          if (j > t.j0) {
 #pragma unroll 1
-              for (int c = 0; c < 2 * HALVES; ++c) {
-                uint32_t o[32];
-                tmem_ld_32x32b_x32(t_o + c * 32, o);
-                tmem_ld_wait();
-                after_wait(o);
+            for (int c = 0; c < 2 * HALVES; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(t_o + c * 32, o);
+              tmem_ld_wait();
+              after_wait(o);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                tmem_st_32x32b_x32(t_o + c * 32, o);
-              }
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st_32x32b_x32(t_o + c * 32, o);
             }
           }
-          const float mc = m == -INFINITY ? 0.0f : m * c2;
-          float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c < chunks) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                const float p0 = ex2(fmaf(__uint_as_float(v[c][k]), c2, -mc));
-                const float p1 = ex2(fmaf(__uint_as_float(v[c][k + 1]), c2, -mc));
-                sum[0] += p0;
-                sum[1] += p1;
-                pk[k >> 1] = XType<T>::pack2(p0, p1);
-              }
-              tmem_st_32x32b_x16(t_s + c * 16, pk);
-            }
-          l += sum[0] + sum[1];
-          tmem_st_wait();
         }
+      };
+      // The weights of chunk c, which take the place of a half of its scores.
+      const auto weigh = [&](auto every, const uint32_t(&v)[32], int c, uint64_t c22, uint64_t mc2) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          float x0, x1;
+          unpair2(fma2(pair2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c22, mc2), x0, x1);
+          exp2_pair<T, decltype(every)::value>(x0, x1, k >> 1);
+          sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair2(x0, x1));
+          pk[k >> 1] = XType<T>::pack2(x0, x1);
+        }
+        tmem_st_32x32b_x16(t_s + c * 16, pk);
+      };
+      const auto give = [&](uint64_t* bar) {  // the products over what was stored can begin
+        tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + rt);
+        if (lane == 0) mbar_arrive(bar);
+      };
+      for (int j = t.j0; j < t.j1; ++j, ++g, ++n_s) {
+        ok = warp_wait(s_full + rt, n_s & 1, abort_flag, a.err, kErrXForward + kWaitS);
+        if (!ok) break;
+        tc_fence_after();
+        const int chunks = x_chunks(t.keys, j);
+        if (!any_row) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(p_full + rt);
+            mbar_arrive(p_rest + rt);
+          }
+        } else {
+          sum[0] = sum[1] = pair2(0.0f, 0.0f);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          const auto search = [&](const uint32_t(&x)[32]) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8)
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                mx[u] = max3(mx[u], __uint_as_float(x[k + 2 * u]), __uint_as_float(x[k + 2 * u + 1]));
+          };
+          if (!masked && !flip && (j + 1) * kXTile <= t.keys) {
+            // 128 kept keys: half of the row stays in registers, the other half is read twice
+            constexpr std::integral_constant<int, kXExpEvery> kShare;
+            uint32_t v0[32], v1[32], v2[32], v3[32];
+            tmem_ld_32x32b_x32(t_s, v0);
+            tmem_ld_32x32b_x32(t_s + 32, v1);
+            tmem_ld_wait();
+            after_wait(v0);
+            after_wait(v1);
+            tmem_ld_32x32b_x32(t_s + 64, v2);
+            tmem_ld_32x32b_x32(t_s + 96, v3);
+            search(v0);
+            search(v1);
+            tmem_ld_wait();
+            after_wait(v2);
+            after_wait(v3);
+            search(v2);
+            search(v3);
+            raise(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), j);
+            const float mc = -m * c2;
+            const uint64_t c22 = pair2(c2, c2), mc2 = pair2(mc, mc);
+            weigh(kShare, v0, 0, c22, mc2);
+            tmem_ld_32x32b_x32(t_s + 64, v2);
+            weigh(kShare, v1, 1, c22, mc2);
+            give(p_full + rt);
+            tmem_ld_wait();
+            after_wait(v2);
+            tmem_ld_32x32b_x32(t_s + 96, v3);
+            weigh(kShare, v2, 2, c22, mc2);
+            tmem_ld_wait();
+            after_wait(v3);
+            weigh(kShare, v3, 3, c22, mc2);
+            give(p_rest + rt);
+          } else {
+            const bool bits = masked || (j + 1) * kXTile > t.keys;
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(words + g % kXMaskSlots);
+            const uint32_t sign = flip ? 0x80000000u : 0u;
+            const auto load = [&](uint32_t(&v)[32], int c) {
+              tmem_ld_32x32b_x32(t_s + c * 32, v);
+              const uint32_t keep = bits ? w[c] : ~0u;
+              tmem_ld_wait();
+              after_wait(v);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] = (keep >> k) & 1u ? v[k] ^ sign : 0xff800000u;
+            };
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+              uint32_t v[32];
+              load(v, c);
+              search(v);
+            }
+            raise(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), j);
+            const float mc = m == -INFINITY ? 0.0f : -m * c2;
+            const uint64_t c22 = pair2(c2, c2), mc2 = pair2(mc, mc);
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+              uint32_t v[32];
+              load(v, c);
+              weigh(std::integral_constant<int, 0>{}, v, c, c22, mc2);  // 2^-inf has to be zero
+              if (c == min(chunks, 2) - 1) give(p_full + rt);
+            }
+            give(p_rest + rt);
+          }
+          float s0, s1;
+          unpair2(add2(sum[0], sum[1]), s0, s1);
+          l += s0 + s1;
+        }
       }
-      if (ok) ok = warp_wait(o_full + rt, n_out & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+      release_stored();
+      if (ok) ok = warp_wait(o_full + rt, n_out & 1, abort_flag, a.err, kErrXForward + kWaitAcc);
       if (!ok) break;
       ++n_out;
       tc_fence_after();
@@ -652,16 +803,19 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
         mbar_arrive(staged + rt);
       }
       if (quad == 0 && lane == 0) {
-        ok = mbar_wait(staged + rt, (n_out - 1) & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+        ok = mbar_wait(staged + rt, (n_out - 1) & 1, abort_flag, a.err, kErrXForward + kWaitStaged);
         if (ok && p.splits == 1) {
           for (int hf = 0; hf < HALVES; ++hf)
             tma_store_4d(&o_map, stage + hf * 16384, hf * 64, t.hv * a.pack, (t.tile0 + rt) * a.tile_tokens, t.b);
           bulk_commit_group();
-          bulk_wait_group_read<0>();
         }
-        if (ok) mbar_arrive(q_empty + qs);
+        if (ok && Ly::kQStages == 1) {
+          bulk_wait_group_read<0>();
+          mbar_arrive(q_empty + qs);
+        }
       }
       ok = __all_sync(0xffffffffu, ok);
+      stored = qs;
       ++n_item;
     }
     if (quad == 0 && lane == 0) bulk_wait_group<0>();

@@ -11,7 +11,9 @@
 //     dV += P^T dO and dK += dS^T Q.
 // That is seven products a tile pair; a single launch would need five, but would add
 // dQ to memory from every key tile.  Both kernels know the rows' log-sum-exp, so no
-// maximum is searched and the 256 softmax threads take 64 columns of a row each.
+// maximum is searched and the 256 softmax threads take 64 columns of a row each.  Two
+// warps issue the products: one the scores and dP, which run ahead into a second score
+// buffer (dQ) or into the columns the softmax has read (dK, dV), one the gradients.
 //
 // P and dS are rounded to the tensors' type (they are matrix operands); scores, dP,
 // statistics and all sums are fp32.
@@ -24,7 +26,8 @@ namespace fp8b {
 struct XBwdParams {
   XAttnParams a;
   int row_tiles;  // row tiles of a (sequence, head group)
-  float2* stats;  // [batch][head groups][row_tiles][128]: (lse in log2 units, +inf where the row has no weight; delta)
+  // [batch][head groups][row_tiles][2][128]: -log-sum-exp in log2 units (-inf where the row has no weight), -delta
+  float* stats;
   int64_t items;
   // x_dkv_kernel
   int q_tiles;    // row tiles that read a key head: (group / pack) * row_tiles
@@ -36,12 +39,12 @@ struct XBwdParams {
 // Sum of the products of eight 16-bit values.
 template <typename T>
 __device__ __forceinline__ float x_dot8(const uint4& x, const uint4& y) {
-  float s = 0.0f;
   const T* u = reinterpret_cast<const T*>(&x);
   const T* v = reinterpret_cast<const T*>(&y);
+  float s[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int k = 0; k < 8; ++k) s = fmaf(to_f32(u[k]), to_f32(v[k]), s);
-  return s;
+  for (int k = 0; k < 8; ++k) s[k & 1] = fmaf(to_f32(u[k]), to_f32(v[k]), s[k & 1]);
+  return s[0] + s[1];
 }
 
 // ============================================================================ dQ
@@ -49,43 +52,25 @@ template <int HALVES>
 struct XDqLayout {
   static constexpr int kTileBytes = HALVES * 16384;
   static constexpr int kQStages = HALVES == 1 ? 3 : 1;  // Q and dO of an item
-  static constexpr int kEntries = HALVES == 1 ? 6 : 5;  // key and value tiles in turn
-  static constexpr int kKV = 2 * kQStages * kTileBytes;
-  static constexpr int kWords = kKV + kEntries * kTileBytes;
-  static constexpr int kBar = kWords + kXMaskSlots * 16;
-  static constexpr int kNumBars = 2 * kQStages + 2 * kEntries + 9;
+  // A key tile stays from its scores to its dQ product, two tiles later; a value tile only for its dP.
+  static constexpr int kKStages = HALVES == 1 ? 4 : 3;
+  static constexpr int kVStages = HALVES == 1 ? 3 : 2;
+  static constexpr int kK = 2 * kQStages * kTileBytes;
+  static constexpr int kV = kK + kKStages * kTileBytes;
+  static constexpr int kWords = kV + kVStages * kTileBytes;
+  static constexpr int kDelta = kWords + kXMaskSlots * 16;  // fp32 [2][128]: the halves of the rows' delta
+  static constexpr int kBar = kDelta + 1024;
+  static constexpr int kNumBars = 2 * (kQStages + kKStages + kVStages) + 13;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;
-  static constexpr int kThreads = 320;
+  static constexpr int kThreads = 352;
 };
 static_assert(XDqLayout<1>::kSmemBytes <= 232448 && XDqLayout<2>::kSmemBytes <= 232448, "dq smem");
 // tensor memory columns: two score buffers (dS over the first half of each 64), dP, dQ
 constexpr uint32_t kXDqS = 0, kXDqDP = 256, kXDqAcc = 384;
 
-// A place in the sequence of (item, key tile) pairs of a CTA.
-template <typename Item>
-struct XCursor {
-  int64_t i;
-  Item t;
-  int j;
-  uint32_t g;       // tiles before this one
-  uint32_t n_item;  // items with tiles before this one
-};
-// Moves to the next tile at or after c; false when there is none.
-template <typename Item, typename MakeItem>
-__device__ __forceinline__ bool x_seek(XCursor<Item>& c, int64_t items, const MakeItem& make) {
-  while (c.j >= c.t.j1) {
-    c.i += gridDim.x;
-    if (c.i >= items) return false;
-    if (c.t.j1 > c.t.j0) ++c.n_item;
-    c.t = make(c.i);
-    c.j = c.t.j0;
-  }
-  return true;
-}
-
 struct XDqItem {
-  int b, hv, tile, keys, j0, j1;
+  int b, hv, tile, keys, tiles;
 };
 __device__ __forceinline__ XDqItem x_dq_item(const XBwdParams& p, int64_t i) {
   XDqItem t;
@@ -95,8 +80,7 @@ __device__ __forceinline__ XDqItem x_dq_item(const XBwdParams& p, int64_t i) {
   t.hv = static_cast<int>(i % hv);
   t.b = static_cast<int>(i / hv);
   t.keys = x_key_count(p.a, t.b);
-  t.j0 = 0;
-  t.j1 = (t.keys + kXTile - 1) / kXTile;
+  t.tiles = (t.keys + kXTile - 1) / kXTile;
   return t;
 }
 
@@ -109,40 +93,52 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint4* words = reinterpret_cast<uint4*>(smem + Ly::kWords);
+  float* delta_half = reinterpret_cast<float*>(smem + Ly::kDelta);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + Ly::kBar);
   uint64_t* q_empty = q_full + Ly::kQStages;
-  uint64_t* kv_full = q_empty + Ly::kQStages;
-  uint64_t* kv_empty = kv_full + Ly::kEntries;
-  uint64_t* s_full = kv_empty + Ly::kEntries;  // [2], by score buffer
-  uint64_t* dp_full = s_full + 2;
+  uint64_t* k_full = q_empty + Ly::kQStages;
+  uint64_t* k_empty = k_full + Ly::kKStages;
+  uint64_t* v_full = k_empty + Ly::kKStages;
+  uint64_t* v_empty = v_full + Ly::kVStages;
+  uint64_t* s_full = v_empty + Ly::kVStages;  // [2], by score buffer
+  uint64_t* s_free = s_full + 2;              // [2]: its dS has been multiplied
+  uint64_t* dp_full = s_free + 2;
   uint64_t* dp_free = dp_full + 1;
   uint64_t* ds_full = dp_free + 1;
   uint64_t* acc_full = ds_full + 1;
   uint64_t* acc_free = acc_full + 1;
   uint64_t* staged = acc_free + 1;
-  uint64_t* drained = staged + 1;
+  uint64_t* delta_full = staged + 1;
+  uint64_t* drained = delta_full + 1;  // [2], by issuing warp
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::kTail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < Ly::kQStages; ++i) {
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 1);
     }
-    for (int i = 0; i < Ly::kEntries; ++i) {
-      mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, 1);
+    for (int i = 0; i < Ly::kKStages; ++i) {
+      mbar_init(k_full + i, 1);
+      mbar_init(k_empty + i, 1);
     }
-    mbar_init(s_full, 2);
-    mbar_init(s_full + 1, 2);
+    for (int i = 0; i < Ly::kVStages; ++i) {
+      mbar_init(v_full + i, 1);
+      mbar_init(v_empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 2);  // the products' commit, and the issuing thread (keep bits)
+      mbar_init(s_free + i, 1);
+      mbar_init(drained + i, 1);
+    }
     mbar_init(dp_full, 1);
     mbar_init(dp_free, 8);
     mbar_init(ds_full, 8);
     mbar_init(acc_full, 1);
     mbar_init(acc_free, 8);
     mbar_init(staged, 8);
-    mbar_init(drained, 1);
+    mbar_init(delta_full, 8);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -159,18 +155,21 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
   const XAttnParams& a = p.a;
   const bool masked = a.key_mask != nullptr;
   const int ksteps = (a.head_dim + 15) >> 4;
-  const auto make = [&](int64_t i) { return x_dq_item(p, i); };
+  const uint32_t s_base = smem_u32(smem);
+  const auto wait = [&](uint64_t* bar, uint32_t phase, int what) {
+    return warp_wait(bar, phase & 1, abort_flag, a.err, kErrXDq + what);
+  };
 
   if (warp == 8) {
     // ------------------------------------------------------------ loads
     const uint32_t q_bytes = static_cast<uint32_t>(a.tile_tokens * a.pack) * 128u * HALVES;
-    uint32_t e = 0, loaded = 0, n_item = 0, g = 0;
+    uint32_t n_item = 0, g = 0, n_k = 0, n_v = 0;  // n_k, n_v: copies started
     bool ok = true;
     for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDqItem t = make(i);
-      if (t.j0 >= t.j1) continue;
+      const XDqItem t = x_dq_item(p, i);
+      if (t.tiles == 0) continue;
       const int qs = n_item % Ly::kQStages;
-      ok = warp_wait(q_empty + qs, ((n_item / Ly::kQStages) & 1) ^ 1, abort_flag, a.err, kErrTimeoutProducer);
+      ok = wait(q_empty + qs, (n_item / Ly::kQStages) ^ 1, kWaitQFree);
       if (!ok) break;
       if (lane == 0) {
         uint8_t* dst = smem + 2 * qs * Ly::kTileBytes;
@@ -183,214 +182,221 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
       }
       ++n_item;
       const int hk = t.hv * a.pack / a.group;
-      for (int j = t.j0; j < t.j1 && ok; ++j, ++g) {
+      for (int j = 0; j < t.tiles; ++j, ++g) {
         if (masked || (j + 1) * kXTile > t.keys) {
           const uint4 w = x_keep_words(a, t.b, j * kXTile, t.keys, lane);
           if (lane == 0) words[g % kXMaskSlots] = w;
         }
-#pragma unroll
-        for (int kv = 0; kv < 2 && ok; ++kv, ++e) {
-          const int slot = e % Ly::kEntries;
-          ok = warp_wait(kv_empty + slot, ((e / Ly::kEntries) & 1) ^ 1, abort_flag, a.err, kErrTimeoutProducer);
-          if (!ok) break;
-          loaded = e + 1;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(kv_full + slot, Ly::kTileBytes);
-            for (int hf = 0; hf < HALVES; ++hf)
-              tma_load_4d(smem + Ly::kKV + slot * Ly::kTileBytes + hf * 16384, kv ? &v_map : &k_map, kv_full + slot,
-                          hf * 64, hk, j * kXTile, t.b);
-          }
+        const int ks = g % Ly::kKStages, vs = g % Ly::kVStages;
+        ok = wait(k_empty + ks, (g / Ly::kKStages) ^ 1, kWaitKFree);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(k_full + ks, Ly::kTileBytes);
+          for (int hf = 0; hf < HALVES; ++hf)
+            tma_load_4d(smem + Ly::kK + ks * Ly::kTileBytes + hf * 16384, &k_map, k_full + ks, hf * 64, hk, j * kXTile, t.b);
         }
+        ++n_k;
+        ok = wait(v_empty + vs, (g / Ly::kVStages) ^ 1, kWaitVFree);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(v_full + vs, Ly::kTileBytes);
+          for (int hf = 0; hf < HALVES; ++hf)
+            tma_load_4d(smem + Ly::kV + vs * Ly::kTileBytes + hf * 16384, &v_map, v_full + vs, hf * 64, hk, j * kXTile, t.b);
+        }
+        ++n_v;
       }
     }
     if (!ok && lane == 0) {  // copies still in flight land before the CTA leaves
       volatile int never = 0;
-      for (uint32_t k = loaded > Ly::kEntries ? loaded - Ly::kEntries : 0; k < loaded; ++k)
-        mbar_wait(kv_full + k % Ly::kEntries, (k / Ly::kEntries) & 1, &never, a.err, kErrTimeoutDrain);
-      for (uint32_t k = n_item > Ly::kQStages ? n_item - Ly::kQStages : 0; k < n_item; ++k)
-        mbar_wait(q_full + k % Ly::kQStages, (k / Ly::kQStages) & 1, &never, a.err, kErrTimeoutDrain);
+      const auto drain = [&](uint64_t* full, uint32_t stages, uint32_t n) {
+        for (uint32_t k = n > stages ? n - stages : 0; k < n; ++k)
+          mbar_wait(full + k % stages, (k / stages) & 1, &never, a.err, kErrXDq + kWaitDrain);
+      };
+      drain(q_full, Ly::kQStages, n_item);
+      drain(k_full, Ly::kKStages, n_k);
+      drain(v_full, Ly::kVStages, n_v);
     }
   } else if (warp == 9) {
-    // ------------------------------------------------------------ products
-    using Cursor = XCursor<XDqItem>;
-    const uint32_t s_base = smem_u32(smem);
+    // ------------------------------------------------------------ products S = Q K^T, dP = dO V^T
+    uint32_t n_item = 0, g = 0;
     bool ok = true;
-    uint32_t n_acc = 0;
-    const auto wait_entry = [&](uint32_t entry, const Cursor& c) {
-      const int slot = entry % Ly::kEntries;
-      if (!warp_wait(kv_full + slot, (entry / Ly::kEntries) & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
-      if (masked || (c.j + 1) * kXTile > c.t.keys) {
-        const uint4 w = words[c.g % kXMaskSlots];
-        if ((w.x & w.y & w.z & w.w) != 0xffffffffu) x_zero_rows<HALVES>(smem + Ly::kKV + slot * Ly::kTileBytes, w, lane);
-      }
-      return true;
-    };
-    // S of a tile into score buffer g % 2
-    const auto issue_s = [&](const Cursor& c) {
-      const int qs = c.n_item % Ly::kQStages;
-      if (c.j == c.t.j0 && !warp_wait(q_full + qs, (c.n_item / Ly::kQStages) & 1, abort_flag, a.err, kErrTimeoutMma))
-        return false;
-      if (!wait_entry(2 * c.g, c)) return false;
-      if (lane == 0) {
-        const uint32_t idesc = x_idesc<T>(x_chunks(c.t.keys, c.j) * 32, 0, 0);
-        const uint32_t sq = s_base + 2 * qs * Ly::kTileBytes;
-        const uint32_t sk = s_base + Ly::kKV + (2 * c.g % Ly::kEntries) * Ly::kTileBytes;
+    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+      const XDqItem t = x_dq_item(p, i);
+      if (t.tiles == 0) continue;
+      const int qs = n_item % Ly::kQStages;
+      ok = wait(q_full + qs, n_item / Ly::kQStages, kWaitQ);
+      const uint64_t sq = k_major_desc(s_base + 2 * qs * Ly::kTileBytes);
+      const uint64_t sdo = k_major_desc(s_base + (2 * qs + 1) * Ly::kTileBytes);
+      for (int j = 0; j < t.tiles && ok; ++j, ++g) {
+        const int ks = g % Ly::kKStages, vs = g % Ly::kVStages, buf = g & 1;
+        const uint32_t idesc = x_idesc<T>(x_chunks(t.keys, j) * 32, 0, 0);
+        const bool bits = masked || (j + 1) * kXTile > t.keys;
+        uint8_t* sk = smem + Ly::kK + ks * Ly::kTileBytes;
+        uint8_t* sv = smem + Ly::kV + vs * Ly::kTileBytes;
+        if (!(ok = wait(k_full + ks, g / Ly::kKStages, kWaitK))) break;
+        uint4 w = make_uint4(~0u, ~0u, ~0u, ~0u);
+        if (bits) w = words[g % kXMaskSlots];
+        const bool holes = (w.x & w.y & w.z & w.w) != 0xffffffffu;
+        if (holes) x_zero_rows<HALVES>(sk, w, lane);
+        if (g >= 2 && !(ok = wait(s_free + buf, (g >> 1) ^ 1, kWaitSFree))) break;
         tc_fence_after();
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          umma_f16_ss(tmem + kXDqS + (c.g & 1) * 128, make_smem_desc(sq + off, 16, 1024), make_smem_desc(sk + off, 16, 1024),
-                      idesc, k > 0 ? 1u : 0u);
+        if (elect_one()) {
+          products_k_major(tmem + kXDqS + buf * 128, sq, k_major_desc(smem_u32(sk)), idesc, ksteps);
+          umma_commit(s_full + buf);
+          mbar_arrive(s_full + buf);
         }
-        umma_commit(s_full + (c.g & 1));
-        mbar_arrive(s_full + (c.g & 1));
-      }
-      __syncwarp();
-      return true;
-    };
-    const auto issue_dp = [&](const Cursor& c) {
-      if (!wait_entry(2 * c.g + 1, c)) return false;
-      if (lane == 0) {
-        const uint32_t idesc = x_idesc<T>(x_chunks(c.t.keys, c.j) * 32, 0, 0);
-        const uint32_t sdo = s_base + (2 * (c.n_item % Ly::kQStages) + 1) * Ly::kTileBytes;
-        const uint32_t entry = 2 * c.g + 1;
-        const uint32_t sv = s_base + Ly::kKV + (entry % Ly::kEntries) * Ly::kTileBytes;
+        __syncwarp();
+        if (!(ok = wait(v_full + vs, g / Ly::kVStages, kWaitV))) break;
+        if (holes) x_zero_rows<HALVES>(sv, w, lane);
+        if (g >= 1 && !(ok = wait(dp_free, g ^ 1, kWaitDPFree))) break;
         tc_fence_after();
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          umma_f16_ss(tmem + kXDqDP, make_smem_desc(sdo + off, 16, 1024), make_smem_desc(sv + off, 16, 1024), idesc,
-                      k > 0 ? 1u : 0u);
+        if (elect_one()) {
+          products_k_major(tmem + kXDqDP, sdo, k_major_desc(smem_u32(sv)), idesc, ksteps);
+          umma_commit(v_empty + vs);
+          umma_commit(dp_full);
         }
-        umma_commit(dp_full);
-        umma_commit(kv_empty + entry % Ly::kEntries);
+        __syncwarp();
       }
-      __syncwarp();
-      return true;
-    };
-    const auto issue_dq = [&](const Cursor& c) {
-      if (!warp_wait(ds_full, c.g & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
-      if (c.j == c.t.j0) {  // the last item's gradient has been read
-        if (n_acc > 0 && !warp_wait(acc_free, (n_acc - 1) & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
-        ++n_acc;
-      }
-      if (lane == 0) {
-        const uint32_t idesc = x_idesc<T>(ksteps * 16, 0, 1);
-        const uint32_t sk = s_base + Ly::kKV + (2 * c.g % Ly::kEntries) * Ly::kTileBytes;
-        const uint32_t ds = tmem + kXDqS + (c.g & 1) * 128;
-        tc_fence_after();
-        const int steps = 2 * x_chunks(c.t.keys, c.j);
-        for (int k = 0; k < steps; ++k)  // dS of columns 64 .. 127 lies at column 64 of the buffer
-          umma_f16_ts(tmem + kXDqAcc, ds + (k >> 2) * 64 + (k & 3) * 8, make_smem_desc(sk + k * 2048, 16384, 1024), idesc,
-                      (c.j > c.t.j0 || k > 0) ? 1u : 0u);
-        umma_commit(kv_empty + 2 * c.g % Ly::kEntries);
-        if (c.j == c.t.j1 - 1) umma_commit(acc_full);
-      }
-      __syncwarp();
-      return true;
-    };
-    const auto next = [&](const Cursor& c, bool* have) {
-      Cursor n = c;
-      ++n.j;
-      ++n.g;
-      *have = x_seek(n, p.items, make);
-      return n;
-    };
-
-    Cursor cur{};
-    cur.i = blockIdx.x;
-    bool have = cur.i < p.items;
-    if (have) {
-      cur.t = make(cur.i);
-      cur.j = cur.t.j0;
-      have = x_seek(cur, p.items, make);
+      ++n_item;
     }
-    // With one Q stage, the next item's Q and dO arrive only after this item's gradient has left: its products
-    // are issued when the last dQ product of this one has been.
-    const auto ahead = [&](const Cursor& from, const Cursor& to) { return Ly::kQStages > 1 || from.i == to.i; };
-    if (have) ok = issue_s(cur) && issue_dp(cur);
-    bool have1 = false;
-    Cursor n1 = cur;
-    if (have) n1 = next(cur, &have1);
-    bool s1 = false;  // S of the next tile has been issued
-    if (ok && have1 && ahead(cur, n1)) {
-      ok = issue_s(n1);
-      s1 = true;
-    }
-    while (have && ok) {
-      bool have2 = false, dp1 = false;
-      Cursor n2 = n1;
-      if (have1) n2 = next(n1, &have2);
-      if (s1) {
-        ok = warp_wait(dp_free, cur.g & 1, abort_flag, a.err, kErrTimeoutMma) && issue_dp(n1);
-        dp1 = true;
-      }
-      ok = ok && issue_dq(cur);
-      if (ok && have1 && !s1) ok = issue_s(n1);
-      if (ok && have1 && !dp1) ok = issue_dp(n1);  // dS of this tile was waited for: dP is free
-      s1 = false;
-      if (ok && have2 && ahead(n1, n2)) {
-        ok = issue_s(n2);
-        s1 = true;
-      }
-      cur = n1;
-      n1 = n2;
-      have = have1;
-      have1 = have2;
-    }
-    if (!ok && lane == 0) {  // the products in flight end before the tensor memory is freed
+    if (!ok && elect_one()) {  // the products in flight end before the tensor memory is freed
       volatile int never = 0;
       umma_commit(drained);
-      mbar_wait(drained, 0, &never, a.err, kErrTimeoutDrain);
+      mbar_wait(drained, 0, &never, a.err, kErrXDq + kWaitDrain);
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------ products dQ += dS K
+    const uint32_t idesc = x_idesc<T>(ksteps * 16, 0, 1);
+    uint32_t n_item = 0, g = 0;
+    bool ok = true;
+    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+      const XDqItem t = x_dq_item(p, i);
+      if (t.tiles == 0) continue;
+      for (int j = 0; j < t.tiles; ++j, ++g) {
+        const int ks = g % Ly::kKStages, buf = g & 1, steps = 2 * x_chunks(t.keys, j);
+        ok = wait(k_full + ks, g / Ly::kKStages, kWaitK) && wait(ds_full, g, kWaitP);
+        if (ok && j == 0 && n_item > 0) ok = wait(acc_free, n_item ^ 1, kWaitAccFree);  // the last item's dQ has been read
+        if (!ok) break;
+        const uint64_t sk = mn_major_desc(s_base + Ly::kK + ks * Ly::kTileBytes);
+        const uint32_t ds = tmem + kXDqS + buf * 128, later = j > 0 ? 1u : 0u;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)  // dS of columns 64 .. 127 lies at column 64 of the buffer
+            if (k < steps)
+              umma_f16_ts(tmem + kXDqAcc, ds + (k >> 2) * 64 + (k & 3) * 8, sk + k * 128, idesc, k > 0 ? 1u : later);
+          umma_commit(s_free + buf);
+          umma_commit(k_empty + ks);
+          if (j == t.tiles - 1) umma_commit(acc_full);
+        }
+        __syncwarp();
+      }
+      ++n_item;
+    }
+    if (!ok && elect_one()) {
+      volatile int never = 0;
+      umma_commit(drained + 1);
+      mbar_wait(drained + 1, 0, &never, a.err, kErrXDq + kWaitDrain);
     }
   } else {
     // ------------------------------------------------------------ dS: thread = row, 64 columns of half wh
     const int wh = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c2 = a.scale * 1.4426950408889634f;
-    const int rows = a.tile_tokens * a.pack;
-    const int hv = a.heads / a.pack;
+    const uint64_t c22 = pair2(c2, c2);
+    const int rows = a.tile_tokens * a.pack, hv = a.heads / a.pack;
+    const int my_token = row / a.pack, my_head = row % a.pack;
+    // Half wh of the channels of this row's output, and its log-sum-exp, for the item to come: asked for while the
+    // products of the item before still run.
+    uint4 o_row[HALVES * 4];
+    float lse = -INFINITY;
+    const auto fetch = [&](int64_t i) {
+      if (i >= p.items) return;
+      const XDqItem t = x_dq_item(p, i);
+      const int token = t.tile * a.tile_tokens + my_token, head = t.hv * a.pack + my_head;
+      const bool live = t.tiles > 0 && row < rows && token < a.q_len;
+      const T* o = static_cast<const T*>(a.o_in) + t.b * a.so.batch + token * a.so.token + head * a.so.head;
+#pragma unroll
+      for (int u = 0; u < HALVES * 4; ++u) {
+        const int c = wh * HALVES * 32 + 8 * u;
+        o_row[u] = live && c < a.head_dim ? *reinterpret_cast<const uint4*>(o + c) : make_uint4(0, 0, 0, 0);
+      }
+      lse = live ? a.lse[(static_cast<int64_t>(t.b) * a.heads + head) * a.q_len + token] : -INFINITY;
+    };
+    fetch(blockIdx.x);
     uint32_t n_item = 0, g = 0;
+    int stored = -1;  // Q stage whose gradient is on its way out
+    const auto release_stored = [&]() {
+      if (stored >= 0 && tid == 0) {
+        bulk_wait_group_read<0>();
+        mbar_arrive(q_empty + stored);
+      }
+      stored = -1;
+    };
     bool ok = true;
     for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDqItem t = make(i);
-      const int token = t.tile * a.tile_tokens + row / a.pack, head = t.hv * a.pack + row % a.pack;
-      const bool live = row < rows && token < a.q_len;
-      float2* stat = p.stats + (((static_cast<int64_t>(t.b) * hv + t.hv) * p.row_tiles + t.tile) * kXTile + row);
-      if (t.j0 >= t.j1) {  // no keys
-        if (wh == 0) *stat = make_float2(INFINITY, 0.0f);
-        if (wh == 0 && live) {
-          T* o = static_cast<T*>(a.dq) + t.b * a.sdq.batch + token * a.sdq.token + head * a.sdq.head;
-          for (int c = 0; c < a.head_dim; c += 8) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
+      const XDqItem t = x_dq_item(p, i);
+      const int token = t.tile * a.tile_tokens + my_token, head = t.hv * a.pack + my_head;
+      float* stat = p.stats + ((static_cast<int64_t>(t.b) * hv + t.hv) * p.row_tiles + t.tile) * (2 * kXTile) + row;
+      if (t.tiles == 0) {  // no keys
+        if (wh == 0) {
+          stat[0] = -INFINITY;
+          stat[kXTile] = 0.0f;
+          if (row < rows && token < a.q_len) {
+            T* o = static_cast<T*>(a.dq) + t.b * a.sdq.batch + token * a.sdq.token + head * a.sdq.head;
+            for (int c = 0; c < a.head_dim; c += 8) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
+          }
         }
+        fetch(i + gridDim.x);
         continue;
       }
-      float lse2 = INFINITY, delta = 0.0f;
-      if (live) {
-        const T* o = static_cast<const T*>(a.o_in) + t.b * a.so.batch + token * a.so.token + head * a.so.head;
-        const T* d = static_cast<const T*>(a.dout) + t.b * a.sdo.batch + token * a.sdo.token + head * a.sdo.head;
-        const float lse = a.lse[(static_cast<int64_t>(t.b) * a.heads + head) * a.q_len + token];
-#pragma unroll 8
-        for (int c = 0; c < a.head_dim; c += 8)
-          delta += x_dot8<T>(__ldg(reinterpret_cast<const uint4*>(o + c)), __ldg(reinterpret_cast<const uint4*>(d + c)));
-        if (lse != -INFINITY) lse2 = lse * 1.4426950408889634f;
+      const int qs = n_item % Ly::kQStages;
+      uint8_t* stage = smem + 2 * qs * Ly::kTileBytes;
+      // ---- delta = do . o, half of the channels each
+      ok = wait(q_full + qs, n_item / Ly::kQStages, kWaitQ);
+      if (!ok) break;
+      const bool dead = lse == -INFINITY;  // no such row, or no kept key
+      float neg_delta = 0.0f;
+#pragma unroll
+      for (int u = 0; u < HALVES * 4; ++u) {
+        const int c = wh * HALVES * 4 + u;  // 16-byte chunk of the row
+        neg_delta -= x_dot8<T>(o_row[u], ld_shared_v4(stage + Ly::kTileBytes + (c >> 3) * 16384 + swizzle128_offset(row, c & 7)));
       }
-      if (wh == 0) *stat = make_float2(lse2, delta);
-      for (int j = t.j0; j < t.j1; ++j, ++g) {
+      delta_half[wh * kXTile + row] = neg_delta;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(delta_full);
+      ok = wait(delta_full, n_item, kWaitDelta);
+      if (!ok) break;
+      neg_delta = dead ? 0.0f : delta_half[row] + delta_half[kXTile + row];
+      const float neg_lse = dead ? -INFINITY : -lse * 1.4426950408889634f;
+      if (wh == 0) {
+        stat[0] = neg_lse;
+        stat[kXTile] = neg_delta;
+      }
+      const uint64_t nl2 = pair2(neg_lse, neg_lse), nd2 = pair2(neg_delta, neg_delta);
+      for (int j = 0; j < t.tiles; ++j, ++g) {
         const int chunks = x_chunks(t.keys, j);
-        const uint32_t t_s = t_lane + kXDqS + (g & 1) * 128 + wh * 64;
-        ok = warp_wait(s_full + (g & 1), (g >> 1) & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+        const uint32_t t_s = t_lane + kXDqS + (g & 1) * 128 + wh * 64, t_dp = t_lane + kXDqDP + wh * 64;
+        const bool two = 2 * wh + 1 < chunks, one = 2 * wh < chunks;  // this half's chunks with keys
+        ok = wait(s_full + (g & 1), g >> 1, kWaitS);
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[2][32], dp[2][32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          if (2 * wh + c < chunks) tmem_ld_32x32b_x32(t_s + c * 32, s[c]);
+        uint32_t s[2][32];
+        if (one) tmem_ld_32x32b_x32(t_s, s[0]);
+        if (two) tmem_ld_32x32b_x32(t_s + 32, s[1]);
         tmem_ld_wait();
         after_wait(s[0]);
         after_wait(s[1]);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int k = 0; k < 32; ++k) s[c][k] = __float_as_uint(ex2(fmaf(__uint_as_float(s[c][k]), c2, -lse2)));
+          for (int k = 0; k < 32; k += 2) {
+            float x0, x1;
+            unpair2(fma2(pair2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), c22, nl2), x0, x1);
+            exp2_pair<T, kXExpEvery>(x0, x1, k >> 1);
+            s[c][k] = __float_as_uint(x0);
+            s[c][k + 1] = __float_as_uint(x1);
+          }
         if (masked || (j + 1) * kXTile > t.keys) {
           const uint4 w4 = words[g % kXMaskSlots];
           const uint32_t w[2] = {wh ? w4.z : w4.x, wh ? w4.w : w4.y};
@@ -399,38 +405,46 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 32; ++k) s[c][k] = (w[c] >> k) & 1u ? s[c][k] : 0u;
         }
-        ok = warp_wait(dp_full, g & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+        ok = wait(dp_full, g, kWaitDP);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          if (2 * wh + c < chunks) tmem_ld_32x32b_x32(t_lane + kXDqDP + wh * 64 + c * 32, dp[c]);
-        tmem_ld_wait();
-        after_wait(dp[0]);
-        after_wait(dp[1]);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dp_free);
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          if (2 * wh + c < chunks) {
+        for (int c = 0; c < 2; ++c) {
+          uint32_t dp[32];
+          if (c == 0 ? one : two) {
+            tmem_ld_32x32b_x32(t_dp + c * 32, dp);
+            tmem_ld_wait();
+            after_wait(dp);
+          }
+          if (c == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(dp_free);
+          }
+          if (c == 0 ? one : two) {
             uint32_t pk[16];
 #pragma unroll
-            for (int k = 0; k < 32; k += 2)
-              pk[k >> 1] = XType<T>::pack2(__uint_as_float(s[c][k]) * (__uint_as_float(dp[c][k]) - delta),
-                                           __uint_as_float(s[c][k + 1]) * (__uint_as_float(dp[c][k + 1]) - delta));
+            for (int k = 0; k < 32; k += 2) {
+              const uint64_t d = add2(pair2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), nd2);
+              float x0, x1;
+              unpair2(mul2(pair2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), d), x0, x1);
+              pk[k >> 1] = XType<T>::pack2(x0, x1);
+            }
             tmem_st_32x32b_x16(t_s + c * 16, pk);
           }
+        }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_full);
       }
-      if (ok) ok = warp_wait(acc_full, n_item & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+      if (!ok) break;
+      fetch(i + gridDim.x);
+      release_stored();
+      ok = wait(acc_full, n_item, kWaitAcc);
       if (!ok) break;
       tc_fence_after();
-      const int qs = n_item % Ly::kQStages;
-      uint8_t* stage = smem + 2 * qs * Ly::kTileBytes;  // Q's tile, read by every product of the item by now
+      // dQ goes out from Q's tile, which every product of the item has read by now
 #pragma unroll
       for (int c = 0; c < HALVES; ++c) {  // this half's share of the channels: [wh * HALVES * 32, + HALVES * 32)
         const int col = (wh * HALVES + c) * 32;
@@ -441,7 +455,7 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
         uint32_t pk[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2)
-          pk[k >> 1] = lse2 == INFINITY ? 0u : XType<T>::pack2(__uint_as_float(o[k]) * a.scale, __uint_as_float(o[k + 1]) * a.scale);
+          pk[k >> 1] = dead ? 0u : XType<T>::pack2(__uint_as_float(o[k]) * a.scale, __uint_as_float(o[k + 1]) * a.scale);
         uint8_t* half = stage + (col >> 6) * 16384;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
@@ -456,16 +470,16 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
         mbar_arrive(staged);
       }
       if (tid == 0) {
-        ok = mbar_wait(staged, n_item & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+        ok = mbar_wait(staged, n_item & 1, abort_flag, a.err, kErrXDq + kWaitStaged);
         if (ok) {
           for (int hf = 0; hf < HALVES; ++hf)
             tma_store_4d(&dq_map, stage + hf * 16384, hf * 64, t.hv * a.pack, t.tile * a.tile_tokens, t.b);
           bulk_commit_group();
-          bulk_wait_group_read<0>();
-          mbar_arrive(q_empty + qs);
         }
       }
       ok = __all_sync(0xffffffffu, ok);
+      if (ok) stored = qs;
+      if (Ly::kQStages == 1) release_stored();
       ++n_item;
     }
     if (tid == 0) bulk_wait_group<0>();
@@ -485,13 +499,13 @@ struct XDkvLayout {
   static constexpr int kKVStages = HALVES == 1 ? 2 : 1;  // K and V of an item
   static constexpr int kEntries = HALVES == 1 ? 8 : 4;   // Q and dO tiles in turn
   static constexpr int kQ = 2 * kKVStages * kTileBytes;
-  static constexpr int kStats = kQ + kEntries * kTileBytes;  // float2 [kEntries / 2][128]
+  static constexpr int kStats = kQ + kEntries * kTileBytes;  // fp32 [kEntries / 2][2][128]
   static constexpr int kWords = kStats + kEntries / 2 * 1024;
   static constexpr int kBar = kWords + 2 * kKVStages * 16;
-  static constexpr int kNumBars = 2 * kKVStages + 2 * kEntries + 8;
+  static constexpr int kNumBars = 2 * kKVStages + 2 * kEntries + 11;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;
-  static constexpr int kThreads = 320;
+  static constexpr int kThreads = 352;
 };
 static_assert(XDkvLayout<1>::kSmemBytes <= 232448 && XDkvLayout<2>::kSmemBytes <= 232448, "dkv smem");
 // tensor memory columns: S^T, dP^T (P^T and dS^T over it), dV, dK
@@ -523,7 +537,7 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
   using Ly = XDkvLayout<HALVES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float2* stats = reinterpret_cast<float2*>(smem + Ly::kStats);
+  float* stats = reinterpret_cast<float*>(smem + Ly::kStats);
   uint4* words = reinterpret_cast<uint4*>(smem + Ly::kWords);
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + Ly::kBar);
   uint64_t* kv_empty = kv_full + Ly::kKVStages;
@@ -532,16 +546,17 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
   uint64_t* s_full = q_empty + Ly::kEntries;
   uint64_t* s_free = s_full + 1;
   uint64_t* dp_full = s_free + 1;
-  uint64_t* ds_full = dp_full + 1;
+  uint64_t* dp_free = dp_full + 1;  // P^T and dS^T have been multiplied
+  uint64_t* ds_full = dp_free + 1;
   uint64_t* acc_full = ds_full + 1;
   uint64_t* acc_free = acc_full + 1;
-  uint64_t* staged = acc_free + 1;
-  uint64_t* drained = staged + 1;
+  uint64_t* staged = acc_free + 1;   // [2], by half of the softmax threads
+  uint64_t* drained = staged + 2;    // [2], by issuing warp
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::kTail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const XAttnParams& a = p.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
   const int rows = a.tile_tokens * a.pack;
   if (tid == 0) {
     for (int i = 0; i < Ly::kKVStages; ++i) {
@@ -552,14 +567,17 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 1);
     }
-    mbar_init(s_full, 2);
+    mbar_init(s_full, 2);  // the products' commit, and the issuing thread (keep bits)
     mbar_init(s_free, 8);
     mbar_init(dp_full, 1);
+    mbar_init(dp_free, 1);
     mbar_init(ds_full, 8);
     mbar_init(acc_full, 1);
     mbar_init(acc_free, 8);
-    mbar_init(staged, 8);
-    mbar_init(drained, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(staged + i, 4);
+      mbar_init(drained + i, 1);
+    }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -580,21 +598,24 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
   pdl_wait();
 
   const int ksteps = (a.head_dim + 15) >> 4;
-  const auto make = [&](int64_t i) { return x_dkv_item(p, i); };
+  const uint32_t s_base = smem_u32(smem);
+  const auto wait = [&](uint64_t* bar, uint32_t phase, int what) {
+    return warp_wait(bar, phase & 1, abort_flag, a.err, kErrXDkv + what);
+  };
 
   if (warp == 8) {
     // ------------------------------------------------------------ loads
     const uint32_t q_bytes = static_cast<uint32_t>(rows) * 128u * HALVES;
     const int per_key_head = a.group / a.pack;  // head groups that read a key head (1 where all are packed)
     const int hv = a.heads / a.pack;
-    uint32_t e = 0, loaded = 0, n_item = 0;
+    uint32_t e = 0, n_item = 0;  // copies started
     bool ok = true;
     for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDkvItem t = make(i);
+      const XDkvItem t = x_dkv_item(p, i);
       if (t.j0 >= t.j1) continue;
       const int ks = n_item % Ly::kKVStages;
       const uint4 w = x_keep_words(a, t.b, t.tile * kXTile, t.keys, lane);
-      ok = warp_wait(kv_empty + ks, ((n_item / Ly::kKVStages) & 1) ^ 1, abort_flag, a.err, kErrTimeoutProducer);
+      ok = wait(kv_empty + ks, (n_item / Ly::kKVStages) ^ 1, kWaitKFree);
       if (!ok) break;
       if (lane == 0) {
         words[n_item % (2 * Ly::kKVStages)] = w;
@@ -609,151 +630,139 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       for (int j = t.j0; j < t.j1 && ok; ++j) {
         const int h = t.hk * per_key_head + j / p.row_tiles, tile = j % p.row_tiles;
 #pragma unroll
-        for (int which = 0; which < 2 && ok; ++which, ++e) {
+        for (int which = 0; which < 2; ++which) {
           const int slot = e % Ly::kEntries;
-          ok = warp_wait(q_empty + slot, ((e / Ly::kEntries) & 1) ^ 1, abort_flag, a.err, kErrTimeoutProducer);
+          ok = wait(q_empty + slot, (e / Ly::kEntries) ^ 1, kWaitQFree);
           if (!ok) break;
-          loaded = e + 1;
           if (lane == 0) {
             mbar_arrive_expect_tx(q_full + slot, q_bytes + (which == 0 ? 1024u : 0u));
             for (int hf = 0; hf < HALVES; ++hf)
               tma_load_4d(smem + Ly::kQ + slot * Ly::kTileBytes + hf * 16384, which ? &do_map : &q_map, q_full + slot,
                           hf * 64, h * a.pack, tile * a.tile_tokens, t.b);
             if (which == 0)
-              bulk_load_1d(stats + (slot >> 1) * kXTile,
-                           p.stats + ((static_cast<int64_t>(t.b) * hv + h) * p.row_tiles + tile) * kXTile, 1024,
+              bulk_load_1d(stats + (slot >> 1) * 2 * kXTile,
+                           p.stats + ((static_cast<int64_t>(t.b) * hv + h) * p.row_tiles + tile) * (2 * kXTile), 1024,
                            q_full + slot);
           }
+          ++e;
         }
       }
     }
     if (!ok && lane == 0) {  // copies still in flight land before the CTA leaves
       volatile int never = 0;
-      for (uint32_t k = loaded > Ly::kEntries ? loaded - Ly::kEntries : 0; k < loaded; ++k)
-        mbar_wait(q_full + k % Ly::kEntries, (k / Ly::kEntries) & 1, &never, a.err, kErrTimeoutDrain);
-      for (uint32_t k = n_item > Ly::kKVStages ? n_item - Ly::kKVStages : 0; k < n_item; ++k)
-        mbar_wait(kv_full + k % Ly::kKVStages, (k / Ly::kKVStages) & 1, &never, a.err, kErrTimeoutDrain);
+      const auto drain = [&](uint64_t* full, uint32_t stages, uint32_t n) {
+        for (uint32_t k = n > stages ? n - stages : 0; k < n; ++k)
+          mbar_wait(full + k % stages, (k / stages) & 1, &never, a.err, kErrXDkv + kWaitDrain);
+      };
+      drain(q_full, Ly::kEntries, e);
+      drain(kv_full, Ly::kKVStages, n_item);
     }
   } else if (warp == 9) {
-    // ------------------------------------------------------------ products
-    using Cursor = XCursor<XDkvItem>;
-    const uint32_t s_base = smem_u32(smem);
-    const uint32_t idesc_s = x_idesc<T>(kXTile, 0, 0), idesc_acc = x_idesc<T>(ksteps * 16, 0, 1);
+    // ------------------------------------------------------------ products S^T = K Q^T, dP^T = V dO^T
+    const uint32_t idesc = x_idesc<T>(kXTile, 0, 0);
+    uint32_t n_item = 0, g = 0;
     bool ok = true;
-    uint32_t n_acc = 0;
-    const auto wait_entry = [&](uint32_t entry) {
-      return warp_wait(q_full + entry % Ly::kEntries, (entry / Ly::kEntries) & 1, abort_flag, a.err, kErrTimeoutMma);
-    };
-    // D[128 keys][128 rows] = (K or V) (Q or dO)^T
-    const auto product_t = [&](uint32_t d, uint32_t sa, uint32_t sb) {
-      for (int k = 0; k < ksteps; ++k) {
-        const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-        umma_f16_ss(tmem + d, make_smem_desc(sa + off, 16, 1024), make_smem_desc(sb + off, 16, 1024), idesc_s,
-                    k > 0 ? 1u : 0u);
+    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+      const XDkvItem t = x_dkv_item(p, i);
+      if (t.j0 >= t.j1) continue;
+      const int ks = n_item % Ly::kKVStages;
+      ok = wait(kv_full + ks, n_item / Ly::kKVStages, kWaitK);
+      if (!ok) break;
+      const uint4 w = words[n_item % (2 * Ly::kKVStages)];
+      if ((w.x & w.y & w.z & w.w) != 0xffffffffu) {
+        x_zero_rows<HALVES>(smem + 2 * ks * Ly::kTileBytes, w, lane);
+        x_zero_rows<HALVES>(smem + (2 * ks + 1) * Ly::kTileBytes, w, lane);
       }
-    };
-    const auto issue_s = [&](const Cursor& c) {
-      const int ks = c.n_item % Ly::kKVStages;
-      if (c.j == c.t.j0) {
-        if (!warp_wait(kv_full + ks, (c.n_item / Ly::kKVStages) & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
-        const uint4 w = words[c.n_item % (2 * Ly::kKVStages)];
-        if ((w.x & w.y & w.z & w.w) != 0xffffffffu) {
-          x_zero_rows<HALVES>(smem + 2 * ks * Ly::kTileBytes, w, lane);
-          x_zero_rows<HALVES>(smem + (2 * ks + 1) * Ly::kTileBytes, w, lane);
+      const uint64_t sk = k_major_desc(s_base + 2 * ks * Ly::kTileBytes);
+      const uint64_t sv = k_major_desc(s_base + (2 * ks + 1) * Ly::kTileBytes);
+      for (int j = t.j0; j < t.j1; ++j, ++g) {
+        const uint32_t eq = 2 * g % Ly::kEntries, phase = 2 * g / Ly::kEntries;
+        ok = wait(q_full + eq, phase, kWaitQ);
+        if (ok && g >= 1) ok = wait(s_free, g ^ 1, kWaitSFree);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          products_k_major(tmem + kXDkvS, sk, k_major_desc(s_base + Ly::kQ + eq * Ly::kTileBytes), idesc, ksteps);
+          umma_commit(s_full);
+          mbar_arrive(s_full);
         }
-      }
-      if (!wait_entry(2 * c.g)) return false;
-      if (lane == 0) {
+        __syncwarp();
+        ok = wait(q_full + eq + 1, phase, kWaitV);
+        if (ok && g >= 1) ok = wait(dp_free, g ^ 1, kWaitDPFree);
+        if (!ok) break;
         tc_fence_after();
-        product_t(kXDkvS, s_base + 2 * ks * Ly::kTileBytes, s_base + Ly::kQ + (2 * c.g % Ly::kEntries) * Ly::kTileBytes);
-        umma_commit(s_full);
-        mbar_arrive(s_full);
+        if (elect_one()) {
+          products_k_major(tmem + kXDkvDP, sv, k_major_desc(s_base + Ly::kQ + (eq + 1) * Ly::kTileBytes), idesc, ksteps);
+          umma_commit(dp_full);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      return true;
-    };
-    const auto issue_dp = [&](const Cursor& c) {
-      if (!wait_entry(2 * c.g + 1)) return false;
-      if (lane == 0) {
-        tc_fence_after();
-        product_t(kXDkvDP, s_base + (2 * (c.n_item % Ly::kKVStages) + 1) * Ly::kTileBytes,
-                  s_base + Ly::kQ + ((2 * c.g + 1) % Ly::kEntries) * Ly::kTileBytes);
-        umma_commit(dp_full);
-      }
-      __syncwarp();
-      return true;
-    };
-    const auto issue_acc = [&](const Cursor& c) {
-      if (!warp_wait(ds_full, c.g & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
-      if (c.j == c.t.j0) {  // the last item's gradients have been read
-        if (n_acc > 0 && !warp_wait(acc_free, (n_acc - 1) & 1, abort_flag, a.err, kErrTimeoutMma)) return false;
-        ++n_acc;
-      }
-      if (lane == 0) {
-        const uint32_t sq = s_base + Ly::kQ + (2 * c.g % Ly::kEntries) * Ly::kTileBytes;
-        const uint32_t sdo = s_base + Ly::kQ + ((2 * c.g + 1) % Ly::kEntries) * Ly::kTileBytes;
-        const uint32_t acc = c.j > c.t.j0 ? 1u : 0u;
-        tc_fence_after();
-        // rows 64 h .. 64 h + 63: P^T at column 64 h of the dP region, dS^T at 64 h + 32
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_f16_ts(tmem + kXDkvV, tmem + kXDkvDP + (k >> 2) * 64 + (k & 3) * 8, make_smem_desc(sdo + k * 2048, 16384, 1024),
-                      idesc_acc, acc | (k > 0 ? 1u : 0u));
-        umma_commit(q_empty + (2 * c.g + 1) % Ly::kEntries);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_f16_ts(tmem + kXDkvV + HALVES * 64, tmem + kXDkvDP + 32 + (k >> 2) * 64 + (k & 3) * 8,
-                      make_smem_desc(sq + k * 2048, 16384, 1024), idesc_acc, acc | (k > 0 ? 1u : 0u));
-        umma_commit(q_empty + 2 * c.g % Ly::kEntries);
-        if (c.j == c.t.j1 - 1) umma_commit(acc_full);
-      }
-      __syncwarp();
-      return true;
-    };
-
-    Cursor cur{};
-    cur.i = blockIdx.x;
-    bool have = cur.i < p.items;
-    if (have) {
-      cur.t = make(cur.i);
-      cur.j = cur.t.j0;
-      have = x_seek(cur, p.items, make);
+      ++n_item;
     }
-    if (have) ok = issue_s(cur);
-    while (have && ok) {
-      ok = issue_dp(cur);
-      Cursor nxt = cur;
-      ++nxt.j;
-      ++nxt.g;
-      const bool more = x_seek(nxt, p.items, make);
-      // with one K / V stage the next item's tiles arrive only after this item's gradients have left
-      const bool apart = Ly::kKVStages == 1 && more && nxt.j == nxt.t.j0;
-      const auto next_s = [&]() {
-        return warp_wait(s_free, cur.g & 1, abort_flag, a.err, kErrTimeoutMma) && issue_s(nxt);
-      };
-      if (ok && more && !apart) ok = next_s();
-      ok = ok && issue_acc(cur);
-      if (ok && more && apart) ok = next_s();
-      cur = nxt;
-      have = more;
-    }
-    if (!ok && lane == 0) {  // the products in flight end before the tensor memory is freed
+    if (!ok && elect_one()) {  // the products in flight end before the tensor memory is freed
       volatile int never = 0;
       umma_commit(drained);
-      mbar_wait(drained, 0, &never, a.err, kErrTimeoutDrain);
+      mbar_wait(drained, 0, &never, a.err, kErrXDkv + kWaitDrain);
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------ products dV += P^T dO, dK += dS^T Q
+    const uint32_t idesc = x_idesc<T>(ksteps * 16, 0, 1);
+    uint32_t n_item = 0, g = 0;
+    bool ok = true;
+    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+      const XDkvItem t = x_dkv_item(p, i);
+      if (t.j0 >= t.j1) continue;
+      for (int j = t.j0; j < t.j1; ++j, ++g) {
+        const uint32_t eq = 2 * g % Ly::kEntries, phase = 2 * g / Ly::kEntries;
+        ok = wait(q_full + eq, phase, kWaitQ) && wait(q_full + eq + 1, phase, kWaitV) && wait(ds_full, g, kWaitP);
+        if (ok && j == t.j0 && n_item > 0) ok = wait(acc_free, n_item ^ 1, kWaitAccFree);  // the last item's sums have been read
+        if (!ok) break;
+        const uint64_t sq = mn_major_desc(s_base + Ly::kQ + eq * Ly::kTileBytes);
+        const uint64_t sdo = mn_major_desc(s_base + Ly::kQ + (eq + 1) * Ly::kTileBytes);
+        const uint32_t later = j > t.j0 ? 1u : 0u;
+        tc_fence_after();
+        if (elect_one()) {
+          // 32 rows' P^T and dS^T lie side by side, 16 columns each
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            umma_f16_ts(tmem + kXDkvV, tmem + kXDkvDP + (k >> 1) * 32 + (k & 1) * 8, sdo + k * 128, idesc, k > 0 ? 1u : later);
+          umma_commit(q_empty + eq + 1);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            umma_f16_ts(tmem + kXDkvV + HALVES * 64, tmem + kXDkvDP + 16 + (k >> 1) * 32 + (k & 1) * 8, sq + k * 128, idesc,
+                        k > 0 ? 1u : later);
+          umma_commit(q_empty + eq);
+          umma_commit(dp_free);
+          if (j == t.j1 - 1) umma_commit(acc_full);
+        }
+        __syncwarp();
+      }
+      ++n_item;
+    }
+    if (!ok && elect_one()) {
+      volatile int never = 0;
+      umma_commit(drained + 1);
+      mbar_wait(drained + 1, 0, &never, a.err, kErrXDkv + kWaitDrain);
     }
   } else {
     // ------------------------------------------------------------ P^T, dS^T: thread = key, 64 rows of half wh
     const int wh = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c2 = a.scale * 1.4426950408889634f;
+    const uint64_t c22 = pair2(c2, c2);
     uint32_t n_item = 0, g = 0;
+    int stored = -1;  // K / V stage whose gradient is on its way out
+    const auto release_stored = [&]() {
+      if (stored >= 0 && quad == 0 && lane == 0) {
+        bulk_wait_group_read<0>();
+        mbar_arrive(kv_empty + stored);
+      }
+      stored = -1;
+    };
     bool ok = true;
     for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDkvItem t = make(i);
+      const XDkvItem t = x_dkv_item(p, i);
       const int j_key = t.tile * kXTile + key;
-      T* const grad = wh == 0 ? static_cast<T*>(a.dv) + t.b * a.sdv.batch + static_cast<int64_t>(j_key) * a.sdv.token + t.hk * a.sdv.head
-                              : static_cast<T*>(a.dk) + t.b * a.sdk.batch + static_cast<int64_t>(j_key) * a.sdk.token + t.hk * a.sdk.head;
       const auto part = [&](int c) {  // this row of the split's partial sums
         return p.part + ((((static_cast<int64_t>(t.split) * 2 + wh) * a.batch + t.b) * a.k_len + j_key) * a.kv_heads + t.hk) *
                             a.head_dim + c;
@@ -763,6 +772,8 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
           if (p.splits > 1) {
             for (int c = 0; c < a.head_dim; c += 4) *reinterpret_cast<float4*>(part(c)) = make_float4(0, 0, 0, 0);
           } else {
+            T* grad = wh == 0 ? static_cast<T*>(a.dv) + t.b * a.sdv.batch + j_key * a.sdv.token + t.hk * a.sdv.head
+                              : static_cast<T*>(a.dk) + t.b * a.sdk.batch + j_key * a.sdk.token + t.hk * a.sdk.head;
             for (int c = 0; c < a.head_dim; c += 8) *reinterpret_cast<uint4*>(grad + c) = make_uint4(0, 0, 0, 0);
           }
         }
@@ -770,67 +781,81 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       }
       bool kept = false;
       for (int j = t.j0; j < t.j1; ++j, ++g) {
-        ok = warp_wait(s_full, g & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+        ok = wait(s_full, g, kWaitS);
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[2][32], dp[2][32];
+        uint32_t s[2][32];
         tmem_ld_32x32b_x32(t_lane + kXDkvS + wh * 64, s[0]);
         tmem_ld_32x32b_x32(t_lane + kXDkvS + wh * 64 + 32, s[1]);
+        const float4* neg_lse = reinterpret_cast<const float4*>(stats + g % (Ly::kEntries / 2) * 2 * kXTile + wh * 64);
+        const float4* neg_delta = neg_lse + kXTile / 4;
+        if (j == t.j0) {
+          const uint4 w = words[n_item % (2 * Ly::kKVStages)];
+          kept = ((quad == 0 ? w.x : quad == 1 ? w.y : quad == 2 ? w.z : w.w) >> lane) & 1u;
+        }
         tmem_ld_wait();
         after_wait(s[0]);
         after_wait(s[1]);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);
-        if (j == t.j0) {
-          const uint4 w = words[n_item % (2 * Ly::kKVStages)];
-          kept = ((quad == 0 ? w.x : quad == 1 ? w.y : quad == 2 ? w.z : w.w) >> lane) & 1u;
-        }
-        const float4* st = reinterpret_cast<const float4*>(stats + (g % (Ly::kEntries / 2)) * kXTile + wh * 64);
         uint32_t pk[2][16];
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float4 r = st[c * 16 + (k >> 1)];  // (lse, delta) of two rows
-            const float p0 = ex2(fmaf(__uint_as_float(s[c][k]), c2, -r.x));
-            const float p1 = ex2(fmaf(__uint_as_float(s[c][k + 1]), c2, -r.z));
-            s[c][k] = __float_as_uint(p0);
-            s[c][k + 1] = __float_as_uint(p1);
-            pk[c][k >> 1] = XType<T>::pack2(p0, p1);
+          for (int k = 0; k < 32; k += 4) {
+            const float4 nl = neg_lse[c * 8 + (k >> 2)];
+            float x0, x1, x2, x3;
+            unpair2(fma2(pair2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), c22, pair2(nl.x, nl.y)), x0, x1);
+            unpair2(fma2(pair2(__uint_as_float(s[c][k + 2]), __uint_as_float(s[c][k + 3])), c22, pair2(nl.z, nl.w)), x2, x3);
+            exp2_pair<T, kXExpEvery>(x0, x1, k >> 1);
+            exp2_pair<T, kXExpEvery>(x2, x3, (k >> 1) + 1);
+            s[c][k] = __float_as_uint(x0);
+            s[c][k + 1] = __float_as_uint(x1);
+            s[c][k + 2] = __float_as_uint(x2);
+            s[c][k + 3] = __float_as_uint(x3);
+            pk[c][k >> 1] = XType<T>::pack2(x0, x1);
+            pk[c][(k >> 1) + 1] = XType<T>::pack2(x2, x3);
           }
-        ok = warp_wait(dp_full, g & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+        ok = wait(dp_full, g, kWaitDP);
         if (!ok) break;
         tc_fence_after();
         const uint32_t t_dp = t_lane + kXDkvDP + wh * 64;
-        tmem_ld_32x32b_x32(t_dp, dp[0]);
-        tmem_ld_32x32b_x32(t_dp + 32, dp[1]);
-        tmem_ld_wait();
-        after_wait(dp[0]);
-        after_wait(dp[1]);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          tmem_st_32x32b_x16(t_dp + c * 16, pk[c]);
+          uint32_t dp[32];
+          tmem_ld_32x32b_x32(t_dp + c * 32, dp);
+          tmem_ld_wait();
+          after_wait(dp);
+          tmem_st_32x32b_x16(t_dp + c * 32, pk[c]);
+          uint32_t ds[16];
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float4 r = st[c * 16 + (k >> 1)];
-            pk[c][k >> 1] = XType<T>::pack2(__uint_as_float(s[c][k]) * (__uint_as_float(dp[c][k]) - r.y),
-                                            __uint_as_float(s[c][k + 1]) * (__uint_as_float(dp[c][k + 1]) - r.w));
+          for (int k = 0; k < 32; k += 4) {
+            const float4 nd = neg_delta[c * 8 + (k >> 2)];
+            float x0, x1, x2, x3;
+            unpair2(mul2(pair2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])),
+                         add2(pair2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), pair2(nd.x, nd.y))), x0, x1);
+            unpair2(mul2(pair2(__uint_as_float(s[c][k + 2]), __uint_as_float(s[c][k + 3])),
+                         add2(pair2(__uint_as_float(dp[k + 2]), __uint_as_float(dp[k + 3])), pair2(nd.z, nd.w))), x2, x3);
+            ds[k >> 1] = XType<T>::pack2(x0, x1);
+            ds[(k >> 1) + 1] = XType<T>::pack2(x2, x3);
           }
-          tmem_st_32x32b_x16(t_dp + 32 + c * 16, pk[c]);
+          tmem_st_32x32b_x16(t_dp + c * 32 + 16, ds);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_full);
       }
-      if (ok) ok = warp_wait(acc_full, n_item & 1, abort_flag, a.err, kErrTimeoutEpilogue);
+      if (!ok) break;
+      release_stored();
+      ok = wait(acc_full, n_item, kWaitAcc);
       if (!ok) break;
       tc_fence_after();
       const int ks = n_item % Ly::kKVStages;
       // dV goes out by the first half of the threads from V's tile, dK by the second from K's
       uint8_t* stage = smem + (2 * ks + 1 - wh) * Ly::kTileBytes;
-      const float f = !kept ? 0.0f : wh == 0 ? 1.0f : a.scale;
+      const float f = wh == 0 ? 1.0f : a.scale;
 #pragma unroll
       for (int c = 0; c < 2 * HALVES; ++c) {
         uint32_t o[32];
@@ -840,11 +865,12 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 32; ++k) o[k] = kept ? __float_as_uint(__uint_as_float(o[k]) * f) : 0u;
         if (p.splits > 1) {
-          if (j_key < a.k_len)
+          if (j_key < a.k_len) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4)
               if (c * 32 + k < a.head_dim)
                 *reinterpret_cast<uint4*>(part(c * 32 + k)) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          }
         } else {
           uint32_t pk[16];
 #pragma unroll
@@ -861,21 +887,19 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(acc_free);
-        mbar_arrive(staged);
+        mbar_arrive(staged + wh);
       }
       if (quad == 0 && lane == 0) {
-        ok = mbar_wait(staged, n_item & 1, abort_flag, a.err, kErrTimeoutEpilogue);
-        if (ok) {
-          if (p.splits == 1) {
-            for (int hf = 0; hf < HALVES; ++hf)
-              tma_store_4d(wh == 0 ? &dv_map : &dk_map, stage + hf * 16384, hf * 64, t.hk, t.tile * kXTile, t.b);
-            bulk_commit_group();
-            bulk_wait_group_read<0>();
-          }
-          mbar_arrive(kv_empty + ks);
+        ok = mbar_wait(staged + wh, n_item & 1, abort_flag, a.err, kErrXDkv + kWaitStaged);
+        if (ok && p.splits == 1) {
+          for (int hf = 0; hf < HALVES; ++hf)
+            tma_store_4d(wh == 0 ? &dv_map : &dk_map, stage + hf * 16384, hf * 64, t.hk, t.tile * kXTile, t.b);
+          bulk_commit_group();
         }
       }
       ok = __all_sync(0xffffffffu, ok);
+      if (ok) stored = ks;
+      if (Ly::kKVStages == 1) release_stored();
       ++n_item;
     }
     if (quad == 0 && lane == 0) bulk_wait_group<0>();
