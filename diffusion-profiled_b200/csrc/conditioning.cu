@@ -188,7 +188,7 @@ int x_fwd_launch(const XFwdParams& f, const CUtensorMap (&maps)[4], int64_t slot
   using Ly = XFwdLayout<HALVES, NT>;
   FP8_CUDA_TRY(cudaFuncSetAttribute(x_fwd_kernel<T, HALVES, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     Ly::kSmemBytes));
-  FP8_CUDA_TRY(launch_kernel(x_fwd_kernel<T, HALVES, NT>, dim3(static_cast<unsigned>(std::min(f.items, slots))),
+  FP8_CUDA_TRY(launch_kernel(x_fwd_kernel<T, HALVES, NT>, dim3(static_cast<unsigned>(std::min<int64_t>(f.items, slots))),
                              dim3(Ly::kThreads), Ly::kSmemBytes, stream, 1, kTensorKernel, f, maps[0], maps[1], maps[2],
                              maps[3]));
   count_launches(1);
@@ -201,12 +201,13 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
   XFwdParams f{};
   f.a = a;
   f.row_tiles = w.row_tiles;
+  f.hv = w.hv;
   f.key_chunk = w.key_chunk;
   f.splits = w.splits;
   f.part_o = static_cast<float*>(workspace);
   f.part_lse = f.part_o == nullptr ? nullptr : f.part_o + static_cast<int64_t>(w.splits) * w.rows * a.head_dim;
   f.rows = w.rows;
-  f.items = w.items;
+  f.items = static_cast<uint32_t>(w.items);
   if (int s = bind_context()) return s;
   CUtensorMap maps[4];
   const int dt = args->dtype;
@@ -275,10 +276,11 @@ int x_bwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XBwd
   XBwdParams p{};
   p.a = a;
   p.row_tiles = w.row_tiles;
+  p.hv = a.heads / a.pack;
   p.stats = static_cast<float*>(workspace);
-  p.items = w.dq_items;
+  p.items = static_cast<uint32_t>(w.dq_items);
   XBwdParams kv = p;
-  kv.items = w.dkv_items;
+  kv.items = static_cast<uint32_t>(w.dkv_items);
   kv.q_tiles = w.q_tiles;
   kv.q_chunk = w.q_chunk;
   kv.splits = w.splits;
@@ -333,6 +335,7 @@ int fp8_cross_attention_fwd(const fp8_cross_attention_args* a, void* workspace, 
   DeviceState* st = nullptr;
   if (int s = device_state(&st)) return s;
   const XPlan w = x_plan(a, st->sm_count);
+  FP8_REQUIRE(w.items < (1ll << 31), FP8_ERR_UNSUPPORTED, "cross attention: too many row tiles (%lld)", (long long)w.items);
   const size_t need = x_fwd_workspace(a, w);
   FP8_REQUIRE(need == 0 || (workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= need),
               FP8_ERR_WORKSPACE, "cross attention: workspace too small or not 16-byte aligned (%zu bytes, needs %zu)",
@@ -348,6 +351,8 @@ int fp8_cross_attention_bwd(const fp8_cross_attention_args* a, void* workspace, 
   DeviceState* st = nullptr;
   if (int s = device_state(&st)) return s;
   const XBwdPlan w = x_bwd_plan(a, st->sm_count);
+  FP8_REQUIRE(w.dq_items < (1ll << 31) && w.dkv_items < (1ll << 31), FP8_ERR_UNSUPPORTED,
+              "cross attention backward: too many tiles (%lld, %lld)", (long long)w.dq_items, (long long)w.dkv_items);
   const size_t need = w.stats_bytes + w.part_bytes;
   FP8_REQUIRE(workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= need, FP8_ERR_WORKSPACE,
               "cross attention backward: workspace too small or not 16-byte aligned (%zu bytes, needs %zu)",

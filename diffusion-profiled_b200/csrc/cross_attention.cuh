@@ -38,8 +38,6 @@
 
 #include <cuda_fp16.h>
 
-#include <type_traits>
-
 #include "dropout.cuh"
 #include "sm100_common.cuh"
 
@@ -51,7 +49,7 @@ constexpr int kXTile = 128;  // rows of a query tile and keys of a key tile
 enum XError : int { kErrXForward = 300, kErrXDq = 320, kErrXDkv = 340 };
 enum XWait : int {
   kWaitQFree = 1, kWaitKFree, kWaitVFree, kWaitQ, kWaitK, kWaitV, kWaitS, kWaitSFree, kWaitDP, kWaitDPFree, kWaitP,
-  kWaitPRest, kWaitAcc, kWaitAccFree, kWaitStaged, kWaitDelta, kWaitDrain
+  kWaitPRest, kWaitTurn, kWaitAcc, kWaitAccFree, kWaitStaged, kWaitDelta, kWaitDrain
 };
 
 struct XStrides {
@@ -74,9 +72,11 @@ struct XAttnParams {
   int* err;
 };
 
-__device__ __forceinline__ int x_key_count(const XAttnParams& p, int b) {
-  return p.key_lengths == nullptr ? p.k_len : max(0, min(p.k_len, p.key_lengths[b]));
+// A sequence's key count as given, and clamped.  (Apart, so that the load can be under way before it is needed.)
+__device__ __forceinline__ int x_raw_count(const XAttnParams& p, int b) {
+  return p.key_lengths == nullptr ? p.k_len : __ldg(p.key_lengths + b);
 }
+__device__ __forceinline__ int x_key_count(const XAttnParams& p, int raw) { return max(0, min(p.k_len, raw)); }
 __device__ __forceinline__ bool x_key_kept(const XAttnParams& p, int b, int j) {
   return p.key_mask == nullptr || p.key_mask[b * p.mask_stride + j] != 0;
 }
@@ -203,14 +203,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 2^x for two values in fp32 arithmetic, for a share of the exponentials: the special-function unit makes 16 a cycle
-// and SM, which for heads of 64 is half of what the two products of a score take.  x = n + f with n the nearest
-// integer (read from the low bits of x + 1.5 * 2^23) and f in [-1/2, 1/2]; 2^f by the polynomial of least largest
-// relative error (fitted for this kernel: 7.5e-5 in degree 3, for weights rounded to bf16's 2^-9; 2.6e-6 in degree 4,
-// for fp16's 2^-12), and n added to its exponent.  x below -125 gives 2^-125; NaN stays NaN.
-template <int DEGREE>
-__device__ __forceinline__ void exp2_fma(float& x0, float& x1);
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -242,48 +234,38 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return d;
 }
 
-template <int DEGREE>
-__device__ __forceinline__ void exp2_fma(float& x0, float& x1) {
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(x0), "f"(-125.0f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(x1), "f"(-125.0f));
-  const uint64_t x = pair2(x0, x1);
-  const uint64_t t = add2(x, pair2(12582912.0f, 12582912.0f));
-  const uint64_t n = add2(t, pair2(-12582912.0f, -12582912.0f));
-  const uint64_t f = fma2(n, pair2(-1.0f, -1.0f), x);
-  const auto c = [](float v) { return pair2(v, v); };
-  uint64_t r;
-  if constexpr (DEGREE == 3) {
-    r = fma2(c(0.05517166853f), f, c(0.24261112511f));
-    r = fma2(r, f, c(0.69326096773f));
-    r = fma2(r, f, c(0.99992805719f));
-  } else {
-    r = fma2(c(0.00957010220f), f, c(0.05591785908f));
-    r = fma2(r, f, c(0.24024744332f));
-    r = fma2(r, f, c(0.69312179089f));
-    r = fma2(r, f, c(0.99999928474f));
-  }
-  float t0, t1, r0, r1;
-  unpair2(t, t0, t1);
-  unpair2(r, r0, r1);
-  x0 = __uint_as_float(__float_as_uint(r0) + (__float_as_uint(t0) << 23));
-  x1 = __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t1) << 23));
-}
-
-// 2^x of the pair-th pair of a row, in place; one pair of every EVERY goes by exp2_fma (0: none).
-template <typename T, int EVERY>
-__device__ __forceinline__ void exp2_pair(float& x0, float& x1, int pair) {
-  if (EVERY > 0 && pair % (EVERY > 0 ? EVERY : 1) == EVERY - 1) {
-    exp2_fma<XType<T>::kFormat == 1u ? 3 : 4>(x0, x1);
-  } else {
-    x0 = ex2(x0);
-    x1 = ex2(x1);
-  }
-}
-
 // A wait whose outcome the whole warp shares (the loads of tensor memory are warp-wide).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
                                           int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
+}
+
+// A number written in mixed radix, (d0, d1, d2, d3) with radices r0, r1, r2: an item's place (row tile, split, head,
+// sequence).  A CTA goes from item to item by adding the grid's digits, without a division.
+struct XCount {
+  int d0, d1, d2, d3;
+};
+__device__ __forceinline__ XCount x_count(uint32_t i, uint32_t r0, uint32_t r1, uint32_t r2) {
+  XCount c;
+  c.d0 = static_cast<int>(i % r0);
+  i /= r0;
+  c.d1 = static_cast<int>(i % r1);
+  i /= r1;
+  c.d2 = static_cast<int>(i % r2);
+  c.d3 = static_cast<int>(i / r2);
+  return c;
+}
+__device__ __forceinline__ void x_advance(XCount& c, const XCount& by, int r0, int r1, int r2) {
+  c.d0 += by.d0;
+  const int a = c.d0 >= r0;
+  c.d0 -= a ? r0 : 0;
+  c.d1 += by.d1 + a;
+  const int b = c.d1 >= r1;
+  c.d1 -= b ? r1 : 0;
+  c.d2 += by.d2 + b;
+  const int e = c.d2 >= r2;
+  c.d2 -= e ? r2 : 0;
+  c.d3 += by.d3 + e;
 }
 
 // The 128 keep bits of the keys [j0, j0 + 128) of sequence b (whole warp).
@@ -297,36 +279,41 @@ __device__ __forceinline__ uint4 x_keep_words(const XAttnParams& p, int b, int j
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Zeroes the rows of a [128][64 * HALVES] tile (128-byte swizzled rows, halves 16 KB apart) whose keep bit is 0
-// (whole warp): a weight of zero times an infinity or NaN stored there would not be zero.
+// Zeroes the rows below `used` of a [128][64 * HALVES] tile (128-byte rows, halves 16 KB apart) whose keep bit is 0
+// (whole warp): a weight of zero times an infinity or NaN stored there would not be zero.  Four rows a step, eight
+// lanes a row: a row's 128 bytes meet all banks once.  (One row a lane took 2,000 cycles for 51 rows, this takes 150.)
 template <int HALVES>
-__device__ __forceinline__ void x_zero_rows(uint8_t* tile, const uint4& keep, int lane) {
+__device__ __forceinline__ void x_zero_rows(uint8_t* tile, const uint4& keep, int used, int lane) {
   const uint32_t w[4] = {keep.x, keep.y, keep.z, keep.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if ((w[i] >> lane) & 1u) continue;
-    uint8_t* row = tile + (32 * i + lane) * 128;
-    for (int hf = 0; hf < HALVES; ++hf)
+    if (32 * i >= used || w[i] == 0xffffffffu) continue;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(row + hf * 16384 + c * 16) = make_uint4(0, 0, 0, 0);
+    for (int r = 0; r < 32; r += 4) {
+      if (((w[i] >> r) & 15u) == 15u) continue;
+      if (!((w[i] >> (r + (lane >> 3))) & 1u))
+#pragma unroll
+        for (int hf = 0; hf < HALVES; ++hf)
+          st_shared_v4(tile + hf * 16384 + (32 * i + r) * 128 + lane * 16, 0, 0, 0, 0);
+    }
   }
   fence_proxy_async_smem();
   __syncwarp();
 }
 
 // ============================================================================ forward
-constexpr int kXExpEvery = 4;  // one pair of exponentials in so many goes by exp2_fma
 constexpr int kXMaskSlots = 8;  // key tiles whose keep bits are held: more than are ever between load and use
 
 struct XFwdParams {
   XAttnParams a;
   int row_tiles;    // row tiles of a (sequence, head group)
+  int hv;           // head groups: heads / pack
   int key_chunk;    // key tiles of a split; splits == 1: all of them
   int splits;
   float* part_o;    // [splits][batch * heads * q_len][head_dim], with splits > 1
   float* part_lse;  // [splits][batch * heads * q_len], base-2 logarithm
   int64_t rows;     // batch * heads * q_len
-  int64_t items;    // (sequence, head group, row tile group, split)
+  uint32_t items;   // (sequence, head group, row tile group, split)
 };
 
 // NT row tiles of HALVES * 64 channels a CTA.
@@ -339,7 +326,7 @@ struct XFwdLayout {
   static constexpr int kKV = NT * kTileBytes * kQStages;
   static constexpr int kWords = kKV + kEntries * kTileBytes;
   static constexpr int kBar = kWords + kXMaskSlots * 16;
-  static constexpr int kNumBars = 2 * kQStages + 2 * kEntries + 7 * NT;
+  static constexpr int kNumBars = 2 * kQStages + 2 * kEntries + 8 * NT;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;  // + alignment slack
   static constexpr int kThreads = NT * 128 + 32 + NT * 32;  // softmax, loads, products of each row tile
@@ -353,24 +340,37 @@ static_assert(XFwdLayout<2, 1>::kSmemBytes <= 115712 && XFwdLayout<1, 1>::kSmemB
 struct XItem {
   int b, hv, tile0, tiles, split, keys, j0, j1;
 };
+// A CTA's items in turn.  The next one's key count is asked for an item ahead, so that it is not waited for.
 template <int NT>
-__device__ __forceinline__ XItem x_item(const XFwdParams& p, int64_t i) {
-  XItem t;
-  const int groups = (p.row_tiles + NT - 1) / NT;
-  t.tile0 = static_cast<int>(i % groups) * NT;
-  i /= groups;
-  t.split = static_cast<int>(i % p.splits);
-  i /= p.splits;
-  const int hv = p.a.heads / p.a.pack;
-  t.hv = static_cast<int>(i % hv);
-  t.b = static_cast<int>(i / hv);
-  t.tiles = min(NT, p.row_tiles - t.tile0);
-  t.keys = x_key_count(p.a, t.b);
-  const int n = (t.keys + kXTile - 1) / kXTile;
-  t.j0 = min(n, t.split * p.key_chunk);
-  t.j1 = min(n, t.j0 + p.key_chunk);
-  return t;
-}
+struct XItems {
+  const XFwdParams& p;
+  const int groups, hv;
+  const XCount by;
+  uint32_t i;
+  XCount at;
+  int keys = 0;
+  __device__ __forceinline__ explicit XItems(const XFwdParams& q)
+      : p(q), groups((q.row_tiles + NT - 1) / NT), hv(q.hv), by(x_count(gridDim.x, groups, q.splits, q.hv)), i(blockIdx.x),
+        at(x_count(blockIdx.x, groups, q.splits, q.hv)) {
+    if (i < p.items) keys = x_raw_count(p.a, at.d3);
+  }
+  __device__ __forceinline__ bool next(XItem& t) {
+    if (i >= p.items) return false;
+    t.tile0 = at.d0 * NT;
+    t.tiles = min(NT, p.row_tiles - t.tile0);
+    t.split = at.d1;
+    t.hv = at.d2;
+    t.b = at.d3;
+    t.keys = x_key_count(p.a, keys);
+    const int n = (t.keys + kXTile - 1) / kXTile;
+    t.j0 = min(n, t.split * p.key_chunk);
+    t.j1 = min(n, t.j0 + p.key_chunk);
+    i += gridDim.x;
+    x_advance(at, by, groups, p.splits, hv);
+    if (i < p.items) keys = x_raw_count(p.a, at.d3);
+    return true;
+  }
+};
 // 32-key chunks of key tile j that hold keys.
 __device__ __forceinline__ int x_chunks(int keys, int j) { return (min(kXTile, keys - j * kXTile) + 31) >> 5; }
 
@@ -392,7 +392,8 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
   uint64_t* o_free = o_full + NT;
   uint64_t* staged = o_free + NT;
   uint64_t* p_rest = staged + NT;
-  uint64_t* drained = p_rest + NT;
+  uint64_t* turn = p_rest + NT;
+  uint64_t* drained = turn + NT;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::kTail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -413,6 +414,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       mbar_init(o_free + i, 4);
       mbar_init(staged + i, 4);
       mbar_init(p_rest + i, 4);
+      mbar_init(turn + i, 1);
       mbar_init(drained + i, 1);
     }
     *abort_flag = 0;
@@ -442,8 +444,9 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
     const uint32_t q_bytes = static_cast<uint32_t>(a.tile_tokens * a.pack) * 128u * HALVES;
     uint32_t e = 0, loaded = 0, n_item = 0, g = 0;  // `loaded`: entries whose copy was started
     bool ok = true;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XItem t = x_item<NT>(p, i);
+    XItems<NT> items(p);
+    XItem t;
+    while (ok && items.next(t)) {
       if (t.j0 >= t.j1) continue;
       const int qs = n_item % Ly::kQStages;
       ok = warp_wait(q_empty + qs, ((n_item / Ly::kQStages) & 1) ^ 1, abort_flag, a.err, kErrXForward + kWaitQFree);
@@ -494,20 +497,36 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
     const uint32_t t_s = tmem + r * 128, t_o = tmem + NT * 128 + r * HALVES * 64;
     uint32_t n_item = 0, g = 0, n_s = 0, n_out = 0;  // items and key tiles of the CTA; key tiles and items of this row tile
     bool ok = true;
+    // Two row tiles take turns at the tensor cores, from the second half of a P V to the next S: products that two
+    // warps issue at a time run mixed, both end late, and then both softmaxes run at a time while the tensor cores
+    // are idle (heads of 128, 4096 keys: 3,860 cycles a pair of tiles; in turns they stay half a period apart).
+    uint32_t n_turn = 0;
+    const auto take_turn = [&]() {
+      if (NT == 1) return true;
+      ++n_turn;
+      // the first row tile begins
+      if (r == 0 && n_turn == 1) return true;
+      return warp_wait(turn + r, (n_turn - (r == 0 ? 2 : 1)) & 1, abort_flag, a.err, kErrXForward + kWaitTurn);
+    };
+    const auto pass_turn = [&]() {
+      if (NT == 2 && lane == 0) mbar_arrive(turn + 1 - r);
+    };
     // Entry e (K of key tile e / 2, or its V) has arrived, with zeros in the rows that are not kept.  (Each row tile's
     // warp writes them: the same zeros.)
-    const auto entry = [&](uint32_t e, bool bits) {
+    const auto entry = [&](uint32_t e, bool bits, int used) {
       const int slot = e % Ly::kEntries;
       if (!warp_wait(kv_full + slot, (e / Ly::kEntries) & 1, abort_flag, a.err, kErrXForward + kWaitK + (e & 1)))
         return false;
       if (bits) {
         const uint4 w = words[(e >> 1) % kXMaskSlots];
-        if ((w.x & w.y & w.z & w.w) != 0xffffffffu) x_zero_rows<HALVES>(smem + Ly::kKV + slot * Ly::kTileBytes, w, lane);
+        if ((w.x & w.y & w.z & w.w) != 0xffffffffu)
+          x_zero_rows<HALVES>(smem + Ly::kKV + slot * Ly::kTileBytes, w, used, lane);
       }
       return true;
     };
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XItem t = x_item<NT>(p, i);
+    XItems<NT> items(p);
+    XItem t;
+    while (ok && items.next(t)) {
       if (t.j0 >= t.j1) continue;
       const int qs = n_item % Ly::kQStages;
       if (r >= t.tiles) {  // no rows: the entries are only passed on
@@ -517,6 +536,10 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
             const int slot = e % Ly::kEntries;
             ok = ok && warp_wait(kv_full + slot, (e / Ly::kEntries) & 1, abort_flag, a.err, kErrXForward + kWaitK + (e & 1));
             if (ok && lane == 0) mbar_arrive(kv_empty + slot);
+            if (e & 1) {
+              ok = ok && take_turn();
+              if (ok) pass_turn();
+            }
           }
         ++n_item;
         continue;
@@ -527,7 +550,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
         const int chunks = x_chunks(t.keys, j);
         const bool bits = masked || (j + 1) * kXTile > t.keys;
         // S over the last tile's P, whose product was issued before it (products run in their order)
-        if (!(ok = entry(2 * g, bits))) break;
+        if (!(ok = entry(2 * g, bits, chunks * 32))) break;
         tc_fence_after();
         if (elect_one()) {
           products_k_major(t_s, sq, k_major_desc(s_base + Ly::kKV + (2 * g % Ly::kEntries) * Ly::kTileBytes),
@@ -537,8 +560,9 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
           umma_commit(kv_empty + 2 * g % Ly::kEntries);
         }
         __syncwarp();
+        if (j > t.j0) pass_turn();
         // O += P V, its first half as soon as the first 64 weights are there
-        ok = entry(2 * g + 1, bits) && warp_wait(p_full + r, n_s & 1, abort_flag, a.err, kErrXForward + kWaitP);
+        ok = entry(2 * g + 1, bits, chunks * 32) && warp_wait(p_full + r, n_s & 1, abort_flag, a.err, kErrXForward + kWaitP);
         if (ok && j == t.j0 && n_out > 0)  // the last item's output has been read
           ok = warp_wait(o_free + r, (n_out - 1) & 1, abort_flag, a.err, kErrXForward + kWaitAccFree);
         if (!ok) break;
@@ -551,7 +575,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
             if (k < 2 * chunks) umma_f16_ts(t_o, t_s + k * 8, sv + k * 128, idesc_o, k > 0 ? 1u : later);
         }
         __syncwarp();
-        ok = warp_wait(p_rest + r, n_s & 1, abort_flag, a.err, kErrXForward + kWaitPRest);
+        ok = warp_wait(p_rest + r, n_s & 1, abort_flag, a.err, kErrXForward + kWaitPRest) && take_turn();
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -562,6 +586,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
           if (j == t.j1 - 1) umma_commit(o_full + r);
         }
         __syncwarp();
+        if (j == t.j1 - 1) pass_turn();  // the next item's Q may be long in coming
       }
       ++n_out;
       ++n_item;
@@ -579,7 +604,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
     const bool flip = a.scale < 0.0f;  // the largest score is the smallest product
     // log2 units; a zero scale keeps a factor that leaves -inf at -inf
     const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
-    const int rows = a.tile_tokens * a.pack;
+    const int rows = a.tile_tokens * a.pack, my_token = row / a.pack, my_head = row % a.pack;
     uint32_t n_s = 0, n_out = 0, n_item = 0, g = 0;
     int stored = -1;  // Q stage whose output is on its way out
     // The stage is free for a new Q once the output has been read from it; asked for as late as can be.
@@ -591,11 +616,12 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       stored = -1;
     };
     bool ok = true;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XItem t = x_item<NT>(p, i);
-      const int token = (t.tile0 + rt) * a.tile_tokens + row / a.pack;
+    XItems<NT> items(p);
+    XItem t;
+    while (ok && items.next(t)) {
+      const int token = (t.tile0 + rt) * a.tile_tokens + my_token;
       const bool live = rt < t.tiles && row < rows && token < a.q_len;
-      const int head = t.hv * a.pack + row % a.pack;
+      const int head = t.hv * a.pack + my_head;
       const int64_t r_index = (static_cast<int64_t>(t.b) * a.heads + head) * a.q_len + token;
       if (t.j0 >= t.j1) {  // no keys
         if (live) {
@@ -646,13 +672,14 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
         }
       };
       // The weights of chunk c, which take the place of a half of its scores.
-      const auto weigh = [&](auto every, const uint32_t(&v)[32], int c, uint64_t c22, uint64_t mc2) {
+      const auto weigh = [&](const uint32_t(&v)[32], int c, uint64_t c22, uint64_t mc2) {
         uint32_t pk[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
           float x0, x1;
           unpair2(fma2(pair2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c22, mc2), x0, x1);
-          exp2_pair<T, decltype(every)::value>(x0, x1, k >> 1);
+          x0 = ex2(x0);
+          x1 = ex2(x1);
           sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair2(x0, x1));
           pk[k >> 1] = XType<T>::pack2(x0, x1);
         }
@@ -686,69 +713,40 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
               for (int u = 0; u < 4; ++u)
                 mx[u] = max3(mx[u], __uint_as_float(x[k + 2 * u]), __uint_as_float(x[k + 2 * u + 1]));
           };
-          if (!masked && !flip && (j + 1) * kXTile <= t.keys) {
-            // 128 kept keys: half of the row stays in registers, the other half is read twice
-            constexpr std::integral_constant<int, kXExpEvery> kShare;
-            uint32_t v0[32], v1[32], v2[32], v3[32];
-            tmem_ld_32x32b_x32(t_s, v0);
-            tmem_ld_32x32b_x32(t_s + 32, v1);
-            tmem_ld_wait();
-            after_wait(v0);
-            after_wait(v1);
-            tmem_ld_32x32b_x32(t_s + 64, v2);
-            tmem_ld_32x32b_x32(t_s + 96, v3);
-            search(v0);
-            search(v1);
-            tmem_ld_wait();
-            after_wait(v2);
-            after_wait(v3);
-            search(v2);
-            search(v3);
-            raise(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), j);
-            const float mc = -m * c2;
-            const uint64_t c22 = pair2(c2, c2), mc2 = pair2(mc, mc);
-            weigh(kShare, v0, 0, c22, mc2);
-            tmem_ld_32x32b_x32(t_s + 64, v2);
-            weigh(kShare, v1, 1, c22, mc2);
-            give(p_full + rt);
-            tmem_ld_wait();
-            after_wait(v2);
-            tmem_ld_32x32b_x32(t_s + 96, v3);
-            weigh(kShare, v2, 2, c22, mc2);
-            tmem_ld_wait();
-            after_wait(v3);
-            weigh(kShare, v3, 3, c22, mc2);
-            give(p_rest + rt);
-          } else {
-            const bool bits = masked || (j + 1) * kXTile > t.keys;
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(words + g % kXMaskSlots);
-            const uint32_t sign = flip ? 0x80000000u : 0u;
-            const auto load = [&](uint32_t(&v)[32], int c) {
-              tmem_ld_32x32b_x32(t_s + c * 32, v);
-              const uint32_t keep = bits ? w[c] : ~0u;
-              tmem_ld_wait();
-              after_wait(v);
+          // The chunks that hold keys, twice (for the maximum, then for the weights), the next one read meanwhile: with
+          // the whole row kept between the two its scores alone take 128 of 168 registers, and it is no faster.
+          const bool bits = masked || (j + 1) * kXTile > t.keys;
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(words + g % kXMaskSlots);
+          const uint32_t sign = flip ? 0x80000000u : 0u;
+          const auto pass = [&](auto&& use) {
+            uint32_t v[2][32];
+            tmem_ld_32x32b_x32(t_s, v[0]);
+#pragma unroll 1
+            for (int c0 = 0; c0 < chunks; c0 += 2)
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] = (keep >> k) & 1u ? v[k] ^ sign : 0xff800000u;
-            };
-#pragma unroll 1
-            for (int c = 0; c < chunks; ++c) {
-              uint32_t v[32];
-              load(v, c);
-              search(v);
-            }
-            raise(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), j);
-            const float mc = m == -INFINITY ? 0.0f : -m * c2;
-            const uint64_t c22 = pair2(c2, c2), mc2 = pair2(mc, mc);
-#pragma unroll 1
-            for (int c = 0; c < chunks; ++c) {
-              uint32_t v[32];
-              load(v, c);
-              weigh(std::integral_constant<int, 0>{}, v, c, c22, mc2);  // 2^-inf has to be zero
-              if (c == min(chunks, 2) - 1) give(p_full + rt);
-            }
-            give(p_rest + rt);
-          }
+              for (int u = 0; u < 2; ++u) {
+                const int c = c0 + u;
+                if (c >= chunks) break;
+                const uint32_t keep = bits ? w[c] : ~0u;
+                tmem_ld_wait();
+                after_wait(v[u]);
+                if (c + 1 < chunks) tmem_ld_32x32b_x32(t_s + (c + 1) * 32, v[1 - u]);
+                if (keep != ~0u || flip) {
+#pragma unroll
+                  for (int k = 0; k < 32; ++k) v[u][k] = (keep >> k) & 1u ? v[u][k] ^ sign : 0xff800000u;
+                }
+                use(v[u], c);
+              }
+          };
+          pass([&](const uint32_t(&v)[32], int) { search(v); });
+          raise(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), j);
+          const float mc = m == -INFINITY ? 0.0f : -m * c2;
+          const uint64_t c22 = pair2(c2, c2), mc2 = pair2(mc, mc);
+          pass([&](const uint32_t(&v)[32], int c) {
+            weigh(v, c, c22, mc2);
+            if (c == min(chunks, 2) - 1) give(p_full + rt);
+          });
+          give(p_rest + rt);
           float s0, s1;
           unpair2(add2(sum[0], sum[1]), s0, s1);
           l += s0 + s1;

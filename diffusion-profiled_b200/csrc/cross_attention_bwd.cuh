@@ -26,9 +26,10 @@ namespace fp8b {
 struct XBwdParams {
   XAttnParams a;
   int row_tiles;  // row tiles of a (sequence, head group)
+  int hv;         // head groups: heads / pack
   // [batch][head groups][row_tiles][2][128]: -log-sum-exp in log2 units (-inf where the row has no weight), -delta
   float* stats;
-  int64_t items;
+  uint32_t items;
   // x_dkv_kernel
   int q_tiles;    // row tiles that read a key head: (group / pack) * row_tiles
   int q_chunk;    // row tiles of a split; splits == 1: all of them
@@ -72,17 +73,34 @@ constexpr uint32_t kXDqS = 0, kXDqDP = 256, kXDqAcc = 384;
 struct XDqItem {
   int b, hv, tile, keys, tiles;
 };
-__device__ __forceinline__ XDqItem x_dq_item(const XBwdParams& p, int64_t i) {
-  XDqItem t;
-  t.tile = static_cast<int>(i % p.row_tiles);
-  i /= p.row_tiles;
-  const int hv = p.a.heads / p.a.pack;
-  t.hv = static_cast<int>(i % hv);
-  t.b = static_cast<int>(i / hv);
-  t.keys = x_key_count(p.a, t.b);
-  t.tiles = (t.keys + kXTile - 1) / kXTile;
-  return t;
-}
+// As XItems; `ahead` is the item after the one that next() gave.
+struct XDqItems {
+  const XBwdParams& p;
+  const XCount by;
+  uint32_t i;
+  XCount at;
+  int keys = 0;
+  __device__ __forceinline__ explicit XDqItems(const XBwdParams& q)
+      : p(q), by(x_count(gridDim.x, q.row_tiles, q.hv, 1u << 30)), i(blockIdx.x),
+        at(x_count(blockIdx.x, q.row_tiles, q.hv, 1u << 30)) {
+    if (i < p.items) keys = x_raw_count(p.a, at.d2);
+  }
+  __device__ __forceinline__ bool ahead(XDqItem& t) const {
+    t.tile = at.d0;
+    t.hv = at.d1;
+    t.b = at.d2;
+    t.keys = x_key_count(p.a, keys);
+    t.tiles = (t.keys + kXTile - 1) / kXTile;
+    return i < p.items;
+  }
+  __device__ __forceinline__ bool next(XDqItem& t) {
+    if (!ahead(t)) return false;
+    i += gridDim.x;
+    x_advance(at, by, p.row_tiles, p.hv, 1 << 30);
+    if (i < p.items) keys = x_raw_count(p.a, at.d2);
+    return true;
+  }
+};
 
 template <typename T, int HALVES>
 __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
@@ -165,8 +183,9 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
     const uint32_t q_bytes = static_cast<uint32_t>(a.tile_tokens * a.pack) * 128u * HALVES;
     uint32_t n_item = 0, g = 0, n_k = 0, n_v = 0;  // n_k, n_v: copies started
     bool ok = true;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDqItem t = x_dq_item(p, i);
+    XDqItems items(p);
+    XDqItem t;
+    while (ok && items.next(t)) {
       if (t.tiles == 0) continue;
       const int qs = n_item % Ly::kQStages;
       ok = wait(q_empty + qs, (n_item / Ly::kQStages) ^ 1, kWaitQFree);
@@ -220,8 +239,9 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
     // ------------------------------------------------------------ products S = Q K^T, dP = dO V^T
     uint32_t n_item = 0, g = 0;
     bool ok = true;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDqItem t = x_dq_item(p, i);
+    XDqItems items(p);
+    XDqItem t;
+    while (ok && items.next(t)) {
       if (t.tiles == 0) continue;
       const int qs = n_item % Ly::kQStages;
       ok = wait(q_full + qs, n_item / Ly::kQStages, kWaitQ);
@@ -237,7 +257,7 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
         uint4 w = make_uint4(~0u, ~0u, ~0u, ~0u);
         if (bits) w = words[g % kXMaskSlots];
         const bool holes = (w.x & w.y & w.z & w.w) != 0xffffffffu;
-        if (holes) x_zero_rows<HALVES>(sk, w, lane);
+        if (holes) x_zero_rows<HALVES>(sk, w, x_chunks(t.keys, j) * 32, lane);
         if (g >= 2 && !(ok = wait(s_free + buf, (g >> 1) ^ 1, kWaitSFree))) break;
         tc_fence_after();
         if (elect_one()) {
@@ -247,7 +267,7 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
         }
         __syncwarp();
         if (!(ok = wait(v_full + vs, g / Ly::kVStages, kWaitV))) break;
-        if (holes) x_zero_rows<HALVES>(sv, w, lane);
+        if (holes) x_zero_rows<HALVES>(sv, w, x_chunks(t.keys, j) * 32, lane);
         if (g >= 1 && !(ok = wait(dp_free, g ^ 1, kWaitDPFree))) break;
         tc_fence_after();
         if (elect_one()) {
@@ -269,8 +289,9 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
     const uint32_t idesc = x_idesc<T>(ksteps * 16, 0, 1);
     uint32_t n_item = 0, g = 0;
     bool ok = true;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDqItem t = x_dq_item(p, i);
+    XDqItems items(p);
+    XDqItem t;
+    while (ok && items.next(t)) {
       if (t.tiles == 0) continue;
       for (int j = 0; j < t.tiles; ++j, ++g) {
         const int ks = g % Ly::kKStages, buf = g & 1, steps = 2 * x_chunks(t.keys, j);
@@ -304,17 +325,17 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c2 = a.scale * 1.4426950408889634f;
     const uint64_t c22 = pair2(c2, c2);
-    const int rows = a.tile_tokens * a.pack, hv = a.heads / a.pack;
+    const int rows = a.tile_tokens * a.pack;
     const int my_token = row / a.pack, my_head = row % a.pack;
     // Half wh of the channels of this row's output, and its log-sum-exp, for the item to come: asked for while the
     // products of the item before still run.
     uint4 o_row[HALVES * 4];
     float lse = -INFINITY;
-    const auto fetch = [&](int64_t i) {
-      if (i >= p.items) return;
-      const XDqItem t = x_dq_item(p, i);
+    const auto fetch = [&](const XDqItems& items) {
+      XDqItem t;
+      const bool exists = items.ahead(t);
       const int token = t.tile * a.tile_tokens + my_token, head = t.hv * a.pack + my_head;
-      const bool live = t.tiles > 0 && row < rows && token < a.q_len;
+      const bool live = exists && t.tiles > 0 && row < rows && token < a.q_len;
       const T* o = static_cast<const T*>(a.o_in) + t.b * a.so.batch + token * a.so.token + head * a.so.head;
 #pragma unroll
       for (int u = 0; u < HALVES * 4; ++u) {
@@ -323,7 +344,6 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
       }
       lse = live ? a.lse[(static_cast<int64_t>(t.b) * a.heads + head) * a.q_len + token] : -INFINITY;
     };
-    fetch(blockIdx.x);
     uint32_t n_item = 0, g = 0;
     int stored = -1;  // Q stage whose gradient is on its way out
     const auto release_stored = [&]() {
@@ -334,10 +354,12 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
       stored = -1;
     };
     bool ok = true;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDqItem t = x_dq_item(p, i);
+    XDqItems items(p);
+    XDqItem t;
+    fetch(items);
+    while (ok && items.next(t)) {
       const int token = t.tile * a.tile_tokens + my_token, head = t.hv * a.pack + my_head;
-      float* stat = p.stats + ((static_cast<int64_t>(t.b) * hv + t.hv) * p.row_tiles + t.tile) * (2 * kXTile) + row;
+      float* stat = p.stats + ((static_cast<int64_t>(t.b) * p.hv + t.hv) * p.row_tiles + t.tile) * (2 * kXTile) + row;
       if (t.tiles == 0) {  // no keys
         if (wh == 0) {
           stat[0] = -INFINITY;
@@ -347,7 +369,7 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
             for (int c = 0; c < a.head_dim; c += 8) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
           }
         }
-        fetch(i + gridDim.x);
+        fetch(items);
         continue;
       }
       const int qs = n_item % Ly::kQStages;
@@ -393,9 +415,8 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
           for (int k = 0; k < 32; k += 2) {
             float x0, x1;
             unpair2(fma2(pair2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), c22, nl2), x0, x1);
-            exp2_pair<T, kXExpEvery>(x0, x1, k >> 1);
-            s[c][k] = __float_as_uint(x0);
-            s[c][k + 1] = __float_as_uint(x1);
+            s[c][k] = __float_as_uint(ex2(x0));
+            s[c][k + 1] = __float_as_uint(ex2(x1));
           }
         if (masked || (j + 1) * kXTile > t.keys) {
           const uint4 w4 = words[g % kXMaskSlots];
@@ -439,7 +460,7 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
         if (lane == 0) mbar_arrive(ds_full);
       }
       if (!ok) break;
-      fetch(i + gridDim.x);
+      fetch(items);
       release_stored();
       ok = wait(acc_full, n_item, kWaitAcc);
       if (!ok) break;
@@ -514,20 +535,33 @@ constexpr uint32_t kXDkvS = 0, kXDkvDP = 128, kXDkvV = 256;
 struct XDkvItem {
   int b, hk, tile, split, keys, j0, j1;  // row tiles [j0, j1) of the key head; none where the tile has no keys
 };
-__device__ __forceinline__ XDkvItem x_dkv_item(const XBwdParams& p, int64_t i) {
-  XDkvItem t;
-  const int tiles = (p.a.k_len + kXTile - 1) / kXTile;
-  t.tile = static_cast<int>(i % tiles);
-  i /= tiles;
-  t.split = static_cast<int>(i % p.splits);
-  i /= p.splits;
-  t.hk = static_cast<int>(i % p.a.kv_heads);
-  t.b = static_cast<int>(i / p.a.kv_heads);
-  t.keys = x_key_count(p.a, t.b);
-  t.j0 = min(p.q_tiles, t.split * p.q_chunk);
-  t.j1 = t.tile * kXTile < t.keys ? min(p.q_tiles, t.j0 + p.q_chunk) : t.j0;
-  return t;
-}
+struct XDkvItems {
+  const XBwdParams& p;
+  const int tiles;
+  const XCount by;
+  uint32_t i;
+  XCount at;
+  int keys = 0;
+  __device__ __forceinline__ explicit XDkvItems(const XBwdParams& q)
+      : p(q), tiles((q.a.k_len + kXTile - 1) / kXTile), by(x_count(gridDim.x, tiles, q.splits, q.a.kv_heads)),
+        i(blockIdx.x), at(x_count(blockIdx.x, tiles, q.splits, q.a.kv_heads)) {
+    if (i < p.items) keys = x_raw_count(p.a, at.d3);
+  }
+  __device__ __forceinline__ bool next(XDkvItem& t) {
+    if (i >= p.items) return false;
+    t.tile = at.d0;
+    t.split = at.d1;
+    t.hk = at.d2;
+    t.b = at.d3;
+    t.keys = x_key_count(p.a, keys);
+    t.j0 = min(p.q_tiles, t.split * p.q_chunk);
+    t.j1 = t.tile * kXTile < t.keys ? min(p.q_tiles, t.j0 + p.q_chunk) : t.j0;
+    i += gridDim.x;
+    x_advance(at, by, tiles, p.splits, p.a.kv_heads);
+    if (i < p.items) keys = x_raw_count(p.a, at.d3);
+    return true;
+  }
+};
 
 template <typename T, int HALVES>
 __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
@@ -607,11 +641,11 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
     // ------------------------------------------------------------ loads
     const uint32_t q_bytes = static_cast<uint32_t>(rows) * 128u * HALVES;
     const int per_key_head = a.group / a.pack;  // head groups that read a key head (1 where all are packed)
-    const int hv = a.heads / a.pack;
     uint32_t e = 0, n_item = 0;  // copies started
     bool ok = true;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDkvItem t = x_dkv_item(p, i);
+    XDkvItems items(p);
+    XDkvItem t;
+    while (ok && items.next(t)) {
       if (t.j0 >= t.j1) continue;
       const int ks = n_item % Ly::kKVStages;
       const uint4 w = x_keep_words(a, t.b, t.tile * kXTile, t.keys, lane);
@@ -641,7 +675,7 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
                           hf * 64, h * a.pack, tile * a.tile_tokens, t.b);
             if (which == 0)
               bulk_load_1d(stats + (slot >> 1) * 2 * kXTile,
-                           p.stats + ((static_cast<int64_t>(t.b) * hv + h) * p.row_tiles + tile) * (2 * kXTile), 1024,
+                           p.stats + ((static_cast<int64_t>(t.b) * p.hv + h) * p.row_tiles + tile) * (2 * kXTile), 1024,
                            q_full + slot);
           }
           ++e;
@@ -662,16 +696,18 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
     const uint32_t idesc = x_idesc<T>(kXTile, 0, 0);
     uint32_t n_item = 0, g = 0;
     bool ok = true;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDkvItem t = x_dkv_item(p, i);
+    XDkvItems items(p);
+    XDkvItem t;
+    while (ok && items.next(t)) {
       if (t.j0 >= t.j1) continue;
       const int ks = n_item % Ly::kKVStages;
       ok = wait(kv_full + ks, n_item / Ly::kKVStages, kWaitK);
       if (!ok) break;
       const uint4 w = words[n_item % (2 * Ly::kKVStages)];
       if ((w.x & w.y & w.z & w.w) != 0xffffffffu) {
-        x_zero_rows<HALVES>(smem + 2 * ks * Ly::kTileBytes, w, lane);
-        x_zero_rows<HALVES>(smem + (2 * ks + 1) * Ly::kTileBytes, w, lane);
+        // rows past the states were copied as zeros
+        x_zero_rows<HALVES>(smem + 2 * ks * Ly::kTileBytes, w, a.k_len - t.tile * kXTile, lane);
+        x_zero_rows<HALVES>(smem + (2 * ks + 1) * Ly::kTileBytes, w, a.k_len - t.tile * kXTile, lane);
       }
       const uint64_t sk = k_major_desc(s_base + 2 * ks * Ly::kTileBytes);
       const uint64_t sv = k_major_desc(s_base + (2 * ks + 1) * Ly::kTileBytes);
@@ -709,8 +745,9 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
     const uint32_t idesc = x_idesc<T>(ksteps * 16, 0, 1);
     uint32_t n_item = 0, g = 0;
     bool ok = true;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDkvItem t = x_dkv_item(p, i);
+    XDkvItems items(p);
+    XDkvItem t;
+    while (ok && items.next(t)) {
       if (t.j0 >= t.j1) continue;
       for (int j = t.j0; j < t.j1; ++j, ++g) {
         const uint32_t eq = 2 * g % Ly::kEntries, phase = 2 * g / Ly::kEntries;
@@ -760,8 +797,9 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       stored = -1;
     };
     bool ok = true;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const XDkvItem t = x_dkv_item(p, i);
+    XDkvItems items(p);
+    XDkvItem t;
+    while (ok && items.next(t)) {
       const int j_key = t.tile * kXTile + key;
       const auto part = [&](int c) {  // this row of the split's partial sums
         return p.part + ((((static_cast<int64_t>(t.split) * 2 + wh) * a.batch + t.b) * a.k_len + j_key) * a.kv_heads + t.hk) *
@@ -808,8 +846,10 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
             float x0, x1, x2, x3;
             unpair2(fma2(pair2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), c22, pair2(nl.x, nl.y)), x0, x1);
             unpair2(fma2(pair2(__uint_as_float(s[c][k + 2]), __uint_as_float(s[c][k + 3])), c22, pair2(nl.z, nl.w)), x2, x3);
-            exp2_pair<T, kXExpEvery>(x0, x1, k >> 1);
-            exp2_pair<T, kXExpEvery>(x2, x3, (k >> 1) + 1);
+            x0 = ex2(x0);
+            x1 = ex2(x1);
+            x2 = ex2(x2);
+            x3 = ex2(x3);
             s[c][k] = __float_as_uint(x0);
             s[c][k + 1] = __float_as_uint(x1);
             s[c][k + 2] = __float_as_uint(x2);

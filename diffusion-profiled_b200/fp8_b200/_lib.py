@@ -24,11 +24,6 @@ EPILOGUE_NONE = 0
 EPILOGUE_BIAS = 1
 EPILOGUE_BIAS_SILU = 2
 
-DTYPE_BF16 = 0
-DTYPE_FP32 = 1
-DTYPE_FP16 = 2
-
-
 class HeadStrides(ctypes.Structure):
     """fp8_head_strides."""
 

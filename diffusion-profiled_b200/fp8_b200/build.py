@@ -1,6 +1,7 @@
-"""Ahead-of-time build of the CUDA library ``libfp8ops.so`` (sm_100a only).
+"""Ahead-of-time build of the CUDA library ``libfp8ops.so`` (sm_100a only) and of the torch
+operators over it, ``libfp8torch.so`` (csrc/torch_ops.cpp, host code).
 
-The library is built in-tree next to this file so that it travels with the
+The libraries are built in-tree next to this file so that they travel with the
 source tree; nothing is JIT-compiled at import time.  ``python -m fp8_b200.build``
 (with ``diffusion-profiled_b200`` on ``sys.path``) or ``build_library()`` runs nvcc.
 """
@@ -19,6 +20,8 @@ SRC_DIR = PKG_DIR.parent / "csrc"
 INCLUDE_DIR = PKG_DIR.parent.parent / "include"
 LIB_NAME = "libfp8ops.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+TORCH_LIB_PATH = PKG_DIR / "libfp8torch.so"
+TORCH_SRC = SRC_DIR / "torch_ops.cpp"
 OBJ_DIR = PKG_DIR / "_build"
 
 NVCC_FLAGS = [
@@ -44,7 +47,7 @@ def _nvcc() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted(SRC_DIR.glob("*.cu")) + headers()
+    return sorted(SRC_DIR.glob("*.cu")) + [TORCH_SRC] + headers()
 
 
 def headers() -> list[Path]:
@@ -52,9 +55,9 @@ def headers() -> list[Path]:
 
 
 def needs_rebuild() -> bool:
-    if not LIB_PATH.exists():
+    if not LIB_PATH.exists() or not TORCH_LIB_PATH.exists():
         return True
-    mtime = LIB_PATH.stat().st_mtime
+    mtime = min(LIB_PATH.stat().st_mtime, TORCH_LIB_PATH.stat().st_mtime)
     return any(p.stat().st_mtime > mtime for p in sources())
 
 
@@ -64,6 +67,28 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
         cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
+
+
+def _compile_torch_ops(obj: Path, verbose: bool) -> None:
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    cuda_include = Path(_nvcc()).resolve().parent.parent / "include"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-c", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{INCLUDE_DIR}", *(f"-isystem{p}" for p in (*include_paths(), cuda_include)), "-o", str(obj), str(TORCH_SRC)]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+
+
+def _link_torch_ops(obj: Path) -> None:
+    import torch
+
+    torch_lib = Path(torch.__file__).resolve().parent / "lib"
+    tmp = TORCH_LIB_PATH.with_suffix(".so.tmp")
+    subprocess.run(["g++", "-shared", "-o", str(tmp), str(obj), f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-lc10",
+                    "-lc10_cuda", f"-L{PKG_DIR}", f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN"], check=True)
+    os.replace(tmp, TORCH_LIB_PATH)
 
 
 def build_library(force: bool = False, verbose: bool = False) -> Path:
@@ -79,13 +104,19 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
         obj = OBJ_DIR / (src.stem + ".o")
         if force or not obj.exists() or obj.stat().st_mtime <= max(newest_header, src.stat().st_mtime):
             jobs.append((src, obj))
+    torch_obj = OBJ_DIR / (TORCH_SRC.stem + ".o")
+    torch_newest = max(TORCH_SRC.stat().st_mtime, (INCLUDE_DIR / "fp8ops.h").stat().st_mtime)
     with ThreadPoolExecutor() as pool:
-        for done in [pool.submit(_compile, src, obj, verbose) for src, obj in jobs]:
+        running = [pool.submit(_compile, src, obj, verbose) for src, obj in jobs]
+        if force or not torch_obj.exists() or torch_obj.stat().st_mtime <= torch_newest:
+            running.append(pool.submit(_compile_torch_ops, torch_obj, verbose))
+        for done in running:
             done.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     objs = [str(OBJ_DIR / (src.stem + ".o")) for src in sorted(SRC_DIR.glob("*.cu"))]
     subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", str(tmp), *objs], check=True)
     os.replace(tmp, LIB_PATH)
+    _link_torch_ops(torch_obj)
     return LIB_PATH
 
 

@@ -4,7 +4,9 @@ Each op allocates its outputs and workspaces with the torch caching allocator,
 launches the native kernels on torch's current stream and never synchronises,
 so the ops can be captured in CUDA graphs.  They are registered with
 ``torch.library.custom_op`` plus fake (meta) implementations so that
-``torch.compile`` treats them as opaque nodes.
+``torch.compile`` treats them as opaque nodes; the text-conditioning operators
+(cross attention, token embedding, dropout) are registered by ``libfp8torch.so``,
+which this module loads.
 
 Layouts: 4-D activations and conv weights are channels_last (physically NHWC /
 [Cout][3][3][Cin]); FP8 tensors are ``torch.float8_e4m3fn``; scales are fp32
@@ -19,6 +21,13 @@ from ctypes import c_int64, c_void_p
 import torch
 
 from . import _lib
+from .build import TORCH_LIB_PATH
+
+if not TORCH_LIB_PATH.exists():
+    raise RuntimeError(f"{TORCH_LIB_PATH} is missing: build it with fp8_b200.build.build_library() "
+                       "(or __graft_entry__.build()); there is no fallback implementation")
+_lib.load()  # libfp8ops.so, which the torch operators call
+torch.ops.load_library(str(TORCH_LIB_PATH))
 
 FP8_DTYPE = torch.float8_e4m3fn
 
@@ -43,21 +52,6 @@ def _require_cuda(*tensors: torch.Tensor) -> torch.device:
         if t.device != dev:
             raise RuntimeError(f"tensors on different devices: {t.device} vs {dev}")
     return dev
-
-
-DTYPE_CODES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_FP32, torch.float16: _lib.DTYPE_FP16}
-
-
-def _call_on(dev: torch.device, name: str, *args) -> None:
-    """Call the C entry ``name`` with ``args`` and ``dev``'s current stream (switching device only if needed)."""
-    fn = getattr(_lib.load(), name)
-    if dev.index == torch.cuda.current_device():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    if status:
-        _lib.check(status, name)
 
 
 def _nhwc_dims(t: torch.Tensor) -> tuple[int, int, int, int]:
