@@ -261,9 +261,9 @@ int x_bwd_launch(const XBwdParams& dq, const XBwdParams& dkv, const CUtensorMap 
   FP8_CUDA_TRY(cudaFuncSetAttribute(x_dkv_kernel<T, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     XDkvLayout<HALVES>::kSmemBytes));
   const auto grid = [&](int64_t items) { return dim3(static_cast<unsigned>(std::min<int64_t>(items, st->sm_count))); };
-  FP8_CUDA_TRY(launch_kernel(x_dq_kernel<T, HALVES>, grid(dq.items), dim3(XDqLayout<HALVES>::kThreads),
+  FP8_CUDA_TRY(launch_kernel(x_dq_kernel<T, HALVES>, grid(dq.items), dim3(kXBwdThreads),
                              XDqLayout<HALVES>::kSmemBytes, stream, 1, kTensorKernel, dq, m[0], m[1], m[2], m[3], m[4]));
-  FP8_CUDA_TRY(launch_kernel(x_dkv_kernel<T, HALVES>, grid(dkv.items), dim3(XDkvLayout<HALVES>::kThreads),
+  FP8_CUDA_TRY(launch_kernel(x_dkv_kernel<T, HALVES>, grid(dkv.items), dim3(kXBwdThreads),
                              XDkvLayout<HALVES>::kSmemBytes, stream, 1, kTensorKernel, dkv, m[0], m[1], m[2], m[3], m[5],
                              m[6]));
   count_launches(2);

@@ -157,6 +157,15 @@ __device__ __forceinline__ void products_k_major(uint32_t d_tmem, uint64_t a, ui
   }
 }
 
+// 32 lanes x 16 columns, TMEM -> register.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
 // 32 lanes x 16 columns, register -> TMEM.
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -179,6 +188,11 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void after_wait(uint32_t (&r)[16]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
 // Makes the uses of r come after the asm statements before it (a tcgen05.wait::ld).
 __device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
   asm volatile(""
@@ -713,40 +727,78 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
               for (int u = 0; u < 4; ++u)
                 mx[u] = max3(mx[u], __uint_as_float(x[k + 2 * u]), __uint_as_float(x[k + 2 * u + 1]));
           };
-          // The chunks that hold keys, twice (for the maximum, then for the weights), the next one read meanwhile: with
-          // the whole row kept between the two its scores alone take 128 of 168 registers, and it is no faster.
-          const bool bits = masked || (j + 1) * kXTile > t.keys;
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(words + g % kXMaskSlots);
-          const uint32_t sign = flip ? 0x80000000u : 0u;
-          const auto pass = [&](auto&& use) {
-            uint32_t v[2][32];
-            tmem_ld_32x32b_x32(t_s, v[0]);
+          if (!masked && !flip && (j + 1) * kXTile <= t.keys) {
+            // 128 kept keys: a quarter of the row stays in registers between the search and the weights, the rest is
+            // read twice (with all of it kept the row's scores alone take 128 of the 168 registers)
+            uint32_t v0[32], v1[32], v2[32];
+            tmem_ld_32x32b_x32(t_s, v0);
+            tmem_ld_32x32b_x32(t_s + 32, v1);
+            tmem_ld_wait();
+            after_wait(v0);
+            after_wait(v1);
+            tmem_ld_32x32b_x32(t_s + 64, v2);
+            search(v0);
+            search(v1);
+            tmem_ld_wait();
+            after_wait(v2);
+            tmem_ld_32x32b_x32(t_s + 96, v1);
+            search(v2);
+            tmem_ld_wait();
+            after_wait(v1);
+            search(v1);
+            tmem_ld_32x32b_x32(t_s + 32, v1);
+            raise(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), j);
+            const float mc = -m * c2;
+            const uint64_t c22 = pair2(c2, c2), mc2 = pair2(mc, mc);
+            weigh(v0, 0, c22, mc2);
+            tmem_ld_wait();
+            after_wait(v1);
+            tmem_ld_32x32b_x32(t_s + 64, v2);
+            weigh(v1, 1, c22, mc2);
+            give(p_full + rt);
+            tmem_ld_wait();
+            after_wait(v2);
+            tmem_ld_32x32b_x32(t_s + 96, v0);
+            weigh(v2, 2, c22, mc2);
+            tmem_ld_wait();
+            after_wait(v0);
+            weigh(v0, 3, c22, mc2);
+            give(p_rest + rt);
+          } else {
+            // keys left out, or a negative scale: the chunks that hold keys, twice, the next one read meanwhile
+            const bool bits = masked || (j + 1) * kXTile > t.keys;
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(words + g % kXMaskSlots);
+            const uint32_t sign = flip ? 0x80000000u : 0u;
+            const auto pass = [&](auto&& use) {
+              uint32_t v[2][32];
+              tmem_ld_32x32b_x32(t_s, v[0]);
 #pragma unroll 1
-            for (int c0 = 0; c0 < chunks; c0 += 2)
+              for (int c0 = 0; c0 < chunks; c0 += 2)
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const int c = c0 + u;
-                if (c >= chunks) break;
-                const uint32_t keep = bits ? w[c] : ~0u;
-                tmem_ld_wait();
-                after_wait(v[u]);
-                if (c + 1 < chunks) tmem_ld_32x32b_x32(t_s + (c + 1) * 32, v[1 - u]);
-                if (keep != ~0u || flip) {
+                for (int u = 0; u < 2; ++u) {
+                  const int c = c0 + u;
+                  if (c >= chunks) break;
+                  const uint32_t keep = bits ? w[c] : ~0u;
+                  tmem_ld_wait();
+                  after_wait(v[u]);
+                  if (c + 1 < chunks) tmem_ld_32x32b_x32(t_s + (c + 1) * 32, v[1 - u]);
+                  if (keep != ~0u || flip) {
 #pragma unroll
-                  for (int k = 0; k < 32; ++k) v[u][k] = (keep >> k) & 1u ? v[u][k] ^ sign : 0xff800000u;
+                    for (int k = 0; k < 32; ++k) v[u][k] = (keep >> k) & 1u ? v[u][k] ^ sign : 0xff800000u;
+                  }
+                  use(v[u], c);
                 }
-                use(v[u], c);
-              }
-          };
-          pass([&](const uint32_t(&v)[32], int) { search(v); });
-          raise(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), j);
-          const float mc = m == -INFINITY ? 0.0f : -m * c2;
-          const uint64_t c22 = pair2(c2, c2), mc2 = pair2(mc, mc);
-          pass([&](const uint32_t(&v)[32], int c) {
-            weigh(v, c, c22, mc2);
-            if (c == min(chunks, 2) - 1) give(p_full + rt);
-          });
-          give(p_rest + rt);
+            };
+            pass([&](const uint32_t(&v)[32], int) { search(v); });
+            raise(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), j);
+            const float mc = m == -INFINITY ? 0.0f : -m * c2;
+            const uint64_t c22 = pair2(c2, c2), mc2 = pair2(mc, mc);
+            pass([&](const uint32_t(&v)[32], int c) {
+              weigh(v, c, c22, mc2);
+              if (c == min(chunks, 2) - 1) give(p_full + rt);
+            });
+            give(p_rest + rt);
+          }
           float s0, s1;
           unpair2(add2(sum[0], sum[1]), s0, s1);
           l += s0 + s1;

@@ -11,9 +11,14 @@
 //     dV += P^T dO and dK += dS^T Q.
 // That is seven products a tile pair; a single launch would need five, but would add
 // dQ to memory from every key tile.  Both kernels know the rows' log-sum-exp, so no
-// maximum is searched and the 256 softmax threads take 64 columns of a row each.  Two
-// warps issue the products: one the scores and dP, which run ahead into a second score
-// buffer (dQ) or into the columns the softmax has read (dK, dV), one the gradients.
+// maximum is searched and a row of scores needs no single owner: 16 softmax warps take
+// 32 columns of a row each (four warps a scheduler hide the exponentials' and loads'
+// latency that two with 64 columns do not).  Two
+// warps issue the products: one the scores and dP, one the gradients.  In x_dq_kernel the
+// scores run ahead into a second buffer; in x_dkv_kernel, where tensor memory has no room
+// for one, P^T takes the place of S^T and dS^T that of dP^T, so that dV += P^T dO and the
+// next scores run while dS^T is made, and dK += dS^T Q and the next dP^T while the next
+// exponentials are.
 //
 // P and dS are rounded to the tensors' type (they are matrix operands); scores, dP,
 // statistics and all sums are fp32.
@@ -22,6 +27,9 @@
 #include "cross_attention.cuh"
 
 namespace fp8b {
+
+constexpr int kXBwdWarps = 16;                           // softmax warps
+constexpr int kXBwdThreads = kXBwdWarps * 32 + 96;       // and loads, scores, gradients
 
 struct XBwdParams {
   XAttnParams a;
@@ -64,10 +72,9 @@ struct XDqLayout {
   static constexpr int kNumBars = 2 * (kQStages + kKStages + kVStages) + 13;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;
-  static constexpr int kThreads = 352;
 };
 static_assert(XDqLayout<1>::kSmemBytes <= 232448 && XDqLayout<2>::kSmemBytes <= 232448, "dq smem");
-// tensor memory columns: two score buffers (dS over the first half of each 64), dP, dQ
+// tensor memory columns: two score buffers (dS over the first half of each 32), dP, dQ
 constexpr uint32_t kXDqS = 0, kXDqDP = 256, kXDqAcc = 384;
 
 struct XDqItem {
@@ -103,7 +110,7 @@ struct XDqItems {
 };
 
 template <typename T, int HALVES>
-__global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
+__global__ void __launch_bounds__(kXBwdThreads, 1)
     x_dq_kernel(const XBwdParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap do_map,
                 const __grid_constant__ CUtensorMap dq_map) {
@@ -151,16 +158,16 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
       mbar_init(drained + i, 1);
     }
     mbar_init(dp_full, 1);
-    mbar_init(dp_free, 8);
-    mbar_init(ds_full, 8);
+    mbar_init(dp_free, kXBwdWarps);
+    mbar_init(ds_full, kXBwdWarps);
     mbar_init(acc_full, 1);
-    mbar_init(acc_free, 8);
-    mbar_init(staged, 8);
+    mbar_init(acc_free, kXBwdWarps);
+    mbar_init(staged, kXBwdWarps);
     mbar_init(delta_full, 8);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (warp == kXBwdWarps) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -178,7 +185,7 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
     return warp_wait(bar, phase & 1, abort_flag, a.err, kErrXDq + what);
   };
 
-  if (warp == 8) {
+  if (warp == kXBwdWarps) {
     // ------------------------------------------------------------ loads
     const uint32_t q_bytes = static_cast<uint32_t>(a.tile_tokens * a.pack) * 128u * HALVES;
     uint32_t n_item = 0, g = 0, n_k = 0, n_v = 0;  // n_k, n_v: copies started
@@ -235,7 +242,7 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
       drain(k_full, Ly::kKStages, n_k);
       drain(v_full, Ly::kVStages, n_v);
     }
-  } else if (warp == 9) {
+  } else if (warp == kXBwdWarps + 1) {
     // ------------------------------------------------------------ products S = Q K^T, dP = dO V^T
     uint32_t n_item = 0, g = 0;
     bool ok = true;
@@ -284,7 +291,7 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
       umma_commit(drained);
       mbar_wait(drained, 0, &never, a.err, kErrXDq + kWaitDrain);
     }
-  } else if (warp == 10) {
+  } else if (warp == kXBwdWarps + 2) {
     // ------------------------------------------------------------ products dQ += dS K
     const uint32_t idesc = x_idesc<T>(ksteps * 16, 0, 1);
     uint32_t n_item = 0, g = 0;
@@ -303,9 +310,9 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)  // dS of columns 64 .. 127 lies at column 64 of the buffer
+          for (int k = 0; k < 8; ++k)  // dS of 32 columns lies in the first 16 of them
             if (k < steps)
-              umma_f16_ts(tmem + kXDqAcc, ds + (k >> 2) * 64 + (k & 3) * 8, sk + k * 128, idesc, k > 0 ? 1u : later);
+              umma_f16_ts(tmem + kXDqAcc, ds + (k >> 1) * 32 + (k & 1) * 8, sk + k * 128, idesc, k > 0 ? 1u : later);
           umma_commit(s_free + buf);
           umma_commit(k_empty + ks);
           if (j == t.tiles - 1) umma_commit(acc_full);
@@ -320,27 +327,30 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
       mbar_wait(drained + 1, 0, &never, a.err, kErrXDq + kWaitDrain);
     }
   } else {
-    // ------------------------------------------------------------ dS: thread = row, 64 columns of half wh
-    const int wh = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+    // ------------------------------------------------------------ dS: thread = row, the 32 columns of chunk wq
+    const int wq = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c2 = a.scale * 1.4426950408889634f;
     const uint64_t c22 = pair2(c2, c2);
     const int rows = a.tile_tokens * a.pack;
     const int my_token = row / a.pack, my_head = row % a.pack;
-    // Half wh of the channels of this row's output, and its log-sum-exp, for the item to come: asked for while the
-    // products of the item before still run.
-    uint4 o_row[HALVES * 4];
+    // This row's log-sum-exp and, in the first two chunks' warps, half of the channels of its output, for the item to
+    // come: asked for while the products of the item before still run.  (With heads of 128 the output is read when the
+    // item begins: the registers for it are not there, and items are longer.)
+    uint4 o_row[4];
     float lse = -INFINITY;
     const auto fetch = [&](const XDqItems& items) {
       XDqItem t;
       const bool exists = items.ahead(t);
       const int token = t.tile * a.tile_tokens + my_token, head = t.hv * a.pack + my_head;
       const bool live = exists && t.tiles > 0 && row < rows && token < a.q_len;
-      const T* o = static_cast<const T*>(a.o_in) + t.b * a.so.batch + token * a.so.token + head * a.so.head;
+      if (HALVES == 1 && wq < 2) {
+        const T* o = static_cast<const T*>(a.o_in) + t.b * a.so.batch + token * a.so.token + head * a.so.head;
 #pragma unroll
-      for (int u = 0; u < HALVES * 4; ++u) {
-        const int c = wh * HALVES * 32 + 8 * u;
-        o_row[u] = live && c < a.head_dim ? *reinterpret_cast<const uint4*>(o + c) : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < 4; ++u) {
+          const int c = wq * 32 + 8 * u;
+          o_row[u] = live && c < a.head_dim ? *reinterpret_cast<const uint4*>(o + c) : make_uint4(0, 0, 0, 0);
+        }
       }
       lse = live ? a.lse[(static_cast<int64_t>(t.b) * a.heads + head) * a.q_len + token] : -INFINITY;
     };
@@ -361,7 +371,7 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
       const int token = t.tile * a.tile_tokens + my_token, head = t.hv * a.pack + my_head;
       float* stat = p.stats + ((static_cast<int64_t>(t.b) * p.hv + t.hv) * p.row_tiles + t.tile) * (2 * kXTile) + row;
       if (t.tiles == 0) {  // no keys
-        if (wh == 0) {
+        if (wq == 0) {
           stat[0] = -INFINITY;
           stat[kXTile] = 0.0f;
           if (row < rows && token < a.q_len) {
@@ -374,87 +384,93 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
       }
       const int qs = n_item % Ly::kQStages;
       uint8_t* stage = smem + 2 * qs * Ly::kTileBytes;
-      // ---- delta = do . o, half of the channels each
-      ok = wait(q_full + qs, n_item / Ly::kQStages, kWaitQ);
-      if (!ok) break;
       const bool dead = lse == -INFINITY;  // no such row, or no kept key
-      float neg_delta = 0.0f;
+      // ---- delta = do . o, half of the channels each
+      if (wq < 2) {
+        ok = wait(q_full + qs, n_item / Ly::kQStages, kWaitQ);
+        if (!ok) break;
+        float part = 0.0f;
+        const T* o = static_cast<const T*>(a.o_in) + t.b * a.so.batch + token * a.so.token + head * a.so.head;
 #pragma unroll
-      for (int u = 0; u < HALVES * 4; ++u) {
-        const int c = wh * HALVES * 4 + u;  // 16-byte chunk of the row
-        neg_delta -= x_dot8<T>(o_row[u], ld_shared_v4(stage + Ly::kTileBytes + (c >> 3) * 16384 + swizzle128_offset(row, c & 7)));
+        for (int u = 0; u < HALVES * 4; ++u) {
+          const int c = wq * HALVES * 4 + u;  // 16-byte chunk of the row
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if constexpr (HALVES == 1) {
+            v = o_row[u];
+          } else if (!dead && c * 8 < a.head_dim) {
+            v = *reinterpret_cast<const uint4*>(o + c * 8);
+          }
+          part -= x_dot8<T>(v, ld_shared_v4(stage + Ly::kTileBytes + (c >> 3) * 16384 + swizzle128_offset(row, c & 7)));
+        }
+        delta_half[wq * kXTile + row] = part;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(delta_full);
       }
-      delta_half[wh * kXTile + row] = neg_delta;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(delta_full);
       ok = wait(delta_full, n_item, kWaitDelta);
       if (!ok) break;
-      neg_delta = dead ? 0.0f : delta_half[row] + delta_half[kXTile + row];
+      const float neg_delta = dead ? 0.0f : delta_half[row] + delta_half[kXTile + row];
       const float neg_lse = dead ? -INFINITY : -lse * 1.4426950408889634f;
-      if (wh == 0) {
+      if (wq == 0) {
         stat[0] = neg_lse;
         stat[kXTile] = neg_delta;
       }
       const uint64_t nl2 = pair2(neg_lse, neg_lse), nd2 = pair2(neg_delta, neg_delta);
       for (int j = 0; j < t.tiles; ++j, ++g) {
-        const int chunks = x_chunks(t.keys, j);
-        const uint32_t t_s = t_lane + kXDqS + (g & 1) * 128 + wh * 64, t_dp = t_lane + kXDqDP + wh * 64;
-        const bool two = 2 * wh + 1 < chunks, one = 2 * wh < chunks;  // this half's chunks with keys
+        const uint32_t t_s = t_lane + kXDqS + (g & 1) * 128 + wq * 32;
+        const bool some = wq < x_chunks(t.keys, j);  // the chunk holds keys
         ok = wait(s_full + (g & 1), g >> 1, kWaitS);
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[2][32];
-        if (one) tmem_ld_32x32b_x32(t_s, s[0]);
-        if (two) tmem_ld_32x32b_x32(t_s + 32, s[1]);
-        tmem_ld_wait();
-        after_wait(s[0]);
-        after_wait(s[1]);
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
+        uint32_t s[32];
+        if (some) {
+          tmem_ld_32x32b_x32(t_s, s);
+          tmem_ld_wait();
+          after_wait(s);
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             float x0, x1;
-            unpair2(fma2(pair2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), c22, nl2), x0, x1);
-            s[c][k] = __float_as_uint(ex2(x0));
-            s[c][k + 1] = __float_as_uint(ex2(x1));
+            unpair2(fma2(pair2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c22, nl2), x0, x1);
+            s[k] = __float_as_uint(ex2(x0));
+            s[k + 1] = __float_as_uint(ex2(x1));
           }
-        if (masked || (j + 1) * kXTile > t.keys) {
-          const uint4 w4 = words[g % kXMaskSlots];
-          const uint32_t w[2] = {wh ? w4.z : w4.x, wh ? w4.w : w4.y};
+          if (masked || (j + 1) * kXTile > t.keys) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(words + g % kXMaskSlots)[wq];
+            if (w != ~0u) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int k = 0; k < 32; ++k) s[c][k] = (w[c] >> k) & 1u ? s[c][k] : 0u;
+              for (int k = 0; k < 32; ++k) s[k] = (w >> k) & 1u ? s[k] : 0u;
+            }
+          }
         }
         ok = wait(dp_full, g, kWaitDP);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t dp[32];
-          if (c == 0 ? one : two) {
-            tmem_ld_32x32b_x32(t_dp + c * 32, dp);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t dp[16];
+          if (some) {
+            tmem_ld_32x32b_x16(t_lane + kXDqDP + wq * 32 + h * 16, dp);
             tmem_ld_wait();
             after_wait(dp);
           }
-          if (c == 1) {
+          if (h == 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(dp_free);
           }
-          if (c == 0 ? one : two) {
-            uint32_t pk[16];
+          if (some) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) {
+            for (int k = 0; k < 16; k += 2) {
               const uint64_t d = add2(pair2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), nd2);
               float x0, x1;
-              unpair2(mul2(pair2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), d), x0, x1);
-              pk[k >> 1] = XType<T>::pack2(x0, x1);
+              unpair2(mul2(pair2(__uint_as_float(s[16 * h + k]), __uint_as_float(s[16 * h + k + 1])), d), x0, x1);
+              s[8 * h + (k >> 1)] = XType<T>::pack2(x0, x1);  // the first 16 become dS
             }
-            tmem_st_32x32b_x16(t_s + c * 16, pk);
           }
         }
-        tmem_st_wait();
+        if (some) {
+          tmem_st_32x32b_x16(t_s, reinterpret_cast<const uint32_t(&)[16]>(s));
+          tmem_st_wait();
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_full);
@@ -465,21 +481,21 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
       ok = wait(acc_full, n_item, kWaitAcc);
       if (!ok) break;
       tc_fence_after();
-      // dQ goes out from Q's tile, which every product of the item has read by now
+      // dQ goes out from Q's tile, which every product of the item has read by now: a quarter of the channels each
 #pragma unroll
-      for (int c = 0; c < HALVES; ++c) {  // this half's share of the channels: [wh * HALVES * 32, + HALVES * 32)
-        const int col = (wh * HALVES + c) * 32;
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(t_lane + kXDqAcc + col, o);
+      for (int c = 0; c < HALVES; ++c) {
+        const int col = (wq * HALVES + c) * 16;
+        uint32_t o[16];
+        tmem_ld_32x32b_x16(t_lane + kXDqAcc + col, o);
         tmem_ld_wait();
         after_wait(o);
-        uint32_t pk[16];
+        uint32_t pk[8];
 #pragma unroll
-        for (int k = 0; k < 32; k += 2)
+        for (int k = 0; k < 16; k += 2)
           pk[k >> 1] = dead ? 0u : XType<T>::pack2(__uint_as_float(o[k]) * a.scale, __uint_as_float(o[k + 1]) * a.scale);
         uint8_t* half = stage + (col >> 6) * 16384;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 2; ++u)
           st_shared_v4(half + swizzle128_offset(row, ((col & 63) >> 3) + u), pk[4 * u], pk[4 * u + 1], pk[4 * u + 2],
                        pk[4 * u + 3]);
       }
@@ -507,7 +523,7 @@ __global__ void __launch_bounds__(XDqLayout<HALVES>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kXBwdWarps) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -523,13 +539,12 @@ struct XDkvLayout {
   static constexpr int kStats = kQ + kEntries * kTileBytes;  // fp32 [kEntries / 2][2][128]
   static constexpr int kWords = kStats + kEntries / 2 * 1024;
   static constexpr int kBar = kWords + 2 * kKVStages * 16;
-  static constexpr int kNumBars = 2 * kKVStages + 2 * kEntries + 11;
+  static constexpr int kNumBars = 2 * kKVStages + 2 * kEntries + 12;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;
-  static constexpr int kThreads = 352;
 };
 static_assert(XDkvLayout<1>::kSmemBytes <= 232448 && XDkvLayout<2>::kSmemBytes <= 232448, "dkv smem");
-// tensor memory columns: S^T, dP^T (P^T and dS^T over it), dV, dK
+// tensor memory columns: S^T (P^T over it), dP^T (dS^T over it), dV, dK
 constexpr uint32_t kXDkvS = 0, kXDkvDP = 128, kXDkvV = 256;
 
 struct XDkvItem {
@@ -564,7 +579,7 @@ struct XDkvItems {
 };
 
 template <typename T, int HALVES>
-__global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
+__global__ void __launch_bounds__(kXBwdThreads, 1)
     x_dkv_kernel(const XBwdParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap do_map,
                  const __grid_constant__ CUtensorMap dk_map, const __grid_constant__ CUtensorMap dv_map) {
@@ -578,11 +593,12 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
   uint64_t* q_full = kv_empty + Ly::kKVStages;
   uint64_t* q_empty = q_full + Ly::kEntries;
   uint64_t* s_full = q_empty + Ly::kEntries;
-  uint64_t* s_free = s_full + 1;
-  uint64_t* dp_full = s_free + 1;
-  uint64_t* dp_free = dp_full + 1;  // P^T and dS^T have been multiplied
-  uint64_t* ds_full = dp_free + 1;
-  uint64_t* acc_full = ds_full + 1;
+  uint64_t* p_full = s_full + 1;
+  uint64_t* p_free = p_full + 1;  // P^T has been multiplied
+  uint64_t* dp_full = p_free + 1;
+  uint64_t* ds_full = dp_full + 1;
+  uint64_t* ds_free = ds_full + 1;  // dS^T has been multiplied
+  uint64_t* acc_full = ds_free + 1;
   uint64_t* acc_free = acc_full + 1;
   uint64_t* staged = acc_free + 1;   // [2], by half of the softmax threads
   uint64_t* drained = staged + 2;    // [2], by issuing warp
@@ -599,29 +615,30 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
     }
     for (int i = 0; i < Ly::kEntries; ++i) {
       mbar_init(q_full + i, 1);
-      mbar_init(q_empty + i, 1);
+      mbar_init(q_empty + i, 1 + i % 2);  // Q: its dK product (S^T came before); dO: its dP^T and its dV product
     }
     mbar_init(s_full, 2);  // the products' commit, and the issuing thread (keep bits)
-    mbar_init(s_free, 8);
+    mbar_init(p_full, kXBwdWarps);
+    mbar_init(p_free, 1);
     mbar_init(dp_full, 1);
-    mbar_init(dp_free, 1);
-    mbar_init(ds_full, 8);
+    mbar_init(ds_free, 1);
+    mbar_init(ds_full, kXBwdWarps);
     mbar_init(acc_full, 1);
-    mbar_init(acc_free, 8);
+    mbar_init(acc_free, kXBwdWarps);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(staged + i, 4);
+      mbar_init(staged + i, kXBwdWarps / 2);
       mbar_init(drained + i, 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
   }
   // rows that no copy fills (128 is not a multiple of `pack`) are zero: they are summed over
-  for (int c = tid; c < (kXTile - rows) * 8 * HALVES * Ly::kEntries; c += Ly::kThreads) {
+  for (int c = tid; c < (kXTile - rows) * 8 * HALVES * Ly::kEntries; c += kXBwdThreads) {
     const int r = rows + c / 8 % (kXTile - rows), tile = c / 8 / (kXTile - rows);
     *reinterpret_cast<uint4*>(smem + Ly::kQ + tile * 16384 + r * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
-  if (warp == 8) {
+  if (warp == kXBwdWarps) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -637,7 +654,7 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
     return warp_wait(bar, phase & 1, abort_flag, a.err, kErrXDkv + what);
   };
 
-  if (warp == 8) {
+  if (warp == kXBwdWarps) {
     // ------------------------------------------------------------ loads
     const uint32_t q_bytes = static_cast<uint32_t>(rows) * 128u * HALVES;
     const int per_key_head = a.group / a.pack;  // head groups that read a key head (1 where all are packed)
@@ -691,7 +708,7 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       drain(q_full, Ly::kEntries, e);
       drain(kv_full, Ly::kKVStages, n_item);
     }
-  } else if (warp == 9) {
+  } else if (warp == kXBwdWarps + 1) {
     // ------------------------------------------------------------ products S^T = K Q^T, dP^T = V dO^T
     const uint32_t idesc = x_idesc<T>(kXTile, 0, 0);
     uint32_t n_item = 0, g = 0;
@@ -714,7 +731,7 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       for (int j = t.j0; j < t.j1; ++j, ++g) {
         const uint32_t eq = 2 * g % Ly::kEntries, phase = 2 * g / Ly::kEntries;
         ok = wait(q_full + eq, phase, kWaitQ);
-        if (ok && g >= 1) ok = wait(s_free, g ^ 1, kWaitSFree);
+        if (ok && g >= 1) ok = wait(p_free, g ^ 1, kWaitSFree);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -724,11 +741,12 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
         }
         __syncwarp();
         ok = wait(q_full + eq + 1, phase, kWaitV);
-        if (ok && g >= 1) ok = wait(dp_free, g ^ 1, kWaitDPFree);
+        if (ok && g >= 1) ok = wait(ds_free, g ^ 1, kWaitDPFree);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
           products_k_major(tmem + kXDkvDP, sv, k_major_desc(s_base + Ly::kQ + (eq + 1) * Ly::kTileBytes), idesc, ksteps);
+          umma_commit(q_empty + eq + 1);
           umma_commit(dp_full);
         }
         __syncwarp();
@@ -740,7 +758,7 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       umma_commit(drained);
       mbar_wait(drained, 0, &never, a.err, kErrXDkv + kWaitDrain);
     }
-  } else if (warp == 10) {
+  } else if (warp == kXBwdWarps + 2) {
     // ------------------------------------------------------------ products dV += P^T dO, dK += dS^T Q
     const uint32_t idesc = x_idesc<T>(ksteps * 16, 0, 1);
     uint32_t n_item = 0, g = 0;
@@ -751,25 +769,32 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       if (t.j0 >= t.j1) continue;
       for (int j = t.j0; j < t.j1; ++j, ++g) {
         const uint32_t eq = 2 * g % Ly::kEntries, phase = 2 * g / Ly::kEntries;
-        ok = wait(q_full + eq, phase, kWaitQ) && wait(q_full + eq + 1, phase, kWaitV) && wait(ds_full, g, kWaitP);
-        if (ok && j == t.j0 && n_item > 0) ok = wait(acc_free, n_item ^ 1, kWaitAccFree);  // the last item's sums have been read
-        if (!ok) break;
         const uint64_t sq = mn_major_desc(s_base + Ly::kQ + eq * Ly::kTileBytes);
         const uint64_t sdo = mn_major_desc(s_base + Ly::kQ + (eq + 1) * Ly::kTileBytes);
         const uint32_t later = j > t.j0 ? 1u : 0u;
+        // 32 rows' P^T or dS^T lies in the first 16 of their columns
+        ok = wait(q_full + eq + 1, phase, kWaitV) && wait(p_full, g, kWaitP);
+        if (ok && j == t.j0 && n_item > 0) ok = wait(acc_free, n_item ^ 1, kWaitAccFree);  // the last item's sums have been read
+        if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          // 32 rows' P^T and dS^T lie side by side, 16 columns each
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tmem + kXDkvV, tmem + kXDkvDP + (k >> 1) * 32 + (k & 1) * 8, sdo + k * 128, idesc, k > 0 ? 1u : later);
+            umma_f16_ts(tmem + kXDkvV, tmem + kXDkvS + (k >> 1) * 32 + (k & 1) * 8, sdo + k * 128, idesc, k > 0 ? 1u : later);
+          umma_commit(p_free);
           umma_commit(q_empty + eq + 1);
+        }
+        __syncwarp();
+        ok = wait(q_full + eq, phase, kWaitQ) && wait(ds_full, g, kWaitPRest);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tmem + kXDkvV + HALVES * 64, tmem + kXDkvDP + 16 + (k >> 1) * 32 + (k & 1) * 8, sq + k * 128, idesc,
+            umma_f16_ts(tmem + kXDkvV + HALVES * 64, tmem + kXDkvDP + (k >> 1) * 32 + (k & 1) * 8, sq + k * 128, idesc,
                         k > 0 ? 1u : later);
+          umma_commit(ds_free);
           umma_commit(q_empty + eq);
-          umma_commit(dp_free);
           if (j == t.j1 - 1) umma_commit(acc_full);
         }
         __syncwarp();
@@ -782,15 +807,17 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       mbar_wait(drained + 1, 0, &never, a.err, kErrXDkv + kWaitDrain);
     }
   } else {
-    // ------------------------------------------------------------ P^T, dS^T: thread = key, 64 rows of half wh
-    const int wh = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
+    // ------------------------------------------------------------ P^T, dS^T: thread = key, the 32 rows of chunk wq
+    const int wq = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
+    const int is_k = wq >> 1;  // the first half of the threads hands out dV, the second dK
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c2 = a.scale * 1.4426950408889634f;
     const uint64_t c22 = pair2(c2, c2);
+    const bool hands_out = (warp & 7) == 0 && lane == 0;
     uint32_t n_item = 0, g = 0;
     int stored = -1;  // K / V stage whose gradient is on its way out
     const auto release_stored = [&]() {
-      if (stored >= 0 && quad == 0 && lane == 0) {
+      if (stored >= 0 && hands_out) {
         bulk_wait_group_read<0>();
         mbar_arrive(kv_empty + stored);
       }
@@ -801,18 +828,22 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
     XDkvItem t;
     while (ok && items.next(t)) {
       const int j_key = t.tile * kXTile + key;
-      const auto part = [&](int c) {  // this row of the split's partial sums
-        return p.part + ((((static_cast<int64_t>(t.split) * 2 + wh) * a.batch + t.b) * a.k_len + j_key) * a.kv_heads + t.hk) *
+      const int c0 = (wq & 1) * HALVES * 32;  // this thread's channels: [c0, c0 + HALVES * 32)
+      const auto part = [&](int c) {          // this key's row of the split's partial sums
+        return p.part + ((((static_cast<int64_t>(t.split) * 2 + is_k) * a.batch + t.b) * a.k_len + j_key) * a.kv_heads + t.hk) *
                             a.head_dim + c;
       };
       if (t.j0 >= t.j1) {  // no keys in this tile (or no rows in this split)
         if (j_key < a.k_len) {
-          if (p.splits > 1) {
-            for (int c = 0; c < a.head_dim; c += 4) *reinterpret_cast<float4*>(part(c)) = make_float4(0, 0, 0, 0);
-          } else {
-            T* grad = wh == 0 ? static_cast<T*>(a.dv) + t.b * a.sdv.batch + j_key * a.sdv.token + t.hk * a.sdv.head
-                              : static_cast<T*>(a.dk) + t.b * a.sdk.batch + j_key * a.sdk.token + t.hk * a.sdk.head;
-            for (int c = 0; c < a.head_dim; c += 8) *reinterpret_cast<uint4*>(grad + c) = make_uint4(0, 0, 0, 0);
+          T* grad = is_k ? static_cast<T*>(a.dk) + t.b * a.sdk.batch + j_key * a.sdk.token + t.hk * a.sdk.head
+                         : static_cast<T*>(a.dv) + t.b * a.sdv.batch + j_key * a.sdv.token + t.hk * a.sdv.head;
+          for (int c = c0; c < min(a.head_dim, c0 + HALVES * 32); c += 8) {
+            if (p.splits > 1) {
+              *reinterpret_cast<float4*>(part(c)) = make_float4(0, 0, 0, 0);
+              *reinterpret_cast<float4*>(part(c + 4)) = make_float4(0, 0, 0, 0);
+            } else {
+              *reinterpret_cast<uint4*>(grad + c) = make_uint4(0, 0, 0, 0);
+            }
           }
         }
         continue;
@@ -822,66 +853,57 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
         ok = wait(s_full, g, kWaitS);
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[2][32];
-        tmem_ld_32x32b_x32(t_lane + kXDkvS + wh * 64, s[0]);
-        tmem_ld_32x32b_x32(t_lane + kXDkvS + wh * 64 + 32, s[1]);
-        const float4* neg_lse = reinterpret_cast<const float4*>(stats + g % (Ly::kEntries / 2) * 2 * kXTile + wh * 64);
+        const uint32_t t_s = t_lane + kXDkvS + wq * 32, t_dp = t_lane + kXDkvDP + wq * 32;
+        uint32_t s[32];
+        tmem_ld_32x32b_x32(t_s, s);
+        const float4* neg_lse = reinterpret_cast<const float4*>(stats + g % (Ly::kEntries / 2) * 2 * kXTile + wq * 32);
         const float4* neg_delta = neg_lse + kXTile / 4;
-        if (j == t.j0) {
-          const uint4 w = words[n_item % (2 * Ly::kKVStages)];
-          kept = ((quad == 0 ? w.x : quad == 1 ? w.y : quad == 2 ? w.z : w.w) >> lane) & 1u;
-        }
+        if (j == t.j0)
+          kept = (reinterpret_cast<const uint32_t*>(words + n_item % (2 * Ly::kKVStages))[quad] >> lane) & 1u;
         tmem_ld_wait();
-        after_wait(s[0]);
-        after_wait(s[1]);
+        after_wait(s);
+        uint32_t pk[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 nl = neg_lse[k >> 2];
+          float x0, x1, x2, x3;
+          unpair2(fma2(pair2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c22, pair2(nl.x, nl.y)), x0, x1);
+          unpair2(fma2(pair2(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])), c22, pair2(nl.z, nl.w)), x2, x3);
+          x0 = ex2(x0);
+          x1 = ex2(x1);
+          x2 = ex2(x2);
+          x3 = ex2(x3);
+          s[k] = __float_as_uint(x0);
+          s[k + 1] = __float_as_uint(x1);
+          s[k + 2] = __float_as_uint(x2);
+          s[k + 3] = __float_as_uint(x3);
+          pk[k >> 1] = XType<T>::pack2(x0, x1);
+          pk[(k >> 1) + 1] = XType<T>::pack2(x2, x3);
+        }
+        tmem_st_32x32b_x16(t_s, pk);
+        tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(s_free);
-        uint32_t pk[2][16];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 nl = neg_lse[c * 8 + (k >> 2)];
-            float x0, x1, x2, x3;
-            unpair2(fma2(pair2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), c22, pair2(nl.x, nl.y)), x0, x1);
-            unpair2(fma2(pair2(__uint_as_float(s[c][k + 2]), __uint_as_float(s[c][k + 3])), c22, pair2(nl.z, nl.w)), x2, x3);
-            x0 = ex2(x0);
-            x1 = ex2(x1);
-            x2 = ex2(x2);
-            x3 = ex2(x3);
-            s[c][k] = __float_as_uint(x0);
-            s[c][k + 1] = __float_as_uint(x1);
-            s[c][k + 2] = __float_as_uint(x2);
-            s[c][k + 3] = __float_as_uint(x3);
-            pk[c][k >> 1] = XType<T>::pack2(x0, x1);
-            pk[c][(k >> 1) + 1] = XType<T>::pack2(x2, x3);
-          }
+        if (lane == 0) mbar_arrive(p_full);
         ok = wait(dp_full, g, kWaitDP);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t t_dp = t_lane + kXDkvDP + wh * 64;
+        uint32_t dp[32];
+        tmem_ld_32x32b_x32(t_dp, dp);
+        tmem_ld_wait();
+        after_wait(dp);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t dp[32];
-          tmem_ld_32x32b_x32(t_dp + c * 32, dp);
-          tmem_ld_wait();
-          after_wait(dp);
-          tmem_st_32x32b_x16(t_dp + c * 32, pk[c]);
-          uint32_t ds[16];
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 nd = neg_delta[c * 8 + (k >> 2)];
-            float x0, x1, x2, x3;
-            unpair2(mul2(pair2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])),
-                         add2(pair2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), pair2(nd.x, nd.y))), x0, x1);
-            unpair2(mul2(pair2(__uint_as_float(s[c][k + 2]), __uint_as_float(s[c][k + 3])),
-                         add2(pair2(__uint_as_float(dp[k + 2]), __uint_as_float(dp[k + 3])), pair2(nd.z, nd.w))), x2, x3);
-            ds[k >> 1] = XType<T>::pack2(x0, x1);
-            ds[(k >> 1) + 1] = XType<T>::pack2(x2, x3);
-          }
-          tmem_st_32x32b_x16(t_dp + c * 32 + 16, ds);
+        for (int k = 0; k < 32; k += 4) {
+          const float4 nd = neg_delta[k >> 2];
+          float x0, x1, x2, x3;
+          unpair2(mul2(pair2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
+                       add2(pair2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), pair2(nd.x, nd.y))), x0, x1);
+          unpair2(mul2(pair2(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])),
+                       add2(pair2(__uint_as_float(dp[k + 2]), __uint_as_float(dp[k + 3])), pair2(nd.z, nd.w))), x2, x3);
+          pk[k >> 1] = XType<T>::pack2(x0, x1);
+          pk[(k >> 1) + 1] = XType<T>::pack2(x2, x3);
         }
+        tmem_st_32x32b_x16(t_dp, pk);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -893,13 +915,14 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       if (!ok) break;
       tc_fence_after();
       const int ks = n_item % Ly::kKVStages;
-      // dV goes out by the first half of the threads from V's tile, dK by the second from K's
-      uint8_t* stage = smem + (2 * ks + 1 - wh) * Ly::kTileBytes;
-      const float f = wh == 0 ? 1.0f : a.scale;
+      // dV goes out from V's tile, dK from K's
+      uint8_t* stage = smem + (2 * ks + 1 - is_k) * Ly::kTileBytes;
+      const float f = is_k ? a.scale : 1.0f;
 #pragma unroll
-      for (int c = 0; c < 2 * HALVES; ++c) {
+      for (int c = 0; c < HALVES; ++c) {
+        const int col = c0 + c * 32;
         uint32_t o[32];
-        tmem_ld_32x32b_x32(t_lane + kXDkvV + wh * HALVES * 64 + c * 32, o);
+        tmem_ld_32x32b_x32(t_lane + kXDkvV + is_k * HALVES * 64 + col, o);
         tmem_ld_wait();
         after_wait(o);
 #pragma unroll
@@ -908,17 +931,17 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
           if (j_key < a.k_len) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4)
-              if (c * 32 + k < a.head_dim)
-                *reinterpret_cast<uint4*>(part(c * 32 + k)) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              if (col + k < a.head_dim)
+                *reinterpret_cast<uint4*>(part(col + k)) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
           }
         } else {
           uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 2) pk[k >> 1] = XType<T>::pack2(__uint_as_float(o[k]), __uint_as_float(o[k + 1]));
-          uint8_t* half = stage + (c >> 1) * 16384;
+          uint8_t* half = stage + (col >> 6) * 16384;
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            st_shared_v4(half + swizzle128_offset(key, (c & 1) * 4 + u), pk[4 * u], pk[4 * u + 1], pk[4 * u + 2],
+            st_shared_v4(half + swizzle128_offset(key, ((col & 63) >> 3) + u), pk[4 * u], pk[4 * u + 1], pk[4 * u + 2],
                          pk[4 * u + 3]);
         }
       }
@@ -927,13 +950,13 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(acc_free);
-        mbar_arrive(staged + wh);
+        mbar_arrive(staged + is_k);
       }
-      if (quad == 0 && lane == 0) {
-        ok = mbar_wait(staged + wh, n_item & 1, abort_flag, a.err, kErrXDkv + kWaitStaged);
+      if (hands_out) {
+        ok = mbar_wait(staged + is_k, n_item & 1, abort_flag, a.err, kErrXDkv + kWaitStaged);
         if (ok && p.splits == 1) {
           for (int hf = 0; hf < HALVES; ++hf)
-            tma_store_4d(wh == 0 ? &dv_map : &dk_map, stage + hf * 16384, hf * 64, t.hk, t.tile * kXTile, t.b);
+            tma_store_4d(is_k ? &dk_map : &dv_map, stage + hf * 16384, hf * 64, t.hk, t.tile * kXTile, t.b);
           bulk_commit_group();
         }
       }
@@ -942,11 +965,11 @@ __global__ void __launch_bounds__(XDkvLayout<HALVES>::kThreads, 1)
       if (Ly::kKVStages == 1) release_stored();
       ++n_item;
     }
-    if (quad == 0 && lane == 0) bulk_wait_group<0>();
+    if (hands_out) bulk_wait_group<0>();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kXBwdWarps) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
