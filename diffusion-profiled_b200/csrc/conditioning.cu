@@ -363,6 +363,49 @@ int fp8_cross_attention_bwd(const fp8_cross_attention_args* a, void* workspace, 
 }
 
 // ------------------------------------------------------------------ token embedding
+namespace {
+
+// How an embedding gradient is sorted and summed, and where its workspace lies.  By sizes alone: the order of
+// the sums, and so the result, does not depend on the device.
+struct EmbedPlan {
+  int passes, bits, ctas, per_cta;
+  int chunk, slices;
+  int64_t chunks;
+  size_t key[2], pos[2], counts, row_start, head, tail, bytes;
+};
+EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
+  EmbedPlan w{};
+  int need = 1;  // keys are 0 .. vocab
+  while ((int64_t(1) << need) <= vocab) ++need;
+  w.passes = (need + kSortMaxBits - 1) / kSortMaxBits;
+  w.bits = (need + w.passes - 1) / w.passes;
+  // at least 2048 tokens a CTA: with fewer the passes' barriers cost more than the tokens
+  w.ctas = static_cast<int>(std::min<int64_t>(kSortMaxCtas, std::max<int64_t>(1, (tokens + 2047) / 2048)));
+  w.per_cta = static_cast<int>((tokens + w.ctas * int64_t(kSortThreads) - 1) / (w.ctas * int64_t(kSortThreads))) * kSortThreads;
+  w.slices = (width + kSumSlice - 1) / kSumSlice;
+  // about 2048 chunks of a slice, of 16 tokens at least: enough warps, and few partial sums of a frequent row
+  w.chunk = static_cast<int>(std::max<int64_t>(16, (tokens + 2047) / 2048));
+  w.chunks = (tokens + w.chunk - 1) / w.chunk;
+  size_t at = 0;
+  const auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 15) & ~size_t(15);
+    return here;
+  };
+  for (int i = 0; i < 2; ++i) {
+    w.key[i] = take(sizeof(uint32_t) * static_cast<size_t>(tokens));
+    w.pos[i] = take(sizeof(uint32_t) * static_cast<size_t>(tokens));
+  }
+  w.counts = take(sizeof(uint32_t) * static_cast<size_t>(w.ctas) << w.bits);
+  w.row_start = take(sizeof(uint32_t) * static_cast<size_t>(vocab + 1));
+  w.head = take(sizeof(float) * static_cast<size_t>(w.chunks) * width);
+  w.tail = take(sizeof(float) * static_cast<size_t>(w.chunks) * width);
+  w.bytes = at;
+  return w;
+}
+
+}  // namespace
+
 static int embed_check(const void* ids, int ids64, int64_t tokens, int64_t vocab, int width, int weight_dtype,
                        int out_dtype) {
   FP8_REQUIRE(tokens >= 0 && vocab > 0 && width > 0, FP8_ERR_INVALID_ARGUMENT,
@@ -393,10 +436,14 @@ int fp8_embedding_fwd(const void* ids, int ids64, int64_t tokens, const void* we
   p.width = width;
   p.scale = scale;
   p.err = st->err_ptr;
+  const bool vec = width % 8 == 0 && weight_stride % 8 == 0 && aligned(weight, 16) && aligned(out, 16);
   const int status = with_dtype(weight_dtype, [&](auto w) {
     return with_dtype(out_dtype, [&](auto o) {
-      FP8_CUDA_TRY(launch_kernel(embed_fwd_kernel<decltype(w), decltype(o)>, dim3(grid_for(tokens, 8, st->sm_count, 8)),
-                                 dim3(256), 0, cuda_stream(stream), 1, kStreamingKernel, p));
+      using TW = decltype(w);
+      using TO = decltype(o);
+      FP8_CUDA_TRY(launch_kernel(vec ? embed_fwd_kernel<TW, TO, true> : embed_fwd_kernel<TW, TO, false>,
+                                 dim3(grid_for(tokens, 8, st->sm_count, 8)), dim3(256), 0, cuda_stream(stream), 1,
+                                 kStreamingKernel, p));
       return FP8_OK;
     });
   });
@@ -405,7 +452,10 @@ int fp8_embedding_fwd(const void* ids, int ids64, int64_t tokens, const void* we
   return ok();
 }
 
-size_t fp8_embedding_bwd_workspace_bytes(int64_t, int64_t, int) { return 0; }
+size_t fp8_embedding_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int width) {
+  if (tokens < 0 || vocab <= 0 || width <= 0) return 0;
+  return embed_plan(tokens, vocab, width).bytes;
+}
 
 int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* dout, int out_dtype, void* dweight,
                       int weight_dtype, int64_t vocab, int width, float scale, int64_t padding_idx, void* workspace,
@@ -414,32 +464,80 @@ int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* do
   FP8_REQUIRE((tokens == 0 || dout) && dweight && aligned(dweight, dtype_size(weight_dtype)) &&
                   aligned(dout, dtype_size(out_dtype)),
               FP8_ERR_INVALID_ARGUMENT, "embedding backward: dout or dweight is NULL or misaligned");
-  FP8_REQUIRE(workspace_bytes >= fp8_embedding_bwd_workspace_bytes(tokens, vocab, width), FP8_ERR_WORKSPACE,
-              "embedding backward: workspace too small");
-  (void)workspace;
+  FP8_REQUIRE(tokens < (1ll << 31) - (1 << 20) && vocab < (1ll << 31) - 1, FP8_ERR_UNSUPPORTED,
+              "embedding backward: too many tokens (%lld) or rows (%lld)", (long long)tokens, (long long)vocab);
+  const EmbedPlan w = embed_plan(tokens, vocab, width);
+  FP8_REQUIRE(workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= w.bytes, FP8_ERR_WORKSPACE,
+              "embedding backward: workspace too small or not 16-byte aligned (%zu bytes, needs %zu)", workspace_bytes,
+              w.bytes);
   DeviceState* st = nullptr;
   if (int s = device_state(&st)) return s;
-  EmbedParams p{};
-  p.ids = ids;
-  p.ids64 = ids64;
-  p.dout = dout;
-  p.dweight = dweight;
-  p.tokens = tokens;
-  p.vocab = vocab;
-  p.padding_idx = padding_idx;
-  p.width = width;
-  p.scale = scale;
-  p.err = st->err_ptr;
-  const int status = with_dtype(weight_dtype, [&](auto w) {
-    return with_dtype(out_dtype, [&](auto o) {
-      FP8_CUDA_TRY(launch_kernel(embed_bwd_simple_kernel<decltype(w), decltype(o)>,
-                                 dim3(grid_for(vocab, 8, st->sm_count, 8)), dim3(256), 0, cuda_stream(stream), 1,
-                                 kStreamingKernel, p));
+  char* const ws = static_cast<char*>(workspace);
+  EmbedSortParams so{};
+  so.ids = ids;
+  so.ids64 = ids64;
+  so.vocab = vocab;
+  so.padding_idx = padding_idx;
+  so.tokens = static_cast<int>(tokens);
+  so.passes = w.passes;
+  so.bits = w.bits;
+  so.per_cta = w.per_cta;
+  so.per_warp = w.per_cta / kSortWarps;
+  for (int i = 0; i < 2; ++i) {
+    so.key[i] = reinterpret_cast<uint32_t*>(ws + w.key[i]);
+    so.pos[i] = reinterpret_cast<uint32_t*>(ws + w.pos[i]);
+  }
+  so.counts = reinterpret_cast<uint32_t*>(ws + w.counts);
+  so.row_start = reinterpret_cast<uint32_t*>(ws + w.row_start);
+  so.arrive = fold_counter(st);
+  so.depart = fold_counter(st);
+  so.err = st->err_ptr;
+  const size_t smem = sizeof(uint32_t) * ((kSortWarps + 1) * (size_t(1) << w.bits) + kSortWarps);
+  FP8_CUDA_TRY(cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(w.ctas));
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = cuda_stream(stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeCooperative;  // the CTAs meet between the passes: all resident
+  at[0].val.cooperative = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = w.ctas > 1 ? 1u : 0u;
+  FP8_CUDA_TRY(cudaLaunchKernelEx(&cfg, embed_sort_kernel, so));
+
+  EmbedSumParams su{};
+  su.key = so.key[(w.passes + 1) & 1];
+  su.pos = so.pos[(w.passes + 1) & 1];
+  su.row_start = so.row_start;
+  su.dout = dout;
+  su.dweight = dweight;
+  su.head = reinterpret_cast<float*>(ws + w.head);
+  su.tail = reinterpret_cast<float*>(ws + w.tail);
+  su.vocab = vocab;
+  su.chunk = w.chunk;
+  su.slices = w.slices;
+  su.width = width;
+  su.scale = scale;
+  const bool vec = width % 8 == 0 && aligned(dout, 16) && aligned(dweight, 16);
+  const int64_t joins = w.chunks * w.slices;
+  const int status = with_dtype(weight_dtype, [&](auto wt) {
+    using TW = decltype(wt);
+    const int s = with_dtype(out_dtype, [&](auto o) {
+      using TO = decltype(o);
+      FP8_CUDA_TRY(launch_kernel(vec ? embed_sum_kernel<TW, TO, true> : embed_sum_kernel<TW, TO, false>,
+                                 dim3(grid_for(std::max(joins, vocab), 8, st->sm_count, 8)), dim3(256), 0,
+                                 cuda_stream(stream), 1, kStreamingKernel, su));
       return FP8_OK;
     });
+    if (s || joins == 0) return s;
+    FP8_CUDA_TRY(launch_kernel(vec ? embed_join_kernel<TW, true> : embed_join_kernel<TW, false>,
+                               dim3(grid_for(joins, 8, st->sm_count, 8)), dim3(256), 0, cuda_stream(stream), 1,
+                               kStreamingKernel, su));
+    return FP8_OK;
   });
   if (status) return status;
-  count_launches(1);
+  count_launches(joins > 0 ? 3 : 2);
   return ok();
 }
 
@@ -464,8 +562,12 @@ int fp8_dropout(const void* x, const void* residual, void* y, int dtype, int64_t
   d.thresh = static_cast<uint32_t>(std::lrint(p * 65536.0));
   d.scale = p < 1.0 ? static_cast<float>(1.0 / (1.0 - p)) : 0.0f;
   const int status = with_dtype(dtype, [&](auto t) {
-    FP8_CUDA_TRY(launch_kernel(dropout_kernel<decltype(t)>, dim3(grid_for(n, 8 * kDropoutThreads, st->sm_count, 8)),
-                               dim3(kDropoutThreads), 0, cuda_stream(stream), 1, kStreamingKernel, d));
+    using T = decltype(t);
+    const bool vec = aligned(x, 16) && aligned(y, 16) && aligned(residual, 16);
+    const auto kernel = residual ? (vec ? dropout_kernel<T, true, true> : dropout_kernel<T, false, true>)
+                                 : (vec ? dropout_kernel<T, true, false> : dropout_kernel<T, false, false>);
+    FP8_CUDA_TRY(launch_kernel(kernel, dim3(grid_for(n, 8 * kDropoutThreads, st->sm_count, 8)), dim3(kDropoutThreads), 0,
+                               cuda_stream(stream), 1, kStreamingKernel, d));
     return FP8_OK;
   });
   if (status) return status;

@@ -36,8 +36,7 @@ __device__ int g_fp8_device_error = 0;
 // launch that folds gets the next counter of the ring, so launches that can run
 // at the same time (other streams) use different counters unless more than
 // kFoldCounters folding launches were issued between them.
-constexpr int kFoldCounters = 8192;
-__device__ unsigned int g_fold_counters[kFoldCounters];
+__device__ unsigned int g_fold_counters[fp8host::kFoldCounters];
 
 namespace fp8host {
 
@@ -115,11 +114,6 @@ int get_encode_fn(EncodeTiledFn* out) {
 using namespace fp8host;
 
 namespace {
-
-// The counter of the next launch that folds a scale in its last CTA.
-unsigned int* fold_counter(DeviceState* st) {
-  return st->fold_base + st->fold_next.fetch_add(1, std::memory_order_relaxed) % kFoldCounters;
-}
 
 // ------------------------------------------------------------------ TMA tensor maps
 // 2-D byte matrix [rows][cols] (cols contiguous), box = 128 bytes x box_rows, 128B swizzle.

@@ -38,7 +38,7 @@ void count_launches(unsigned n);
 struct DeviceState {
   int sm_count = 0;
   int* err_ptr = nullptr;             // device error word
-  unsigned int* fold_base = nullptr;  // g_fold_counters on this device
+  unsigned int* fold_base = nullptr;  // the device's counters (fold_counter)
   std::atomic<unsigned int> fold_next{0};
   // Set (release) after the fields above are written; a reader that sees it
   // (acquire) sees them too.
@@ -47,6 +47,13 @@ struct DeviceState {
 
 // The current device's state.
 int device_state(DeviceState** out);
+
+// Counters in device memory that a launch's CTAs meet at, zero between launches.
+constexpr int kFoldCounters = 8192;
+// The counter of the next launch that folds a scale in its last CTA, or holds a grid barrier.
+inline unsigned int* fold_counter(DeviceState* st) {
+  return st->fold_base + st->fold_next.fetch_add(1, std::memory_order_relaxed) % kFoldCounters;
+}
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
