@@ -371,7 +371,7 @@ struct EmbedPlan {
   int passes, bits, ctas, per_cta;
   int chunk, slices;
   int64_t chunks;
-  size_t key[2], pos[2], counts, row_start, head, tail, bytes;
+  size_t key[2], pos[2], counts, live, present, head, tail, bytes;
 };
 EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
   EmbedPlan w{};
@@ -379,8 +379,9 @@ EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
   while ((int64_t(1) << need) <= vocab) ++need;
   w.passes = (need + kSortMaxBits - 1) / kSortMaxBits;
   w.bits = (need + w.passes - 1) / w.passes;
-  // at least 2048 tokens a CTA: with fewer the passes' barriers cost more than the tokens
-  w.ctas = static_cast<int>(std::min<int64_t>(kSortMaxCtas, std::max<int64_t>(1, (tokens + 2047) / 2048)));
+  // One CTA, without barriers between CTAs, up to 16384 tokens; then 4096 a CTA: with fewer the barriers cost more
+  // than the tokens.
+  w.ctas = tokens <= 16384 ? 1 : static_cast<int>(std::min<int64_t>(kSortMaxCtas, (tokens + 4095) / 4096));
   w.per_cta = static_cast<int>((tokens + w.ctas * int64_t(kSortThreads) - 1) / (w.ctas * int64_t(kSortThreads))) * kSortThreads;
   w.slices = (width + kSumSlice - 1) / kSumSlice;
   // about 2048 chunks of a slice, of 16 tokens at least: enough warps, and few partial sums of a frequent row
@@ -397,7 +398,8 @@ EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
     w.pos[i] = take(sizeof(uint32_t) * static_cast<size_t>(tokens));
   }
   w.counts = take(sizeof(uint32_t) * static_cast<size_t>(w.ctas) << w.bits);
-  w.row_start = take(sizeof(uint32_t) * static_cast<size_t>(vocab + 1));
+  w.live = take(sizeof(uint32_t));
+  w.present = take(sizeof(uint32_t) * static_cast<size_t>(vocab / 32 + 1));
   w.head = take(sizeof(float) * static_cast<size_t>(w.chunks) * width);
   w.tail = take(sizeof(float) * static_cast<size_t>(w.chunks) * width);
   w.bytes = at;
@@ -488,7 +490,8 @@ int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* do
     so.pos[i] = reinterpret_cast<uint32_t*>(ws + w.pos[i]);
   }
   so.counts = reinterpret_cast<uint32_t*>(ws + w.counts);
-  so.row_start = reinterpret_cast<uint32_t*>(ws + w.row_start);
+  so.live = reinterpret_cast<uint32_t*>(ws + w.live);
+  so.present = reinterpret_cast<uint32_t*>(ws + w.present);
   so.arrive = fold_counter(st);
   so.depart = fold_counter(st);
   so.err = st->err_ptr;
@@ -509,7 +512,8 @@ int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* do
   EmbedSumParams su{};
   su.key = so.key[(w.passes + 1) & 1];
   su.pos = so.pos[(w.passes + 1) & 1];
-  su.row_start = so.row_start;
+  su.live = so.live;
+  su.present = so.present;
   su.dout = dout;
   su.dweight = dweight;
   su.head = reinterpret_cast<float*>(ws + w.head);
@@ -526,14 +530,13 @@ int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* do
     const int s = with_dtype(out_dtype, [&](auto o) {
       using TO = decltype(o);
       FP8_CUDA_TRY(launch_kernel(vec ? embed_sum_kernel<TW, TO, true> : embed_sum_kernel<TW, TO, false>,
-                                 dim3(grid_for(std::max(joins, vocab), 8, st->sm_count, 8)), dim3(256), 0,
+                                 dim3(grid_for(std::max(joins, vocab / 8 + 1), 8, st->sm_count, 8)), dim3(256), 0,
                                  cuda_stream(stream), 1, kStreamingKernel, su));
       return FP8_OK;
     });
     if (s || joins == 0) return s;
-    FP8_CUDA_TRY(launch_kernel(vec ? embed_join_kernel<TW, true> : embed_join_kernel<TW, false>,
-                               dim3(grid_for(joins, 8, st->sm_count, 8)), dim3(256), 0, cuda_stream(stream), 1,
-                               kStreamingKernel, su));
+    FP8_CUDA_TRY(launch_kernel(embed_join_kernel<TW>, dim3(grid_for(2 * joins, 8, st->sm_count, 8)), dim3(256), 0,
+                               cuda_stream(stream), 1, kStreamingKernel, su));
     return FP8_OK;
   });
   if (status) return status;

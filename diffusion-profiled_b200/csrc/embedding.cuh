@@ -10,7 +10,7 @@
 // Gradient, three launches:
 //   1. embed_sort_kernel sorts (id, position) by id, stably, in radix passes of up to 9
 //      bits inside one cooperative launch (a token's key is its id; padding and ids out of
-//      range take the key `vocab`, behind all others), and finds each row's first place;
+//      range take the key `vocab`, behind all others), and marks the rows that occur;
 //   2. embed_sum_kernel sums the gradient rows in that order.  The sorted tokens are cut
 //      into chunks of equal length whatever the ids, so that a token that is half of the
 //      batch is summed by many warps; a row whose tokens lie in one chunk is written at
@@ -47,37 +47,55 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int ids64, int64_t i
 }
 
 // ============================================================================ lookup
-// One warp per token; VEC: rows of whole 16-byte words (width % 8 == 0, aligned).
+// A warp takes two tokens a step, so that two rows' loads are in flight; VEC: rows of whole 16-byte words (width % 8
+// == 0, aligned).
 template <typename TW, typename TO, bool VEC>
 __global__ void __launch_bounds__(256) embed_fwd_kernel(const EmbedParams p) {
   pdl_sync();
   const int lane = threadIdx.x & 31;
   const int64_t warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; i < p.tokens; i += warps) {
-    const int64_t id = load_id(p.ids, p.ids64, i);
-    const bool valid = id >= 0 && id < p.vocab;
-    if (!valid && lane == 0) record_error(p.err, kErrTokenRange);
-    const TW* w = static_cast<const TW*>(p.weight) + (valid ? id : 0) * p.weight_stride;
-    TO* o = static_cast<TO*>(p.out) + i * p.width;
+  constexpr int kTokens = 2;
+  for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; i0 < p.tokens;
+       i0 += kTokens * warps) {
+    const TW* w[kTokens];
+    TO* o[kTokens];
+    bool there[kTokens], valid[kTokens];
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+      const int64_t i = i0 + t * warps;
+      there[t] = i < p.tokens;
+      const int64_t id = there[t] ? load_id(p.ids, p.ids64, i) : 0;
+      valid[t] = id >= 0 && id < p.vocab;
+      if (!valid[t] && lane == 0) record_error(p.err, kErrTokenRange);
+      w[t] = static_cast<const TW*>(p.weight) + (valid[t] ? id : 0) * p.weight_stride;
+      o[t] = static_cast<TO*>(p.out) + (there[t] ? i : 0) * p.width;
+    }
     if constexpr (VEC) {
-      constexpr int kAtOnce = 4;  // 1024 channels' loads in flight
+      constexpr int kAtOnce = 2;  // 512 channels of each token
       for (int c0 = lane * 8; c0 < p.width; c0 += 256 * kAtOnce) {
-        Words8<TW> v[kAtOnce];
+        Words8<TW> v[kTokens][kAtOnce];
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u)
-          if (c0 + 256 * u < p.width) v[u] = load_words8(w + c0 + 256 * u);
+        for (int t = 0; t < kTokens; ++t)
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u)
-          if (c0 + 256 * u < p.width) {
-            float f[8];
-            widen8(v[u], f);
+          for (int u = 0; u < kAtOnce; ++u)
+            if (there[t] && c0 + 256 * u < p.width) v[t][u] = load_words8(w[t] + c0 + 256 * u);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] = valid ? f[k] * p.scale : 0.0f;
-            store8(o + c0 + 256 * u, f);
-          }
+        for (int t = 0; t < kTokens; ++t)
+#pragma unroll
+          for (int u = 0; u < kAtOnce; ++u)
+            if (there[t] && c0 + 256 * u < p.width) {
+              float f[8];
+              widen8(v[t][u], f);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) f[k] = valid[t] ? f[k] * p.scale : 0.0f;
+              store8(o[t] + c0 + 256 * u, f);
+            }
       }
     } else {
-      for (int c = lane; c < p.width; c += 32) o[c] = from_f32<TO>(valid ? to_f32(w[c]) * p.scale : 0.0f);
+#pragma unroll
+      for (int t = 0; t < kTokens; ++t)
+        if (there[t])
+          for (int c = lane; c < p.width; c += 32) o[t][c] = from_f32<TO>(valid[t] ? to_f32(w[t][c]) * p.scale : 0.0f);
     }
   }
 }
@@ -87,6 +105,7 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortMaxBits = 9;  // 512 digits: one count a warp and digit fits shared memory (64 KB)
 constexpr int kSortMaxCtas = 64;
+constexpr int kSortAhead = 8;    // steps of 32 tokens whose keys are loaded together
 
 struct EmbedSortParams {
   const void* ids;
@@ -98,18 +117,30 @@ struct EmbedSortParams {
   uint32_t* key[2];
   uint32_t* pos[2];
   uint32_t* counts;        // [gridDim.x][1 << bits]
-  uint32_t* row_start;     // [vocab + 1]: first place whose key is at least the row
+  uint32_t* live;          // number of keys below vocab
+  uint32_t* present;       // bit v: row v occurs; [vocab / 32 + 1] words
   unsigned int *arrive, *depart;  // zero between launches
   int* err;
 };
+
+// The lanes whose digit (of `bits` bits) is this lane's, among the lanes with `in` (one vote a bit: a quarter of the
+// time of a match instruction over 32 different digits).
+__device__ __forceinline__ unsigned same_digit(uint32_t d, int bits, bool in) {
+  unsigned same = __ballot_sync(~0u, in);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned ones = __ballot_sync(~0u, (d >> b) & 1u);
+    same &= (d >> b) & 1u ? ones : ~ones;
+  }
+  return same;
+}
 
 // All CTAs' writes so far are visible to all.  `round` counts the barriers of the launch from 1.
 __device__ __forceinline__ bool sort_barrier(const EmbedSortParams& p, unsigned int round) {
   __shared__ int passed;
   __syncthreads();
+  if (gridDim.x == 1) return true;
   if (threadIdx.x == 0) {
-    __threadfence();
-    red_release_gpu_add_u32(p.arrive, 1u);
+    red_release_gpu_add_u32(p.arrive, 1u);  // with what the CTA's other threads wrote before the barrier above
     const uint64_t t0 = globaltimer_ns();
     int ok = 1;
     while (ld_acquire_gpu_u32(p.arrive) < round * gridDim.x) {
@@ -119,7 +150,6 @@ __device__ __forceinline__ bool sort_barrier(const EmbedSortParams& p, unsigned 
         break;
       }
     }
-    __threadfence();
     passed = ok;
   }
   __syncthreads();
@@ -138,6 +168,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
   const int end = min(min(p.tokens, (static_cast<int>(blockIdx.x) + 1) * p.per_cta), begin + p.per_warp);
   uint32_t* mine = warp_count + warp * digits;
   unsigned int round = 0;
+  const int64_t all = static_cast<int64_t>(gridDim.x) * kSortThreads, me = static_cast<int64_t>(blockIdx.x) * kSortThreads + tid;
+  for (int64_t w = me; w <= p.vocab / 32; w += all) p.present[w] = 0;  // set after the passes' barriers
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * p.bits;
     const uint32_t* key_in = p.key[(pass + 1) & 1];
@@ -152,13 +184,19 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
     // ---- this warp's count of each digit over its own stretch of tokens
     for (int d = lane; d < digits; d += 32) mine[d] = 0;
     __syncwarp();
-    for (int i0 = begin; i0 < end; i0 += 32) {
-      const int i = i0 + lane;
-      const bool in = i < end;
-      const uint32_t d = in ? (key_of(i) >> shift) & (digits - 1) : ~0u;
-      const unsigned same = __match_any_sync(~0u, d);
-      if (in && (same & ((1u << lane) - 1)) == 0) mine[d] += __popc(same);
-      __syncwarp();
+    for (int i0 = begin; i0 < end; i0 += 32 * kSortAhead) {
+      uint32_t key[kSortAhead];
+#pragma unroll
+      for (int u = 0; u < kSortAhead; ++u) key[u] = i0 + 32 * u + lane < end ? key_of(i0 + 32 * u + lane) : 0u;
+#pragma unroll
+      for (int u = 0; u < kSortAhead; ++u) {
+        if (i0 + 32 * u >= end) break;
+        const bool in = i0 + 32 * u + lane < end;
+        const uint32_t d = (key[u] >> shift) & (digits - 1);
+        const unsigned same = same_digit(d, p.bits, in);
+        if (in && (same & ((1u << lane) - 1)) == 0) mine[d] += __popc(same);
+        __syncwarp();
+      }
     }
     __syncthreads();
     // ---- the CTA's count, and each warp's place among the CTA's tokens of the digit
@@ -202,39 +240,54 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
     if (tid < digits) base[tid] = (warp > 0 ? scan[warp - 1] : 0u) + incl - total + before;
     __syncthreads();
     // ---- to their places, in order
-    for (int i0 = begin; i0 < end; i0 += 32) {
-      const int i = i0 + lane;
-      const bool in = i < end;
-      const uint32_t key = in ? key_of(i) : 0u;
-      const uint32_t d = in ? (key >> shift) & (digits - 1) : ~0u;
-      const unsigned same = __match_any_sync(~0u, d);
-      const int rank = __popc(same & ((1u << lane) - 1));
-      if (in) {
-        const uint32_t to = base[d] + mine[d] + rank;
-        key_out[to] = key;
-        pos_out[to] = pass > 0 ? __ldcg(pos_in + i) : static_cast<uint32_t>(i);
+    for (int i0 = begin; i0 < end; i0 += 32 * kSortAhead) {
+      uint32_t key[kSortAhead], pos[kSortAhead];
+#pragma unroll
+      for (int u = 0; u < kSortAhead; ++u) {
+        const int i = i0 + 32 * u + lane;
+        key[u] = i < end ? key_of(i) : 0u;
+        pos[u] = pass > 0 && i < end ? __ldcg(pos_in + i) : static_cast<uint32_t>(i);
       }
-      __syncwarp();
-      if (in && rank == 0) mine[d] += __popc(same);
-      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < kSortAhead; ++u) {
+        if (i0 + 32 * u >= end) break;
+        const bool in = i0 + 32 * u + lane < end;
+        const uint32_t d = (key[u] >> shift) & (digits - 1);
+        const unsigned same = same_digit(d, p.bits, in);
+        const int rank = __popc(same & ((1u << lane) - 1));
+        if (in) {
+          const uint32_t to = base[d] + mine[d] + rank;
+          key_out[to] = key[u];
+          pos_out[to] = pos[u];
+        }
+        __syncwarp();
+        if (in && rank == 0) mine[d] += __popc(same);
+        __syncwarp();
+      }
     }
     if (!sort_barrier(p, ++round)) return;
   }
-  // ---- each row's first place, by bisection
+  // ---- the rows that occur: each where its key first does
   const uint32_t* key = p.key[(p.passes + 1) & 1];
-  for (int64_t v = static_cast<int64_t>(blockIdx.x) * kSortThreads + tid; v <= p.vocab;
-       v += static_cast<int64_t>(gridDim.x) * kSortThreads) {
-    int lo = 0, hi = p.tokens;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldcg(key + mid) < static_cast<uint32_t>(v)) lo = mid + 1;
-      else hi = mid;
+  for (int64_t i0 = me; i0 <= p.tokens; i0 += 4 * all) {
+    uint32_t k[4], before[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = i0 + u * all;
+      k[u] = i < p.tokens ? __ldcg(key + i) : static_cast<uint32_t>(p.vocab);
+      before[u] = i > 0 && i <= p.tokens ? __ldcg(key + i - 1) : ~0u;
     }
-    p.row_start[v] = static_cast<uint32_t>(lo);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = i0 + u * all;
+      if (i > p.tokens || (i > 0 && k[u] == before[u])) continue;
+      if (k[u] < p.vocab) atomicOr(p.present + (k[u] >> 5), 1u << (k[u] & 31));
+      else if (i == 0 || before[u] < p.vocab) *p.live = static_cast<uint32_t>(i);
+    }
   }
   // the last CTA to leave sets the counters back
   __syncthreads();
-  if (tid == 0 && atom_add_acq_rel_gpu_u32(p.depart, 1u) == gridDim.x - 1) {
+  if (gridDim.x > 1 && tid == 0 && atom_add_acq_rel_gpu_u32(p.depart, 1u) == gridDim.x - 1) {
     *p.arrive = 0u;
     *p.depart = 0u;
   }
@@ -244,7 +297,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
 constexpr int kSumSlice = 256;  // channels of a warp's work: 8 a lane
 
 struct EmbedSumParams {
-  const uint32_t *key, *pos, *row_start;  // sorted; rows' first places [vocab + 1]
+  const uint32_t *key, *pos;  // sorted
+  const uint32_t *live, *present;
   const void* dout;
   void* dweight;
   float *head, *tail;  // [chunks][width]: sums of the row that began before the chunk / that goes on after it
@@ -260,23 +314,24 @@ template <bool VEC>
 __device__ __forceinline__ int slice_channel(int slice, int lane, int k) {
   return slice * kSumSlice + (VEC ? lane * 8 + k : k * 32 + lane);
 }
+// The 8 channels as loaded (widened only when they are added: loads in flight take half the registers).
 template <typename T, bool VEC>
-__device__ __forceinline__ void slice_load(const T* row, int slice, int lane, int width, float (&f)[8]) {
+__device__ __forceinline__ Words8<T> slice_load(const T* row, int slice, int lane, int width) {
+  Words8<T> v;
   if constexpr (VEC) {
     const int c = slice_channel<true>(slice, lane, 0);
-    if (c < width) {
-      widen8(load_words8(row + c), f);
-      return;
-    }
+    if (c < width) return load_words8(row + c);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = 0.0f;
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) v.w[i] = make_uint4(0, 0, 0, 0);
   } else {
+    T* t = reinterpret_cast<T*>(&v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int c = slice_channel<false>(slice, lane, k);
-      f[k] = c < width ? to_f32(row[c]) : 0.0f;
+      t[k] = c < width ? row[c] : from_f32<T>(0.0f);
     }
   }
+  return v;
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void slice_store(T* row, int slice, int lane, int width, const float (&f)[8]) {
@@ -298,7 +353,7 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedSumParams p) 
   const int lane = threadIdx.x & 31;
   const int64_t warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
   const int64_t me = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int live = static_cast<int>(p.row_start[p.vocab]);  // padding and ids out of range lie behind
+  const int live = static_cast<int>(*p.live);  // padding and ids out of range lie behind
   const int64_t sums = static_cast<int64_t>((live + p.chunk - 1) / p.chunk) * p.slices;
   const TO* dout = static_cast<const TO*>(p.dout);
   TW* dw = static_cast<TW*>(p.dweight);
@@ -319,21 +374,30 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedSumParams p) 
         slice_store<TW, VEC>(dw + static_cast<int64_t>(row) * p.width, slice, lane, p.width, f);
       }
     };
-    for (int p0 = begin; p0 < end; p0 += 32) {
-      const int n = min(32, end - p0);
-      const uint32_t my_key = lane < n ? p.key[p0 + lane] : 0u, my_pos = lane < n ? p.pos[p0 + lane] : 0u;
-      constexpr int kAtOnce = 4;  // rows in flight
-      for (int u0 = 0; u0 < n; u0 += kAtOnce) {
-        float f[kAtOnce][8];
+    // Batches of kAtOnce rows; the next batch's loads are under way while this one is added.
+    constexpr int kAtOnce = 4;
+    Words8<TO> rows[2][kAtOnce];
+    uint32_t my_key = 0, my_pos = 0;
+    const auto fetch = [&](int at, Words8<TO>(&to)[kAtOnce]) {
+      if (((at - begin) & 31) == 0 && at < end) my_pos = at + lane < end ? p.pos[at + lane] : 0u;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const uint32_t pos = __shfl_sync(~0u, my_pos, (at - begin + u) & 31);
+        if (at + u < end) to[u] = slice_load<TO, VEC>(dout + static_cast<int64_t>(pos) * p.width, slice, lane, p.width);
+      }
+    };
+    fetch(begin, rows[0]);
+    for (int at0 = begin; at0 < end; at0 += 2 * kAtOnce)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int at = at0 + half * kAtOnce;
+        if (at >= end) break;
+        if (((at - begin) & 31) == 0) my_key = at + lane < end ? p.key[at + lane] : 0u;
+        fetch(at + kAtOnce, rows[1 - half]);
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
-          const uint32_t pos = __shfl_sync(~0u, my_pos, (u0 + u) & 31);
-          if (u0 + u < n) slice_load<TO, VEC>(dout + static_cast<int64_t>(pos) * p.width, slice, lane, p.width, f[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-          const uint32_t key = __shfl_sync(~0u, my_key, (u0 + u) & 31);
-          if (u0 + u >= n) continue;
+          const uint32_t key = __shfl_sync(~0u, my_key, (at - begin + u) & 31);
+          if (at + u >= end) continue;
           if (key != row) {
             flush(false);
             row = key;
@@ -341,53 +405,73 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedSumParams p) 
 #pragma unroll
             for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
           }
+          float f[8];
+          widen8(rows[half][u], f);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) acc[k] += f[u][k];
+          for (int k = 0; k < 8; ++k) acc[k] += f[k];
         }
       }
-    }
     flush(end < live && p.key[end] == row);
   }
-  // rows without tokens
-  for (int64_t v = me; v < p.vocab; v += warps) {
-    if (p.row_start[v] != p.row_start[v + 1]) continue;
+  // rows without tokens, 8 rows a warp and step
+  for (int64_t v0 = me * 8; v0 < p.vocab; v0 += warps * 8) {
+    uint32_t absent = ~(p.present[v0 >> 5] >> (v0 & 31)) & 0xffu;
+    if (p.vocab - v0 < 8) absent &= (1u << (p.vocab - v0)) - 1;
     const float zero[8] = {};
-    for (int slice = 0; slice < p.slices; ++slice) slice_store<TW, VEC>(dw + v * p.width, slice, lane, p.width, zero);
+    while (absent) {
+      const int64_t v = v0 + __ffs(absent) - 1;
+      absent &= absent - 1;
+      for (int slice = 0; slice < p.slices; ++slice) slice_store<TW, VEC>(dw + v * p.width, slice, lane, p.width, zero);
+    }
   }
 }
 
-// Rows that cross chunks: the partial sum of the chunk the row begins in, then those of the chunks it goes on in.
-template <typename TW, bool VEC>
+// Rows that cross chunks: the partial sum of the chunk the row begins in, then those of the chunks it goes on in.  A
+// warp takes 128 channels (4 a lane), 16 partial sums in flight: a row that is a twentieth of a long batch has over a
+// hundred.
+constexpr int kJoinSlice = 128;
+template <typename TW>
 __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedSumParams p) {
   pdl_sync();
   const int lane = threadIdx.x & 31;
   const int64_t warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
-  const int live = static_cast<int>(p.row_start[p.vocab]);
-  const int64_t items = static_cast<int64_t>((live + p.chunk - 1) / p.chunk) * p.slices;
+  const int live = static_cast<int>(*p.live);
+  const int slices = (p.width + kJoinSlice - 1) / kJoinSlice;
+  const int64_t items = static_cast<int64_t>((live + p.chunk - 1) / p.chunk) * slices;
   for (int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; item < items; item += warps) {
-    const int chunk = static_cast<int>(item / p.slices), slice = static_cast<int>(item % p.slices);
-    const int end = (chunk + 1) * p.chunk;
+    const int chunk = static_cast<int>(item / slices), c0 = static_cast<int>(item % slices) * kJoinSlice + lane;
+    const int begin = chunk * p.chunk, end = begin + p.chunk;
     if (end >= live) continue;
     const uint32_t row = p.key[end];
-    if (p.key[end - 1] != row || static_cast<int>(p.row_start[row]) < chunk * p.chunk) continue;  // ends here, or began before
-    const int last = (static_cast<int>(p.row_start[row + 1]) - 1) / p.chunk;
-    float acc[8];
-    slice_load<float, VEC>(p.tail + static_cast<int64_t>(chunk) * p.width, slice, lane, p.width, acc);
-    constexpr int kAtOnce = 4;
-    for (int c0 = chunk + 1; c0 <= last; c0 += kAtOnce) {
-      float f[kAtOnce][8];
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u)
-        if (c0 + u <= last) slice_load<float, VEC>(p.head + static_cast<int64_t>(c0 + u) * p.width, slice, lane, p.width, f[u]);
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u)
-        if (c0 + u <= last)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) acc[k] += f[u][k];
+    if (p.key[end - 1] != row || (begin > 0 && p.key[begin - 1] == row)) continue;  // ends here, or began before
+    int last = chunk;  // the last chunk that begins with the row: 32 are looked at at a time
+    for (unsigned more = ~0u; more == ~0u; last += __popc(more)) {
+      const int64_t at = (static_cast<int64_t>(last) + 1 + lane) * p.chunk;
+      more = __ballot_sync(~0u, at < live && p.key[at] == row);
     }
+    const auto part = [&](const float* from, int of, float(&f)[4]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) acc[k] *= p.scale;
-    slice_store<TW, VEC>(static_cast<TW*>(p.dweight) + static_cast<int64_t>(row) * p.width, slice, lane, p.width, acc);
+      for (int k = 0; k < 4; ++k)
+        f[k] = c0 + 32 * k < p.width ? from[static_cast<int64_t>(of) * p.width + c0 + 32 * k] : 0.0f;
+    };
+    float acc[4];
+    part(p.tail, chunk, acc);
+    constexpr int kAtOnce = 16;
+    for (int of = chunk + 1; of <= last; of += kAtOnce) {
+      float f[kAtOnce][4];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (of + u <= last) part(p.head, of + u, f[u]);
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (of + u <= last)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[k] += f[u][k];
+    }
+    TW* to = static_cast<TW*>(p.dweight) + static_cast<int64_t>(row) * p.width;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c0 + 32 * k < p.width) to[c0 + 32 * k] = from_f32<TW>(acc[k] * p.scale);
   }
 }
 
