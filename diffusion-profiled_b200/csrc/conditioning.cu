@@ -379,9 +379,9 @@ EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
   while ((int64_t(1) << need) <= vocab) ++need;
   w.passes = (need + kSortMaxBits - 1) / kSortMaxBits;
   w.bits = (need + w.passes - 1) / w.passes;
-  // One CTA, without barriers between CTAs, up to 16384 tokens; then 4096 a CTA: with fewer the barriers cost more
-  // than the tokens.
-  w.ctas = tokens <= 16384 ? 1 : static_cast<int>(std::min<int64_t>(kSortMaxCtas, (tokens + 4095) / 4096));
+  // One CTA, without barriers between CTAs, up to 2048 tokens; then 1024 a CTA, one step of each of its warps, while
+  // there are CTAs: a step of 32 tokens takes its warp about 100 instructions, and 32 warps share an SM's issue.
+  w.ctas = tokens <= 2048 ? 1 : static_cast<int>(std::min<int64_t>(kSortMaxCtas, (tokens + kSortThreads - 1) / kSortThreads));
   w.per_cta = static_cast<int>((tokens + w.ctas * int64_t(kSortThreads) - 1) / (w.ctas * int64_t(kSortThreads))) * kSortThreads;
   w.slices = (width + kSumSlice - 1) / kSumSlice;
   // about 2048 chunks of a slice, of 16 tokens at least: enough warps, and few partial sums of a frequent row

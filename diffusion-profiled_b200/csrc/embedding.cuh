@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const EmbedParams p) {
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortMaxBits = 9;  // 512 digits: one count a warp and digit fits shared memory (64 KB)
-constexpr int kSortMaxCtas = 64;
+constexpr int kSortMaxCtas = 96;
 constexpr int kSortAhead = 8;    // steps of 32 tokens whose keys are loaded together
 
 struct EmbedSortParams {
@@ -127,10 +127,13 @@ struct EmbedSortParams {
 // time of a match instruction over 32 different digits).
 __device__ __forceinline__ unsigned same_digit(uint32_t d, int bits, bool in) {
   unsigned same = __ballot_sync(~0u, in);
-  for (int b = 0; b < bits; ++b) {
-    const unsigned ones = __ballot_sync(~0u, (d >> b) & 1u);
-    same &= (d >> b) & 1u ? ones : ~ones;
-  }
+#pragma unroll
+  for (int b = 0; b < kSortMaxBits; ++b)
+    if (b < bits) {
+      const bool one = (d >> b) & 1u;
+      const unsigned ones = __ballot_sync(~0u, one);
+      same &= one ? ones : ~ones;
+    }
   return same;
 }
 
@@ -201,11 +204,13 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
     __syncthreads();
     // ---- the CTA's count, and each warp's place among the CTA's tokens of the digit
     if (tid < digits) {
-      uint32_t sum = 0;
+      uint32_t c[kSortWarps], sum = 0;
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) c[w] = warp_count[w * digits + tid];
+#pragma unroll
       for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t c = warp_count[w * digits + tid];
         warp_count[w * digits + tid] = sum;
-        sum += c;
+        sum += c[w];
       }
       p.counts[blockIdx.x * digits + tid] = sum;
     }
@@ -213,7 +218,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
     // ---- where the digit begins, and the tokens of the CTAs before this one in it
     uint32_t before = 0, total = 0;
     if (tid < digits)
-#pragma unroll 8
+#pragma unroll 16
       for (int c = 0; c < static_cast<int>(gridDim.x); ++c) {
         const uint32_t n = __ldcg(p.counts + c * digits + tid);
         before += c < static_cast<int>(blockIdx.x) ? n : 0u;
