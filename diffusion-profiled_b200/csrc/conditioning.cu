@@ -184,13 +184,12 @@ size_t x_fwd_workspace(const fp8_cross_attention_args* a, const XPlan& w) {
 }
 
 template <typename T, int HALVES, int NT>
-int x_fwd_launch(const XFwdParams& f, const CUtensorMap (&maps)[4], int64_t slots, cudaStream_t stream) {
+int x_fwd_launch(const XFwdParams& f, const CUtensorMap (&maps)[4], bool one_key_tile, int64_t slots, cudaStream_t stream) {
   using Ly = XFwdLayout<HALVES, NT>;
-  FP8_CUDA_TRY(cudaFuncSetAttribute(x_fwd_kernel<T, HALVES, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    Ly::kSmemBytes));
-  FP8_CUDA_TRY(launch_kernel(x_fwd_kernel<T, HALVES, NT>, dim3(static_cast<unsigned>(std::min<int64_t>(f.items, slots))),
-                             dim3(Ly::kThreads), Ly::kSmemBytes, stream, 1, kTensorKernel, f, maps[0], maps[1], maps[2],
-                             maps[3]));
+  const auto kernel = one_key_tile ? x_fwd_kernel<T, HALVES, NT, true> : x_fwd_kernel<T, HALVES, NT, false>;
+  FP8_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ly::kSmemBytes));
+  FP8_CUDA_TRY(launch_kernel(kernel, dim3(static_cast<unsigned>(std::min<int64_t>(f.items, slots))), dim3(Ly::kThreads),
+                             Ly::kSmemBytes, stream, 1, kTensorKernel, f, maps[0], maps[1], maps[2], maps[3]));
   count_launches(1);
   return FP8_OK;
 }
@@ -215,11 +214,11 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
   if (int s = x_map(&maps[1], a.k, dt, a.sk, a.batch, a.k_len, a.kv_heads, a.head_dim, 1, kXTile)) return s;
   if (int s = x_map(&maps[2], a.v, dt, a.sv, a.batch, a.k_len, a.kv_heads, a.head_dim, 1, kXTile)) return s;
   if (int s = x_map(&maps[3], a.o, dt, a.so, a.batch, a.q_len, a.heads, a.head_dim, a.pack, a.tile_tokens)) return s;
-  int status;
-  if (a.head_dim <= 64)
-    status = w.nt == 1 ? x_fwd_launch<T, 1, 1>(f, maps, w.slots, stream) : x_fwd_launch<T, 1, 2>(f, maps, w.slots, stream);
-  else
-    status = w.nt == 1 ? x_fwd_launch<T, 2, 1>(f, maps, w.slots, stream) : x_fwd_launch<T, 2, 2>(f, maps, w.slots, stream);
+  const bool one = w.n_tiles == 1;
+  const int status = a.head_dim <= 64 ? (w.nt == 1 ? x_fwd_launch<T, 1, 1>(f, maps, one, w.slots, stream)
+                                                   : x_fwd_launch<T, 1, 2>(f, maps, one, w.slots, stream))
+                                      : (w.nt == 1 ? x_fwd_launch<T, 2, 1>(f, maps, one, w.slots, stream)
+                                                   : x_fwd_launch<T, 2, 2>(f, maps, one, w.slots, stream));
   if (status) return status;
   if (w.splits > 1) {
     FP8_CUDA_TRY(launch_kernel(x_combine_kernel<T>, dim3(grid_for(w.rows, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,

@@ -15,22 +15,27 @@
 // values are read once for all of them and their gradients need no second sum.
 //
 // Forward (x_fwd_kernel): one pass over the keys with a running maximum and sum.
-//   * S = Q K^T of a 128-row, 128-key tile on tcgen05 kind::f16 into TMEM (fp32); one
-//     thread owns one row, reads it, and writes P (rounded to the tensors' type, the
-//     tensor cores' operand) over S in TMEM, where the second product O += P V takes
-//     it from;
+//   * S = Q K^T of 128 rows and 64 keys on tcgen05 kind::f16 into TMEM (fp32); one thread
+//     owns one row, reads its 64 scores, and writes P (rounded to the tensors' type, the
+//     tensor cores' operand) over them, where the second product O += P V takes it from;
+//   * two score buffers a row tile: the products of the next 64 keys run while the softmax
+//     of these does.  (With one buffer of 128 keys the softmax, P V and the next S are one
+//     chain: 4,770 cycles a pair of tiles at heads of 128 against 2,050 of products.)
+//     64 keys cost S a third of its rate (its operands' shared-memory reads), which the
+//     overlap more than returns;
 //   * the exponent's reference is the row's maximum so far, raised only when a score
 //     passes it by more than 2^8: then O and the sum are rescaled.  Scores that stay
 //     within that factor need no rescaling pass, and P <= 2^8 keeps its relative
 //     precision in bf16 and fp16;
-//   * with two row tiles a CTA, one's softmax runs while the other's products do; each
-//     has a warp of its own that issues its products (a product's issue takes about as
+//   * a warp of its own issues each row tile's products (a product's issue takes about as
 //     long as the product, so one warp that waits for two softmaxes in turn leaves the
 //     tensor cores idle meanwhile);
-//   * tiles with keys that are not kept: their rows of K and V are zeroed in shared
-//     memory before the products, and their scores are -inf.
+//   * keys that are not kept: their rows of K and V are zeroed in shared memory before the
+//     products, and their scores are -inf.
 // The sums and statistics are fp32; P is the one value rounded before a sum (it is a
-// matrix operand).
+// matrix operand).  Over many keys that rounding averages out against the output's own.
+// Where the states are at most one key tile (SPLIT) it would not, and the products are
+// cheap: there P goes in as the sum of two values of the type, P V = P_hi V + P_lo V.
 //
 // Every mbarrier wait is bounded (mbar_wait); on a timeout the kernel records the error
 // code, skips the remaining work and frees its tensor memory.
@@ -49,7 +54,7 @@ constexpr int kXTile = 128;  // rows of a query tile and keys of a key tile
 enum XError : int { kErrXForward = 300, kErrXDq = 320, kErrXDkv = 340 };
 enum XWait : int {
   kWaitQFree = 1, kWaitKFree, kWaitVFree, kWaitQ, kWaitK, kWaitV, kWaitS, kWaitSFree, kWaitDP, kWaitDPFree, kWaitP,
-  kWaitPRest, kWaitTurn, kWaitAcc, kWaitAccFree, kWaitStaged, kWaitDelta, kWaitDrain
+  kWaitPRest, kWaitPV, kWaitAcc, kWaitAccFree, kWaitStaged, kWaitDelta, kWaitDrain
 };
 
 struct XStrides {
@@ -97,6 +102,14 @@ struct XType<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 };
+
+// Two fp32 values as the sum of two pairs of T: hi = RN(x), lo = RN(x - hi).
+template <typename T>
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  hi = XType<T>::pack2(x0, x1);
+  const T* h = reinterpret_cast<const T*>(&hi);
+  lo = XType<T>::pack2(x0 - to_f32(h[0]), x1 - to_f32(h[1]));
+}
 
 // kind::f16 instruction descriptor for operands of type T, f32 accumulator, M = 128.
 template <typename T>
@@ -157,14 +170,31 @@ __device__ __forceinline__ void products_k_major(uint32_t d_tmem, uint64_t a, ui
   }
 }
 
-// 32 lanes x 16 columns, TMEM -> register.
-__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+// 32 lanes x 32 (16) columns, TMEM -> register, and the wait for them.  One statement, so that nothing can use the
+// registers before the wait, and nothing has to copy them after it (an empty statement that the registers pass through
+// in the wait's place cost a move a register: 2.6 of the forward's 7.6 instructions a score).
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
+      : "r"(taddr)
+      : "memory");
 }
 // 32 lanes x 16 columns, register -> TMEM.
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -187,21 +217,6 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ void after_wait(uint32_t (&r)[16]) {
-  asm volatile(""
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
-}
-// Makes the uses of r come after the asm statements before it (a tcgen05.wait::ld).
-__device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
-  asm volatile(""
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
-                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                 "+r"(r[30]), "+r"(r[31]));
-}
 
 // Tiled TMA store of a {channels, heads, tokens, batch} box.
 __device__ __forceinline__ void tma_store_4d(const void* tmap, const void* src, int c0, int c1, int c2, int c3) {
@@ -337,13 +352,14 @@ struct XFwdLayout {
   static constexpr int kQStages = HALVES == 2 ? 1 : NT == 2 ? 3 : 2;
   // key / value entries: as many as fit the CTA's share of the SM (two CTAs with NT = 1)
   static constexpr int kEntries = NT == 2 ? (HALVES == 1 ? 6 : 4) : (HALVES == 1 ? 4 : 2);
+  static constexpr int kWarps = 4 * NT;  // softmax warps
   static constexpr int kKV = NT * kTileBytes * kQStages;
   static constexpr int kWords = kKV + kEntries * kTileBytes;
   static constexpr int kBar = kWords + kXMaskSlots * 16;
-  static constexpr int kNumBars = 2 * kQStages + 2 * kEntries + 8 * NT;
+  static constexpr int kNumBars = 2 * kQStages + 2 * kEntries + 10 * NT;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;  // + alignment slack
-  static constexpr int kThreads = NT * 128 + 32 + NT * 32;  // softmax, loads, products of each row tile
+  static constexpr int kThreads = kWarps * 32 + 32 + NT * 32;  // softmax, loads, products of each row tile
   static constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
   static constexpr int kCtasPerSm = NT == 2 ? 1 : 2;
 };
@@ -385,10 +401,11 @@ struct XItems {
     return true;
   }
 };
-// 32-key chunks of key tile j that hold keys.
+// 32-key chunks of key tile j that hold keys, and of the 64 keys from u * 64.
 __device__ __forceinline__ int x_chunks(int keys, int j) { return (min(kXTile, keys - j * kXTile) + 31) >> 5; }
+__device__ __forceinline__ int x_chunks64(int keys, int u) { return (min(64, keys - u * 64) + 31) >> 5; }
 
-template <typename T, int HALVES, int NT>
+template <typename T, int HALVES, int NT, bool SPLIT>
 __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<HALVES, NT>::kCtasPerSm)
     x_fwd_kernel(const XFwdParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap o_map) {
@@ -400,14 +417,13 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
   uint64_t* q_empty = q_full + Ly::kQStages;
   uint64_t* kv_full = q_empty + Ly::kQStages;
   uint64_t* kv_empty = kv_full + Ly::kEntries;
-  uint64_t* s_full = kv_empty + Ly::kEntries;
-  uint64_t* p_full = s_full + NT;
-  uint64_t* o_full = p_full + NT;
+  uint64_t* s_full = kv_empty + Ly::kEntries;  // [NT][2], by score buffer
+  uint64_t* p_full = s_full + 2 * NT;          // [NT][2]: a warp may be a step ahead of another of its row tile
+  uint64_t* pv_done = p_full + 2 * NT;         // [NT][2]: a step's P V product is done
+  uint64_t* o_full = pv_done + 2 * NT;         // the item's last one is
   uint64_t* o_free = o_full + NT;
   uint64_t* staged = o_free + NT;
-  uint64_t* p_rest = staged + NT;
-  uint64_t* turn = p_rest + NT;
-  uint64_t* drained = turn + NT;
+  uint64_t* drained = staged + NT;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::kTail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -421,20 +437,21 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       mbar_init(kv_full + i, 1);
       mbar_init(kv_empty + i, NT);
     }
-    for (int i = 0; i < NT; ++i) {
+    for (int i = 0; i < 2 * NT; ++i) {
       mbar_init(s_full + i, 2);  // the products' commit, and the issuing thread (keep bits)
       mbar_init(p_full + i, 4);
+      mbar_init(pv_done + i, 1);
+    }
+    for (int i = 0; i < NT; ++i) {
       mbar_init(o_full + i, 1);
       mbar_init(o_free + i, 4);
       mbar_init(staged + i, 4);
-      mbar_init(p_rest + i, 4);
-      mbar_init(turn + i, 1);
       mbar_init(drained + i, 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 4 * NT) {
+  if (warp == Ly::kWarps) {
     tmem_alloc(tmem_slot, Ly::kTmemCols);
     tmem_relinquish();
   }
@@ -448,7 +465,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
   const bool masked = a.key_mask != nullptr;
   const int ksteps = (a.head_dim + 15) >> 4;  // 16-channel steps of Q K^T, and 16-column steps of P V's width
 
-  if (warp == 4 * NT) {
+  if (warp == Ly::kWarps) {
     // ------------------------------------------------------------ loads
     if (lane == 0) {
       tma_prefetch_desc(&q_map);
@@ -499,32 +516,17 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       volatile int never = 0;
       for (uint32_t k = loaded > Ly::kEntries ? loaded - Ly::kEntries : 0; k < loaded; ++k)
         mbar_wait(kv_full + k % Ly::kEntries, (k / Ly::kEntries) & 1, &never, a.err, kErrXForward + kWaitDrain);
-      if (n_item > 0)
-        mbar_wait(q_full + (n_item - 1) % Ly::kQStages, ((n_item - 1) / Ly::kQStages) & 1, &never, a.err,
-                  kErrXForward + kWaitDrain);
+      for (uint32_t k = n_item > Ly::kQStages ? n_item - Ly::kQStages : 0; k < n_item; ++k)
+        mbar_wait(q_full + k % Ly::kQStages, (k / Ly::kQStages) & 1, &never, a.err, kErrXForward + kWaitDrain);
     }
-  } else if (warp > 4 * NT) {
+  } else if (warp > Ly::kWarps) {
     // ------------------------------------------------------------ products of row tile r
-    const int r = warp - 4 * NT - 1;
+    const int r = warp - Ly::kWarps - 1;
     const uint32_t s_base = smem_u32(smem);
     const uint32_t idesc_o = x_idesc<T>(ksteps * 16, 0, 1);
     const uint32_t t_s = tmem + r * 128, t_o = tmem + NT * 128 + r * HALVES * 64;
-    uint32_t n_item = 0, g = 0, n_s = 0, n_out = 0;  // items and key tiles of the CTA; key tiles and items of this row tile
+    uint32_t n_item = 0, g = 0, n_s = 0, n_p = 0, n_out = 0;  // items, key tiles; scores, weights, items of this row tile
     bool ok = true;
-    // Two row tiles take turns at the tensor cores, from the second half of a P V to the next S: products that two
-    // warps issue at a time run mixed, both end late, and then both softmaxes run at a time while the tensor cores
-    // are idle (heads of 128, 4096 keys: 3,860 cycles a pair of tiles; in turns they stay half a period apart).
-    uint32_t n_turn = 0;
-    const auto take_turn = [&]() {
-      if (NT == 1) return true;
-      ++n_turn;
-      // the first row tile begins
-      if (r == 0 && n_turn == 1) return true;
-      return warp_wait(turn + r, (n_turn - (r == 0 ? 2 : 1)) & 1, abort_flag, a.err, kErrXForward + kWaitTurn);
-    };
-    const auto pass_turn = [&]() {
-      if (NT == 2 && lane == 0) mbar_arrive(turn + 1 - r);
-    };
     // Entry e (K of key tile e / 2, or its V) has arrived, with zeros in the rows that are not kept.  (Each row tile's
     // warp writes them: the same zeros.)
     const auto entry = [&](uint32_t e, bool bits, int used) {
@@ -550,58 +552,63 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
             const int slot = e % Ly::kEntries;
             ok = ok && warp_wait(kv_full + slot, (e / Ly::kEntries) & 1, abort_flag, a.err, kErrXForward + kWaitK + (e & 1));
             if (ok && lane == 0) mbar_arrive(kv_empty + slot);
-            if (e & 1) {
-              ok = ok && take_turn();
-              if (ok) pass_turn();
-            }
           }
         ++n_item;
         continue;
       }
       ok = warp_wait(q_full + qs, (n_item / Ly::kQStages) & 1, abort_flag, a.err, kErrXForward + kWaitQ);
       const uint64_t sq = k_major_desc(s_base + (qs * NT + r) * Ly::kTileBytes);
-      for (int j = t.j0; j < t.j1 && ok; ++j, ++g, ++n_s) {
-        const int chunks = x_chunks(t.keys, j);
-        const bool bits = masked || (j + 1) * kXTile > t.keys;
-        // S over the last tile's P, whose product was issued before it (products run in their order)
-        if (!(ok = entry(2 * g, bits, chunks * 32))) break;
+      const int u_end = min(2 * t.j1, (t.keys + 63) >> 6);  // 64-key steps [2 * j0, u_end)
+      const uint32_t g0 = g - t.j0;                         // a key tile's number in the CTA, less its own
+      // S of step u over P of step u - 2, whose product was issued before it (products run in their order)
+      const auto issue_s = [&](int u) {
+        const uint32_t e = 2 * (g0 + (u >> 1));
+        const int j = u >> 1;
+        if (!(u & 1) && !entry(e, masked || (j + 1) * kXTile > t.keys, x_chunks(t.keys, j) * 32)) return false;
         tc_fence_after();
         if (elect_one()) {
-          products_k_major(t_s, sq, k_major_desc(s_base + Ly::kKV + (2 * g % Ly::kEntries) * Ly::kTileBytes),
-                           x_idesc<T>(chunks * 32, 0, 0), ksteps);
-          umma_commit(s_full + r);
-          mbar_arrive(s_full + r);
-          umma_commit(kv_empty + 2 * g % Ly::kEntries);
+          products_k_major(t_s + (n_s & 1) * 64, sq,
+                           k_major_desc(s_base + Ly::kKV + (e % Ly::kEntries) * Ly::kTileBytes + (u & 1) * 8192),
+                           x_idesc<T>(x_chunks64(t.keys, u) * 32, 0, 0), ksteps);
+          umma_commit(s_full + 2 * r + (n_s & 1));
+          mbar_arrive(s_full + 2 * r + (n_s & 1));
+          if ((u & 1) || u == u_end - 1) umma_commit(kv_empty + e % Ly::kEntries);
         }
         __syncwarp();
-        if (j > t.j0) pass_turn();
-        // O += P V, its first half as soon as the first 64 weights are there
-        ok = entry(2 * g + 1, bits, chunks * 32) && warp_wait(p_full + r, n_s & 1, abort_flag, a.err, kErrXForward + kWaitP);
-        if (ok && j == t.j0 && n_out > 0)  // the last item's output has been read
+        ++n_s;
+        return true;
+      };
+      ok = ok && issue_s(2 * t.j0) && (2 * t.j0 + 1 >= u_end || issue_s(2 * t.j0 + 1));
+      for (int u = 2 * t.j0; u < u_end && ok; ++u) {
+        const uint32_t e = 2 * (g0 + (u >> 1)) + 1;
+        const int j = u >> 1;
+        // O += P V
+        if (!(u & 1)) ok = entry(e, masked || (j + 1) * kXTile > t.keys, x_chunks(t.keys, j) * 32);
+        ok = ok && warp_wait(p_full + 2 * r + (n_p & 1), (n_p >> 1) & 1, abort_flag, a.err, kErrXForward + kWaitP);
+        if (ok && u == 2 * t.j0 && n_out > 0)  // the last item's output has been read
           ok = warp_wait(o_free + r, (n_out - 1) & 1, abort_flag, a.err, kErrXForward + kWaitAccFree);
         if (!ok) break;
-        const uint64_t sv = mn_major_desc(s_base + Ly::kKV + ((2 * g + 1) % Ly::kEntries) * Ly::kTileBytes);
-        const uint32_t later = j > t.j0 ? 1u : 0u;
+        const uint64_t sv = mn_major_desc(s_base + Ly::kKV + (e % Ly::kEntries) * Ly::kTileBytes + (u & 1) * 8192);
+        const uint32_t later = u > 2 * t.j0 ? 1u : 0u, weights = t_s + (n_p & 1) * 64;
+        const int steps = 2 * x_chunks64(t.keys, u);
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (k < 2 * chunks) umma_f16_ts(t_o, t_s + k * 8, sv + k * 128, idesc_o, k > 0 ? 1u : later);
+          for (int k = 0; k < 4; ++k)  // a chunk's P lies in the first 16 of its 32 columns, the low part in the others
+            if (k < steps) {
+              const uint32_t w = weights + (k >> 1) * 32 + (k & 1) * 8;
+              umma_f16_ts(t_o, w, sv + k * 128, idesc_o, k > 0 ? 1u : later);
+              if (SPLIT) umma_f16_ts(t_o, w + 16, sv + k * 128, idesc_o, 1u);
+            }
+          umma_commit(pv_done + 2 * r + (n_p & 1));
+          if (u == u_end - 1) umma_commit(o_full + r);
+          if ((u & 1) || u == u_end - 1) umma_commit(kv_empty + e % Ly::kEntries);
         }
         __syncwarp();
-        ok = warp_wait(p_rest + r, n_s & 1, abort_flag, a.err, kErrXForward + kWaitPRest) && take_turn();
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 4; k < 8; ++k)
-            if (k < 2 * chunks) umma_f16_ts(t_o, t_s + k * 8, sv + k * 128, idesc_o, 1u);
-          umma_commit(kv_empty + (2 * g + 1) % Ly::kEntries);
-          if (j == t.j1 - 1) umma_commit(o_full + r);
-        }
-        __syncwarp();
-        if (j == t.j1 - 1) pass_turn();  // the next item's Q may be long in coming
+        ++n_p;
+        if (u + 2 < u_end) ok = issue_s(u + 2);
       }
+      g += t.j1 - t.j0;
       ++n_out;
       ++n_item;
     }
@@ -618,12 +625,14 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
     const bool flip = a.scale < 0.0f;  // the largest score is the smallest product
     // log2 units; a zero scale keeps a factor that leaves -inf at -inf
     const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
+    const uint64_t c22 = pair2(c2, c2);
     const int rows = a.tile_tokens * a.pack, my_token = row / a.pack, my_head = row % a.pack;
-    uint32_t n_s = 0, n_out = 0, n_item = 0, g = 0;
+    const bool hands_out = quad == 0 && lane == 0;
+    uint32_t n_s = 0, n_out = 0, n_item = 0, g = 0;  // 64-key steps and items of this row tile; items, key tiles
     int stored = -1;  // Q stage whose output is on its way out
     // The stage is free for a new Q once the output has been read from it; asked for as late as can be.
     const auto release_stored = [&]() {
-      if (Ly::kQStages > 1 && stored >= 0 && quad == 0 && lane == 0) {
+      if (Ly::kQStages > 1 && stored >= 0 && hands_out) {
         bulk_wait_group_read<0>();
         mbar_arrive(q_empty + stored);
       }
@@ -662,198 +671,143 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       }
       // rows of this warp that exist: a warp without any keeps only the barriers
       const bool any_row = __any_sync(0xffffffffu, live);
-      float m = -INFINITY, l = 0.0f;
-      uint64_t sum[2];  // of the tile's weights, four partial sums
-      // Raises the exponent's reference to at least the row's maximum mt over 2^8, with what was summed so far.
-      const auto raise = [&](float mt, int j) {
-        if (__any_sync(0xffffffffu, live && ((mt - m) * c2 > 8.0f || m == -INFINITY))) {
-          const float mn = fmaxf(m, mt);
-          const float f = m == -INFINITY ? 0.0f : ex2((m - mn) * c2);
-          l *= f;
-          m = mn;
-          if (j > t.j0) {
-#pragma unroll 1
-            for (int c = 0; c < 2 * HALVES; ++c) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(t_o + c * 32, o);
-              tmem_ld_wait();
-              after_wait(o);
-#pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tmem_st_32x32b_x32(t_o + c * 32, o);
-            }
-          }
-        }
-      };
-      // The weights of chunk c, which take the place of a half of its scores.
-      const auto weigh = [&](const uint32_t(&v)[32], int c, uint64_t c22, uint64_t mc2) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          float x0, x1;
-          unpair2(fma2(pair2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c22, mc2), x0, x1);
-          x0 = ex2(x0);
-          x1 = ex2(x1);
-          sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair2(x0, x1));
-          pk[k >> 1] = XType<T>::pack2(x0, x1);
-        }
-        tmem_st_32x32b_x16(t_s + c * 16, pk);
-      };
-      const auto give = [&](uint64_t* bar) {  // the products over what was stored can begin
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
-      };
-      for (int j = t.j0; j < t.j1; ++j, ++g, ++n_s) {
-        ok = warp_wait(s_full + rt, n_s & 1, abort_flag, a.err, kErrXForward + kWaitS);
+      float m = -INFINITY, l = 0.0f;  // reference of the row's exponent, and the sum
+      const int u_end = min(2 * t.j1, (t.keys + 63) >> 6);
+      for (int u = 2 * t.j0; u < u_end; ++u, ++n_s) {
+        const uint32_t scores = t_s + (n_s & 1) * 64;
+        ok = warp_wait(s_full + 2 * rt + (n_s & 1), (n_s >> 1) & 1, abort_flag, a.err, kErrXForward + kWaitS);
         if (!ok) break;
         tc_fence_after();
-        const int chunks = x_chunks(t.keys, j);
-        if (!any_row) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(p_full + rt);
-            mbar_arrive(p_rest + rt);
-          }
-        } else {
-          sum[0] = sum[1] = pair2(0.0f, 0.0f);
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          const auto search = [&](const uint32_t(&x)[32]) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 8)
-#pragma unroll
-              for (int u = 0; u < 4; ++u)
-                mx[u] = max3(mx[u], __uint_as_float(x[k + 2 * u]), __uint_as_float(x[k + 2 * u + 1]));
-          };
-          if (!masked && !flip && (j + 1) * kXTile <= t.keys) {
-            // 128 kept keys: a quarter of the row stays in registers between the search and the weights, the rest is
-            // read twice (with all of it kept the row's scores alone take 128 of the 168 registers)
-            uint32_t v0[32], v1[32], v2[32];
-            tmem_ld_32x32b_x32(t_s, v0);
-            tmem_ld_32x32b_x32(t_s + 32, v1);
-            tmem_ld_wait();
-            after_wait(v0);
-            after_wait(v1);
-            tmem_ld_32x32b_x32(t_s + 64, v2);
-            search(v0);
-            search(v1);
-            tmem_ld_wait();
-            after_wait(v2);
-            tmem_ld_32x32b_x32(t_s + 96, v1);
-            search(v2);
-            tmem_ld_wait();
-            after_wait(v1);
-            search(v1);
-            tmem_ld_32x32b_x32(t_s + 32, v1);
-            raise(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), j);
-            const float mc = -m * c2;
-            const uint64_t c22 = pair2(c2, c2), mc2 = pair2(mc, mc);
-            weigh(v0, 0, c22, mc2);
-            tmem_ld_wait();
-            after_wait(v1);
-            tmem_ld_32x32b_x32(t_s + 64, v2);
-            weigh(v1, 1, c22, mc2);
-            give(p_full + rt);
-            tmem_ld_wait();
-            after_wait(v2);
-            tmem_ld_32x32b_x32(t_s + 96, v0);
-            weigh(v2, 2, c22, mc2);
-            tmem_ld_wait();
-            after_wait(v0);
-            weigh(v0, 3, c22, mc2);
-            give(p_rest + rt);
-          } else {
-            // keys left out, or a negative scale: the chunks that hold keys, twice, the next one read meanwhile
-            const bool bits = masked || (j + 1) * kXTile > t.keys;
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(words + g % kXMaskSlots);
+        if (any_row) {
+          const bool two = x_chunks64(t.keys, u) == 2;
+          uint32_t v[2][32];
+          tmem_read(scores, v[0]);
+          if (two) tmem_read(scores + 32, v[1]);
+          if (masked || flip || (u + 1) * 64 > t.keys) {
+            uint2 keep = make_uint2(~0u, ~0u);
+            if (masked || ((u >> 1) + 1) * kXTile > t.keys)
+              keep = reinterpret_cast<const uint2*>(words + (g + (u >> 1) - t.j0) % kXMaskSlots)[u & 1];
             const uint32_t sign = flip ? 0x80000000u : 0u;
-            const auto pass = [&](auto&& use) {
-              uint32_t v[2][32];
-              tmem_ld_32x32b_x32(t_s, v[0]);
-#pragma unroll 1
-              for (int c0 = 0; c0 < chunks; c0 += 2)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                  const int c = c0 + u;
-                  if (c >= chunks) break;
-                  const uint32_t keep = bits ? w[c] : ~0u;
-                  tmem_ld_wait();
-                  after_wait(v[u]);
-                  if (c + 1 < chunks) tmem_ld_32x32b_x32(t_s + (c + 1) * 32, v[1 - u]);
-                  if (keep != ~0u || flip) {
+            for (int k = 0; k < 32; ++k) v[0][k] = (keep.x >> k) & 1u ? v[0][k] ^ sign : 0xff800000u;
+            if (two) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[u][k] = (keep >> k) & 1u ? v[u][k] ^ sign : 0xff800000u;
-                  }
-                  use(v[u], c);
-                }
-            };
-            pass([&](const uint32_t(&v)[32], int) { search(v); });
-            raise(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), j);
-            const float mc = m == -INFINITY ? 0.0f : -m * c2;
-            const uint64_t c22 = pair2(c2, c2), mc2 = pair2(mc, mc);
-            pass([&](const uint32_t(&v)[32], int c) {
-              weigh(v, c, c22, mc2);
-              if (c == min(chunks, 2) - 1) give(p_full + rt);
-            });
-            give(p_rest + rt);
+              for (int k = 0; k < 32; ++k) v[1][k] = (keep.y >> k) & 1u ? v[1][k] ^ sign : 0xff800000u;
+            }
           }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            if (c == 0 || two) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 8)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  mx[i] = max3(mx[i], __uint_as_float(v[c][k + 2 * i]), __uint_as_float(v[c][k + 2 * i + 1]));
+            }
+          const float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+          // raises the reference where the row's maximum passes it by more than 2^8, with what was summed so far
+          if (__any_sync(0xffffffffu, live && ((mt - m) * c2 > 8.0f || m == -INFINITY))) {
+            const float mn = fmaxf(m, mt);
+            const float f = m == -INFINITY ? 0.0f : ex2((m - mn) * c2);
+            l *= f;
+            m = mn;
+            if (u > 2 * t.j0) {
+              // the product of the step before is done (the one before that was when this step's scores came)
+              ok = warp_wait(pv_done + 2 * rt + ((n_s - 1) & 1), ((n_s - 1) >> 1) & 1, abort_flag, a.err,
+                             kErrXForward + kWaitPV);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < 4 * HALVES; ++c) {
+                uint32_t o[16];
+                tmem_read(t_o + c * 16, o);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                tmem_st_32x32b_x16(t_o + c * 16, o);
+              }
+            }
+          }
+          const float mc = m == -INFINITY ? 0.0f : -m * c2;
+          const uint64_t mc2 = pair2(mc, mc);
+          uint64_t sum[2] = {pair2(0.0f, 0.0f), pair2(0.0f, 0.0f)};
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            if (c == 0 || two) {
+              uint32_t pk[16], lo[16];
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                float x0, x1;
+                unpair2(fma2(pair2(__uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1])), c22, mc2), x0, x1);
+                x0 = ex2(x0);
+                x1 = ex2(x1);
+                sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair2(x0, x1));
+                if constexpr (SPLIT) split2<T>(x0, x1, pk[k >> 1], lo[k >> 1]);
+                else pk[k >> 1] = XType<T>::pack2(x0, x1);
+              }
+              tmem_st_32x32b_x16(scores + c * 32, pk);  // the weights take the place of their scores
+              if constexpr (SPLIT) tmem_st_32x32b_x16(scores + c * 32 + 16, lo);
+            }
           float s0, s1;
           unpair2(add2(sum[0], sum[1]), s0, s1);
           l += s0 + s1;
+          tmem_st_wait();
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 2 * rt + (n_s & 1));
       }
-      release_stored();
-      if (ok) ok = warp_wait(o_full + rt, n_out & 1, abort_flag, a.err, kErrXForward + kWaitAcc);
       if (!ok) break;
-      ++n_out;
+      g += t.j1 - t.j0;
+      release_stored();
+      ok = warp_wait(o_full + rt, n_out & 1, abort_flag, a.err, kErrXForward + kWaitAcc);
+      if (!ok) break;
       tc_fence_after();
       const float inv = l > 0.0f ? __fdividef(1.0f, l) : (l == l ? 0.0f : l);
       uint8_t* stage = smem + (qs * NT + rt) * Ly::kTileBytes;  // Q's tile, read by every product of the item by now
+      if (any_row) {
 #pragma unroll
-      for (int c = 0; c < 2 * HALVES; ++c) {
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(t_o + c * 32, o);
-        tmem_ld_wait();
-        after_wait(o);
-        if (p.splits > 1) {
-          if (live) {
-            float* dst = p.part_o + (t.split * p.rows + r_index) * a.head_dim + c * 32;
+        for (int c = 0; c < 2 * HALVES; ++c) {
+          const int col = c * 32;
+          uint32_t o[32];
+          tmem_read(t_o + col, o);
+          if (p.splits > 1) {
+            if (live) {
+              float* dst = p.part_o + (t.split * p.rows + r_index) * a.head_dim + col;
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              if (c * 32 + k < a.head_dim)
-                *reinterpret_cast<float4*>(dst + k) =
-                    make_float4(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv,
-                                __uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
+              for (int k = 0; k < 32; k += 4)
+                if (col + k < a.head_dim)
+                  *reinterpret_cast<float4*>(dst + k) =
+                      make_float4(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv,
+                                  __uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
+            }
+          } else {
+            uint32_t pk[16];
+#pragma unroll
+            for (int k = 0; k < 32; k += 2)
+              pk[k >> 1] = XType<T>::pack2(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              st_shared_v4(stage + (col >> 6) * 16384 + swizzle128_offset(row, ((col & 63) >> 3) + u), pk[4 * u],
+                           pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
           }
-        } else {
-          uint32_t pk[16];
-#pragma unroll
-          for (int k = 0; k < 32; k += 2)
-            pk[k >> 1] = XType<T>::pack2(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
-          uint8_t* half = stage + (c >> 1) * 16384;
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            st_shared_v4(half + swizzle128_offset(row, (c & 1) * 4 + u), pk[4 * u], pk[4 * u + 1], pk[4 * u + 2],
-                         pk[4 * u + 3]);
+        }
+        if (live) {
+          // lse in base 2; the natural one is log(2) times it
+          const float lse2 = l > 0.0f ? m * c2 + __log2f(l) : (l == l ? -INFINITY : l);
+          if (p.splits > 1) p.part_lse[t.split * p.rows + r_index] = lse2;
+          else if (a.lse != nullptr) a.lse[r_index] = lse2 * 0.6931471805599453f;
         }
       }
       tc_fence_before();
-      if (live) {
-        // lse in base 2; the natural one is log(2) times it
-        const float lse2 = l > 0.0f ? m * c2 + __log2f(l) : (l == l ? -INFINITY : l);
-        if (p.splits > 1) p.part_lse[t.split * p.rows + r_index] = lse2;
-        else if (a.lse != nullptr) a.lse[r_index] = lse2 * 0.6931471805599453f;
-      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(o_free + rt);
         mbar_arrive(staged + rt);
       }
-      if (quad == 0 && lane == 0) {
-        ok = mbar_wait(staged + rt, (n_out - 1) & 1, abort_flag, a.err, kErrXForward + kWaitStaged);
+      if (hands_out) {
+        ok = mbar_wait(staged + rt, n_out & 1, abort_flag, a.err, kErrXForward + kWaitStaged);
         if (ok && p.splits == 1) {
           for (int hf = 0; hf < HALVES; ++hf)
             tma_store_4d(&o_map, stage + hf * 16384, hf * 64, t.hv * a.pack, (t.tile0 + rt) * a.tile_tokens, t.b);
@@ -866,13 +820,14 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       }
       ok = __all_sync(0xffffffffu, ok);
       stored = qs;
+      ++n_out;
       ++n_item;
     }
-    if (quad == 0 && lane == 0) bulk_wait_group<0>();
+    if (hands_out) bulk_wait_group<0>();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4 * NT) {
+  if (warp == Ly::kWarps) {
     tc_fence_after();
     tmem_dealloc(tmem, Ly::kTmemCols);
   }

@@ -423,9 +423,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         tc_fence_after();
         uint32_t s[32];
         if (some) {
-          tmem_ld_32x32b_x32(t_s, s);
-          tmem_ld_wait();
-          after_wait(s);
+          tmem_read(t_s, s);
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             float x0, x1;
@@ -448,9 +446,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         for (int h = 0; h < 2; ++h) {
           uint32_t dp[16];
           if (some) {
-            tmem_ld_32x32b_x16(t_lane + kXDqDP + wq * 32 + h * 16, dp);
-            tmem_ld_wait();
-            after_wait(dp);
+            tmem_read(t_lane + kXDqDP + wq * 32 + h * 16, dp);
           }
           if (h == 1) {
             tc_fence_before();
@@ -486,9 +482,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       for (int c = 0; c < HALVES; ++c) {
         const int col = (wq * HALVES + c) * 16;
         uint32_t o[16];
-        tmem_ld_32x32b_x16(t_lane + kXDqAcc + col, o);
-        tmem_ld_wait();
-        after_wait(o);
+        tmem_read(t_lane + kXDqAcc + col, o);
         uint32_t pk[8];
 #pragma unroll
         for (int k = 0; k < 16; k += 2)
@@ -854,14 +848,12 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         if (!ok) break;
         tc_fence_after();
         const uint32_t t_s = t_lane + kXDkvS + wq * 32, t_dp = t_lane + kXDkvDP + wq * 32;
-        uint32_t s[32];
-        tmem_ld_32x32b_x32(t_s, s);
         const float4* neg_lse = reinterpret_cast<const float4*>(stats + g % (Ly::kEntries / 2) * 2 * kXTile + wq * 32);
         const float4* neg_delta = neg_lse + kXTile / 4;
         if (j == t.j0)
           kept = (reinterpret_cast<const uint32_t*>(words + n_item % (2 * Ly::kKVStages))[quad] >> lane) & 1u;
-        tmem_ld_wait();
-        after_wait(s);
+        uint32_t s[32];
+        tmem_read(t_s, s);
         uint32_t pk[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
@@ -889,9 +881,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         if (!ok) break;
         tc_fence_after();
         uint32_t dp[32];
-        tmem_ld_32x32b_x32(t_dp, dp);
-        tmem_ld_wait();
-        after_wait(dp);
+        tmem_read(t_dp, dp);
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
           const float4 nd = neg_delta[k >> 2];
@@ -922,9 +912,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       for (int c = 0; c < HALVES; ++c) {
         const int col = c0 + c * 32;
         uint32_t o[32];
-        tmem_ld_32x32b_x32(t_lane + kXDkvV + is_k * HALVES * 64 + col, o);
-        tmem_ld_wait();
-        after_wait(o);
+        tmem_read(t_lane + kXDkvV + is_k * HALVES * 64 + col, o);
 #pragma unroll
         for (int k = 0; k < 32; ++k) o[k] = kept ? __float_as_uint(__uint_as_float(o[k]) * f) : 0u;
         if (p.splits > 1) {
