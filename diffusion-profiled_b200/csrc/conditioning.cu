@@ -252,17 +252,17 @@ XBwdPlan x_bwd_plan(const fp8_cross_attention_args* a, int sm_count) {
   return w;
 }
 
-template <typename T, int HALVES>
+template <typename T, int HALVES, bool SPLIT>
 int x_bwd_launch(const XBwdParams& dq, const XBwdParams& dkv, const CUtensorMap (&m)[7], DeviceState* st,
                  cudaStream_t stream) {
-  FP8_CUDA_TRY(cudaFuncSetAttribute(x_dq_kernel<T, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    XDqLayout<HALVES>::kSmemBytes));
-  FP8_CUDA_TRY(cudaFuncSetAttribute(x_dkv_kernel<T, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  FP8_CUDA_TRY(cudaFuncSetAttribute(x_dq_kernel<T, HALVES, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    XDqLayout<HALVES, SPLIT>::kSmemBytes));
+  FP8_CUDA_TRY(cudaFuncSetAttribute(x_dkv_kernel<T, HALVES, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     XDkvLayout<HALVES>::kSmemBytes));
   const auto grid = [&](int64_t items) { return dim3(static_cast<unsigned>(std::min<int64_t>(items, st->sm_count))); };
-  FP8_CUDA_TRY(launch_kernel(x_dq_kernel<T, HALVES>, grid(dq.items), dim3(kXBwdThreads),
-                             XDqLayout<HALVES>::kSmemBytes, stream, 1, kTensorKernel, dq, m[0], m[1], m[2], m[3], m[4]));
-  FP8_CUDA_TRY(launch_kernel(x_dkv_kernel<T, HALVES>, grid(dkv.items), dim3(kXBwdThreads),
+  FP8_CUDA_TRY(launch_kernel(x_dq_kernel<T, HALVES, SPLIT>, grid(dq.items), dim3(kXBwdThreads),
+                             XDqLayout<HALVES, SPLIT>::kSmemBytes, stream, 1, kTensorKernel, dq, m[0], m[1], m[2], m[3], m[4]));
+  FP8_CUDA_TRY(launch_kernel(x_dkv_kernel<T, HALVES, SPLIT>, grid(dkv.items), dim3(kXBwdThreads),
                              XDkvLayout<HALVES>::kSmemBytes, stream, 1, kTensorKernel, dkv, m[0], m[1], m[2], m[3], m[5],
                              m[6]));
   count_launches(2);
@@ -300,8 +300,12 @@ int x_bwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XBwd
   if (int s = q_side(&m[4], a.dq, a.sdq)) return s;
   if (int s = k_side(&m[5], a.dk, a.sdk)) return s;
   if (int s = k_side(&m[6], a.dv, a.sdv)) return s;
-  if (int s = a.head_dim <= 64 ? x_bwd_launch<T, 1>(p, kv, m, st, stream) : x_bwd_launch<T, 2>(p, kv, m, st, stream))
-    return s;
+  const bool one = a.k_len <= kXTile;  // the states are one key tile
+  const int status = a.head_dim <= 64 ? (one ? x_bwd_launch<T, 1, true>(p, kv, m, st, stream)
+                                             : x_bwd_launch<T, 1, false>(p, kv, m, st, stream))
+                                      : (one ? x_bwd_launch<T, 2, true>(p, kv, m, st, stream)
+                                             : x_bwd_launch<T, 2, false>(p, kv, m, st, stream));
+  if (status) return status;
   if (w.splits > 1) {
     const int64_t quads = 2ll * a.batch * a.k_len * a.kv_heads * (a.head_dim / 4);
     FP8_CUDA_TRY(launch_kernel(x_dkv_join_kernel<T>, dim3(grid_for(quads, 256, st->sm_count, 8)), dim3(256), 0, stream, 1,

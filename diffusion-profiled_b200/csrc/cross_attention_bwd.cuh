@@ -2,34 +2,35 @@
 //
 // Two launches, each with its sums in tensor memory from beginning to end, so that no
 // gradient is added to memory by several CTAs (no atomics, one order of addition):
-//   * x_dq_kernel: a row tile of queries against its key tiles.  delta_i = do_i . o_i
-//     first (fp32; stored for the second launch with the row's log-sum-exp), then per
-//     key tile S = Q K^T and dP = dO V^T, dS = P (dP - delta), dQ += dS K;
-//   * x_dkv_kernel: a key tile against the row tiles that read it, all heads that share
-//     it among them.  The scores are formed transposed, S^T = K Q^T and dP^T = V dO^T
-//     (lane = key), so that P^T and dS^T lie in tensor memory as the first operands of
-//     dV += P^T dO and dK += dS^T Q.
+//   * x_dq_kernel: a row tile of queries against the keys, 64 at a step.  Per step
+//     S = Q K^T and dP = dO V^T, dS = P (dP - delta), dQ += dS K.  It also leaves each
+//     row's -log-sum-exp and -delta for the second launch;
+//   * x_dkv_kernel: a key tile against the rows that read it, 64 at a step, all heads that
+//     share it among them.  The scores are formed transposed, S^T = K Q^T and
+//     dP^T = V dO^T (lane = key), so that P^T and dS^T lie in tensor memory as the first
+//     operands of dV += P^T dO and dK += dS^T Q.
 // That is seven products a tile pair; a single launch would need five, but would add
-// dQ to memory from every key tile.  Both kernels know the rows' log-sum-exp, so no
-// maximum is searched and a row of scores needs no single owner: 16 softmax warps take
-// 32 columns of a row each (four warps a scheduler hide the exponentials' and loads'
-// latency that two with 64 columns do not).  Two
-// warps issue the products: one the scores and dP, one the gradients.  In x_dq_kernel the
-// scores run ahead into a second buffer; in x_dkv_kernel, where tensor memory has no room
-// for one, P^T takes the place of S^T and dS^T that of dP^T, so that dV += P^T dO and the
-// next scores run while dS^T is made, and dK += dS^T Q and the next dP^T while the next
-// exponentials are.
+// dQ to memory from every key tile.
 //
-// P and dS are rounded to the tensors' type (they are matrix operands); scores, dP,
-// statistics and all sums are fp32.
+// Both kernels have two buffers for the scores and for dP, and two groups of four softmax
+// warps that take the steps in turn, a thread one row (or key) and 64 columns: while one
+// group works on a step, the products of the next run.  (With one buffer of 128 columns
+// and all warps on it, softmax and products of a tile followed one another: 3,300 to 4,100
+// cycles a tile at heads of 128.)  One warp issues the scores and dP, one the gradients.
+//
+// delta_i = do_i . o_i from the forward's output; where the states are at most one key
+// tile (SPLIT), delta_i = sum_j p_ij dp_ij in fp32 instead, without the output's rounding
+// (with few keys it does not average out), and P and dS go into the products as the sum of
+// two values of the tensors' type.  Otherwise P and dS are rounded to it once (they are
+// matrix operands); scores, dP, statistics and all sums are fp32.
 #pragma once
 
 #include "cross_attention.cuh"
 
 namespace fp8b {
 
-constexpr int kXBwdWarps = 16;                           // softmax warps
-constexpr int kXBwdThreads = kXBwdWarps * 32 + 96;       // and loads, scores, gradients
+constexpr int kXBwdWarps = 16;                      // softmax warps, two groups of eight
+constexpr int kXBwdThreads = kXBwdWarps * 32 + 96;  // and loads, scores, gradients
 
 struct XBwdParams {
   XAttnParams a;
@@ -56,25 +57,59 @@ __device__ __forceinline__ float x_dot8(const uint4& x, const uint4& y) {
   return s[0] + s[1];
 }
 
+// All lanes have done what came before.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// Weights and score gradients of a chunk of 32 columns, as operands over the columns they were made from.
+template <typename T, bool SPLIT>
+__device__ __forceinline__ void x_store_operand(uint32_t taddr, const float (&x)[32]) {
+  uint32_t hi[16], lo[16];
+#pragma unroll
+  for (int k = 0; k < 32; k += 2) {
+    if constexpr (SPLIT) split2<T>(x[k], x[k + 1], hi[k >> 1], lo[k >> 1]);
+    else hi[k >> 1] = XType<T>::pack2(x[k], x[k + 1]);
+  }
+  tmem_st_32x32b_x16(taddr, hi);
+  if constexpr (SPLIT) tmem_st_32x32b_x16(taddr + 16, lo);
+}
+
+// D += A B over `steps` (of at most MAX) 16-column steps of an operand stored by x_store_operand and a tile read across
+// its rows (one elected thread).
+template <bool SPLIT, int MAX>
+__device__ __forceinline__ void x_products_mn(uint32_t d, uint32_t operand, uint64_t b, uint32_t idesc, int steps,
+                                              uint32_t accumulate) {
+#pragma unroll
+  for (int k = 0; k < MAX; ++k)
+    if (k < steps) {
+      const uint32_t w = operand + (k >> 1) * 32 + (k & 1) * 8;
+      umma_f16_ts(d, w, b + k * 128, idesc, k > 0 ? 1u : accumulate);
+      if (SPLIT) umma_f16_ts(d, w + 16, b + k * 128, idesc, 1u);
+    }
+}
+
 // ============================================================================ dQ
-template <int HALVES>
+template <int HALVES, bool SPLIT>
 struct XDqLayout {
   static constexpr int kTileBytes = HALVES * 16384;
   static constexpr int kQStages = HALVES == 1 ? 3 : 1;  // Q and dO of an item
   // A key tile stays from its scores to its dQ product, two tiles later; a value tile only for its dP.
-  static constexpr int kKStages = HALVES == 1 ? 4 : 3;
+  static constexpr int kKStages = HALVES == 1 ? 4 : SPLIT ? 2 : 3;
   static constexpr int kVStages = HALVES == 1 ? 3 : 2;
   static constexpr int kK = 2 * kQStages * kTileBytes;
   static constexpr int kV = kK + kKStages * kTileBytes;
   static constexpr int kWords = kV + kVStages * kTileBytes;
-  static constexpr int kDelta = kWords + kXMaskSlots * 16;  // fp32 [2][128]: the halves of the rows' delta
-  static constexpr int kBar = kDelta + 1024;
-  static constexpr int kNumBars = 2 * (kQStages + kKStages + kVStages) + 13;
+  static constexpr int kDelta = kWords + kXMaskSlots * 16;  // fp32: the rows' delta in parts, [2][128] or with SPLIT [4][128]
+  static constexpr int kBar = kDelta + (SPLIT ? 2048 : 1024);
+  static constexpr int kNumBars = 2 * (kQStages + kKStages + kVStages) + 14;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;
 };
-static_assert(XDqLayout<1>::kSmemBytes <= 232448 && XDqLayout<2>::kSmemBytes <= 232448, "dq smem");
-// tensor memory columns: two score buffers (dS over the first half of each 32), dP, dQ
+static_assert(XDqLayout<1, true>::kSmemBytes <= 232448 && XDqLayout<2, true>::kSmemBytes <= 232448 &&
+                  XDqLayout<1, false>::kSmemBytes <= 232448 && XDqLayout<2, false>::kSmemBytes <= 232448, "dq smem");
+// tensor memory columns: two score buffers (dS over them), dP, dQ
 constexpr uint32_t kXDqS = 0, kXDqDP = 256, kXDqAcc = 384;
 
 struct XDqItem {
@@ -109,16 +144,16 @@ struct XDqItems {
   }
 };
 
-template <typename T, int HALVES>
+template <typename T, int HALVES, bool SPLIT>
 __global__ void __launch_bounds__(kXBwdThreads, 1)
     x_dq_kernel(const XBwdParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap do_map,
                 const __grid_constant__ CUtensorMap dq_map) {
-  using Ly = XDqLayout<HALVES>;
+  using Ly = XDqLayout<HALVES, SPLIT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint4* words = reinterpret_cast<uint4*>(smem + Ly::kWords);
-  float* delta_half = reinterpret_cast<float*>(smem + Ly::kDelta);
+  float* delta_part = reinterpret_cast<float*>(smem + Ly::kDelta);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + Ly::kBar);
   uint64_t* q_empty = q_full + Ly::kQStages;
   uint64_t* k_full = q_empty + Ly::kQStages;
@@ -129,8 +164,8 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
   uint64_t* s_free = s_full + 2;              // [2]: its dS has been multiplied
   uint64_t* dp_full = s_free + 2;
   uint64_t* dp_free = dp_full + 1;
-  uint64_t* ds_full = dp_free + 1;
-  uint64_t* acc_full = ds_full + 1;
+  uint64_t* ds_full = dp_free + 1;            // [2], by score buffer: a warp may be a tile ahead of another
+  uint64_t* acc_full = ds_full + 2;
   uint64_t* acc_free = acc_full + 1;
   uint64_t* staged = acc_free + 1;
   uint64_t* delta_full = staged + 1;
@@ -155,15 +190,15 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 2);  // the products' commit, and the issuing thread (keep bits)
       mbar_init(s_free + i, 1);
+      mbar_init(ds_full + i, kXBwdWarps);
       mbar_init(drained + i, 1);
     }
     mbar_init(dp_full, 1);
     mbar_init(dp_free, kXBwdWarps);
-    mbar_init(ds_full, kXBwdWarps);
     mbar_init(acc_full, 1);
     mbar_init(acc_free, kXBwdWarps);
     mbar_init(staged, kXBwdWarps);
-    mbar_init(delta_full, 8);
+    mbar_init(delta_full, SPLIT ? kXBwdWarps : 8);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -302,17 +337,13 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       if (t.tiles == 0) continue;
       for (int j = 0; j < t.tiles; ++j, ++g) {
         const int ks = g % Ly::kKStages, buf = g & 1, steps = 2 * x_chunks(t.keys, j);
-        ok = wait(k_full + ks, g / Ly::kKStages, kWaitK) && wait(ds_full, g, kWaitP);
+        ok = wait(k_full + ks, g / Ly::kKStages, kWaitK) && wait(ds_full + buf, g >> 1, kWaitP);
         if (ok && j == 0 && n_item > 0) ok = wait(acc_free, n_item ^ 1, kWaitAccFree);  // the last item's dQ has been read
         if (!ok) break;
         const uint64_t sk = mn_major_desc(s_base + Ly::kK + ks * Ly::kTileBytes);
-        const uint32_t ds = tmem + kXDqS + buf * 128, later = j > 0 ? 1u : 0u;
         tc_fence_after();
         if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)  // dS of 32 columns lies in the first 16 of them
-            if (k < steps)
-              umma_f16_ts(tmem + kXDqAcc, ds + (k >> 1) * 32 + (k & 1) * 8, sk + k * 128, idesc, k > 0 ? 1u : later);
+          x_products_mn<SPLIT, 8>(tmem + kXDqAcc, tmem + kXDqS + buf * 128, sk, idesc, steps, j > 0 ? 1u : 0u);
           umma_commit(s_free + buf);
           umma_commit(k_empty + ks);
           if (j == t.tiles - 1) umma_commit(acc_full);
@@ -344,7 +375,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       const bool exists = items.ahead(t);
       const int token = t.tile * a.tile_tokens + my_token, head = t.hv * a.pack + my_head;
       const bool live = exists && t.tiles > 0 && row < rows && token < a.q_len;
-      if (HALVES == 1 && wq < 2) {
+      if (!SPLIT && HALVES == 1 && wq < 2) {
         const T* o = static_cast<const T*>(a.o_in) + t.b * a.so.batch + token * a.so.token + head * a.so.head;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -385,8 +416,9 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       const int qs = n_item % Ly::kQStages;
       uint8_t* stage = smem + 2 * qs * Ly::kTileBytes;
       const bool dead = lse == -INFINITY;  // no such row, or no kept key
-      // ---- delta = do . o, half of the channels each
-      if (wq < 2) {
+      const float neg_lse = dead ? -INFINITY : -lse * 1.4426950408889634f;
+      float neg_delta = 0.0f;
+      if (!SPLIT && wq < 2) {  // delta = do . o, half of the channels each
         ok = wait(q_full + qs, n_item / Ly::kQStages, kWaitQ);
         if (!ok) break;
         float part = 0.0f;
@@ -402,19 +434,27 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
           }
           part -= x_dot8<T>(v, ld_shared_v4(stage + Ly::kTileBytes + (c >> 3) * 16384 + swizzle128_offset(row, c & 7)));
         }
-        delta_half[wq * kXTile + row] = part;
+        delta_part[wq * kXTile + row] = part;
         __syncwarp();
         if (lane == 0) mbar_arrive(delta_full);
       }
-      ok = wait(delta_full, n_item, kWaitDelta);
-      if (!ok) break;
-      const float neg_delta = dead ? 0.0f : delta_half[row] + delta_half[kXTile + row];
-      const float neg_lse = dead ? -INFINITY : -lse * 1.4426950408889634f;
-      if (wq == 0) {
-        stat[0] = neg_lse;
-        stat[kXTile] = neg_delta;
+      // this row's delta, from its parts, and the statistics that the second launch needs
+      const auto join_delta = [&]() {
+        if (!wait(delta_full, n_item, kWaitDelta)) return false;
+        neg_delta = delta_part[row] + delta_part[kXTile + row];
+        if (SPLIT) neg_delta += delta_part[2 * kXTile + row] + delta_part[3 * kXTile + row];
+        if (dead) neg_delta = 0.0f;
+        if (wq == 0) {
+          stat[0] = neg_lse;
+          stat[kXTile] = neg_delta;
+        }
+        return true;
+      };
+      if (!SPLIT) {
+        ok = join_delta();
+        if (!ok) break;
       }
-      const uint64_t nl2 = pair2(neg_lse, neg_lse), nd2 = pair2(neg_delta, neg_delta);
+      const uint64_t nl2 = pair2(neg_lse, neg_lse);
       for (int j = 0; j < t.tiles; ++j, ++g) {
         const uint32_t t_s = t_lane + kXDqS + (g & 1) * 128 + wq * 32;
         const bool some = wq < x_chunks(t.keys, j);  // the chunk holds keys
@@ -422,6 +462,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         if (!ok) break;
         tc_fence_after();
         uint32_t s[32];
+        bool single = false;  // one kept key: its weight is 1 whatever its score, and no gradient goes through it
         if (some) {
           tmem_read(t_s, s);
 #pragma unroll
@@ -433,6 +474,10 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
           }
           if (masked || (j + 1) * kXTile > t.keys) {
             const uint32_t w = reinterpret_cast<const uint32_t*>(words + g % kXMaskSlots)[wq];
+            if (SPLIT) {
+              const uint4 all = words[g % kXMaskSlots];
+              single = __popc(all.x) + __popc(all.y) + __popc(all.z) + __popc(all.w) == 1;
+            }
             if (w != ~0u) {
 #pragma unroll
               for (int k = 0; k < 32; ++k) s[k] = (w >> k) & 1u ? s[k] : 0u;
@@ -442,16 +487,34 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         ok = wait(dp_full, g, kWaitDP);
         if (!ok) break;
         tc_fence_after();
+        if constexpr (SPLIT) {  // delta = sum p dP, a chunk of it by each warp of these rows
+          float s0 = 0.0f, s1 = 0.0f;
+          if (some) {
+            uint64_t sum = pair2(0.0f, 0.0f);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t dp[16];
+              tmem_read(t_lane + kXDqDP + wq * 32 + h * 16, dp);
+#pragma unroll
+              for (int k = 0; k < 16; k += 2)
+                sum = fma2(pair2(__uint_as_float(s[16 * h + k]), __uint_as_float(s[16 * h + k + 1])),
+                           pair2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), sum);
+            }
+            unpair2(sum, s0, s1);
+          }
+          delta_part[wq * kXTile + row] = -(s0 + s1);
+          warp_arrive(delta_full);
+          ok = join_delta();
+          if (!ok) break;
+        }
+        const uint64_t nd2 = pair2(neg_delta, neg_delta);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t dp[16];
-          if (some) {
-            tmem_read(t_lane + kXDqDP + wq * 32 + h * 16, dp);
-          }
+          if (some) tmem_read(t_lane + kXDqDP + wq * 32 + h * 16, dp);
           if (h == 1) {
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(dp_free);
+            warp_arrive(dp_free);
           }
           if (some) {
 #pragma unroll
@@ -459,17 +522,29 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
               const uint64_t d = add2(pair2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), nd2);
               float x0, x1;
               unpair2(mul2(pair2(__uint_as_float(s[16 * h + k]), __uint_as_float(s[16 * h + k + 1])), d), x0, x1);
-              s[8 * h + (k >> 1)] = XType<T>::pack2(x0, x1);  // the first 16 become dS
+              // in the place of the weights
+              if constexpr (SPLIT) {
+                if (single) x0 = x1 = 0.0f;
+                split2<T>(x0, x1, s[16 * h + k], s[16 * h + k + 1]);
+              } else {
+                s[16 * h + k] = XType<T>::pack2(x0, x1);
+              }
             }
           }
         }
         if (some) {
-          tmem_st_32x32b_x16(t_s, reinterpret_cast<const uint32_t(&)[16]>(s));
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            hi[k] = s[2 * k];
+            lo[k] = s[2 * k + 1];
+          }
+          tmem_st_32x32b_x16(t_s, hi);
+          if constexpr (SPLIT) tmem_st_32x32b_x16(t_s + 16, lo);
           tmem_st_wait();
         }
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ds_full);
+        warp_arrive(ds_full + (g & 1));
       }
       if (!ok) break;
       fetch(items);
@@ -497,8 +572,8 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(acc_free);
         mbar_arrive(staged);
+        mbar_arrive(acc_free);
       }
       if (tid == 0) {
         ok = mbar_wait(staged, n_item & 1, abort_flag, a.err, kErrXDq + kWaitStaged);
@@ -533,12 +608,12 @@ struct XDkvLayout {
   static constexpr int kStats = kQ + kEntries * kTileBytes;  // fp32 [kEntries / 2][2][128]
   static constexpr int kWords = kStats + kEntries / 2 * 1024;
   static constexpr int kBar = kWords + 2 * kKVStages * 16;
-  static constexpr int kNumBars = 2 * kKVStages + 2 * kEntries + 12;
+  static constexpr int kNumBars = 2 * kKVStages + 2 * kEntries + 14;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;
 };
 static_assert(XDkvLayout<1>::kSmemBytes <= 232448 && XDkvLayout<2>::kSmemBytes <= 232448, "dkv smem");
-// tensor memory columns: S^T (P^T over it), dP^T (dS^T over it), dV, dK
+// tensor memory columns: two buffers of S^T (P^T over it) and of dP^T (dS^T over it), dV, dK
 constexpr uint32_t kXDkvS = 0, kXDkvDP = 128, kXDkvV = 256;
 
 struct XDkvItem {
@@ -572,7 +647,12 @@ struct XDkvItems {
   }
 };
 
-template <typename T, int HALVES>
+// 64-row steps of row tile `tile` of a head group.
+__device__ __forceinline__ int x_row_steps(const XAttnParams& a, int tile) {
+  return (min(a.tile_tokens, a.q_len - tile * a.tile_tokens) * a.pack + 63) >> 6;
+}
+
+template <typename T, int HALVES, bool SPLIT>
 __global__ void __launch_bounds__(kXBwdThreads, 1)
     x_dkv_kernel(const XBwdParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap do_map,
@@ -586,16 +666,15 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
   uint64_t* kv_empty = kv_full + Ly::kKVStages;
   uint64_t* q_full = kv_empty + Ly::kKVStages;
   uint64_t* q_empty = q_full + Ly::kEntries;
+  // [2], by buffer
   uint64_t* s_full = q_empty + Ly::kEntries;
-  uint64_t* p_full = s_full + 1;
-  uint64_t* p_free = p_full + 1;  // P^T has been multiplied
-  uint64_t* dp_full = p_free + 1;
-  uint64_t* ds_full = dp_full + 1;
-  uint64_t* ds_free = ds_full + 1;  // dS^T has been multiplied
-  uint64_t* acc_full = ds_free + 1;
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* ds_full = dp_full + 2;  // P^T and dS^T are there
+  uint64_t* ds_free = ds_full + 2;  // and have been multiplied
+  uint64_t* staged = ds_free + 2;   // [2], by group
+  uint64_t* drained = staged + 2;   // [2], by issuing warp
+  uint64_t* acc_full = drained + 2;
   uint64_t* acc_free = acc_full + 1;
-  uint64_t* staged = acc_free + 1;   // [2], by half of the softmax threads
-  uint64_t* drained = staged + 2;    // [2], by issuing warp
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::kTail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -609,20 +688,18 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
     }
     for (int i = 0; i < Ly::kEntries; ++i) {
       mbar_init(q_full + i, 1);
-      mbar_init(q_empty + i, 1 + i % 2);  // Q: its dK product (S^T came before); dO: its dP^T and its dV product
+      mbar_init(q_empty + i, 1);  // by the dK or dV products, before which S^T and dP^T were done
     }
-    mbar_init(s_full, 2);  // the products' commit, and the issuing thread (keep bits)
-    mbar_init(p_full, kXBwdWarps);
-    mbar_init(p_free, 1);
-    mbar_init(dp_full, 1);
-    mbar_init(ds_free, 1);
-    mbar_init(ds_full, kXBwdWarps);
-    mbar_init(acc_full, 1);
-    mbar_init(acc_free, kXBwdWarps);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(staged + i, kXBwdWarps / 2);
+      mbar_init(s_full + i, 2);  // the products' commit, and the issuing thread (keep bits)
+      mbar_init(dp_full + i, 1);
+      mbar_init(ds_full + i, 8);
+      mbar_init(ds_free + i, 1);
+      mbar_init(staged + i, 8);
       mbar_init(drained + i, 1);
     }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_free, kXBwdWarps);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -704,8 +781,8 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
     }
   } else if (warp == kXBwdWarps + 1) {
     // ------------------------------------------------------------ products S^T = K Q^T, dP^T = V dO^T
-    const uint32_t idesc = x_idesc<T>(kXTile, 0, 0);
-    uint32_t n_item = 0, g = 0;
+    const uint32_t idesc = x_idesc<T>(64, 0, 0);
+    uint32_t n_item = 0, g = 0, n = 0;  // items, row tiles, 64-row steps
     bool ok = true;
     XDkvItems items(p);
     XDkvItem t;
@@ -722,28 +799,31 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       }
       const uint64_t sk = k_major_desc(s_base + 2 * ks * Ly::kTileBytes);
       const uint64_t sv = k_major_desc(s_base + (2 * ks + 1) * Ly::kTileBytes);
-      for (int j = t.j0; j < t.j1; ++j, ++g) {
+      for (int j = t.j0; j < t.j1 && ok; ++j, ++g) {
         const uint32_t eq = 2 * g % Ly::kEntries, phase = 2 * g / Ly::kEntries;
-        ok = wait(q_full + eq, phase, kWaitQ);
-        if (ok && g >= 1) ok = wait(p_free, g ^ 1, kWaitSFree);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          products_k_major(tmem + kXDkvS, sk, k_major_desc(s_base + Ly::kQ + eq * Ly::kTileBytes), idesc, ksteps);
-          umma_commit(s_full);
-          mbar_arrive(s_full);
+        const int steps = x_row_steps(a, j % p.row_tiles);
+        for (int u = 0; u < steps; ++u, ++n) {
+          const int buf = n & 1;
+          if (u == 0) ok = wait(q_full + eq, phase, kWaitQ);
+          if (ok && n >= 2) ok = wait(ds_free + buf, (n >> 1) ^ 1, kWaitSFree);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            products_k_major(tmem + kXDkvS + buf * 64, sk, k_major_desc(s_base + Ly::kQ + eq * Ly::kTileBytes + u * 8192), idesc,
+                             ksteps);
+            umma_commit(s_full + buf);
+            mbar_arrive(s_full + buf);
+          }
+          __syncwarp();
+          if (u == 0 && !(ok = wait(q_full + eq + 1, phase, kWaitV))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            products_k_major(tmem + kXDkvDP + buf * 64, sv,
+                             k_major_desc(s_base + Ly::kQ + (eq + 1) * Ly::kTileBytes + u * 8192), idesc, ksteps);
+            umma_commit(dp_full + buf);
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        ok = wait(q_full + eq + 1, phase, kWaitV);
-        if (ok && g >= 1) ok = wait(ds_free, g ^ 1, kWaitDPFree);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          products_k_major(tmem + kXDkvDP, sv, k_major_desc(s_base + Ly::kQ + (eq + 1) * Ly::kTileBytes), idesc, ksteps);
-          umma_commit(q_empty + eq + 1);
-          umma_commit(dp_full);
-        }
-        __syncwarp();
       }
       ++n_item;
     }
@@ -755,43 +835,35 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
   } else if (warp == kXBwdWarps + 2) {
     // ------------------------------------------------------------ products dV += P^T dO, dK += dS^T Q
     const uint32_t idesc = x_idesc<T>(ksteps * 16, 0, 1);
-    uint32_t n_item = 0, g = 0;
+    uint32_t n_item = 0, g = 0, n = 0;
     bool ok = true;
     XDkvItems items(p);
     XDkvItem t;
     while (ok && items.next(t)) {
       if (t.j0 >= t.j1) continue;
-      for (int j = t.j0; j < t.j1; ++j, ++g) {
+      for (int j = t.j0; j < t.j1 && ok; ++j, ++g) {
         const uint32_t eq = 2 * g % Ly::kEntries, phase = 2 * g / Ly::kEntries;
-        const uint64_t sq = mn_major_desc(s_base + Ly::kQ + eq * Ly::kTileBytes);
-        const uint64_t sdo = mn_major_desc(s_base + Ly::kQ + (eq + 1) * Ly::kTileBytes);
-        const uint32_t later = j > t.j0 ? 1u : 0u;
-        // 32 rows' P^T or dS^T lies in the first 16 of their columns
-        ok = wait(q_full + eq + 1, phase, kWaitV) && wait(p_full, g, kWaitP);
-        if (ok && j == t.j0 && n_item > 0) ok = wait(acc_free, n_item ^ 1, kWaitAccFree);  // the last item's sums have been read
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tmem + kXDkvV, tmem + kXDkvS + (k >> 1) * 32 + (k & 1) * 8, sdo + k * 128, idesc, k > 0 ? 1u : later);
-          umma_commit(p_free);
-          umma_commit(q_empty + eq + 1);
+        const int steps = x_row_steps(a, j % p.row_tiles);
+        for (int u = 0; u < steps; ++u, ++n) {
+          const int buf = n & 1;
+          if (u == 0) ok = wait(q_full + eq, phase, kWaitQ) && wait(q_full + eq + 1, phase, kWaitV);
+          ok = ok && wait(ds_full + buf, n >> 1, kWaitP);
+          if (ok && j == t.j0 && u == 0 && n_item > 0) ok = wait(acc_free, n_item ^ 1, kWaitAccFree);  // the last item's sums have been read
+          if (!ok) break;
+          const uint64_t sq = mn_major_desc(s_base + Ly::kQ + eq * Ly::kTileBytes + u * 8192);
+          const uint64_t sdo = mn_major_desc(s_base + Ly::kQ + (eq + 1) * Ly::kTileBytes + u * 8192);
+          const uint32_t later = j > t.j0 || u > 0 ? 1u : 0u;
+          tc_fence_after();
+          if (elect_one()) {
+            x_products_mn<SPLIT, 4>(tmem + kXDkvV, tmem + kXDkvS + buf * 64, sdo, idesc, 4, later);
+            if (u == steps - 1) umma_commit(q_empty + eq + 1);
+            x_products_mn<SPLIT, 4>(tmem + kXDkvV + HALVES * 64, tmem + kXDkvDP + buf * 64, sq, idesc, 4, later);
+            if (u == steps - 1) umma_commit(q_empty + eq);
+            umma_commit(ds_free + buf);
+            if (j == t.j1 - 1 && u == steps - 1) umma_commit(acc_full);
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        ok = wait(q_full + eq, phase, kWaitQ) && wait(ds_full, g, kWaitPRest);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tmem + kXDkvV + HALVES * 64, tmem + kXDkvDP + (k >> 1) * 32 + (k & 1) * 8, sq + k * 128, idesc,
-                        k > 0 ? 1u : later);
-          umma_commit(ds_free);
-          umma_commit(q_empty + eq);
-          if (j == t.j1 - 1) umma_commit(acc_full);
-        }
-        __syncwarp();
       }
       ++n_item;
     }
@@ -801,14 +873,14 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       mbar_wait(drained + 1, 0, &never, a.err, kErrXDkv + kWaitDrain);
     }
   } else {
-    // ------------------------------------------------------------ P^T, dS^T: thread = key, the 32 rows of chunk wq
-    const int wq = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
-    const int is_k = wq >> 1;  // the first half of the threads hands out dV, the second dK
+    // ------------------------------------------------------------ P^T, dS^T: thread = key and 32 rows, the steps of group gp
+    const int gp = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3, key = quad * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t t_s = t_lane + kXDkvS + gp * 64 + half * 32, t_dp = t_s + (kXDkvDP - kXDkvS);  // a group's steps use one buffer
     const float c2 = a.scale * 1.4426950408889634f;
     const uint64_t c22 = pair2(c2, c2);
-    const bool hands_out = (warp & 7) == 0 && lane == 0;
-    uint32_t n_item = 0, g = 0;
+    const bool hands_out = (warp & 7) == 0 && lane == 0;  // of dV (group 0) or dK (group 1)
+    uint32_t n_item = 0, g = 0, n = 0;
     int stored = -1;  // K / V stage whose gradient is on its way out
     const auto release_stored = [&]() {
       if (stored >= 0 && hands_out) {
@@ -822,16 +894,15 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
     XDkvItem t;
     while (ok && items.next(t)) {
       const int j_key = t.tile * kXTile + key;
-      const int c0 = (wq & 1) * HALVES * 32;  // this thread's channels: [c0, c0 + HALVES * 32)
-      const auto part = [&](int c) {          // this key's row of the split's partial sums
-        return p.part + ((((static_cast<int64_t>(t.split) * 2 + is_k) * a.batch + t.b) * a.k_len + j_key) * a.kv_heads + t.hk) *
+      const auto part = [&](int c) {  // this key's row of the split's partial sums
+        return p.part + ((((static_cast<int64_t>(t.split) * 2 + gp) * a.batch + t.b) * a.k_len + j_key) * a.kv_heads + t.hk) *
                             a.head_dim + c;
       };
       if (t.j0 >= t.j1) {  // no keys in this tile (or no rows in this split)
-        if (j_key < a.k_len) {
-          T* grad = is_k ? static_cast<T*>(a.dk) + t.b * a.sdk.batch + j_key * a.sdk.token + t.hk * a.sdk.head
-                         : static_cast<T*>(a.dv) + t.b * a.sdv.batch + j_key * a.sdv.token + t.hk * a.sdv.head;
-          for (int c = c0; c < min(a.head_dim, c0 + HALVES * 32); c += 8) {
+        if (j_key < a.k_len && half == 0) {
+          T* grad = gp ? static_cast<T*>(a.dk) + t.b * a.sdk.batch + j_key * a.sdk.token + t.hk * a.sdk.head
+                       : static_cast<T*>(a.dv) + t.b * a.sdv.batch + j_key * a.sdv.token + t.hk * a.sdv.head;
+          for (int c = 0; c < a.head_dim; c += 8) {
             if (p.splits > 1) {
               *reinterpret_cast<float4*>(part(c)) = make_float4(0, 0, 0, 0);
               *reinterpret_cast<float4*>(part(c + 4)) = make_float4(0, 0, 0, 0);
@@ -842,62 +913,55 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         }
         continue;
       }
-      bool kept = false;
-      for (int j = t.j0; j < t.j1; ++j, ++g) {
-        ok = wait(s_full, g, kWaitS);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t t_s = t_lane + kXDkvS + wq * 32, t_dp = t_lane + kXDkvDP + wq * 32;
-        const float4* neg_lse = reinterpret_cast<const float4*>(stats + g % (Ly::kEntries / 2) * 2 * kXTile + wq * 32);
-        const float4* neg_delta = neg_lse + kXTile / 4;
-        if (j == t.j0)
-          kept = (reinterpret_cast<const uint32_t*>(words + n_item % (2 * Ly::kKVStages))[quad] >> lane) & 1u;
-        uint32_t s[32];
-        tmem_read(t_s, s);
-        uint32_t pk[16];
+      for (int j = t.j0; j < t.j1 && ok; ++j, ++g) {
+        const int steps = x_row_steps(a, j % p.row_tiles);
+        for (int u = 0; u < steps; ++u, ++n) {
+          if ((n & 1) != static_cast<uint32_t>(gp)) continue;
+          ok = wait(s_full + gp, n >> 1, kWaitS);
+          if (!ok) break;
+          tc_fence_after();
+          const float4* neg_lse =
+              reinterpret_cast<const float4*>(stats + g % (Ly::kEntries / 2) * 2 * kXTile + u * 64 + half * 32);
+          const float4* neg_delta = neg_lse + kXTile / 4;
+          float pr[32];
+          {
+            uint32_t s[32];
+            tmem_read(t_s, s);
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          const float4 nl = neg_lse[k >> 2];
-          float x0, x1, x2, x3;
-          unpair2(fma2(pair2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c22, pair2(nl.x, nl.y)), x0, x1);
-          unpair2(fma2(pair2(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])), c22, pair2(nl.z, nl.w)), x2, x3);
-          x0 = ex2(x0);
-          x1 = ex2(x1);
-          x2 = ex2(x2);
-          x3 = ex2(x3);
-          s[k] = __float_as_uint(x0);
-          s[k + 1] = __float_as_uint(x1);
-          s[k + 2] = __float_as_uint(x2);
-          s[k + 3] = __float_as_uint(x3);
-          pk[k >> 1] = XType<T>::pack2(x0, x1);
-          pk[(k >> 1) + 1] = XType<T>::pack2(x2, x3);
-        }
-        tmem_st_32x32b_x16(t_s, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
-        ok = wait(dp_full, g, kWaitDP);
-        if (!ok) break;
-        tc_fence_after();
-        uint32_t dp[32];
-        tmem_read(t_dp, dp);
+            for (int k = 0; k < 32; k += 4) {
+              const float4 nl = neg_lse[k >> 2];
+              float x0, x1, x2, x3;
+              unpair2(fma2(pair2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c22, pair2(nl.x, nl.y)), x0, x1);
+              unpair2(fma2(pair2(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])), c22, pair2(nl.z, nl.w)), x2, x3);
+              pr[k] = ex2(x0);
+              pr[k + 1] = ex2(x1);
+              pr[k + 2] = ex2(x2);
+              pr[k + 3] = ex2(x3);
+            }
+            x_store_operand<T, SPLIT>(t_s, pr);
+          }
+          ok = wait(dp_full + gp, n >> 1, kWaitDP);
+          if (!ok) break;
+          tc_fence_after();
+          {
+            uint32_t dp[32];
+            tmem_read(t_dp, dp);
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          const float4 nd = neg_delta[k >> 2];
-          float x0, x1, x2, x3;
-          unpair2(mul2(pair2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
-                       add2(pair2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), pair2(nd.x, nd.y))), x0, x1);
-          unpair2(mul2(pair2(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])),
-                       add2(pair2(__uint_as_float(dp[k + 2]), __uint_as_float(dp[k + 3])), pair2(nd.z, nd.w))), x2, x3);
-          pk[k >> 1] = XType<T>::pack2(x0, x1);
-          pk[(k >> 1) + 1] = XType<T>::pack2(x2, x3);
+            for (int k = 0; k < 32; k += 4) {
+              const float4 nd = neg_delta[k >> 2];
+              unpair2(mul2(pair2(pr[k], pr[k + 1]),
+                           add2(pair2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), pair2(nd.x, nd.y))),
+                      pr[k], pr[k + 1]);
+              unpair2(mul2(pair2(pr[k + 2], pr[k + 3]),
+                           add2(pair2(__uint_as_float(dp[k + 2]), __uint_as_float(dp[k + 3])), pair2(nd.z, nd.w))),
+                      pr[k + 2], pr[k + 3]);
+            }
+            x_store_operand<T, SPLIT>(t_dp, pr);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          warp_arrive(ds_full + gp);
         }
-        tmem_st_32x32b_x16(t_dp, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ds_full);
       }
       if (!ok) break;
       release_stored();
@@ -905,16 +969,21 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       if (!ok) break;
       tc_fence_after();
       const int ks = n_item % Ly::kKVStages;
+      const uint4 w = words[n_item % (2 * Ly::kKVStages)];
+      const bool kept = ((quad == 0 ? w.x : quad == 1 ? w.y : quad == 2 ? w.z : w.w) >> lane) & 1u;
+      // where one key is all there is, its weight is 1 whatever its score
+      const bool single = SPLIT && __popc(w.x) + __popc(w.y) + __popc(w.z) + __popc(w.w) == 1;
       // dV goes out from V's tile, dK from K's
-      uint8_t* stage = smem + (2 * ks + 1 - is_k) * Ly::kTileBytes;
-      const float f = is_k ? a.scale : 1.0f;
+      uint8_t* stage = smem + (2 * ks + 1 - gp) * Ly::kTileBytes;
+      const float f = gp ? a.scale : 1.0f;
+      const bool zero = !kept || (gp && single);
 #pragma unroll
       for (int c = 0; c < HALVES; ++c) {
-        const int col = c0 + c * 32;
+        const int col = (half * HALVES + c) * 32;
         uint32_t o[32];
-        tmem_read(t_lane + kXDkvV + is_k * HALVES * 64 + col, o);
+        tmem_read(t_lane + kXDkvV + gp * HALVES * 64 + col, o);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] = kept ? __float_as_uint(__uint_as_float(o[k]) * f) : 0u;
+        for (int k = 0; k < 32; ++k) o[k] = zero ? 0u : __float_as_uint(__uint_as_float(o[k]) * f);
         if (p.splits > 1) {
           if (j_key < a.k_len) {
 #pragma unroll
@@ -926,25 +995,25 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
           uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 2) pk[k >> 1] = XType<T>::pack2(__uint_as_float(o[k]), __uint_as_float(o[k + 1]));
-          uint8_t* half = stage + (col >> 6) * 16384;
+          uint8_t* dst = stage + (col >> 6) * 16384;
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            st_shared_v4(half + swizzle128_offset(key, ((col & 63) >> 3) + u), pk[4 * u], pk[4 * u + 1], pk[4 * u + 2],
-                         pk[4 * u + 3]);
+          for (int i = 0; i < 4; ++i)
+            st_shared_v4(dst + swizzle128_offset(key, ((col & 63) >> 3) + i), pk[4 * i], pk[4 * i + 1], pk[4 * i + 2],
+                         pk[4 * i + 3]);
         }
       }
       tc_fence_before();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
+        mbar_arrive(staged + gp);
         mbar_arrive(acc_free);
-        mbar_arrive(staged + is_k);
       }
       if (hands_out) {
-        ok = mbar_wait(staged + is_k, n_item & 1, abort_flag, a.err, kErrXDkv + kWaitStaged);
+        ok = mbar_wait(staged + gp, n_item & 1, abort_flag, a.err, kErrXDkv + kWaitStaged);
         if (ok && p.splits == 1) {
           for (int hf = 0; hf < HALVES; ++hf)
-            tma_store_4d(is_k ? &dk_map : &dv_map, stage + hf * 16384, hf * 64, t.hk, t.tile * kXTile, t.b);
+            tma_store_4d(gp ? &dk_map : &dv_map, stage + hf * 16384, hf * 64, t.hk, t.tile * kXTile, t.b);
           bulk_commit_group();
         }
       }
