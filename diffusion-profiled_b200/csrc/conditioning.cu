@@ -409,6 +409,11 @@ EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
   return w;
 }
 
+// embed_few_kernel takes the gradient: see kFewTokens (and its grid stays small).
+bool embed_few(int64_t tokens, int width) {
+  return tokens <= kFewTokens && tokens * ((width + kSumSlice - 1) / kSumSlice) <= 1 << 16;
+}
+
 }  // namespace
 
 static int embed_check(const void* ids, int ids64, int64_t tokens, int64_t vocab, int width, int weight_dtype,
@@ -459,7 +464,7 @@ int fp8_embedding_fwd(const void* ids, int ids64, int64_t tokens, const void* we
 
 size_t fp8_embedding_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int width) {
   if (tokens < 0 || vocab <= 0 || width <= 0) return 0;
-  return embed_plan(tokens, vocab, width).bytes;
+  return embed_few(tokens, width) ? 0 : embed_plan(tokens, vocab, width).bytes;
 }
 
 int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* dout, int out_dtype, void* dweight,
@@ -471,12 +476,40 @@ int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* do
               FP8_ERR_INVALID_ARGUMENT, "embedding backward: dout or dweight is NULL or misaligned");
   FP8_REQUIRE(tokens < (1ll << 31) - (1 << 20) && vocab < (1ll << 31) - 1, FP8_ERR_UNSUPPORTED,
               "embedding backward: too many tokens (%lld) or rows (%lld)", (long long)tokens, (long long)vocab);
+  DeviceState* st = nullptr;
+  if (int s = device_state(&st)) return s;
+  const bool vec = width % 8 == 0 && aligned(dout, 16) && aligned(dweight, 16);
+  if (embed_few(tokens, width)) {
+    EmbedFewParams f{};
+    f.ids = ids;
+    f.ids64 = ids64;
+    f.tokens = static_cast<int>(tokens);
+    f.dout = dout;
+    f.dweight = dweight;
+    f.vocab = vocab;
+    f.padding_idx = padding_idx;
+    f.slices = (width + kSumSlice - 1) / kSumSlice;
+    f.width = width;
+    f.zero_ctas = static_cast<int>(grid_for(vocab, kFewRows, st->sm_count, 8));
+    f.scale = scale;
+    const int status = with_dtype(weight_dtype, [&](auto wt) {
+      return with_dtype(out_dtype, [&](auto o) {
+        using TW = decltype(wt);
+        using TO = decltype(o);
+        FP8_CUDA_TRY(launch_kernel(vec ? embed_few_kernel<TW, TO, true> : embed_few_kernel<TW, TO, false>,
+                                   dim3(static_cast<unsigned>(f.zero_ctas + f.tokens * f.slices)), dim3(kFewThreads), 0,
+                                   cuda_stream(stream), 1, kStreamingKernel, f));
+        return FP8_OK;
+      });
+    });
+    if (status) return status;
+    count_launches(1);
+    return ok();
+  }
   const EmbedPlan w = embed_plan(tokens, vocab, width);
   FP8_REQUIRE(workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= w.bytes, FP8_ERR_WORKSPACE,
               "embedding backward: workspace too small or not 16-byte aligned (%zu bytes, needs %zu)", workspace_bytes,
               w.bytes);
-  DeviceState* st = nullptr;
-  if (int s = device_state(&st)) return s;
   char* const ws = static_cast<char*>(workspace);
   EmbedSortParams so{};
   so.ids = ids;
@@ -526,7 +559,6 @@ int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* do
   su.slices = w.slices;
   su.width = width;
   su.scale = scale;
-  const bool vec = width % 8 == 0 && aligned(dout, 16) && aligned(dweight, 16);
   const int64_t joins = w.chunks * w.slices;
   const int status = with_dtype(weight_dtype, [&](auto wt) {
     using TW = decltype(wt);

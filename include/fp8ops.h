@@ -576,7 +576,8 @@ int fp8_embedding_fwd(const void* ids, int ids64, int64_t tokens, const void* we
 /* Its gradient: dweight[v][c] = scale * sum of dout[i][c] over the tokens i with
  * ids[i] = v, zero for tokens that do not occur and for padding_idx (< 0: none).
  * Every element of the dense [vocab][width] dweight is written.  The sums are fp32,
- * in an order that the ids alone fix: the same call gives the same bits. */
+ * in an order that the ids alone fix: the same call gives the same bits.  Few tokens
+ * need no workspace (0 bytes; NULL will do). */
 size_t fp8_embedding_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int width);
 int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* dout, int out_dtype, void* dweight,
                       int weight_dtype, int64_t vocab, int width, float scale, int64_t padding_idx, void* workspace,

@@ -65,6 +65,21 @@ def test_lookup_and_gradient(cuda, n, vocab, width, wdtype, dtype):
         assert torch.count_nonzero(wd.grad[pad]) == 0
 
 
+# one launch up to 1024 tokens (of rows that are not too wide), three beyond
+@pytest.mark.parametrize("kind", ["one", "uniform", "zipf"])
+@pytest.mark.parametrize("n,vocab,width", [(255, 65, 777), (257, 64, 72), (1023, 63, 264), (1024, 4001, 250),
+                                           (1025, 4001, 250), (2049, 1, 64), (1024, 5, 16648)])
+def test_gradient_at_the_choice_of_launches(cuda, kind, n, vocab, width):
+    from fp8_b200.embedding import embedding_bwd
+
+    ids, _, dout = _case(n, vocab, width, FP32, BF16, kind, seed=n)
+    ids[n // 2] = vocab  # one id outside the vocabulary adds to nothing
+    got = embedding_bwd(ids.to(cuda), dout.to(cuda), vocab, 0.5, vocab - 1, FP32)
+    inside = ids < vocab
+    _check_grad(got, ids[inside], dout[inside], vocab, 0.5, vocab - 1)
+    assert torch.equal(got, embedding_bwd(ids.to(cuda).int(), dout.to(cuda), vocab, 0.5, vocab - 1, FP32))
+
+
 @pytest.mark.parametrize("kind", ["one", "uniform", "zipf"])
 @pytest.mark.parametrize("n", [31, 1024, 20000])
 def test_gradient_is_the_same_every_time(cuda, kind, n):
