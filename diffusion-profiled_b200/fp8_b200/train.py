@@ -52,9 +52,10 @@ class LinearSchedule:
         return self.mix(x, eps, t), eps, t
 
 
-def diffusion_loss(model: torch.nn.Module, x: torch.Tensor, sched: LinearSchedule) -> torch.Tensor:
+def diffusion_loss(model: torch.nn.Module, x: torch.Tensor, sched: LinearSchedule, *prompt: torch.Tensor) -> torch.Tensor:
+    """``prompt``: ids and lengths, for a UNet that is conditioned on them."""
     x_t, eps, t = sched.noise(x)
-    return F.mse_loss(model(x_t, t), eps)
+    return F.mse_loss(model(x_t, t, *prompt), eps)
 
 
 # ----------------------------------------------------------------------------- gradient all-reduce
@@ -236,6 +237,12 @@ class GraphedTrainStep:
         self.external_noise = external_noise
         self.static_t = torch.zeros(cfg.batch_size, dtype=torch.int64, device=device)
         self.static_eps = torch.zeros_like(self.static_batch)
+        # a prompt for each image, for a UNet that takes them (step(images, prompt_ids=.., prompt_lengths=..))
+        self.static_prompt: tuple[torch.Tensor, ...] = ()
+        if model.config.prompt_vocab > 0:
+            self.static_prompt = (
+                torch.zeros(cfg.batch_size, model.config.prompt_tokens, dtype=torch.int64, device=device),
+                torch.full((cfg.batch_size,), model.config.prompt_tokens, dtype=torch.int32, device=device))
         self.loss_acc = torch.zeros((), device=device)
         self.graph = None
         self.use_graph = use_graph
@@ -251,9 +258,9 @@ class GraphedTrainStep:
         with torch.autocast(device_type="cuda", dtype=torch.bfloat16):
             if self.external_noise:
                 x_t = self.sched.mix(self.static_batch, self.static_eps, self.static_t)
-                loss = F.mse_loss(self.model(x_t, self.static_t), self.static_eps)
+                loss = F.mse_loss(self.model(x_t, self.static_t, *self.static_prompt), self.static_eps)
             else:
-                loss = diffusion_loss(self.model, self.static_batch, self.sched)
+                loss = diffusion_loss(self.model, self.static_batch, self.sched, *self.static_prompt)
         self.loss_acc.add_(loss.detach())
         loss.backward()
         if self.dp is not None:
@@ -296,13 +303,17 @@ class GraphedTrainStep:
         self.loss_acc.zero_()
 
     def step(self, images: torch.Tensor | None = None, t: torch.Tensor | None = None,
-             eps: torch.Tensor | None = None) -> None:
+             eps: torch.Tensor | None = None, prompt_ids: torch.Tensor | None = None,
+             prompt_lengths: torch.Tensor | None = None) -> None:
         if images is not None:
             self.static_batch.copy_(images, non_blocking=True)
         if t is not None:
             self.static_t.copy_(t, non_blocking=True)
         if eps is not None:
             self.static_eps.copy_(eps, non_blocking=True)
+        for static, given in zip(self.static_prompt, (prompt_ids, prompt_lengths)):
+            if given is not None:
+                static.copy_(given, non_blocking=True)
         if self.graph is not None:
             self.graph.replay()
         else:
@@ -318,13 +329,14 @@ class GraphedTrainStep:
 def build_model(fp8: bool = True, scaling: str = "delayed", attn_resolutions=(16,), p_drop: float = 0.1,
                 device: torch.device | str = "cuda", seed: int = 0, fused_norm: bool = True,
                 fused_resample: bool | None = None, plain: bool = False, skip_empty: bool = False,
-                fp8_attention: bool = False, extended_shapes: bool = False) -> UNet:
+                fp8_attention: bool = False, extended_shapes: bool = False, prompt_vocab: int = 0) -> UNet:
     """The reference UNet; ``fused_norm`` / ``fused_resample`` (default: as ``fused_norm``) route its
     norm -> activation chains and its resampling + concatenation to this library's kernels.
     ``plain``: the reference's op structure throughout (every FP8 conv a ``triton_conv2d_fp8`` call,
     scale windows kept by torch ops in the module).  ``skip_empty``: ``fp8_history_skip_empty``.
     ``fp8_attention``: the attention blocks on the FP8 attention kernels.  ``extended_shapes``:
-    ``fp8_extended_shapes`` (FP8 also for the 3x3 convs outside the reference's whitelist)."""
+    ``fp8_extended_shapes`` (FP8 also for the 3x3 convs outside the reference's whitelist).
+    ``prompt_vocab``: condition on prompts of that many token ids (``UNetConfig.prompt_vocab``)."""
     torch.manual_seed(seed)
     if plain:
         fused_norm, fused_resample = False, False
@@ -333,7 +345,7 @@ def build_model(fp8: bool = True, scaling: str = "delayed", attn_resolutions=(16
                      p_drop=p_drop, fused_norm=fused_norm, fused_resample=fr, fused_residual=fr,
                      batched_time_embed=fr, fused_skip_cast=fr, batched_weight_cast=fr,
                      device_scale_history=not plain, fp8_history_skip_empty=skip_empty,
-                     fp8_attention=fp8_attention, fp8_extended_shapes=extended_shapes)
+                     fp8_attention=fp8_attention, fp8_extended_shapes=extended_shapes, prompt_vocab=prompt_vocab)
     model = UNet(cfg).to(memory_format=torch.channels_last)
     return model.to(device)
 

@@ -29,6 +29,7 @@ import torch.nn.functional as F
 
 from . import _lib, ops
 from .attention import attention_supported, fp8_attention
+from .conditioning import PromptAttention, PromptEncoder
 from .delayed import ConvFP8Delayed, GroupNormActConvFP8Delayed, quantize_conv_weights
 from .fp8_kernels import SUPPORTED_UNET_SHAPES, triton_conv2d_fp8
 from .resample import downsample_nearest, residual_join, upsample_cat, upsample_cat_pair
@@ -87,6 +88,13 @@ class UNetConfig:
     # (fp8_b200.attention: e4m3 q, k, v per image and head, FP8 QK^T and PV) instead of the
     # reference's bf16 scaled_dot_product_attention (unet.py:197).  Off by default.
     fp8_attention: bool = False
+    # condition on a prompt (fp8_b200.conditioning): the number of token ids, 0 for the reference's
+    # unconditional UNet.  Each attention block is followed by one over the prompt's states, and
+    # forward takes the ids [B, up to prompt_tokens] and each prompt's length.
+    prompt_vocab: int = 0
+    prompt_width: int = 512
+    prompt_tokens: int = 77
+    prompt_padding_idx: int | None = None
 
     def as_dict(self):
         return asdict(self)
@@ -326,10 +334,17 @@ class Stage(nn.Module):
         self.attns = nn.ModuleList(
             CHWAttention(config, widths[i + 1]) if attention else nn.Identity() for i in range(num_blocks)
         )
+        self.prompt_attns = None
+        if attention and config.prompt_vocab > 0:
+            self.prompt_attns = nn.ModuleList(
+                PromptAttention(widths[i + 1], config.prompt_width, config.n_heads, config.p_drop) for i in range(num_blocks)
+            )
 
-    def forward(self, x: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
-        for block, attn in zip(self.blocks, self.attns):
+    def forward(self, x: torch.Tensor, t: torch.Tensor, prompt=None) -> torch.Tensor:
+        for i, (block, attn) in enumerate(zip(self.blocks, self.attns)):
             x = attn(block(x, t))
+            if prompt is not None and self.prompt_attns is not None:
+                x = self.prompt_attns[i](x, *prompt)
         return x
 
 
@@ -362,6 +377,10 @@ class UNet(nn.Module):
             nn.GroupNorm(32, chans[0]), nn.SiLU(),
             nn.Conv2d(chans[0], config.in_channels, (3, 3), padding=1, bias=False),
         )
+        self.prompt = None
+        if config.prompt_vocab > 0:
+            self.prompt = PromptEncoder(config.prompt_vocab, config.prompt_width, config.prompt_tokens,
+                                        config.prompt_padding_idx, config.p_drop)
         self.time_embed = nn.Sequential(
             nn.Linear(base, 4 * base, bias=False), nn.SiLU(), nn.Linear(4 * base, 4 * base, bias=False), nn.SiLU(),
         )
@@ -384,8 +403,11 @@ class UNet(nn.Module):
             emb = F.pad(emb, (0, 1))
         return emb
 
-    def forward(self, x: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, t: torch.Tensor, prompt_ids: torch.Tensor | None = None,
+                prompt_lengths: torch.Tensor | None = None) -> torch.Tensor:
         cfg = self.config
+        if (prompt_ids is None) != (self.prompt is None):
+            raise RuntimeError("the UNet takes prompt ids if and only if it was built with prompt_vocab > 0")
         if cfg.fp8_convs_enabled and cfg.fp8_scaling_type == "delayed" and cfg.device_scale_history:
             # process-wide mode, read by the history-updating launches of this step (forward and backward)
             _lib.set_empty_tensor_history(1 if cfg.fp8_history_skip_empty else 0)
@@ -400,7 +422,8 @@ class UNet(nn.Module):
             self.dropout_seed.add_(1)
             for i, b in enumerate(self._res_blocks):
                 b._seed = seeds[i]
-        out = self._forward(x, t)
+        prompt = None if prompt_ids is None else (self.prompt(prompt_ids), prompt_lengths)
+        out = self._forward(x, t, prompt)
         for b in self._res_blocks:
             b._seed = None
         convs = [m for m in self.modules() if isinstance(m, Conv2dFP8) and m.used_fp8_delayed]
@@ -443,7 +466,7 @@ class UNet(nn.Module):
         for b, part in zip(blocks, torch.split(e, [w.shape[0] for w in weights], dim=1)):
             b._emb = part[:, :, None, None]
 
-    def _forward(self, x: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
+    def _forward(self, x: torch.Tensor, t: torch.Tensor, prompt=None) -> torch.Tensor:
         w16, self._time_w16 = self._time_w16, None
         if w16 is None:
             t_emb = self.time_embed(self._timestep(t))
@@ -458,9 +481,9 @@ class UNet(nn.Module):
         for i, stage in enumerate(self.down_stages):
             if i > 0:
                 act = downsample_nearest(act) if fused else F.interpolate(act, scale_factor=0.5, mode="nearest")
-            act = stage(act, t_emb)
+            act = stage(act, t_emb, prompt)
             skips.append(act)
-        act = self.mid(act, t_emb)
+        act = self.mid(act, t_emb, prompt)
         for i, stage in enumerate(self.up_stages):
             h = skips.pop()
             if fused:
@@ -469,10 +492,10 @@ class UNet(nn.Module):
                     y, blk._skip_in = upsample_cat_pair(act, h, 2 if i > 0 else 1)
                 else:
                     y = upsample_cat(act, h, 2 if i > 0 else 1)
-                act = stage(y, t_emb)
+                act = stage(y, t_emb, prompt)
             else:
                 up = F.interpolate(act, scale_factor=2.0, mode="nearest") if i > 0 else act
-                act = stage(torch.cat([up, h], dim=1), t_emb)
+                act = stage(torch.cat([up, h], dim=1), t_emb, prompt)
         if self.config.fused_norm and fused_norm_supported(act, self.out[0]):
             return self.out[2](group_norm_act(act, self.out[0]))
         return self.out(act)
