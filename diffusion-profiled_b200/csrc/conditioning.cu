@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "cross_attention.cuh"
@@ -147,12 +148,30 @@ int bind_context() {
   return FP8_OK;
 }
 
-constexpr int kXMaxSplits = 128;
 
 // How a forward call divides its work.
+// Counters at which the splits of a forward call meet, zero between launches.  A launch takes the next ones of a ring:
+// half as many as it has CTAs at most, so launches that can run at the same time use different ones unless some 7,000
+// of them were issued between the two.
+__device__ unsigned int g_x_join_counters[kXJoinCounters];
+
+int x_join_counters(DeviceState* st, uint32_t n, unsigned int** ring, uint32_t* at) {
+  static std::atomic<uint32_t> next{0};
+  *ring = st->join_base.load(std::memory_order_relaxed);
+  if (*ring == nullptr) {  // every caller finds the same address
+    void* p = nullptr;
+    FP8_CUDA_TRY(cudaGetSymbolAddress(&p, g_x_join_counters));
+    *ring = static_cast<unsigned int*>(p);
+    st->join_base.store(*ring, std::memory_order_relaxed);
+  }
+  *at = next.fetch_add(n, std::memory_order_relaxed);
+  return FP8_OK;
+}
+
 struct XPlan {
   int row_tiles, hv, n_tiles, nt, splits, key_chunk;
   int64_t rows, items, slots;
+  bool join_inside;  // x_join
 };
 XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
   XPlan w{};
@@ -177,6 +196,7 @@ XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
     w.splits = (w.n_tiles + w.key_chunk - 1) / w.key_chunk;
   }
   w.items = base * w.splits;
+  w.join_inside = few_rows && w.splits > 1 && w.items <= w.slots;
   return w;
 }
 size_t x_fwd_workspace(const fp8_cross_attention_args* a, const XPlan& w) {
@@ -208,6 +228,8 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
   f.rows = w.rows;
   f.items = static_cast<uint32_t>(w.items);
   if (int s = bind_context()) return s;
+  if (w.join_inside)
+    if (int s = x_join_counters(st, static_cast<uint32_t>(w.items / w.splits), &f.join, &f.join_at)) return s;
   CUtensorMap maps[4];
   const int dt = args->dtype;
   if (int s = x_map(&maps[0], a.q, dt, a.sq, a.batch, a.q_len, a.heads, a.head_dim, a.pack, a.tile_tokens)) return s;
@@ -220,7 +242,7 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
                                       : (w.nt == 1 ? x_fwd_launch<T, 2, 1>(f, maps, one, w.slots, stream)
                                                    : x_fwd_launch<T, 2, 2>(f, maps, one, w.slots, stream));
   if (status) return status;
-  if (w.splits > 1) {
+  if (w.splits > 1 && !w.join_inside) {
     FP8_CUDA_TRY(launch_kernel(x_combine_kernel<T>, dim3(grid_for(w.rows, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,
                                kStreamingKernel, f));
     count_launches(1);

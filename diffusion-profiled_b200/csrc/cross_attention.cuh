@@ -171,8 +171,7 @@ __device__ __forceinline__ void products_k_major(uint32_t d_tmem, uint64_t a, ui
 }
 
 // 32 lanes x 32 (16) columns, TMEM -> register, and the wait for them.  One statement, so that nothing can use the
-// registers before the wait, and nothing has to copy them after it (an empty statement that the registers pass through
-// in the wait's place cost a move a register: 2.6 of the forward's 7.6 instructions a score).
+// registers before the wait.
 __device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -203,17 +202,6 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -343,7 +331,13 @@ struct XFwdParams {
   float* part_lse;  // [splits][batch * heads * q_len], base-2 logarithm
   int64_t rows;     // batch * heads * q_len
   uint32_t items;   // (sequence, head group, row tile group, split)
+  // where the launch itself joins the splits (x_join): a ring of counters, zero between launches, of which it has those
+  // from join_at on, one for each (sequence, head group); else null
+  unsigned int* join;
+  uint32_t join_at;
 };
+constexpr uint32_t kXJoinCounters = 1u << 20;
+constexpr int kXMaxSplits = 128;
 
 // NT row tiles of HALVES * 64 channels a CTA.
 template <int HALVES, int NT>
@@ -404,6 +398,84 @@ struct XItems {
 // 32-key chunks of key tile j that hold keys, and of the 64 keys from u * 64.
 __device__ __forceinline__ int x_chunks(int keys, int j) { return (min(kXTile, keys - j * kXTile) + 31) >> 5; }
 __device__ __forceinline__ int x_chunks64(int keys, int u) { return (min(64, keys - u * 64) + 31) >> 5; }
+
+// This warp's rows of a split are written.  The warp that is the last of the splits to say so joins them, in the order
+// of the splits: o = sum_s 2^(lse_s - lse) o_s.  For calls of one warp's rows a (sequence, head group) and one item a
+// CTA: it takes as long as x_combine_kernel does (one query, 1,024 keys: 10.6 us in all), but no launch, whose time on
+// the host such a call waits for.  Where a CTA goes on with other items, the wait for the memory's answer, behind the
+// copies under way, holds them up: 32 queries over 8,192 keys took 161 us, with the second launch 97.
+// r_index: this lane's row; o_at: where its output goes.
+template <typename T>
+__device__ __forceinline__ void x_join(const XFwdParams& p, uint32_t counter, bool live, int64_t r_index, int64_t o_at) {
+  const int lane = threadIdx.x & 31;
+  unsigned int* const arrived = p.join + (p.join_at + counter) % kXJoinCounters;
+  __syncwarp();  // the other lanes' writes come before this one's release
+  unsigned int before = 0;
+  if (lane == 0) before = atom_add_acq_rel_gpu_u32(arrived, 1u);
+  if (__shfl_sync(~0u, before, 0) + 1 != static_cast<unsigned int>(p.splits)) return;
+  if (lane == 0) *arrived = 0;
+  const int head_dim = p.a.head_dim, rows = __popc(__ballot_sync(~0u, live));  // the first lanes
+  // ---- lane = row: the sum of the splits' weights
+  constexpr int kAtOnce = 8;
+  float m = -INFINITY, total = 0.0f;
+  for (int s0 = 0; s0 < p.splits; s0 += kAtOnce) {
+    float x[kAtOnce], most = m;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      x[u] = live && s0 + u < p.splits ? __ldcg(p.part_lse + (s0 + u) * p.rows + r_index) : -INFINITY;
+      most = fmaxf(most, x[u]);
+    }
+    const float ref = most == -INFINITY ? 0.0f : most;
+    total *= ex2(m - ref);
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) total += ex2(x[u] - ref);
+    m = most;
+  }
+  const float ref = m == -INFINITY ? 0.0f : m;
+  const float inv = total > 0.0f ? __fdividef(1.0f, total) : (total == total ? 0.0f : total);
+  if (p.a.lse != nullptr && live)
+    p.a.lse[r_index] = total > 0.0f ? (ref + __log2f(total)) * 0.6931471805599453f : (total == total ? -INFINITY : total);
+  // ---- lane = four channels: row after row and split after split, eight loads under way
+  const bool mine = lane * 4 < head_dim;
+  float acc[4] = {};
+  int row = 0, s = 0;  // of the next load, and (to_row, to_s) of the next sum
+  int to_row = 0, to_s = 0;
+  while (to_row < rows) {
+    float4 v[kAtOnce];
+    float f[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int64_t at = __shfl_sync(~0u, r_index, row & 31) + s * p.rows;
+      f[u] = row < rows ? __ldcg(p.part_lse + at) : -INFINITY;
+      v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (mine && row < rows) v[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * head_dim) + lane);
+      if (++s == p.splits) {
+        s = 0;
+        ++row;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (to_row >= rows) break;
+      const float w = ex2(f[u] - __shfl_sync(~0u, ref, to_row)) * __shfl_sync(~0u, inv, to_row);
+      if (f[u] != -INFINITY) {  // a split without keys wrote no output
+        acc[0] = fmaf(w, v[u].x, acc[0]);
+        acc[1] = fmaf(w, v[u].y, acc[1]);
+        acc[2] = fmaf(w, v[u].z, acc[2]);
+        acc[3] = fmaf(w, v[u].w, acc[3]);
+      }
+      if (++to_s == p.splits) {
+        T* const o = static_cast<T*>(p.a.o) + __shfl_sync(~0u, o_at, to_row);
+        if (mine)
+          *reinterpret_cast<uint2*>(o + lane * 4) =
+              make_uint2(XType<T>::pack2(acc[0], acc[1]), XType<T>::pack2(acc[2], acc[3]));
+        acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+        to_s = 0;
+        ++to_row;
+      }
+    }
+  }
+}
 
 template <typename T, int HALVES, int NT, bool SPLIT>
 __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<HALVES, NT>::kCtasPerSm)
@@ -646,16 +718,24 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       const bool live = rt < t.tiles && row < rows && token < a.q_len;
       const int head = t.hv * a.pack + my_head;
       const int64_t r_index = (static_cast<int64_t>(t.b) * a.heads + head) * a.q_len + token;
+      // rows of this warp that exist: a warp without any keeps only the barriers
+      const bool any_row = __any_sync(0xffffffffu, live);
+      const int64_t o_at = t.b * a.so.batch + token * a.so.token + head * a.so.head;
+      const auto join = [&]() {
+        if constexpr (NT == 1 && !SPLIT)  // (more row tiles, or one key tile, are not joined here)
+          if (p.join != nullptr && any_row) x_join<T>(p, static_cast<uint32_t>(t.b) * p.hv + t.hv, live, r_index, o_at);
+      };
       if (t.j0 >= t.j1) {  // no keys
         if (live) {
           if (p.splits > 1) {
             p.part_lse[t.split * p.rows + r_index] = -INFINITY;
           } else {
-            T* o = static_cast<T*>(a.o) + t.b * a.so.batch + token * a.so.token + head * a.so.head;
+            T* o = static_cast<T*>(a.o) + o_at;
             for (int c = 0; c < a.head_dim; c += 8) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
             if (a.lse != nullptr) a.lse[r_index] = -INFINITY;
           }
         }
+        join();
         continue;
       }
       const int qs = n_item % Ly::kQStages;
@@ -669,8 +749,6 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
         g += t.j1 - t.j0;
         continue;
       }
-      // rows of this warp that exist: a warp without any keeps only the barriers
-      const bool any_row = __any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.0f;  // reference of the row's exponent, and the sum
       const int u_end = min(2 * t.j1, (t.keys + 63) >> 6);
       for (int u = 2 * t.j0; u < u_end; ++u, ++n_s) {
@@ -819,6 +897,8 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
         }
       }
       ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      join();
       stored = qs;
       ++n_out;
       ++n_item;
@@ -833,7 +913,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
   }
 }
 
-// Joins the splits of a row: o = sum_s 2^(lse_s - lse) o_s, in the order of the splits.  One warp per row.
+// Joins the splits of a row in a launch of its own (see x_join): o = sum_s 2^(lse_s - lse) o_s, in the order of the splits.  One warp per row.
 template <typename T>
 __global__ void __launch_bounds__(256) x_combine_kernel(const XFwdParams p) {
   pdl_sync();

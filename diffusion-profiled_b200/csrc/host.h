@@ -40,6 +40,7 @@ struct DeviceState {
   int* err_ptr = nullptr;             // device error word
   unsigned int* fold_base = nullptr;  // the device's counters (fold_counter)
   std::atomic<unsigned int> fold_next{0};
+  std::atomic<unsigned int*> join_base{nullptr};  // the device's counters of the attention's splits (conditioning.cu)
   // Set (release) after the fields above are written; a reader that sees it
   // (acquire) sees them too.
   std::atomic<bool> init{false};

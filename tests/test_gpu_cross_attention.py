@@ -109,6 +109,25 @@ def test_few_queries_over_long_states(cuda, size, mask):
     _check(_run(cuda, q, k, v, None, lengths, keep), oracle.cross_attention(q, k, v, None, lengths, keep))
 
 
+@pytest.mark.parametrize("size", [(1, 1, 1024, 4, 4, 64), (40, 2, 1000, 8, 4, 80)], ids=["inside", "launch"])
+def test_joined_splits_are_the_same_every_time(cuda, size):
+    """One after another, and on two streams side by side (joined inside the launch, or by a second one)."""
+    from fp8_b200.cross_attention import cross_attention
+
+    q, k, v, _ = (None if x is None else x.to(cuda) for x in _inputs(*size, BF16, seed=1))
+    lengths = torch.randint(0, size[2] + 1, (size[0],), generator=torch.Generator().manual_seed(4), dtype=torch.int32)
+    lengths = lengths.to(cuda)
+    first = cross_attention(q, k, v, lengths)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(cuda) for _ in range(2)]
+    got = []
+    for i in range(8):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(cross_attention(q, k, v, lengths))
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, o) for o in got)
+
+
 @pytest.mark.parametrize("d,dtype", [(64, BF16), (128, FP16)])
 def test_what_is_not_kept_is_never_used(cuda, d, dtype):
     """Infinities and NaN behind the lengths and the mask change nothing; their gradients are zero."""
