@@ -599,13 +599,14 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
     const uint32_t t_s = tmem + r * 128, t_o = tmem + NT * 128 + r * HALVES * 64;
     uint32_t n_item = 0, g = 0, n_s = 0, n_p = 0, n_out = 0;  // items, key tiles; scores, weights, items of this row tile
     bool ok = true;
-    // Entry e (K of key tile e / 2, or its V) has arrived, with zeros in the rows that are not kept.  (Each row tile's
-    // warp writes them: the same zeros.)
+    // Entry e (K of key tile e / 2, or its V) has arrived, V with zeros in the rows that are not kept, which their
+    // weights of zero would not keep out if they held an infinity.  (Each row tile's warp writes them: the same zeros.
+    // What K has in those rows only reaches scores that the softmax replaces.)
     const auto entry = [&](uint32_t e, bool bits, int used) {
       const int slot = e % Ly::kEntries;
       if (!warp_wait(kv_full + slot, (e / Ly::kEntries) & 1, abort_flag, a.err, kErrXForward + kWaitK + (e & 1)))
         return false;
-      if (bits) {
+      if (bits && (e & 1)) {
         const uint4 w = words[(e >> 1) % kXMaskSlots];
         if ((w.x & w.y & w.z & w.w) != 0xffffffffu)
           x_zero_rows<HALVES>(smem + Ly::kKV + slot * Ly::kTileBytes, w, used, lane);
