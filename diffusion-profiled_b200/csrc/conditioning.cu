@@ -169,7 +169,7 @@ int x_join_counters(DeviceState* st, uint32_t n, unsigned int** ring, uint32_t* 
 }
 
 struct XPlan {
-  int row_tiles, hv, n_tiles, nt, splits, key_chunk;
+  int row_tiles, hv, n_tiles, splits, key_chunk;
   int64_t rows, items, slots;
   bool join_inside;  // x_join
 };
@@ -179,17 +179,16 @@ XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
   w.row_tiles = (a->q_len + tokens - 1) / tokens;
   w.hv = a->heads / pack;
   w.n_tiles = (a->k_len + kXTile - 1) / kXTile;
-  w.nt = w.row_tiles > 1 ? 2 : 1;
   w.rows = static_cast<int64_t>(a->batch) * a->heads * a->q_len;
-  w.slots = static_cast<int64_t>(sm_count) * (w.nt == 1 ? 2 : 1);
-  const int64_t base = static_cast<int64_t>(a->batch) * w.hv * ((w.row_tiles + w.nt - 1) / w.nt);
+  w.slots = static_cast<int64_t>(sm_count) * kXFwdCtasPerSm;
+  const int64_t base = static_cast<int64_t>(a->batch) * w.hv * w.row_tiles;
   w.splits = 1;
   w.key_chunk = w.n_tiles;
   // A split writes its rows' partial outputs in fp32.  With a few rows a tile that is nothing, and pieces that
   // are a quarter of an even share even out sequences of different lengths; with whole tiles of rows the keys
   // are split only to reach SMs that would have no work at all.
   const bool few_rows = w.row_tiles == 1 && a->q_len * pack <= 16;
-  const int64_t pieces = few_rows ? 4 * w.slots : w.slots;
+  const int64_t pieces = few_rows ? 4 * w.slots : sm_count;
   if (w.n_tiles > 1 && 2 * base <= pieces) {
     w.key_chunk = static_cast<int>(std::max<int64_t>((w.n_tiles * base + pieces - 1) / pieces,
                                                      (w.n_tiles + kXMaxSplits - 1) / kXMaxSplits));
@@ -203,10 +202,10 @@ size_t x_fwd_workspace(const fp8_cross_attention_args* a, const XPlan& w) {
   return w.splits == 1 ? 0 : sizeof(float) * static_cast<size_t>(w.splits) * w.rows * (a->head_dim + 1);
 }
 
-template <typename T, int HALVES, int NT>
+template <typename T, int HALVES>
 int x_fwd_launch(const XFwdParams& f, const CUtensorMap (&maps)[4], bool one_key_tile, int64_t slots, cudaStream_t stream) {
-  using Ly = XFwdLayout<HALVES, NT>;
-  const auto kernel = one_key_tile ? x_fwd_kernel<T, HALVES, NT, true> : x_fwd_kernel<T, HALVES, NT, false>;
+  using Ly = XFwdLayout<HALVES>;
+  const auto kernel = one_key_tile ? x_fwd_kernel<T, HALVES, true> : x_fwd_kernel<T, HALVES, false>;
   FP8_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ly::kSmemBytes));
   FP8_CUDA_TRY(launch_kernel(kernel, dim3(static_cast<unsigned>(std::min<int64_t>(f.items, slots))), dim3(Ly::kThreads),
                              Ly::kSmemBytes, stream, 1, kTensorKernel, f, maps[0], maps[1], maps[2], maps[3]));
@@ -237,10 +236,8 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
   if (int s = x_map(&maps[2], a.v, dt, a.sv, a.batch, a.k_len, a.kv_heads, a.head_dim, 1, kXTile)) return s;
   if (int s = x_map(&maps[3], a.o, dt, a.so, a.batch, a.q_len, a.heads, a.head_dim, a.pack, a.tile_tokens)) return s;
   const bool one = w.n_tiles == 1;
-  const int status = a.head_dim <= 64 ? (w.nt == 1 ? x_fwd_launch<T, 1, 1>(f, maps, one, w.slots, stream)
-                                                   : x_fwd_launch<T, 1, 2>(f, maps, one, w.slots, stream))
-                                      : (w.nt == 1 ? x_fwd_launch<T, 2, 1>(f, maps, one, w.slots, stream)
-                                                   : x_fwd_launch<T, 2, 2>(f, maps, one, w.slots, stream));
+  const int status = a.head_dim <= 64 ? x_fwd_launch<T, 1>(f, maps, one, w.slots, stream)
+                                      : x_fwd_launch<T, 2>(f, maps, one, w.slots, stream);
   if (status) return status;
   if (w.splits > 1 && !w.join_inside) {
     FP8_CUDA_TRY(launch_kernel(x_combine_kernel<T>, dim3(grid_for(w.rows, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,

@@ -339,49 +339,47 @@ struct XFwdParams {
 constexpr uint32_t kXJoinCounters = 1u << 20;
 constexpr int kXMaxSplits = 128;
 
-// NT row tiles of HALVES * 64 channels a CTA.
-template <int HALVES, int NT>
+// A CTA works on one row tile of HALVES * 64 channels at a time, and an SM holds two CTAs: while one begins or ends an
+// item, the other computes.  (One CTA with two row tiles, which share its key and value tiles, took 3 to 16 % longer:
+// their items begin and end together.  64 x 1024 queries of 4 heads of 64 over up to 256 keys: 39.6 us against 38.2;
+// of 128 over 77 keys: 57 against 50.)
+template <int HALVES>
 struct XFwdLayout {
   static constexpr int kTileBytes = HALVES * 16384;
-  static constexpr int kQStages = HALVES == 2 ? 1 : NT == 2 ? 3 : 2;
-  // key / value entries: as many as fit the CTA's share of the SM (two CTAs with NT = 1)
-  static constexpr int kEntries = NT == 2 ? (HALVES == 1 ? 6 : 4) : (HALVES == 1 ? 4 : 2);
-  static constexpr int kWarps = 4 * NT;  // softmax warps
-  static constexpr int kKV = NT * kTileBytes * kQStages;
+  static constexpr int kQStages = HALVES == 2 ? 1 : 2;
+  static constexpr int kEntries = HALVES == 1 ? 4 : 2;  // key / value tiles: as many as fit half of the SM
+  static constexpr int kWarps = 4;                      // softmax warps
+  static constexpr int kKV = kTileBytes * kQStages;
   static constexpr int kWords = kKV + kEntries * kTileBytes;
   static constexpr int kBar = kWords + kXMaskSlots * 16;
-  static constexpr int kNumBars = 2 * kQStages + 2 * kEntries + 10 * NT;
+  static constexpr int kNumBars = 2 * kQStages + 2 * kEntries + 10;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;  // + alignment slack
-  static constexpr int kThreads = kWarps * 32 + 32 + NT * 32;  // softmax, loads, products of each row tile
-  static constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
-  static constexpr int kCtasPerSm = NT == 2 ? 1 : 2;
+  static constexpr int kThreads = kWarps * 32 + 64;     // softmax, loads, products
+  static constexpr uint32_t kTmemCols = 256;            // two score buffers of 64, output
 };
-static_assert(XFwdLayout<2, 2>::kSmemBytes <= 232448 && XFwdLayout<1, 2>::kSmemBytes <= 232448, "one CTA per SM");
-static_assert(XFwdLayout<2, 1>::kSmemBytes <= 115712 && XFwdLayout<1, 1>::kSmemBytes <= 115712, "two CTAs per SM");
+constexpr int kXFwdCtasPerSm = 2;
+static_assert(XFwdLayout<2>::kSmemBytes <= 115712 && XFwdLayout<1>::kSmemBytes <= 115712, "two CTAs per SM");
 
-// One unit of work: the row tiles [tile0, tile0 + tiles) of a head group against the key tiles [j0, j1).
+// One unit of work: a row tile of a head group against the key tiles [j0, j1).
 struct XItem {
-  int b, hv, tile0, tiles, split, keys, j0, j1;
+  int b, hv, tile, split, keys, j0, j1;
 };
 // A CTA's items in turn.  The next one's key count is asked for an item ahead, so that it is not waited for.
-template <int NT>
 struct XItems {
   const XFwdParams& p;
-  const int groups, hv;
   const XCount by;
   uint32_t i;
   XCount at;
   int keys = 0;
   __device__ __forceinline__ explicit XItems(const XFwdParams& q)
-      : p(q), groups((q.row_tiles + NT - 1) / NT), hv(q.hv), by(x_count(gridDim.x, groups, q.splits, q.hv)), i(blockIdx.x),
-        at(x_count(blockIdx.x, groups, q.splits, q.hv)) {
+      : p(q), by(x_count(gridDim.x, q.row_tiles, q.splits, q.hv)), i(blockIdx.x),
+        at(x_count(blockIdx.x, q.row_tiles, q.splits, q.hv)) {
     if (i < p.items) keys = x_raw_count(p.a, at.d3);
   }
   __device__ __forceinline__ bool next(XItem& t) {
     if (i >= p.items) return false;
-    t.tile0 = at.d0 * NT;
-    t.tiles = min(NT, p.row_tiles - t.tile0);
+    t.tile = at.d0;
     t.split = at.d1;
     t.hv = at.d2;
     t.b = at.d3;
@@ -390,7 +388,7 @@ struct XItems {
     t.j0 = min(n, t.split * p.key_chunk);
     t.j1 = min(n, t.j0 + p.key_chunk);
     i += gridDim.x;
-    x_advance(at, by, groups, p.splits, hv);
+    x_advance(at, by, p.row_tiles, p.splits, p.hv);
     if (i < p.items) keys = x_raw_count(p.a, at.d3);
     return true;
   }
@@ -477,11 +475,11 @@ __device__ __forceinline__ void x_join(const XFwdParams& p, uint32_t counter, bo
   }
 }
 
-template <typename T, int HALVES, int NT, bool SPLIT>
-__global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<HALVES, NT>::kCtasPerSm)
+template <typename T, int HALVES, bool SPLIT>
+__global__ void __launch_bounds__(XFwdLayout<HALVES>::kThreads, kXFwdCtasPerSm)
     x_fwd_kernel(const XFwdParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap o_map) {
-  using Ly = XFwdLayout<HALVES, NT>;
+  using Ly = XFwdLayout<HALVES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint4* words = reinterpret_cast<uint4*>(smem + Ly::kWords);
@@ -489,13 +487,13 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
   uint64_t* q_empty = q_full + Ly::kQStages;
   uint64_t* kv_full = q_empty + Ly::kQStages;
   uint64_t* kv_empty = kv_full + Ly::kEntries;
-  uint64_t* s_full = kv_empty + Ly::kEntries;  // [NT][2], by score buffer
-  uint64_t* p_full = s_full + 2 * NT;          // [NT][2]: a warp may be a step ahead of another of its row tile
-  uint64_t* pv_done = p_full + 2 * NT;         // [NT][2]: a step's P V product is done
-  uint64_t* o_full = pv_done + 2 * NT;         // the item's last one is
-  uint64_t* o_free = o_full + NT;
-  uint64_t* staged = o_free + NT;
-  uint64_t* drained = staged + NT;
+  uint64_t* s_full = kv_empty + Ly::kEntries;  // [2], by score buffer
+  uint64_t* p_full = s_full + 2;               // [2]: a warp may be a step ahead of another
+  uint64_t* pv_done = p_full + 2;              // [2]: a step's P V product is done
+  uint64_t* o_full = pv_done + 2;              // the item's last one is
+  uint64_t* o_free = o_full + 1;
+  uint64_t* staged = o_free + 1;
+  uint64_t* drained = staged + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::kTail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -503,23 +501,21 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
   if (tid == 0) {
     for (int i = 0; i < Ly::kQStages; ++i) {
       mbar_init(q_full + i, 1);
-      mbar_init(q_empty + i, NT);
+      mbar_init(q_empty + i, 1);
     }
     for (int i = 0; i < Ly::kEntries; ++i) {
       mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, NT);
+      mbar_init(kv_empty + i, 1);
     }
-    for (int i = 0; i < 2 * NT; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 2);  // the products' commit, and the issuing thread (keep bits)
       mbar_init(p_full + i, 4);
       mbar_init(pv_done + i, 1);
     }
-    for (int i = 0; i < NT; ++i) {
-      mbar_init(o_full + i, 1);
-      mbar_init(o_free + i, 4);
-      mbar_init(staged + i, 4);
-      mbar_init(drained + i, 1);
-    }
+    mbar_init(o_full, 1);
+    mbar_init(o_free, 4);
+    mbar_init(staged, 4);
+    mbar_init(drained, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -547,7 +543,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
     const uint32_t q_bytes = static_cast<uint32_t>(a.tile_tokens * a.pack) * 128u * HALVES;
     uint32_t e = 0, loaded = 0, n_item = 0, g = 0;  // `loaded`: entries whose copy was started
     bool ok = true;
-    XItems<NT> items(p);
+    XItems items(p);
     XItem t;
     while (ok && items.next(t)) {
       if (t.j0 >= t.j1) continue;
@@ -555,11 +551,10 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       ok = warp_wait(q_empty + qs, ((n_item / Ly::kQStages) & 1) ^ 1, abort_flag, a.err, kErrXForward + kWaitQFree);
       if (!ok) break;
       if (lane == 0) {
-        mbar_arrive_expect_tx(q_full + qs, q_bytes * t.tiles);
-        for (int r = 0; r < t.tiles; ++r)
-          for (int hf = 0; hf < HALVES; ++hf)
-            tma_load_4d(smem + (qs * NT + r) * Ly::kTileBytes + hf * 16384, &q_map, q_full + qs, hf * 64, t.hv * a.pack,
-                        (t.tile0 + r) * a.tile_tokens, t.b);
+        mbar_arrive_expect_tx(q_full + qs, q_bytes);
+        for (int hf = 0; hf < HALVES; ++hf)
+          tma_load_4d(smem + qs * Ly::kTileBytes + hf * 16384, &q_map, q_full + qs, hf * 64, t.hv * a.pack,
+                      t.tile * a.tile_tokens, t.b);
       }
       ++n_item;
       const int hk = t.hv * a.pack / a.group;
@@ -592,16 +587,15 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
         mbar_wait(q_full + k % Ly::kQStages, (k / Ly::kQStages) & 1, &never, a.err, kErrXForward + kWaitDrain);
     }
   } else if (warp > Ly::kWarps) {
-    // ------------------------------------------------------------ products of row tile r
-    const int r = warp - Ly::kWarps - 1;
+    // ------------------------------------------------------------ products
     const uint32_t s_base = smem_u32(smem);
     const uint32_t idesc_o = x_idesc<T>(ksteps * 16, 0, 1);
-    const uint32_t t_s = tmem + r * 128, t_o = tmem + NT * 128 + r * HALVES * 64;
-    uint32_t n_item = 0, g = 0, n_s = 0, n_p = 0, n_out = 0;  // items, key tiles; scores, weights, items of this row tile
+    const uint32_t t_s = tmem, t_o = tmem + 128;
+    uint32_t n_item = 0, g = 0, n_s = 0, n_p = 0;  // items, key tiles, scores, weights
     bool ok = true;
     // Entry e (K of key tile e / 2, or its V) has arrived, V with zeros in the rows that are not kept, which their
-    // weights of zero would not keep out if they held an infinity.  (Each row tile's warp writes them: the same zeros.
-    // What K has in those rows only reaches scores that the softmax replaces.)
+    // weights of zero would not keep out if they held an infinity.
+    // (What K has in those rows only reaches scores that the softmax replaces.)
     const auto entry = [&](uint32_t e, bool bits, int used) {
       const int slot = e % Ly::kEntries;
       if (!warp_wait(kv_full + slot, (e / Ly::kEntries) & 1, abort_flag, a.err, kErrXForward + kWaitK + (e & 1)))
@@ -613,24 +607,13 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       }
       return true;
     };
-    XItems<NT> items(p);
+    XItems items(p);
     XItem t;
     while (ok && items.next(t)) {
       if (t.j0 >= t.j1) continue;
       const int qs = n_item % Ly::kQStages;
-      if (r >= t.tiles) {  // no rows: the entries are only passed on
-        for (int j = t.j0; j < t.j1 && ok; ++j, ++g)
-#pragma unroll
-          for (uint32_t e = 2 * g; e < 2 * g + 2; ++e) {
-            const int slot = e % Ly::kEntries;
-            ok = ok && warp_wait(kv_full + slot, (e / Ly::kEntries) & 1, abort_flag, a.err, kErrXForward + kWaitK + (e & 1));
-            if (ok && lane == 0) mbar_arrive(kv_empty + slot);
-          }
-        ++n_item;
-        continue;
-      }
       ok = warp_wait(q_full + qs, (n_item / Ly::kQStages) & 1, abort_flag, a.err, kErrXForward + kWaitQ);
-      const uint64_t sq = k_major_desc(s_base + (qs * NT + r) * Ly::kTileBytes);
+      const uint64_t sq = k_major_desc(s_base + qs * Ly::kTileBytes);
       const int u_end = min(2 * t.j1, (t.keys + 63) >> 6);  // 64-key steps [2 * j0, u_end)
       const uint32_t g0 = g - t.j0;                         // a key tile's number in the CTA, less its own
       // S of step u over P of step u - 2, whose product was issued before it (products run in their order)
@@ -643,8 +626,8 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
           products_k_major(t_s + (n_s & 1) * 64, sq,
                            k_major_desc(s_base + Ly::kKV + (e % Ly::kEntries) * Ly::kTileBytes + (u & 1) * 8192),
                            x_idesc<T>(x_chunks64(t.keys, u) * 32, 0, 0), ksteps);
-          umma_commit(s_full + 2 * r + (n_s & 1));
-          mbar_arrive(s_full + 2 * r + (n_s & 1));
+          umma_commit(s_full + (n_s & 1));
+          mbar_arrive(s_full + (n_s & 1));
           if ((u & 1) || u == u_end - 1) umma_commit(kv_empty + e % Ly::kEntries);
         }
         __syncwarp();
@@ -657,9 +640,9 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
         const int j = u >> 1;
         // O += P V
         if (!(u & 1)) ok = entry(e, masked || (j + 1) * kXTile > t.keys, x_chunks(t.keys, j) * 32);
-        ok = ok && warp_wait(p_full + 2 * r + (n_p & 1), (n_p >> 1) & 1, abort_flag, a.err, kErrXForward + kWaitP);
-        if (ok && u == 2 * t.j0 && n_out > 0)  // the last item's output has been read
-          ok = warp_wait(o_free + r, (n_out - 1) & 1, abort_flag, a.err, kErrXForward + kWaitAccFree);
+        ok = ok && warp_wait(p_full + (n_p & 1), (n_p >> 1) & 1, abort_flag, a.err, kErrXForward + kWaitP);
+        if (ok && u == 2 * t.j0 && n_item > 0)  // the last item's output has been read
+          ok = warp_wait(o_free, (n_item - 1) & 1, abort_flag, a.err, kErrXForward + kWaitAccFree);
         if (!ok) break;
         const uint64_t sv = mn_major_desc(s_base + Ly::kKV + (e % Ly::kEntries) * Ly::kTileBytes + (u & 1) * 8192);
         const uint32_t later = u > 2 * t.j0 ? 1u : 0u, weights = t_s + (n_p & 1) * 64;
@@ -673,8 +656,8 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
               umma_f16_ts(t_o, w, sv + k * 128, idesc_o, k > 0 ? 1u : later);
               if (SPLIT) umma_f16_ts(t_o, w + 16, sv + k * 128, idesc_o, 1u);
             }
-          umma_commit(pv_done + 2 * r + (n_p & 1));
-          if (u == u_end - 1) umma_commit(o_full + r);
+          umma_commit(pv_done + (n_p & 1));
+          if (u == u_end - 1) umma_commit(o_full);
           if ((u & 1) || u == u_end - 1) umma_commit(kv_empty + e % Ly::kEntries);
         }
         __syncwarp();
@@ -682,26 +665,25 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
         if (u + 2 < u_end) ok = issue_s(u + 2);
       }
       g += t.j1 - t.j0;
-      ++n_out;
       ++n_item;
     }
     if (!ok && elect_one()) {  // the products in flight end before the tensor memory is freed
       volatile int never = 0;
-      umma_commit(drained + r);
-      mbar_wait(drained + r, 0, &never, a.err, kErrXForward + kWaitDrain);
+      umma_commit(drained);
+      mbar_wait(drained, 0, &never, a.err, kErrXForward + kWaitDrain);
     }
   } else {
-    // ------------------------------------------------------------ softmax: thread = row of row tile rt
-    const int rt = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+    // ------------------------------------------------------------ softmax: thread = row
+    const int quad = warp, row = quad * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t t_s = t_lane + rt * 128, t_o = t_lane + NT * 128 + rt * HALVES * 64;
+    const uint32_t t_s = t_lane, t_o = t_lane + 128;
     const bool flip = a.scale < 0.0f;  // the largest score is the smallest product
     // log2 units; a zero scale keeps a factor that leaves -inf at -inf
     const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
     const uint64_t c22 = pair2(c2, c2);
     const int rows = a.tile_tokens * a.pack, my_token = row / a.pack, my_head = row % a.pack;
     const bool hands_out = quad == 0 && lane == 0;
-    uint32_t n_s = 0, n_out = 0, n_item = 0, g = 0;  // 64-key steps and items of this row tile; items, key tiles
+    uint32_t n_s = 0, n_item = 0, g = 0;  // 64-key steps, items, key tiles
     int stored = -1;  // Q stage whose output is on its way out
     // The stage is free for a new Q once the output has been read from it; asked for as late as can be.
     const auto release_stored = [&]() {
@@ -712,18 +694,18 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       stored = -1;
     };
     bool ok = true;
-    XItems<NT> items(p);
+    XItems items(p);
     XItem t;
     while (ok && items.next(t)) {
-      const int token = (t.tile0 + rt) * a.tile_tokens + my_token;
-      const bool live = rt < t.tiles && row < rows && token < a.q_len;
+      const int token = t.tile * a.tile_tokens + my_token;
+      const bool live = row < rows && token < a.q_len;
       const int head = t.hv * a.pack + my_head;
       const int64_t r_index = (static_cast<int64_t>(t.b) * a.heads + head) * a.q_len + token;
       // rows of this warp that exist: a warp without any keeps only the barriers
       const bool any_row = __any_sync(0xffffffffu, live);
       const int64_t o_at = t.b * a.so.batch + token * a.so.token + head * a.so.head;
       const auto join = [&]() {
-        if constexpr (NT == 1 && !SPLIT)  // (more row tiles, or one key tile, are not joined here)
+        if constexpr (!SPLIT)  // (one key tile is not split)
           if (p.join != nullptr && any_row) x_join<T>(p, static_cast<uint32_t>(t.b) * p.hv + t.hv, live, r_index, o_at);
       };
       if (t.j0 >= t.j1) {  // no keys
@@ -740,21 +722,11 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
         continue;
       }
       const int qs = n_item % Ly::kQStages;
-      if (rt >= t.tiles) {  // this row tile has no rows in the item
-        release_stored();
-        if (quad == 0) {
-          ok = warp_wait(q_full + qs, (n_item / Ly::kQStages) & 1, abort_flag, a.err, kErrXForward + kWaitQ);
-          if (ok && lane == 0) mbar_arrive(q_empty + qs);
-        }
-        ++n_item;
-        g += t.j1 - t.j0;
-        continue;
-      }
       float m = -INFINITY, l = 0.0f;  // reference of the row's exponent, and the sum
       const int u_end = min(2 * t.j1, (t.keys + 63) >> 6);
       for (int u = 2 * t.j0; u < u_end; ++u, ++n_s) {
         const uint32_t scores = t_s + (n_s & 1) * 64;
-        ok = warp_wait(s_full + 2 * rt + (n_s & 1), (n_s >> 1) & 1, abort_flag, a.err, kErrXForward + kWaitS);
+        ok = warp_wait(s_full + (n_s & 1), (n_s >> 1) & 1, abort_flag, a.err, kErrXForward + kWaitS);
         if (!ok) break;
         tc_fence_after();
         if (any_row) {
@@ -793,7 +765,7 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
             m = mn;
             if (u > 2 * t.j0) {
               // the product of the step before is done (the one before that was when this step's scores came)
-              ok = warp_wait(pv_done + 2 * rt + ((n_s - 1) & 1), ((n_s - 1) >> 1) & 1, abort_flag, a.err,
+              ok = warp_wait(pv_done + ((n_s - 1) & 1), ((n_s - 1) >> 1) & 1, abort_flag, a.err,
                              kErrXForward + kWaitPV);
               if (!ok) break;
               tc_fence_after();
@@ -834,16 +806,16 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + 2 * rt + (n_s & 1));
+        if (lane == 0) mbar_arrive(p_full + (n_s & 1));
       }
       if (!ok) break;
       g += t.j1 - t.j0;
       release_stored();
-      ok = warp_wait(o_full + rt, n_out & 1, abort_flag, a.err, kErrXForward + kWaitAcc);
+      ok = warp_wait(o_full, n_item & 1, abort_flag, a.err, kErrXForward + kWaitAcc);
       if (!ok) break;
       tc_fence_after();
       const float inv = l > 0.0f ? __fdividef(1.0f, l) : (l == l ? 0.0f : l);
-      uint8_t* stage = smem + (qs * NT + rt) * Ly::kTileBytes;  // Q's tile, read by every product of the item by now
+      uint8_t* stage = smem + qs * Ly::kTileBytes;  // Q's tile, read by every product of the item by now
       if (any_row) {
 #pragma unroll
         for (int c = 0; c < 2 * HALVES; ++c) {
@@ -882,14 +854,14 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(o_free + rt);
-        mbar_arrive(staged + rt);
+        mbar_arrive(staged);
+        mbar_arrive(o_free);
       }
       if (hands_out) {
-        ok = mbar_wait(staged + rt, n_out & 1, abort_flag, a.err, kErrXForward + kWaitStaged);
+        ok = mbar_wait(staged, n_item & 1, abort_flag, a.err, kErrXForward + kWaitStaged);
         if (ok && p.splits == 1) {
           for (int hf = 0; hf < HALVES; ++hf)
-            tma_store_4d(&o_map, stage + hf * 16384, hf * 64, t.hv * a.pack, (t.tile0 + rt) * a.tile_tokens, t.b);
+            tma_store_4d(&o_map, stage + hf * 16384, hf * 64, t.hv * a.pack, t.tile * a.tile_tokens, t.b);
           bulk_commit_group();
         }
         if (ok && Ly::kQStages == 1) {
@@ -901,7 +873,6 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES, NT>::kThreads, XFwdLayout<H
       if (!ok) break;
       join();
       stored = qs;
-      ++n_out;
       ++n_item;
     }
     if (hands_out) bulk_wait_group<0>();
