@@ -94,16 +94,19 @@ __device__ __forceinline__ void x_products_mn(uint32_t d, uint32_t operand, uint
 template <int HALVES, bool SPLIT>
 struct XDqLayout {
   static constexpr int kTileBytes = HALVES * 16384;
-  static constexpr int kQStages = HALVES == 1 ? 3 : 1;  // Q and dO of an item
+  // Sums of dQ in tensor memory.  With two, an item's is handed out while the next item's products run; with heads of
+  // more than 64 there is room for one (and items are longer).
+  static constexpr int kAccs = HALVES == 1 ? 2 : 1;
+  static constexpr int kQStages = HALVES == 1 ? (SPLIT ? 4 : 3) : 1;  // Q and dO of an item
   // A key tile stays from its scores to its dQ product, two tiles later; a value tile only for its dP.
-  static constexpr int kKStages = HALVES == 1 ? 4 : SPLIT ? 2 : 3;
-  static constexpr int kVStages = HALVES == 1 ? 3 : 2;
+  static constexpr int kKStages = HALVES == 1 ? (SPLIT ? 3 : 4) : SPLIT ? 2 : 3;
+  static constexpr int kVStages = HALVES == 1 && !SPLIT ? 3 : 2;
   static constexpr int kK = 2 * kQStages * kTileBytes;
   static constexpr int kV = kK + kKStages * kTileBytes;
   static constexpr int kWords = kV + kVStages * kTileBytes;
-  static constexpr int kDelta = kWords + kXMaskSlots * 16;  // fp32: the rows' delta in parts, [2][128] or with SPLIT [4][128]
-  static constexpr int kBar = kDelta + (SPLIT ? 2048 : 1024);
-  static constexpr int kNumBars = 2 * (kQStages + kKStages + kVStages) + 14;
+  static constexpr int kDelta = kWords + kXMaskSlots * 16;  // fp32: the rows' delta in parts, [kAccs][2][128] or with SPLIT [4][128]
+  static constexpr int kBar = kDelta + (SPLIT ? 2048 : kAccs * 1024);
+  static constexpr int kNumBars = 2 * (kQStages + kKStages + kVStages) + 17;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;
 };
@@ -165,10 +168,10 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
   uint64_t* dp_full = s_free + 2;
   uint64_t* dp_free = dp_full + 1;
   uint64_t* ds_full = dp_free + 1;            // [2], by score buffer: a warp may be a tile ahead of another
-  uint64_t* acc_full = ds_full + 2;
-  uint64_t* acc_free = acc_full + 1;
-  uint64_t* staged = acc_free + 1;
-  uint64_t* delta_full = staged + 1;
+  uint64_t* acc_full = ds_full + 2;  // [2], by sum
+  uint64_t* acc_free = acc_full + 2;
+  uint64_t* staged = acc_free + 2;
+  uint64_t* delta_full = staged + 2;
   uint64_t* drained = delta_full + 1;  // [2], by issuing warp
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::kTail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -192,12 +195,12 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       mbar_init(s_free + i, 1);
       mbar_init(ds_full + i, kXBwdWarps);
       mbar_init(drained + i, 1);
+      mbar_init(acc_full + i, 1);
+      mbar_init(acc_free + i, kXBwdWarps);
+      mbar_init(staged + i, kXBwdWarps);
     }
     mbar_init(dp_full, 1);
     mbar_init(dp_free, kXBwdWarps);
-    mbar_init(acc_full, 1);
-    mbar_init(acc_free, kXBwdWarps);
-    mbar_init(staged, kXBwdWarps);
     mbar_init(delta_full, SPLIT ? kXBwdWarps : 8);
     *abort_flag = 0;
     fence_barrier_init();
@@ -338,15 +341,16 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       for (int j = 0; j < t.tiles; ++j, ++g) {
         const int ks = g % Ly::kKStages, buf = g & 1, steps = 2 * x_chunks(t.keys, j);
         ok = wait(k_full + ks, g / Ly::kKStages, kWaitK) && wait(ds_full + buf, g >> 1, kWaitP);
-        if (ok && j == 0 && n_item > 0) ok = wait(acc_free, n_item ^ 1, kWaitAccFree);  // the last item's dQ has been read
+        if (ok && j == 0 && n_item >= Ly::kAccs)  // the last dQ summed here has been read
+          ok = wait(acc_free + n_item % Ly::kAccs, (n_item / Ly::kAccs) ^ 1, kWaitAccFree);
         if (!ok) break;
         const uint64_t sk = mn_major_desc(s_base + Ly::kK + ks * Ly::kTileBytes);
         tc_fence_after();
         if (elect_one()) {
-          x_products_mn<SPLIT, 8>(tmem + kXDqAcc, tmem + kXDqS + buf * 128, sk, idesc, steps, j > 0 ? 1u : 0u);
+          x_products_mn<SPLIT, 8>(tmem + kXDqAcc + n_item % Ly::kAccs * 64, tmem + kXDqS + buf * 128, sk, idesc, steps, j > 0 ? 1u : 0u);
           umma_commit(s_free + buf);
           umma_commit(k_empty + ks);
-          if (j == t.tiles - 1) umma_commit(acc_full);
+          if (j == t.tiles - 1) umma_commit(acc_full + n_item % Ly::kAccs);
         }
         __syncwarp();
       }
@@ -394,7 +398,58 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       }
       stored = -1;
     };
-    bool ok = true;
+    // The gradient of item n, from its sum by way of Q's tile, which every product of the item has read by then: a quarter
+    // of the channels each.
+    struct Done {
+      uint32_t n;
+      int b, hv, tile;
+      bool dead;
+    };
+    const auto hand_out = [&](const Done& w) {
+      const uint32_t acc = w.n % Ly::kAccs, phase = w.n / Ly::kAccs;
+      const int qs = w.n % Ly::kQStages;
+      uint8_t* stage = smem + 2 * qs * Ly::kTileBytes;
+      release_stored();
+      if (!wait(acc_full + acc, phase, kWaitAcc)) return false;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < HALVES; ++c) {
+        const int col = (wq * HALVES + c) * 16;
+        uint32_t o[16];
+        tmem_read(t_lane + kXDqAcc + acc * 64 + col, o);
+        uint32_t pk[8];
+#pragma unroll
+        for (int k = 0; k < 16; k += 2)
+          pk[k >> 1] = w.dead ? 0u : XType<T>::pack2(__uint_as_float(o[k]) * a.scale, __uint_as_float(o[k + 1]) * a.scale);
+        uint8_t* half = stage + (col >> 6) * 16384;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          st_shared_v4(half + swizzle128_offset(row, ((col & 63) >> 3) + u), pk[4 * u], pk[4 * u + 1], pk[4 * u + 2],
+                       pk[4 * u + 3]);
+      }
+      tc_fence_before();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(staged + acc);
+        mbar_arrive(acc_free + acc);
+      }
+      bool ok = true;
+      if (tid == 0) {
+        ok = mbar_wait(staged + acc, phase & 1, abort_flag, a.err, kErrXDq + kWaitStaged);
+        if (ok) {
+          for (int hf = 0; hf < HALVES; ++hf)
+            tma_store_4d(&dq_map, stage + hf * 16384, hf * 64, w.hv * a.pack, w.tile * a.tile_tokens, w.b);
+          bulk_commit_group();
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) stored = qs;
+      if (Ly::kQStages == 1) release_stored();
+      return ok;
+    };
+    Done done{};  // not handed out yet, with two sums
+    bool any_done = false, ok = true;
     XDqItems items(p);
     XDqItem t;
     fetch(items);
@@ -418,6 +473,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       const bool dead = lse == -INFINITY;  // no such row, or no kept key
       const float neg_lse = dead ? -INFINITY : -lse * 1.4426950408889634f;
       float neg_delta = 0.0f;
+      float* parts = delta_part + (SPLIT ? 0 : n_item % Ly::kAccs * (2 * kXTile));
       if (!SPLIT && wq < 2) {  // delta = do . o, half of the channels each
         ok = wait(q_full + qs, n_item / Ly::kQStages, kWaitQ);
         if (!ok) break;
@@ -434,15 +490,14 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
           }
           part -= x_dot8<T>(v, ld_shared_v4(stage + Ly::kTileBytes + (c >> 3) * 16384 + swizzle128_offset(row, c & 7)));
         }
-        delta_part[wq * kXTile + row] = part;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(delta_full);
+        parts[wq * kXTile + row] = part;
+        warp_arrive(delta_full);
       }
       // this row's delta, from its parts, and the statistics that the second launch needs
       const auto join_delta = [&]() {
         if (!wait(delta_full, n_item, kWaitDelta)) return false;
-        neg_delta = delta_part[row] + delta_part[kXTile + row];
-        if (SPLIT) neg_delta += delta_part[2 * kXTile + row] + delta_part[3 * kXTile + row];
+        neg_delta = parts[row] + parts[kXTile + row];
+        if (SPLIT) neg_delta += parts[2 * kXTile + row] + parts[3 * kXTile + row];
         if (dead) neg_delta = 0.0f;
         if (wq == 0) {
           stat[0] = neg_lse;
@@ -484,6 +539,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
             }
           }
         }
+        if (Ly::kAccs > 1) release_stored();
         ok = wait(dp_full, g, kWaitDP);
         if (!ok) break;
         tc_fence_after();
@@ -502,7 +558,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
             }
             unpair2(sum, s0, s1);
           }
-          delta_part[wq * kXTile + row] = -(s0 + s1);
+          parts[wq * kXTile + row] = -(s0 + s1);
           warp_arrive(delta_full);
           ok = join_delta();
           if (!ok) break;
@@ -548,46 +604,13 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       }
       if (!ok) break;
       fetch(items);
-      release_stored();
-      ok = wait(acc_full, n_item, kWaitAcc);
-      if (!ok) break;
-      tc_fence_after();
-      // dQ goes out from Q's tile, which every product of the item has read by now: a quarter of the channels each
-#pragma unroll
-      for (int c = 0; c < HALVES; ++c) {
-        const int col = (wq * HALVES + c) * 16;
-        uint32_t o[16];
-        tmem_read(t_lane + kXDqAcc + col, o);
-        uint32_t pk[8];
-#pragma unroll
-        for (int k = 0; k < 16; k += 2)
-          pk[k >> 1] = dead ? 0u : XType<T>::pack2(__uint_as_float(o[k]) * a.scale, __uint_as_float(o[k + 1]) * a.scale);
-        uint8_t* half = stage + (col >> 6) * 16384;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          st_shared_v4(half + swizzle128_offset(row, ((col & 63) >> 3) + u), pk[4 * u], pk[4 * u + 1], pk[4 * u + 2],
-                       pk[4 * u + 3]);
-      }
-      tc_fence_before();
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(staged);
-        mbar_arrive(acc_free);
-      }
-      if (tid == 0) {
-        ok = mbar_wait(staged, n_item & 1, abort_flag, a.err, kErrXDq + kWaitStaged);
-        if (ok) {
-          for (int hf = 0; hf < HALVES; ++hf)
-            tma_store_4d(&dq_map, stage + hf * 16384, hf * 64, t.hv * a.pack, t.tile * a.tile_tokens, t.b);
-          bulk_commit_group();
-        }
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) stored = qs;
-      if (Ly::kQStages == 1) release_stored();
+      const Done now{n_item, t.b, t.hv, t.tile, dead};
+      if (Ly::kAccs == 1 || any_done) ok = hand_out(Ly::kAccs == 1 ? now : done);
+      done = now;
+      any_done = true;
       ++n_item;
     }
+    if (ok && Ly::kAccs > 1 && any_done) hand_out(done);
     if (tid == 0) bulk_wait_group<0>();
   }
   tc_fence_before();
