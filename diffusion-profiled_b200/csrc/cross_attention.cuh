@@ -18,20 +18,24 @@
 //   * S = Q K^T of 128 rows and 64 keys on tcgen05 kind::f16 into TMEM (fp32); one thread
 //     owns one row, reads its 64 scores, and writes P (rounded to the tensors' type, the
 //     tensor cores' operand) over them, where the second product O += P V takes it from;
-//   * two score buffers a row tile: the products of the next 64 keys run while the softmax
-//     of these does.  (With one buffer of 128 keys the softmax, P V and the next S are one
-//     chain: 4,770 cycles a pair of tiles at heads of 128 against 2,050 of products.)
-//     64 keys cost S a third of its rate (its operands' shared-memory reads), which the
-//     overlap more than returns;
+//   * two score buffers: the products of the next 64 keys run while the softmax of these
+//     does.  (With one buffer of 128 keys the softmax, P V and the next S are one chain:
+//     170 us against 154 for 2 x 4096 queries of 8 heads of 128 over 4096 keys.)  64 keys
+//     cost S a third of its rate (its operands' shared-memory reads), which the overlap
+//     more than returns;
 //   * the exponent's reference is the row's maximum so far, raised only when a score
 //     passes it by more than 2^8: then O and the sum are rescaled.  Scores that stay
 //     within that factor need no rescaling pass, and P <= 2^8 keeps its relative
 //     precision in bf16 and fp16;
-//   * a warp of its own issues each row tile's products (a product's issue takes about as
-//     long as the product, so one warp that waits for two softmaxes in turn leaves the
-//     tensor cores idle meanwhile);
-//   * keys that are not kept: their rows of K and V are zeroed in shared memory before the
-//     products, and their scores are -inf.
+//   * keys that are not kept: their scores are replaced by -inf, and their rows of V are
+//     zeroed in shared memory before the product.
+// What bounds it: with many queries the softmax (an exponential a score, 16 a clock and
+// SM) and the products by turns: the 2 x 4096 x 4096 above takes 150 us now, 919 TFLOP/s,
+// 55 % of the measured peak, and 13 % of it is the last wave (512 row tiles on 296 CTAs);
+// with few keys the beginning and end of an item (3,000 of 8,000 cycles at 160 keys), which
+// the other CTA of the SM fills in part; with single queries the bytes of K and V (32
+// queries of 16 heads over 8192 keys of 4: 342 MB in 88 us, 3.9 TB/s, of which 25 us do
+// not depend on the bytes: 6.5 TB/s is the rate of what more bytes add).
 // The sums and statistics are fp32; P is the one value rounded before a sum (it is a
 // matrix operand).  Over many keys that rounding averages out against the output's own.
 // Where the states are at most one key tile (SPLIT) it would not, and the products are
@@ -54,7 +58,7 @@ constexpr int kXTile = 128;  // rows of a query tile and keys of a key tile
 enum XError : int { kErrXForward = 300, kErrXDq = 320, kErrXDkv = 340 };
 enum XWait : int {
   kWaitQFree = 1, kWaitKFree, kWaitVFree, kWaitQ, kWaitK, kWaitV, kWaitS, kWaitSFree, kWaitDP, kWaitDPFree, kWaitP,
-  kWaitPRest, kWaitPV, kWaitAcc, kWaitAccFree, kWaitStaged, kWaitDelta, kWaitDrain
+  kWaitPV, kWaitAcc, kWaitAccFree, kWaitStaged, kWaitDelta, kWaitDrain
 };
 
 struct XStrides {

@@ -2,27 +2,40 @@
 //
 // Two launches, each with its sums in tensor memory from beginning to end, so that no
 // gradient is added to memory by several CTAs (no atomics, one order of addition):
-//   * x_dq_kernel: a row tile of queries against the keys, 64 at a step.  Per step
-//     S = Q K^T and dP = dO V^T, dS = P (dP - delta), dQ += dS K.  It also leaves each
-//     row's -log-sum-exp and -delta for the second launch;
+//   * x_dq_kernel: a row tile of queries against its key tiles, 128 keys at a step.  Per
+//     step S = Q K^T and dP = dO V^T, dS = P (dP - delta), dQ += dS K.  It also leaves
+//     each row's -log-sum-exp and -delta for the second launch;
 //   * x_dkv_kernel: a key tile against the rows that read it, 64 at a step, all heads that
 //     share it among them.  The scores are formed transposed, S^T = K Q^T and
 //     dP^T = V dO^T (lane = key), so that P^T and dS^T lie in tensor memory as the first
 //     operands of dV += P^T dO and dK += dS^T Q.
 // That is seven products a tile pair; a single launch would need five, but would add
-// dQ to memory from every key tile.
+// dQ to memory from every key tile.  Both kernels know the rows' log-sum-exp, so no
+// maximum is searched and a row of scores needs no single owner: 16 softmax warps take
+// 32 columns of a row each.  One warp issues the scores and dP, one the gradients.
 //
-// Both kernels have two buffers for the scores and for dP, and two groups of four softmax
-// warps that take the steps in turn, a thread one row (or key) and 64 columns: while one
-// group works on a step, the products of the next run.  (With one buffer of 128 columns
-// and all warps on it, softmax and products of a tile followed one another: 3,300 to 4,100
-// cycles a tile at heads of 128.)  One warp issues the scores and dP, one the gradients.
+// What runs side by side.  x_dq_kernel: the scores run a tile ahead into a second buffer,
+// dP one tile ahead of its use as soon as the last has been read; all 16 warps work on one
+// tile.  (64 keys at a step, two groups of warps by turns as in x_dkv_kernel: 257 to 279 us
+// against 198 for 2 x 4096 queries of 8 heads of 128 over 4096 keys: products of 64 columns
+// run at two thirds of the rate, and dQ's sum leaves tensor memory room enough without
+// them.)  x_dkv_kernel, whose two sums leave room for one tile's scores and dP only: two
+// buffers of 64 rows, and two groups of eight warps that take the steps by turns, so that
+// one group's exponentials run during the other's products.  (One buffer of 128 rows: 298 us
+// against 275.)  Both are bound by the products and the softmax by turns, at 1,040 and 1,000
+// TFLOP/s of the seven products they do, 60 to 63 % of the measured peak; 13 % of the time is
+// the last wave of 512 tiles on 148 SMs.
 //
 // delta_i = do_i . o_i from the forward's output; where the states are at most one key
 // tile (SPLIT), delta_i = sum_j p_ij dp_ij in fp32 instead, without the output's rounding
-// (with few keys it does not average out), and P and dS go into the products as the sum of
-// two values of the tensors' type.  Otherwise P and dS are rounded to it once (they are
-// matrix operands); scores, dP, statistics and all sums are fp32.
+// (with few keys it does not average out), P and dS go into the products as the sum of two
+// values of the tensors' type, and a sequence of one key gets the exact zero that its dS
+// is.  Otherwise P and dS are rounded to the type once (they are matrix operands); scores,
+// dP, statistics and all sums are fp32.
+//
+// A barrier that warps arrive on has one copy for each buffer, and the buffer is reused only
+// after its phase: with one for all, a warp that is a step ahead completes a phase that
+// another has not reached.
 #pragma once
 
 #include "cross_attention.cuh"

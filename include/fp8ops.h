@@ -518,7 +518,13 @@ int fp8_attention_bwd(const void* qkv, const void* o, const void* dout, const fl
                       void* dqkv, int batch, int seq, int heads, int head_dim, int ld_qkv, int ld_o,
                       fp8_stream_t stream);
 
-/* ------------------------------------------------------------ text conditioning */
+/* ------------------------------------------------------------ text conditioning
+ *
+ * Device errors (fp8_device_error) of these kernels: 201, a token id outside the
+ * vocabulary (the call's other rows are right); 202 and 301 to 358, a bounded wait
+ * that ran out: the embedding gradient's sort, the attention's forward (300 and the
+ * barrier's number), dq (320) and dk, dv (340).  After one of the latter the call's
+ * outputs are not valid. */
 
 /* Element types of the operators below. */
 #define FP8_DTYPE_BF16 0
