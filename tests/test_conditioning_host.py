@@ -44,3 +44,20 @@ def test_prompts_and_the_model_go_together():
 def test_there_is_no_kernel_on_the_cpu():
     with pytest.raises((RuntimeError, NotImplementedError)):
         PromptEncoder(10, 16, 4)(torch.zeros(1, 3, dtype=torch.int64))
+
+
+def test_shapes_without_data():
+    """The operators' meta kernels, which tracing asks for shapes and types."""
+    from fp8_b200.cross_attention import cross_attention, cross_attention_packed
+    from fp8_b200.dropout import dropout_add
+    from fp8_b200.embedding import embed_tokens, embedding_bwd
+
+    meta = lambda *s, dtype=torch.bfloat16: torch.empty(s, dtype=dtype, device="meta")  # noqa: E731
+    q, kv = meta(2, 9, 8, 40), meta(2, 5, 2, 4, 40)
+    for o in (cross_attention_packed(q, kv), cross_attention(q, kv[:, :, 0], kv[:, :, 1])):
+        assert o.shape == q.shape and o.dtype == q.dtype and o.device.type == "meta"
+    ids, w = meta(3, 7, dtype=torch.int64), meta(50, 16, dtype=torch.float32)
+    assert embed_tokens(ids, w, dtype=torch.float16).shape == (3, 7, 16)
+    assert embedding_bwd(ids, meta(3, 7, 16), 50, 1.0, -1, torch.float32).shape == (50, 16)
+    x = meta(3, 4)
+    assert dropout_add(x, x, 0.1, meta(dtype=torch.int64)).shape == (3, 4)

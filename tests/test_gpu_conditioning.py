@@ -152,3 +152,41 @@ def test_training_step_with_prompts(cuda, graph):
     late[ids[1, :30]] = False
     assert torch.count_nonzero(grad[late]) == 0
     step.release()
+
+
+def test_operators_in_a_captured_graph(cuda):
+    """The forms that meet across CTAs (split keys, sorted gradient) leave their counters as a replay needs them."""
+    from fp8_b200.cross_attention import cross_attention
+    from fp8_b200.dropout import dropout
+    from fp8_b200.embedding import embedding_bwd
+
+    g = torch.Generator(device=cuda).manual_seed(5)
+    new = lambda *s: torch.randn(*s, device=cuda, generator=g).to(torch.bfloat16)  # noqa: E731
+    q, k, v, dout = new(2, 1, 4, 64), new(2, 1500, 4, 64), new(2, 1500, 4, 64), new(5000, 72)
+    ids = torch.randint(0, 300, (5000,), device=cuda, generator=g)
+    seed = torch.tensor(7, device=cuda)
+
+    def run():
+        out = cross_attention(q, k, v), embedding_bwd(ids, dout, 300, 1.0, -1, torch.float32), dropout(dout, 0.5, seed)
+        seed.add_(1)
+        return out
+
+    side = torch.cuda.Stream(cuda)
+    side.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(side):
+        want = [x.clone() for x in run()]
+    torch.cuda.current_stream(cuda).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    masks = []
+    for _ in range(3):
+        q.neg_(), q.neg_()
+        graph.replay()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        masks.append(got[2] != 0)
+    assert not torch.equal(masks[0], masks[1]) and not torch.equal(masks[1], masks[2])
+    # other inputs at the same addresses
+    q.neg_()
+    graph.replay()
+    assert torch.equal(got[0], cross_attention(q, k, v)) and not torch.equal(got[0], want[0])
