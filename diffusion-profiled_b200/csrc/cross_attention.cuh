@@ -341,7 +341,7 @@ struct XFwdParams {
   uint32_t join_at;
 };
 constexpr uint32_t kXJoinCounters = 1u << 20;
-constexpr int kXMaxSplits = 128;
+constexpr int kXMaxSplits = 128;  // four a lane
 
 // A CTA works on one row tile of HALVES * 64 channels at a time, and an SM holds two CTAs: while one begins or ends an
 // item, the other computes.  (One CTA with two row tiles, which share its key and value tiles, took 3 to 16 % longer:
@@ -899,25 +899,41 @@ __global__ void __launch_bounds__(256) x_combine_kernel(const XFwdParams p) {
        r += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
     const int token = static_cast<int>(r % a.q_len), head = static_cast<int>(r / a.q_len % a.heads),
               b = static_cast<int>(r / a.q_len / a.heads);
-    float m = -INFINITY;
-    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_lse[s * p.rows + r]);
+    float w[kXMaxSplits / 32], m = -INFINITY;  // lane = split
+#pragma unroll
+    for (int k = 0; k < kXMaxSplits / 32; ++k) {
+      w[k] = k * 32 + lane < p.splits ? p.part_lse[(k * 32 + lane) * p.rows + r] : -INFINITY;
+      m = fmaxf(m, w[k]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float ref = m == -INFINITY ? 0.0f : m;
     float total = 0.0f, o[4] = {};
-    for (int s = 0; s < p.splits; ++s) {
-      const float lse = p.part_lse[s * p.rows + r];
-      if (lse == -INFINITY) continue;  // a split without keys wrote no output
-      const float w = ex2(lse - ref);
-      total += w;
-      if (lane * 4 < a.head_dim) {
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * p.rows + r) * a.head_dim + lane * 4);
-        o[0] = fmaf(w, v.x, o[0]);
-        o[1] = fmaf(w, v.y, o[1]);
-        o[2] = fmaf(w, v.z, o[2]);
-        o[3] = fmaf(w, v.w, o[3]);
+#pragma unroll
+    for (int k = 0; k < kXMaxSplits / 32; ++k) total += w[k] = ex2(w[k] - ref);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    constexpr int kAtOnce = 8;  // loads under way
+#pragma unroll
+    for (int k = 0; k < kXMaxSplits / 32; ++k)
+      for (int s0 = k * 32; s0 < min(p.splits, k * 32 + 32); s0 += kAtOnce) {
+        float4 v[kAtOnce];
+        float f[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          f[u] = __shfl_sync(0xffffffffu, w[k], (s0 + u) & 31);  // 0 beyond the splits
+          v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (f[u] != 0.0f && lane * 4 < a.head_dim)  // a split without keys wrote no output
+            v[u] = *reinterpret_cast<const float4*>(p.part_o + ((s0 + u) * p.rows + r) * a.head_dim + lane * 4);
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          o[0] = fmaf(f[u], v[u].x, o[0]);
+          o[1] = fmaf(f[u], v[u].y, o[1]);
+          o[2] = fmaf(f[u], v[u].z, o[2]);
+          o[3] = fmaf(f[u], v[u].w, o[3]);
+        }
       }
-    }
     const float inv = total > 0.0f ? __fdividef(1.0f, total) : (total == total ? 0.0f : total);
     if (lane * 4 < a.head_dim)
       *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + b * a.so.batch + token * a.so.token + head * a.so.head + lane * 4) =

@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedSumParams p) 
 }
 
 // Rows that cross chunks: the partial sum of the chunk the row begins in, then those of the chunks it goes on in.  A
-// warp takes 128 channels (4 a lane), 16 partial sums in flight: a row that is a twentieth of a long batch has over a
+// warp takes 128 channels (4 a lane), 8 partial sums in flight: a row that is a twentieth of a long batch has over a
 // hundred.
 constexpr int kJoinSlice = 128;
 template <typename TW>
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedSumParams p)
     };
     float acc[4];
     part(p.tail, chunk, acc);
-    constexpr int kAtOnce = 16;
+    constexpr int kAtOnce = 8;
     for (int of = chunk + 1; of <= last; of += kAtOnce) {
       float f[kAtOnce][4];
 #pragma unroll
