@@ -403,9 +403,9 @@ __device__ __forceinline__ int x_chunks64(int keys, int u) { return (min(64, key
 
 // This warp's rows of a split are written.  The warp that is the last of the splits to say so joins them, in the order
 // of the splits: o = sum_s 2^(lse_s - lse) o_s.  For calls of one warp's rows a (sequence, head group) and one item a
-// CTA: it takes as long as x_combine_kernel does (one query, 1,024 keys: 10.6 us in all), but no launch, whose time on
-// the host such a call waits for.  Where a CTA goes on with other items, the wait for the memory's answer, behind the
-// copies under way, holds them up: 32 queries over 8,192 keys took 161 us, with the second launch 97.
+// CTA: it takes as long as a launch of x_combine_kernel does (one query, 1,024 keys: 9.4 us in all), but not that
+// launch's time on the host, which such a call waits for.  Where a CTA goes on with other items, the wait for the memory's answer, behind the
+// copies under way, holds them up: 32 queries over 8,192 keys took 161 us, with the second launch 93.
 // r_index: this lane's row; o_at: where its output goes.
 template <typename T>
 __device__ __forceinline__ void x_join(const XFwdParams& p, uint32_t counter, bool live, int64_t r_index, int64_t o_at) {
