@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       mbar_init(acc_free + i, kXBwdWarps);
       mbar_init(staged + i, kXBwdWarps);
     }
-    mbar_init(dp_full, 1);
+    mbar_init(dp_full, 2);  // the products' commit, and the issuing warp (rows of K zeroed)
     mbar_init(dp_free, kXBwdWarps);
     mbar_init(delta_full, SPLIT ? kXBwdWarps : 8);
     *abort_flag = 0;
@@ -315,7 +315,6 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         uint4 w = make_uint4(~0u, ~0u, ~0u, ~0u);
         if (bits) w = words[g % kXMaskSlots];
         const bool holes = (w.x & w.y & w.z & w.w) != 0xffffffffu;
-        if (holes) x_zero_rows<HALVES>(sk, w, x_chunks(t.keys, j) * 32, lane);
         if (g >= 2 && !(ok = wait(s_free + buf, (g >> 1) ^ 1, kWaitSFree))) break;
         tc_fence_after();
         if (elect_one()) {
@@ -324,6 +323,9 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
           mbar_arrive(s_full + buf);
         }
         __syncwarp();
+        // Keys that are not kept: K with zeros for dQ, where the zeros of dS would not keep an infinity out (what the scores
+        // read there is replaced), V for dP, so that dS gets them.
+        if (holes) x_zero_rows<HALVES>(sk, w, x_chunks(t.keys, j) * 32, lane);
         if (!(ok = wait(v_full + vs, g / Ly::kVStages, kWaitV))) break;
         if (holes) x_zero_rows<HALVES>(sv, w, x_chunks(t.keys, j) * 32, lane);
         if (g >= 1 && !(ok = wait(dp_free, g ^ 1, kWaitDPFree))) break;
@@ -332,6 +334,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
           products_k_major(tmem + kXDqDP, sdo, k_major_desc(smem_u32(sv)), idesc, ksteps);
           umma_commit(v_empty + vs);
           umma_commit(dp_full);
+          mbar_arrive(dp_full);
         }
         __syncwarp();
       }
@@ -827,12 +830,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       const int ks = n_item % Ly::kKVStages;
       ok = wait(kv_full + ks, n_item / Ly::kKVStages, kWaitK);
       if (!ok) break;
-      const uint4 w = words[n_item % (2 * Ly::kKVStages)];
-      if ((w.x & w.y & w.z & w.w) != 0xffffffffu) {
-        // rows past the states were copied as zeros
-        x_zero_rows<HALVES>(smem + 2 * ks * Ly::kTileBytes, w, a.k_len - t.tile * kXTile, lane);
-        x_zero_rows<HALVES>(smem + (2 * ks + 1) * Ly::kTileBytes, w, a.k_len - t.tile * kXTile, lane);
-      }
+      // (What lies at a key that is not kept reaches that key's lane alone, whose gradients are zeroed at the end.)
       const uint64_t sk = k_major_desc(s_base + 2 * ks * Ly::kTileBytes);
       const uint64_t sv = k_major_desc(s_base + (2 * ks + 1) * Ly::kTileBytes);
       for (int j = t.j0; j < t.j1 && ok; ++j, ++g) {
