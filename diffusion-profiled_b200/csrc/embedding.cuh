@@ -94,10 +94,21 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const EmbedParams p) {
             }
       }
     } else {
+      constexpr int kAtOnce = 8;  // 256 channels of each token
+      for (int c0 = lane; c0 < p.width; c0 += 32 * kAtOnce) {
+        TW v[kTokens][kAtOnce];
 #pragma unroll
-      for (int t = 0; t < kTokens; ++t)
-        if (there[t])
-          for (int c = lane; c < p.width; c += 32) o[t][c] = from_f32<TO>(valid[t] ? to_f32(w[t][c]) * p.scale : 0.0f);
+        for (int t = 0; t < kTokens; ++t)
+#pragma unroll
+          for (int u = 0; u < kAtOnce; ++u)
+            if (there[t] && c0 + 32 * u < p.width) v[t][u] = w[t][c0 + 32 * u];
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t)
+#pragma unroll
+          for (int u = 0; u < kAtOnce; ++u)
+            if (there[t] && c0 + 32 * u < p.width)
+              o[t][c0 + 32 * u] = from_f32<TO>(valid[t] ? to_f32(v[t][u]) * p.scale : 0.0f);
+      }
     }
   }
 }
