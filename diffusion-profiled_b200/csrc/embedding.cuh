@@ -24,6 +24,8 @@
 // sort 36, sums 158 (805 MB, 5.1 TB/s), join 20: 332 us against 246 of bytes.
 #pragma once
 
+#include <type_traits>
+
 #include "dropout.cuh"
 #include "sm100_common.cuh"
 
@@ -94,21 +96,44 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const EmbedParams p) {
             }
       }
     } else {
-      constexpr int kAtOnce = 8;  // 256 channels of each token
-      for (int c0 = lane; c0 < p.width; c0 += 32 * kAtOnce) {
-        TW v[kTokens][kAtOnce];
+      // 16-bit outputs in pairs from the row's first 4-byte boundary on, so that a warp's store fills whole sectors but
+      // for its ends (100,000 x 777 bf16: 67 us, with 2-byte stores 108)
+      constexpr int kPer = sizeof(TO) == 2 ? 2 : 1, kAtOnce = 8 / kPer;  // 256 channels of each token
+      int head[kTokens];
+#pragma unroll
+      for (int t = 0; t < kTokens; ++t) head[t] = kPer == 2 ? (reinterpret_cast<uintptr_t>(o[t]) >> 1) & 1 : 0;
+      for (int c0 = lane * kPer; c0 < p.width; c0 += 256) {
+        TW v[kTokens][kAtOnce][kPer];
 #pragma unroll
         for (int t = 0; t < kTokens; ++t)
 #pragma unroll
           for (int u = 0; u < kAtOnce; ++u)
-            if (there[t] && c0 + 32 * u < p.width) v[t][u] = w[t][c0 + 32 * u];
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+              const int c = head[t] + c0 + 32 * kPer * u;
+              if (there[t] && c + kPer <= p.width) v[t][u][k] = w[t][c + k];
+            }
 #pragma unroll
         for (int t = 0; t < kTokens; ++t)
 #pragma unroll
-          for (int u = 0; u < kAtOnce; ++u)
-            if (there[t] && c0 + 32 * u < p.width)
-              o[t][c0 + 32 * u] = from_f32<TO>(valid[t] ? to_f32(v[t][u]) * p.scale : 0.0f);
+          for (int u = 0; u < kAtOnce; ++u) {
+            const int c = head[t] + c0 + 32 * kPer * u;
+            if (!there[t] || c + kPer > p.width) continue;
+            struct alignas(sizeof(TO) * kPer) {
+              TO x[kPer];
+            } out;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) out.x[k] = from_f32<TO>(valid[t] ? to_f32(v[t][u][k]) * p.scale : 0.0f);
+            *reinterpret_cast<decltype(out)*>(o[t] + c) = out;
+          }
       }
+      if constexpr (kPer == 2)  // the row's first and last value where they are not of a pair
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) {
+          const int c = lane == 0 ? 0 : p.width - 1;
+          if (there[t] && ((lane == 0 && head[t] == 1) || (lane == 1 && p.width > head[t] && ((p.width - head[t]) & 1))))
+            o[t][c] = from_f32<TO>(valid[t] ? to_f32(w[t][c]) * p.scale : 0.0f);
+        }
     }
   }
 }
@@ -332,24 +357,50 @@ template <bool VEC>
 __device__ __forceinline__ int slice_channel(int slice, int lane, int k) {
   return slice * kSumSlice + (VEC ? lane * 8 + k : k * 32 + lane);
 }
-// The 8 channels as loaded (widened only when they are added: loads in flight take half the registers).
+// The 8 channels as loaded (widened only when they are added: loads in flight take half the registers).  16-bit values
+// that are loaded one by one stay in a register each: to pack two, the warp would wait for them (100,000 x 777 bf16:
+// 66 us, packed 147).
 template <typename T, bool VEC>
-__device__ __forceinline__ Words8<T> slice_load(const T* row, int slice, int lane, int width) {
-  Words8<T> v;
+struct SliceWords {
+  Words8<T> w;
+};
+template <typename T>
+struct SliceWords<T, false> {
+  uint32_t r[8];
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ SliceWords<T, VEC> slice_load(const T* row, int slice, int lane, int width) {
+  SliceWords<T, VEC> v;
   if constexpr (VEC) {
     const int c = slice_channel<true>(slice, lane, 0);
-    if (c < width) return load_words8(row + c);
+    if (c < width) {
+      v.w = load_words8(row + c);
+    } else {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) v.w[i] = make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) v.w.w[i] = make_uint4(0, 0, 0, 0);
+    }
   } else {
-    T* t = reinterpret_cast<T*>(&v);
+    using Bits = std::conditional_t<sizeof(T) == 2, unsigned short, uint32_t>;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int c = slice_channel<false>(slice, lane, k);
-      t[k] = c < width ? row[c] : from_f32<T>(0.0f);
+      v.r[k] = c < width ? __ldg(reinterpret_cast<const Bits*>(row) + c) : 0u;
     }
   }
   return v;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void slice_widen(const SliceWords<T, VEC>& v, float (&f)[8]) {
+  if constexpr (VEC) {
+    widen8(v.w, f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if constexpr (sizeof(T) == 4) f[k] = __uint_as_float(v.r[k]);
+      else if constexpr (std::is_same_v<T, __half>) f[k] = __half2float(__ushort_as_half(static_cast<unsigned short>(v.r[k])));
+      else f[k] = __uint_as_float(v.r[k] << 16);
+    }
+  }
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void slice_store(T* row, int slice, int lane, int width, const float (&f)[8]) {
@@ -394,9 +445,9 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedSumParams p) 
     };
     // Batches of kAtOnce rows; the next batch's loads are under way while this one is added.
     constexpr int kAtOnce = 4;
-    Words8<TO> rows[2][kAtOnce];
+    SliceWords<TO, VEC> rows[2][kAtOnce];
     uint32_t my_key = 0, my_pos = 0;
-    const auto fetch = [&](int at, Words8<TO>(&to)[kAtOnce]) {
+    const auto fetch = [&](int at, SliceWords<TO, VEC>(&to)[kAtOnce]) {
       if (((at - begin) & 31) == 0 && at < end) my_pos = at + lane < end ? p.pos[at + lane] : 0u;
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
@@ -424,7 +475,7 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedSumParams p) 
             for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
           }
           float f[8];
-          widen8(rows[half][u], f);
+          slice_widen<TO, VEC>(rows[half][u], f);
 #pragma unroll
           for (int k = 0; k < 8; ++k) acc[k] += f[k];
         }
@@ -560,7 +611,7 @@ __global__ void __launch_bounds__(kFewThreads) embed_few_kernel(const EmbedFewPa
   for (int s = 0; s < kSteps; ++s)
     for (unsigned left = same[s]; left != 0;) {
       constexpr int kAtOnce = 4;
-      Words8<TO> rows[kAtOnce];
+      SliceWords<TO, VEC> rows[kAtOnce];
       bool in[kAtOnce];
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
@@ -573,7 +624,7 @@ __global__ void __launch_bounds__(kFewThreads) embed_few_kernel(const EmbedFewPa
       for (int u = 0; u < kAtOnce; ++u)
         if (in[u]) {
           float f[8];
-          widen8(rows[u], f);
+          slice_widen<TO, VEC>(rows[u], f);
 #pragma unroll
           for (int k = 0; k < 8; ++k) acc[k] += f[k];
         }
