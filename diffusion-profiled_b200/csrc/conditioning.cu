@@ -152,6 +152,8 @@ int bind_context() {
 // half as many as it has CTAs at most, so launches that can run at the same time use different ones unless some 7,000
 // of them were issued between the two.
 __device__ unsigned int g_x_join_counters[kXJoinCounters];
+static_assert(kXJoinCounters == kJoinCounters, "what fp8_device_error sets back");
+static_assert(kErrXForward + 1 == kFirstForwardError && kErrXDq - 1 == kLastForwardError, "the forward's codes");
 
 int x_join_counters(DeviceState* st, uint32_t n, unsigned int** ring, uint32_t* at) {
   static std::atomic<uint32_t> next{0};
@@ -183,11 +185,11 @@ XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
   const int64_t base = static_cast<int64_t>(a->batch) * w.hv * w.row_tiles;
   w.splits = 1;
   w.key_chunk = w.n_tiles;
-  // A split writes its rows' partial outputs in fp32.  With a few rows a tile that is nothing, and pieces that
-  // are a quarter of an even share even out sequences of different lengths (finer ones only make the join longer: 32
-  // queries over 8192 keys, 88 us and the join at four pieces a CTA, the same at eight and twelve, 92 at sixteen); with whole tiles of rows
-  // the keys are split only to reach SMs that would have no work at all (5 x 333 queries of 8 heads over 1021 keys, 110
-  // row tiles: 28 us unsplit, 36 split for two CTAs an SM).
+  // A split writes its rows' partial outputs in fp32.  With a few rows a tile that is nothing, and pieces that are a
+  // quarter of an even share even out sequences of different lengths (finer ones only make the join longer: 32 queries
+  // over 8192 keys, 88 us and the join at four pieces a CTA, the same at eight and twelve, 92 at sixteen).  With whole
+  // tiles of rows the keys are split only to reach SMs that would have no work at all (5 x 333 queries of 8 heads over
+  // 1021 keys, 110 row tiles: 28 us unsplit, 36 split for two CTAs an SM).
   const bool few_rows = w.row_tiles == 1 && a->q_len * pack <= 16;
   const int64_t pieces = few_rows ? 4 * w.slots : sm_count;
   if (w.n_tiles > 1 && 2 * base <= pieces) {

@@ -49,6 +49,11 @@ struct DeviceState {
 // The current device's state.
 int device_state(DeviceState** out);
 
+// Counters of the attention's splits (join_base): a forward launch that gave up leaves its own as they are, so
+// fp8_device_error sets all back when it reports one.
+constexpr unsigned int kJoinCounters = 1u << 20;
+constexpr int kFirstForwardError = 301, kLastForwardError = 319;
+
 // Counters in device memory that a launch's CTAs meet at, zero between launches.
 constexpr int kFoldCounters = 8192;
 // The counter of the next launch that folds a scale in its last CTA, or holds a grid barrier.
