@@ -298,3 +298,34 @@ def test_refusals(cuda):
                 lambda: cross_attention(q, k, k, scale=float("nan")), lambda: cross_attention_packed(q, k)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_states_whose_offsets_pass_32_bits(cuda):
+    """Packed states of 4.6e9 values: only a few keys of each sequence are kept, the last one's far behind 2^32."""
+    from fp8_b200.cross_attention import cross_attention_packed
+
+    b, lk, hkv, d = 2, 1_130_000, 8, 128
+    kv = torch.empty(b, lk, 2, hkv, d, dtype=BF16, device=cuda)  # what is not kept is whatever was there
+    assert kv.numel() > 2**32
+    g = torch.Generator(device=cuda).manual_seed(0)
+    keep = torch.zeros(b, lk, dtype=torch.bool, device=cuda)
+    at = [[5, 70_000, lk - 1], [0, 130, lk - 2]]
+    few = torch.randn(b, 3, 2, hkv, d, device=cuda, generator=g).to(BF16)
+    for i in range(b):
+        keep[i, at[i]] = True
+        kv[i, at[i]] = few[i]
+    q = torch.randn(b, 3, hkv, d, device=cuda, generator=g).to(BF16).requires_grad_(True)
+    dout = torch.randn(b, 3, hkv, d, device=cuda, generator=g).to(BF16)
+    kv.requires_grad_(True)
+    out = cross_attention_packed(q, kv, key_mask=keep)
+    dq, dkv = torch.autograd.grad(out, (q, kv), dout)
+    want = oracle.cross_attention(q.detach().cpu(), few[:, :, 0].cpu(), few[:, :, 1].cpu(), dout.cpu(), None, None)
+    picked = torch.stack([dkv[i, at[i]] for i in range(b)])
+    got = {"o": out, "dq": dq, "dk": picked[:, :, 0], "dv": picked[:, :, 1]}
+    for name, x in got.items():
+        exact, bound = want[name]
+        worst = oracle.excess(x.detach().cpu(), exact, bound)
+        assert worst <= 1.0, f"{name}: {worst:.3f} of its bound"
+    for i in range(b):
+        for near in (at[i][1] - 1, at[i][1] + 1, lk - 3):
+            assert torch.count_nonzero(dkv[i, near]) == 0

@@ -166,3 +166,20 @@ def test_refusals(cuda):
                 lambda: embed_tokens(ids, w, padding_idx=-5), lambda: embed_tokens(ids, w[:0])):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_rows_whose_offsets_pass_32_bits(cuda):
+    from fp8_b200.embedding import embed_tokens, embedding_bwd
+
+    vocab, width = 70_000, 65_536  # 4.6e9 values
+    w = torch.empty(vocab, width, dtype=BF16, device=cuda)
+    ids = torch.tensor([69_999, 3, 69_999, 40_001], device=cuda)
+    rows = torch.randn(4, width, device=cuda).to(BF16)
+    w[ids] = rows
+    assert torch.equal(embed_tokens(ids, w), w[ids])
+    del w
+    dout = torch.randn(4, width, device=cuda).to(BF16)
+    dw = embedding_bwd(ids, dout, vocab, 1.0, -1, BF16)
+    assert torch.equal(dw[3], dout[1]) and torch.equal(dw[40_001], dout[3])
+    assert torch.equal(dw[69_999], (dout[0].float() + dout[2].float()).to(BF16))
+    assert torch.count_nonzero(dw[69_998]) == 0 and torch.count_nonzero(dw[40_000]) == 0
