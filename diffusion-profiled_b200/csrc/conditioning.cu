@@ -4,7 +4,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 
 #include "cross_attention.cuh"
@@ -148,26 +147,6 @@ int bind_context() {
   return FP8_OK;
 }
 
-// Counters at which the splits of a forward call meet, zero between launches.  A launch takes the next ones of a ring:
-// half as many as it has CTAs at most, so launches that can run at the same time use different ones unless some 7,000
-// of them were issued between the two.
-__device__ unsigned int g_x_join_counters[kXJoinCounters];
-static_assert(kXJoinCounters == kJoinCounters, "what fp8_device_error sets back");
-static_assert(kErrXForward + 1 == kFirstForwardError && kErrXDq - 1 == kLastForwardError, "the forward's codes");
-
-int x_join_counters(DeviceState* st, uint32_t n, unsigned int** ring, uint32_t* at) {
-  static std::atomic<uint32_t> next{0};
-  *ring = st->join_base.load(std::memory_order_relaxed);
-  if (*ring == nullptr) {  // every caller finds the same address
-    void* p = nullptr;
-    FP8_CUDA_TRY(cudaGetSymbolAddress(&p, g_x_join_counters));
-    *ring = static_cast<unsigned int*>(p);
-    st->join_base.store(*ring, std::memory_order_relaxed);
-  }
-  *at = next.fetch_add(n, std::memory_order_relaxed);
-  return FP8_OK;
-}
-
 // How a forward call divides its work.
 struct XPlan {
   int row_tiles, hv, n_tiles, splits, key_chunk;
@@ -201,8 +180,15 @@ XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
   w.join_inside = few_rows && w.splits > 1 && w.items <= w.slots;
   return w;
 }
+// The workspace: the splits' outputs, their log-sum-exps and, where the launch joins them, its counters.  (The counters
+// are the call's own, zeroed before its launch: neither another call nor a replay of a captured one can meet them, and a
+// launch that gave up leaves nothing behind.)
+size_t x_part_floats(const fp8_cross_attention_args* a, const XPlan& w) {
+  return w.splits == 1 ? 0 : static_cast<size_t>(w.splits) * w.rows * (a->head_dim + 1);
+}
+size_t x_join_counters(const XPlan& w) { return w.join_inside ? static_cast<size_t>(w.items / w.splits) : 0; }
 size_t x_fwd_workspace(const fp8_cross_attention_args* a, const XPlan& w) {
-  return w.splits == 1 ? 0 : sizeof(float) * static_cast<size_t>(w.splits) * w.rows * (a->head_dim + 1);
+  return sizeof(float) * x_part_floats(a, w) + sizeof(unsigned int) * x_join_counters(w);
 }
 
 template <typename T, int HALVES>
@@ -230,8 +216,10 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
   f.rows = w.rows;
   f.items = static_cast<uint32_t>(w.items);
   if (int s = bind_context()) return s;
-  if (w.join_inside)
-    if (int s = x_join_counters(st, static_cast<uint32_t>(w.items / w.splits), &f.join, &f.join_at)) return s;
+  if (w.join_inside) {
+    f.join = reinterpret_cast<unsigned int*>(f.part_o + x_part_floats(args, w));
+    FP8_CUDA_TRY(cudaMemsetAsync(f.join, 0, sizeof(unsigned int) * x_join_counters(w), stream));
+  }
   CUtensorMap maps[4];
   const int dt = args->dtype;
   if (int s = x_map(&maps[0], a.q, dt, a.sq, a.batch, a.q_len, a.heads, a.head_dim, a.pack, a.tile_tokens)) return s;

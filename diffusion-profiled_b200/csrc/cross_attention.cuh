@@ -335,12 +335,10 @@ struct XFwdParams {
   float* part_lse;  // [splits][batch * heads * q_len], base-2 logarithm
   int64_t rows;     // batch * heads * q_len
   uint32_t items;   // (sequence, head group, row tile group, split)
-  // where the launch itself joins the splits (x_join): a ring of counters, zero between launches, of which it has those
-  // from join_at on, one for each (sequence, head group); else null
+  // where the launch itself joins the splits (x_join): a counter for each (sequence, head group), zero when it starts;
+  // else null
   unsigned int* join;
-  uint32_t join_at;
 };
-constexpr uint32_t kXJoinCounters = 1u << 20;
 constexpr int kXMaxSplits = 128;  // four a lane
 
 // A CTA works on one row tile of HALVES * 64 channels at a time, and an SM holds two CTAs: while one begins or ends an
@@ -403,19 +401,19 @@ __device__ __forceinline__ int x_chunks64(int keys, int u) { return (min(64, key
 
 // This warp's rows of a split are written.  The warp that is the last of the splits to say so joins them, in the order
 // of the splits: o = sum_s 2^(lse_s - lse) o_s.  For calls of one warp's rows a (sequence, head group) and one item a
-// CTA: it takes as long as a launch of x_combine_kernel does (one query, 1,024 keys: 9.4 us in all), but not that
-// launch's time on the host, which such a call waits for.  Where a CTA goes on with other items, the wait for the memory's answer, behind the
-// copies under way, holds them up: 32 queries over 8,192 keys took 161 us, with the second launch 93.
+// CTA, which wait for the host: zeroing the counters and joining here takes less of its time than a launch of
+// x_combine_kernel (one query over 1,024 keys: 12.3 us a call against 13.2).  Where a CTA goes on with other items, the
+// wait for the memory's answer, behind the copies under way, holds them up: 32 queries over 8,192 keys took 161 us, with
+// the second launch 93.
 // r_index: this lane's row; o_at: where its output goes.
 template <typename T>
 __device__ __forceinline__ void x_join(const XFwdParams& p, uint32_t counter, bool live, int64_t r_index, int64_t o_at) {
   const int lane = threadIdx.x & 31;
-  unsigned int* const arrived = p.join + (p.join_at + counter) % kXJoinCounters;
   __syncwarp();  // the other lanes' writes come before this one's release
   unsigned int before = 0;
-  if (lane == 0) before = atom_add_acq_rel_gpu_u32(arrived, 1u);
+  if (lane == 0) before = atom_add_acq_rel_gpu_u32(p.join + counter, 1u);
   if (__shfl_sync(~0u, before, 0) + 1 != static_cast<unsigned int>(p.splits)) return;
-  if (lane == 0) *arrived = 0;
+  __syncwarp();  // and this one's acquire before what the others read (the shuffle orders no memory)
   const int head_dim = p.a.head_dim, rows = __popc(__ballot_sync(~0u, live));  // the first lanes
   // ---- lane = row: the sum of the splits' weights
   constexpr int kAtOnce = 8;

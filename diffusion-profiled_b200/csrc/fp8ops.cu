@@ -915,11 +915,6 @@ int fp8_device_error(int* code_out, fp8_stream_t stream) {
   if (code != 0) {
     const int zero = 0;
     FP8_CUDA_TRY(cudaMemcpyToSymbol(g_fp8_device_error, &zero, sizeof(int)));
-    unsigned int* const join = st->join_base.load(std::memory_order_relaxed);
-    if (join != nullptr && code >= kFirstForwardError && code <= kLastForwardError) {
-      FP8_CUDA_TRY(cudaDeviceSynchronize());
-      FP8_CUDA_TRY(cudaMemset(join, 0, sizeof(unsigned int) * kJoinCounters));
-    }
   }
   *code_out = code;
   return ok();

@@ -40,7 +40,6 @@ struct DeviceState {
   int* err_ptr = nullptr;             // device error word
   unsigned int* fold_base = nullptr;  // the device's counters (fold_counter)
   std::atomic<unsigned int> fold_next{0};
-  std::atomic<unsigned int*> join_base{nullptr};  // the device's counters of the attention's splits (conditioning.cu)
   // Set (release) after the fields above are written; a reader that sees it
   // (acquire) sees them too.
   std::atomic<bool> init{false};
@@ -48,11 +47,6 @@ struct DeviceState {
 
 // The current device's state.
 int device_state(DeviceState** out);
-
-// Counters of the attention's splits (join_base): a forward launch that gave up leaves its own as they are, so
-// fp8_device_error sets all back when it reports one.
-constexpr unsigned int kJoinCounters = 1u << 20;
-constexpr int kFirstForwardError = 301, kLastForwardError = 319;
 
 // Counters in device memory that a launch's CTAs meet at, zero between launches.
 constexpr int kFoldCounters = 8192;

@@ -1,0 +1,83 @@
+"""GPU tests of what the conditioning operators share between calls: nothing.
+
+Where CTAs of a launch meet, they meet at counters of the call's own workspace, which the
+call zeroes: whatever the workspace held, whatever runs beside the call, and however often a
+captured call is replayed, the results are the same.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import conditioning_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def _single_queries(cuda, b, lk, h, hkv, d, seed=0):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    new = lambda *s: torch.randn(*s, device=cuda, generator=g).to(BF16)  # noqa: E731
+    return new(b, 1, h, d), new(b, lk, hkv, d), new(b, lk, hkv, d)
+
+
+def _attention_args(q, k, v, o):
+    from fp8_b200 import _lib
+
+    a = _lib.CrossAttentionArgs(batch=q.shape[0], q_len=q.shape[1], k_len=k.shape[1], heads=q.shape[2], kv_heads=k.shape[2],
+                                head_dim=q.shape[3], dtype=0, scale=q.shape[3] ** -0.5)
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", o)):
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_stride", _lib.HeadStrides(*t.stride()[:3]))
+    return a
+
+
+def test_attention_joins_at_counters_of_its_workspace(cuda):
+    from fp8_b200 import _lib
+
+    lib = _lib.load()
+    q, k, v = _single_queries(cuda, 3, 1000, 4, 2, 64)
+    o = torch.empty_like(q)
+    a = _attention_args(q, k, v, o)
+    splits = 8  # one of each 128 keys
+    partial = 4 * splits * 3 * 4 * (64 + 1)
+    need = lib.fp8_cross_attention_workspace_bytes(ctypes.byref(a), 0)
+    assert need == partial + 4 * 3 * 2  # a counter for each sequence and key head
+    ws = torch.empty(need, dtype=torch.uint8, device=cuda)
+    stream = torch.cuda.current_stream(cuda).cuda_stream
+    want = oracle.cross_attention(q, k, v)["o"]
+    for fill in (0, 255, 1):
+        ws.fill_(fill)
+        o.fill_(torch.nan)
+        assert lib.fp8_cross_attention_fwd(ctypes.byref(a), ws.data_ptr(), need, stream) == 0, _lib.last_error()
+        assert oracle.excess(o, *want) <= 1.0
+    assert lib.fp8_cross_attention_fwd(ctypes.byref(a), ws.data_ptr(), need - 4, stream) != 0
+
+
+def test_a_replayed_attention_beside_many_calls(cuda):
+    """A captured call replayed on one stream while another stream issues 9,000 calls of 128 joins each."""
+    from fp8_b200.cross_attention import cross_attention
+
+    q, k, v = _single_queries(cuda, 32, 256, 4, 4, 64, seed=1)
+    want = cross_attention(q, k, v)
+    assert oracle.excess(want, *oracle.cross_attention(q, k, v)["o"]) <= 1.0
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = cross_attention(q, k, v)
+    replays, eager = torch.cuda.Stream(cuda), torch.cuda.Stream(cuda)
+    wrong = torch.zeros((), dtype=torch.int64, device=cuda)
+    torch.cuda.synchronize()
+    for i in range(9000):
+        with torch.cuda.stream(eager):
+            last = cross_attention(q, k, v)
+        if i % 4 == 0:
+            with torch.cuda.stream(replays):
+                got.fill_(torch.nan)
+                graph.replay()
+                wrong += (got != want).any()
+    torch.cuda.synchronize()
+    assert wrong.item() == 0 and torch.equal(last, want)
