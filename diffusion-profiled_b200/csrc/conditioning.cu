@@ -384,7 +384,7 @@ struct EmbedPlan {
   int passes, bits, ctas, per_cta;
   int chunk, slices;
   int64_t chunks;
-  size_t key[2], pos[2], counts, live, present, head, tail, bytes;
+  size_t key[2], pos[2], counts, live, arrive, present, head, tail, bytes;
 };
 EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
   EmbedPlan w{};
@@ -412,6 +412,8 @@ EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
   }
   w.counts = take(sizeof(uint32_t) * static_cast<size_t>(w.ctas) << w.bits);
   w.live = take(sizeof(uint32_t));
+  // (the call's own, as the attention's: zeroed before the launch whose CTAs meet there)
+  w.arrive = take(sizeof(uint32_t));
   w.present = take(sizeof(uint32_t) * static_cast<size_t>(vocab / 32 + 1));
   w.head = take(sizeof(float) * static_cast<size_t>(w.chunks) * width);
   w.tail = take(sizeof(float) * static_cast<size_t>(w.chunks) * width);
@@ -538,8 +540,8 @@ int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* do
   so.counts = reinterpret_cast<uint32_t*>(ws + w.counts);
   so.live = reinterpret_cast<uint32_t*>(ws + w.live);
   so.present = reinterpret_cast<uint32_t*>(ws + w.present);
-  so.arrive = fold_counter(st);
-  so.depart = fold_counter(st);
+  so.arrive = reinterpret_cast<unsigned int*>(ws + w.arrive);
+  if (w.ctas > 1) FP8_CUDA_TRY(cudaMemsetAsync(so.arrive, 0, sizeof(unsigned int), cuda_stream(stream)));
   so.err = st->err_ptr;
   const size_t smem = sizeof(uint32_t) * ((kSortWarps + 1) * (size_t(1) << w.bits) + kSortWarps);
   FP8_CUDA_TRY(cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));

@@ -157,7 +157,7 @@ struct EmbedSortParams {
   uint32_t* counts;        // [gridDim.x][1 << bits]
   uint32_t* live;          // number of keys below vocab
   uint32_t* present;       // bit v: row v occurs; [vocab / 32 + 1] words
-  unsigned int *arrive, *depart;  // zero between launches
+  unsigned int* arrive;    // the call's own, zero when the launch starts (gridDim.x > 1)
   int* err;
 };
 
@@ -327,12 +327,6 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
       if (k[u] < p.vocab) atomicOr(p.present + (k[u] >> 5), 1u << (k[u] & 31));
       else if (i == 0 || before[u] < p.vocab) *p.live = static_cast<uint32_t>(i);
     }
-  }
-  // the last CTA to leave sets the counters back
-  __syncthreads();
-  if (gridDim.x > 1 && tid == 0 && atom_add_acq_rel_gpu_u32(p.depart, 1u) == gridDim.x - 1) {
-    *p.arrive = 0u;
-    *p.depart = 0u;
   }
 }
 

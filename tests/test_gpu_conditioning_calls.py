@@ -81,3 +81,67 @@ def test_a_replayed_attention_beside_many_calls(cuda):
                 wrong += (got != want).any()
     torch.cuda.synchronize()
     assert wrong.item() == 0 and torch.equal(last, want)
+
+
+def _tokens(cuda, n, vocab, width, seed=0):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    ids = torch.randint(0, vocab, (n,), device=cuda, generator=g)
+    return ids, torch.randn(n, width, device=cuda, generator=g).to(BF16)
+
+
+def _embedding_bwd(ids, dout, dw, ws, need=None):
+    from fp8_b200 import _lib
+
+    return _lib.load().fp8_embedding_bwd(ids.data_ptr(), 1, ids.numel(), dout.data_ptr(), 0, dw.data_ptr(), 1, dw.shape[0],
+                                         dw.shape[1], 1.0, -1, ws.data_ptr(), ws.numel() if need is None else need,
+                                         torch.cuda.current_stream().cuda_stream)
+
+
+def _gradient_error(dw, ids, dout):
+    exact, mag = oracle.embedding_grad(ids, dout, dw.shape[0], 1.0, None)
+    count = torch.bincount(ids.cpu(), minlength=dw.shape[0]).double()[:, None]
+    return oracle.excess(dw, exact, 2.0**-24 * exact.abs() + (count + 2) * 2.0**-24 * mag)
+
+
+def test_embedding_sort_meets_at_a_counter_of_its_workspace(cuda):
+    from fp8_b200 import _lib
+
+    ids, dout = _tokens(cuda, 20_000, 700, 72)
+    need = _lib.load().fp8_embedding_bwd_workspace_bytes(20_000, 700, 72)
+    ws, dw = torch.empty(need, dtype=torch.uint8, device=cuda), torch.empty(700, 72, device=cuda)
+    for fill in (0, 255, 1):
+        ws.fill_(fill)
+        dw.fill_(torch.nan)
+        assert _embedding_bwd(ids, dout, dw, ws) == 0, _lib.last_error()
+        assert _gradient_error(dw, ids, dout) <= 1.0
+    assert _embedding_bwd(ids, dout, dw, ws, need - 16) != 0
+    assert _lib.device_error() == 0
+
+
+def test_a_replayed_gradient_beside_many_calls(cuda):
+    """4,500 calls beside the replays: counters shared in a ring (of 8,192, two a call) would come round."""
+    from fp8_b200 import _lib
+    from fp8_b200.embedding import embedding_bwd
+
+    ids, dout = _tokens(cuda, 5000, 300, 40, seed=1)
+    run = lambda: embedding_bwd(ids, dout, 300, 1.0, -1, torch.float32)  # noqa: E731
+    want = run()
+    assert _gradient_error(want, ids, dout) <= 1.0
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    replays, eager = torch.cuda.Stream(cuda), torch.cuda.Stream(cuda)
+    wrong = torch.zeros((), dtype=torch.int64, device=cuda)
+    torch.cuda.synchronize()
+    for i in range(4500):
+        with torch.cuda.stream(eager):
+            last = run()
+        if i % 4 == 0:
+            with torch.cuda.stream(replays):
+                got.fill_(torch.nan)
+                graph.replay()
+                wrong += (got != want).any()
+    torch.cuda.synchronize()
+    assert wrong.item() == 0 and torch.equal(last, want)
+    assert _lib.device_error() == 0
