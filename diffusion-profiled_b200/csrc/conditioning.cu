@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "cross_attention.cuh"
@@ -411,8 +412,9 @@ EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
     w.pos[i] = take(sizeof(uint32_t) * static_cast<size_t>(tokens));
   }
   w.counts = take(sizeof(uint32_t) * static_cast<size_t>(w.ctas) << w.bits);
+  // zeroed before the sort: the number of live keys, and the counter where its CTAs meet (the call's own, as the
+  // attention's)
   w.live = take(sizeof(uint32_t));
-  // (the call's own, as the attention's: zeroed before the launch whose CTAs meet there)
   w.arrive = take(sizeof(uint32_t));
   w.present = take(sizeof(uint32_t) * static_cast<size_t>(vocab / 32 + 1));
   w.head = take(sizeof(float) * static_cast<size_t>(w.chunks) * width);
@@ -420,6 +422,10 @@ EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
   w.bytes = at;
   return w;
 }
+
+// The sort's waits: fp8_selftest_sort_timeout.
+std::atomic<uint64_t> g_sort_limit_ns{FP8_WAIT_TIMEOUT_NS};
+std::atomic<unsigned int> g_sort_missing{0};
 
 // embed_few_kernel takes the gradient: see kFewTokens (and its grid stays small).
 bool embed_few(int64_t tokens, int width) {
@@ -541,7 +547,10 @@ int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* do
   so.live = reinterpret_cast<uint32_t*>(ws + w.live);
   so.present = reinterpret_cast<uint32_t*>(ws + w.present);
   so.arrive = reinterpret_cast<unsigned int*>(ws + w.arrive);
-  if (w.ctas > 1) FP8_CUDA_TRY(cudaMemsetAsync(so.arrive, 0, sizeof(unsigned int), cuda_stream(stream)));
+  so.meet = static_cast<unsigned int>(w.ctas) + g_sort_missing.load(std::memory_order_relaxed);
+  so.limit_ns = g_sort_limit_ns.load(std::memory_order_relaxed);
+  if (so.meet > 1)  // (one CTA waits for none, and always says how many keys are live)
+    FP8_CUDA_TRY(cudaMemsetAsync(so.live, 0, w.arrive + sizeof(uint32_t) - w.live, cuda_stream(stream)));
   so.err = st->err_ptr;
   const size_t smem = sizeof(uint32_t) * ((kSortWarps + 1) * (size_t(1) << w.bits) + kSortWarps);
   FP8_CUDA_TRY(cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
@@ -588,6 +597,13 @@ int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* do
   });
   if (status) return status;
   count_launches(joins > 0 ? 3 : 2);
+  return ok();
+}
+
+int fp8_selftest_sort_timeout(uint64_t limit_ns) {
+  FP8_REQUIRE(limit_ns <= 1000000000ull, FP8_ERR_INVALID_ARGUMENT, "limit_ns must be at most 1e9");
+  g_sort_missing.store(limit_ns == 0 ? 0u : 1u, std::memory_order_relaxed);
+  g_sort_limit_ns.store(limit_ns == 0 ? FP8_WAIT_TIMEOUT_NS : limit_ns, std::memory_order_relaxed);
   return ok();
 }
 

@@ -155,9 +155,11 @@ struct EmbedSortParams {
   uint32_t* key[2];
   uint32_t* pos[2];
   uint32_t* counts;        // [gridDim.x][1 << bits]
-  uint32_t* live;          // number of keys below vocab
+  uint32_t* live;          // number of keys below vocab; zero when the launch starts, and so it stays if a CTA gives up
   uint32_t* present;       // bit v: row v occurs; [vocab / 32 + 1] words
-  unsigned int* arrive;    // the call's own, zero when the launch starts (gridDim.x > 1)
+  unsigned int* arrive;    // the call's own, zero when the launch starts
+  unsigned int meet;       // CTAs that a barrier waits for: gridDim.x (more in the self-test, for a wait that runs out)
+  uint64_t limit_ns;       // and how long it waits
   int* err;
 };
 
@@ -175,17 +177,19 @@ __device__ __forceinline__ unsigned same_digit(uint32_t d, int bits, bool in) {
   return same;
 }
 
-// All CTAs' writes so far are visible to all.  `round` counts the barriers of the launch from 1.
+// All CTAs' writes so far are visible to all.  `round` counts the barriers of the launch from 1.  A CTA that gives up
+// leaves: none of the others passes a later barrier, so `live` stays zero unless the keys are sorted, and the launches
+// behind sum nothing (they never read keys that were not written).
 __device__ __forceinline__ bool sort_barrier(const EmbedSortParams& p, unsigned int round) {
   __shared__ int passed;
   __syncthreads();
-  if (gridDim.x == 1) return true;
+  if (p.meet == 1) return true;
   if (threadIdx.x == 0) {
     red_release_gpu_add_u32(p.arrive, 1u);  // with what the CTA's other threads wrote before the barrier above
     const uint64_t t0 = globaltimer_ns();
     int ok = 1;
-    while (ld_acquire_gpu_u32(p.arrive) < round * gridDim.x) {
-      if (globaltimer_ns() - t0 > FP8_WAIT_TIMEOUT_NS) {
+    while (ld_acquire_gpu_u32(p.arrive) < round * p.meet) {
+      if (globaltimer_ns() - t0 > p.limit_ns) {
         record_error(p.err, kErrTimeoutSort);
         ok = 0;
         break;

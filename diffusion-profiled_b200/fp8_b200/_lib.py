@@ -195,6 +195,7 @@ _SIGNATURES: dict[str, tuple] = {
     "fp8_embedding_bwd": (
         c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_float, c_int64,
                 c_void_p, c_size_t, c_void_p]),
+    "fp8_selftest_sort_timeout": (c_int, [ctypes.c_uint64]),
     "fp8_dropout": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, ctypes.c_double, c_void_p, c_void_p]),
     "fp8_set_conv_algo": (c_int, [c_int]),
     "fp8_set_pdl": (c_int, [c_int]),

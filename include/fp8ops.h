@@ -589,6 +589,11 @@ int fp8_embedding_bwd(const void* ids, int ids64, int64_t tokens, const void* do
                       int weight_dtype, int64_t vocab, int width, float scale, int64_t padding_idx, void* workspace,
                       size_t workspace_bytes, fp8_stream_t stream);
 
+/* Failure-path self test: with 0 < limit_ns <= 1e9, the sort of the embedding
+ * gradients called from now on waits limit_ns for a CTA that does not exist, gives up,
+ * records 202, and the call writes zeros; 0 sets the sort right again.  Process-wide. */
+int fp8_selftest_sort_timeout(uint64_t limit_ns);
+
 /* Dropout with a mask made from a counter: y[e] = keep(e) ? x[e] / (1 - p) : 0, plus
  * residual[e] where residual is not NULL, in fp32, rounded once to dtype.  keep(e):
  * the (e mod 4)-th 16 bits of splitmix64(*seed ^ (e / 4) * 0xD1B54A32D192ED03) are

@@ -145,3 +145,27 @@ def test_a_replayed_gradient_beside_many_calls(cuda):
     torch.cuda.synchronize()
     assert wrong.item() == 0 and torch.equal(last, want)
     assert _lib.device_error() == 0
+
+
+def test_a_sort_that_gives_up_reads_nothing_and_leaves_nothing_behind(cuda):
+    from fp8_b200 import _lib
+
+    lib = _lib.load()
+    assert _lib.device_error() == 0
+    ids, dout = _tokens(cuda, 20_000, 700, 72, seed=2)
+    need = lib.fp8_embedding_bwd_workspace_bytes(20_000, 700, 72)
+    ws, dw = torch.empty(need, dtype=torch.uint8, device=cuda), torch.empty(700, 72, device=cuda)
+    assert lib.fp8_selftest_sort_timeout(10**9 + 1) != 0
+    try:
+        assert lib.fp8_selftest_sort_timeout(20_000_000) == 0
+        ws.fill_(255)
+        dw.fill_(torch.nan)
+        assert _embedding_bwd(ids, dout, dw, ws) == 0, _lib.last_error()
+        assert _lib.device_error(torch.cuda.current_stream().cuda_stream) == 202
+        assert torch.count_nonzero(dw) == 0
+    finally:
+        assert lib.fp8_selftest_sort_timeout(0) == 0
+    for _ in range(2):  # in the same workspace as it was left
+        assert _embedding_bwd(ids, dout, dw, ws) == 0, _lib.last_error()
+        assert _gradient_error(dw, ids, dout) <= 1.0
+    assert _lib.device_error() == 0
