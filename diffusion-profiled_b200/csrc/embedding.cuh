@@ -31,7 +31,6 @@
 
 namespace fp8b {
 
-constexpr int kErrTokenRange = 201;   // a token id outside [0, vocab)
 constexpr int kErrTimeoutSort = 202;  // a CTA gave up waiting for the others between two passes
 
 struct EmbedParams {

@@ -51,8 +51,13 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
   return t;
 }
 
+// A token id outside [0, vocab): the one code that is not a wait that ran out.
+constexpr int kErrTokenRange = 201;
+
+// The first code stays, but that a wait which ran out, after which outputs are not valid, takes the place of an id.
 __device__ __forceinline__ void record_error(int* err, int code) {
-  if (err != nullptr) atomicCAS(err, 0, code);
+  if (err == nullptr) return;
+  if (atomicCAS(err, 0, code) == kErrTokenRange && code != kErrTokenRange) atomicCAS(err, kErrTokenRange, code);
 }
 
 // ---------------------------------------------------------------- mbarrier

@@ -55,8 +55,9 @@ int fp8_abi_version(void);
 int fp8_last_error(char* buf, size_t len);
 
 /* Reads and clears the device-side error word of the current device (kernels
- * record a code there when a bounded wait inside them times out).  Synchronises
- * `stream`.  *code_out = 0 means no device error was recorded. */
+ * record a code there when a bounded wait inside them times out; the first one
+ * stays, but that a time-out takes the place of 201, a token id outside the
+ * vocabulary).  Synchronises `stream`.  *code_out = 0 means no device error was recorded. */
 int fp8_device_error(int* code_out, fp8_stream_t stream);
 
 /* Failure-path self test (no counterpart in the reference, which has no

@@ -169,3 +169,23 @@ def test_a_sort_that_gives_up_reads_nothing_and_leaves_nothing_behind(cuda):
         assert _embedding_bwd(ids, dout, dw, ws) == 0, _lib.last_error()
         assert _gradient_error(dw, ids, dout) <= 1.0
     assert _lib.device_error() == 0
+
+
+def test_an_id_outside_the_vocabulary_does_not_hide_a_time_out(cuda):
+    from fp8_b200 import _lib
+    from fp8_b200.embedding import embed_tokens, embedding_bwd
+
+    lib = _lib.load()
+    assert _lib.device_error() == 0
+    ids, dout = _tokens(cuda, 5000, 300, 40, seed=3)
+    stray = lambda: embed_tokens(torch.full((2,), 300, device=cuda), torch.zeros(300, 8, device=cuda))  # noqa: E731
+    stray()
+    try:
+        assert lib.fp8_selftest_sort_timeout(20_000_000) == 0
+        embedding_bwd(ids, dout, 300, 1.0, -1, torch.float32)
+    finally:
+        assert lib.fp8_selftest_sort_timeout(0) == 0
+    stray()  # and does not take its place
+    assert _lib.device_error() == 202
+    stray()
+    assert _lib.device_error() == 201 and _lib.device_error() == 0
