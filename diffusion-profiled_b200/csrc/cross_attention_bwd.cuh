@@ -110,6 +110,7 @@ struct XDqLayout {
   // Sums of dQ in tensor memory.  With two, an item's is handed out while the next item's products run; with heads of
   // more than 64 there is room for one (and items are longer).
   static constexpr int kAccs = HALVES == 1 ? 2 : 1;
+  static constexpr int kDeltas = SPLIT ? 1 : kAccs;  // buffers of the rows' delta in parts
   static constexpr int kQStages = HALVES == 1 ? (SPLIT ? 4 : 3) : 1;  // Q and dO of an item
   // A key tile stays from its scores to its dQ product, two tiles later; a value tile only for its dP.
   static constexpr int kKStages = HALVES == 1 ? (SPLIT ? 3 : 4) : SPLIT ? 2 : 3;
@@ -117,9 +118,9 @@ struct XDqLayout {
   static constexpr int kK = 2 * kQStages * kTileBytes;
   static constexpr int kV = kK + kKStages * kTileBytes;
   static constexpr int kWords = kV + kVStages * kTileBytes;
-  static constexpr int kDelta = kWords + kXMaskSlots * 16;  // fp32: the rows' delta in parts, [kAccs][2][128] or with SPLIT [4][128]
-  static constexpr int kBar = kDelta + (SPLIT ? 2048 : kAccs * 1024);
-  static constexpr int kNumBars = 2 * (kQStages + kKStages + kVStages) + 17;
+  static constexpr int kDelta = kWords + kXMaskSlots * 16;  // fp32 [kDeltas][2 or, with SPLIT, 4][128]
+  static constexpr int kBar = kDelta + (SPLIT ? 2048 : kDeltas * 1024);
+  static constexpr int kNumBars = 2 * (kQStages + kKStages + kVStages) + 18;
   static constexpr int kTail = kBar + kNumBars * 8;
   static constexpr int kSmemBytes = kTail + 16 + 1024;
 };
@@ -184,8 +185,8 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
   uint64_t* acc_full = ds_full + 2;  // [2], by sum
   uint64_t* acc_free = acc_full + 2;
   uint64_t* staged = acc_free + 2;
-  uint64_t* delta_full = staged + 2;
-  uint64_t* drained = delta_full + 1;  // [2], by issuing warp
+  uint64_t* delta_full = staged + 2;   // [2], by buffer of delta
+  uint64_t* drained = delta_full + 2;  // [2], by issuing warp
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::kTail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -211,10 +212,10 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       mbar_init(acc_full + i, 1);
       mbar_init(acc_free + i, kXBwdWarps);
       mbar_init(staged + i, kXBwdWarps);
+      mbar_init(delta_full + i, SPLIT ? kXBwdWarps : 8);
     }
     mbar_init(dp_full, 2);  // the products' commit, and the issuing warp (rows of K zeroed)
     mbar_init(dp_free, kXBwdWarps);
-    mbar_init(delta_full, SPLIT ? kXBwdWarps : 8);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -489,7 +490,11 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       const bool dead = lse == -INFINITY;  // no such row, or no kept key
       const float neg_lse = dead ? -INFINITY : -lse * 1.4426950408889634f;
       float neg_delta = 0.0f;
-      float* parts = delta_part + (SPLIT ? 0 : n_item % Ly::kAccs * (2 * kXTile));
+      float* parts = delta_part + n_item % Ly::kDeltas * (2 * kXTile);
+      // (Half of the warps arrive and all wait.  An item of one key tile may let those that arrive go on to the next item's
+      // delta before the others have seen this one's; the one after that they reach only behind dP of the next item, which
+      // waits for all to have read dP of this one: two copies.)
+      uint64_t* const delta_here = delta_full + n_item % Ly::kDeltas;
       if (!SPLIT && wq < 2) {  // delta = do . o, half of the channels each
         ok = wait(q_full + qs, n_item / Ly::kQStages, kWaitQ);
         if (!ok) break;
@@ -507,11 +512,11 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
           part -= x_dot8<T>(v, ld_shared_v4(stage + Ly::kTileBytes + (c >> 3) * 16384 + swizzle128_offset(row, c & 7)));
         }
         parts[wq * kXTile + row] = part;
-        warp_arrive(delta_full);
+        warp_arrive(delta_here);
       }
       // this row's delta, from its parts, and the statistics that the second launch needs
       const auto join_delta = [&]() {
-        if (!wait(delta_full, n_item, kWaitDelta)) return false;
+        if (!wait(delta_here, n_item / Ly::kDeltas, kWaitDelta)) return false;
         neg_delta = parts[row] + parts[kXTile + row];
         if (SPLIT) neg_delta += parts[2 * kXTile + row] + parts[3 * kXTile + row];
         if (dead) neg_delta = 0.0f;
@@ -575,7 +580,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
             unpair2(sum, s0, s1);
           }
           parts[wq * kXTile + row] = -(s0 + s1);
-          warp_arrive(delta_full);
+          warp_arrive(delta_here);
           ok = join_delta();
           if (!ok) break;
         }
