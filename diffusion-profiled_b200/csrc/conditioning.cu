@@ -152,7 +152,8 @@ int bind_context() {
 struct XPlan {
   int row_tiles, hv, n_tiles, splits, key_chunk;
   int64_t rows, items, slots;
-  bool join_inside;  // x_join
+  bool two_values;   // P in two values of the type: x_fwd_kernel's SPLIT
+  bool join_inside;  // x_join (with two_values only)
 };
 XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
   XPlan w{};
@@ -178,6 +179,7 @@ XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
     w.splits = (w.n_tiles + w.key_chunk - 1) / w.key_chunk;
   }
   w.items = base * w.splits;
+  w.two_values = w.n_tiles == 1 || few_rows;
   w.join_inside = few_rows && w.splits > 1 && w.items <= w.slots;
   return w;
 }
@@ -193,9 +195,9 @@ size_t x_fwd_workspace(const fp8_cross_attention_args* a, const XPlan& w) {
 }
 
 template <typename T, int HALVES>
-int x_fwd_launch(const XFwdParams& f, const CUtensorMap (&maps)[4], bool one_key_tile, int64_t slots, cudaStream_t stream) {
+int x_fwd_launch(const XFwdParams& f, const CUtensorMap (&maps)[4], bool two_values, int64_t slots, cudaStream_t stream) {
   using Ly = XFwdLayout<HALVES>;
-  const auto kernel = one_key_tile ? x_fwd_kernel<T, HALVES, true> : x_fwd_kernel<T, HALVES, false>;
+  const auto kernel = two_values ? x_fwd_kernel<T, HALVES, true> : x_fwd_kernel<T, HALVES, false>;
   FP8_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ly::kSmemBytes));
   FP8_CUDA_TRY(launch_kernel(kernel, dim3(static_cast<unsigned>(std::min<int64_t>(f.items, slots))), dim3(Ly::kThreads),
                              Ly::kSmemBytes, stream, 1, kTensorKernel, f, maps[0], maps[1], maps[2], maps[3]));
@@ -227,9 +229,8 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
   if (int s = x_map(&maps[1], a.k, dt, a.sk, a.batch, a.k_len, a.kv_heads, a.head_dim, 1, kXTile)) return s;
   if (int s = x_map(&maps[2], a.v, dt, a.sv, a.batch, a.k_len, a.kv_heads, a.head_dim, 1, kXTile)) return s;
   if (int s = x_map(&maps[3], a.o, dt, a.so, a.batch, a.q_len, a.heads, a.head_dim, a.pack, a.tile_tokens)) return s;
-  const bool one = w.n_tiles == 1;
-  const int status = a.head_dim <= 64 ? x_fwd_launch<T, 1>(f, maps, one, w.slots, stream)
-                                      : x_fwd_launch<T, 2>(f, maps, one, w.slots, stream);
+  const int status = a.head_dim <= 64 ? x_fwd_launch<T, 1>(f, maps, w.two_values, w.slots, stream)
+                                      : x_fwd_launch<T, 2>(f, maps, w.two_values, w.slots, stream);
   if (status) return status;
   if (w.splits > 1 && !w.join_inside) {
     FP8_CUDA_TRY(launch_kernel(x_combine_kernel<T>, dim3(grid_for(w.rows, 8, st->sm_count, 8)), dim3(256), 0, stream, 1,
