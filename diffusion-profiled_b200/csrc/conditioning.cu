@@ -244,7 +244,8 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
 struct XBwdPlan {
   int row_tiles, q_tiles, q_chunk, splits;
   int64_t dq_items, dkv_items;
-  size_t stats_bytes, part_bytes;
+  size_t stats_bytes, part_bytes, row_norm_bytes, max_norm_bytes;  // the workspace, in this order; the norms for fp16
+  size_t bytes() const { return stats_bytes + part_bytes + row_norm_bytes + max_norm_bytes; }
 };
 XBwdPlan x_bwd_plan(const fp8_cross_attention_args* a, int sm_count) {
   const XPlan f = x_plan(a, sm_count);
@@ -261,6 +262,9 @@ XBwdPlan x_bwd_plan(const fp8_cross_attention_args* a, int sm_count) {
   w.dkv_items = base * w.splits;
   w.stats_bytes = static_cast<size_t>(w.dq_items) * 2 * kXTile * sizeof(float);
   w.part_bytes = w.splits == 1 ? 0 : sizeof(float) * 2 * w.splits * a->batch * a->k_len * static_cast<size_t>(a->kv_heads) * a->head_dim;
+  const bool norms = a->dtype == FP8_DTYPE_FP16;
+  w.row_norm_bytes = norms ? sizeof(float) * f.rows : 0;
+  w.max_norm_bytes = norms ? sizeof(unsigned int) * 2 * a->batch * a->kv_heads : 0;
   return w;
 }
 
@@ -290,6 +294,8 @@ int x_bwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XBwd
   p.hv = a.heads / a.pack;
   p.stats = static_cast<float*>(workspace);
   p.items = static_cast<uint32_t>(w.dq_items);
+  p.row_norm2 = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.stats_bytes + w.part_bytes);
+  p.max_norm2 = reinterpret_cast<unsigned int*>(reinterpret_cast<char*>(p.row_norm2) + w.row_norm_bytes);
   XBwdParams kv = p;
   kv.items = static_cast<uint32_t>(w.dkv_items);
   kv.q_tiles = w.q_tiles;
@@ -312,6 +318,13 @@ int x_bwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XBwd
   if (int s = q_side(&m[4], a.dq, a.sdq)) return s;
   if (int s = k_side(&m[5], a.dk, a.sdk)) return s;
   if (int s = k_side(&m[6], a.dv, a.sdv)) return s;
+  if constexpr (kXScaled<T>) {
+    FP8_CUDA_TRY(cudaMemsetAsync(p.max_norm2, 0, w.max_norm_bytes, stream));
+    const int64_t chunks = (static_cast<int64_t>(a.q_len) * a.group + a.k_len + kXNormRows - 1) / kXNormRows * a.batch * a.kv_heads;
+    FP8_CUDA_TRY(launch_kernel(x_norms_kernel<T>, dim3(grid_for(chunks, 1, st->sm_count, 8)), dim3(256), 0, stream, 1,
+                               kStreamingKernel, p));
+    count_launches(1);
+  }
   const bool one = a.k_len <= kXTile;  // the states are one key tile
   const int status = a.head_dim <= 64 ? (one ? x_bwd_launch<T, 1, true>(p, kv, m, st, stream)
                                              : x_bwd_launch<T, 1, false>(p, kv, m, st, stream))
@@ -339,7 +352,7 @@ size_t fp8_cross_attention_workspace_bytes(const fp8_cross_attention_args* a, in
   if (device_state(&st)) return 0;
   if (backward) {
     const XBwdPlan w = x_bwd_plan(a, st->sm_count);
-    return w.stats_bytes + w.part_bytes;
+    return w.bytes();
   }
   return x_fwd_workspace(a, x_plan(a, st->sm_count));
 }
@@ -368,7 +381,7 @@ int fp8_cross_attention_bwd(const fp8_cross_attention_args* a, void* workspace, 
   const XBwdPlan w = x_bwd_plan(a, st->sm_count);
   FP8_REQUIRE(w.dq_items < (1ll << 31) && w.dkv_items < (1ll << 31), FP8_ERR_UNSUPPORTED,
               "cross attention backward: too many tiles (%lld, %lld)", (long long)w.dq_items, (long long)w.dkv_items);
-  const size_t need = w.stats_bytes + w.part_bytes;
+  const size_t need = w.bytes();
   FP8_REQUIRE(workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= need, FP8_ERR_WORKSPACE,
               "cross attention backward: workspace too small or not 16-byte aligned (%zu bytes, needs %zu)",
               workspace_bytes, need);

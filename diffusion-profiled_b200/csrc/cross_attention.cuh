@@ -25,8 +25,8 @@
 //     more than returns;
 //   * the exponent's reference is the row's maximum so far, raised only when a score
 //     passes it by more than 2^8: then O and the sum are rescaled.  Scores that stay
-//     within that factor need no rescaling pass, and P <= 2^8 keeps its relative
-//     precision in bf16 and fp16;
+//     within that factor need no rescaling pass.  P <= 2^8 keeps its relative precision
+//     in bf16; in fp16 what is below 2^-14 is a multiple of 2^-24, beside a sum of 1 or more;
 //   * keys that are not kept: their scores are replaced by -inf, and their rows of V are
 //     zeroed in shared memory before the product.
 // What bounds it: with many queries the softmax (an exponential a score, 16 a clock and
@@ -49,6 +49,8 @@
 #pragma once
 
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "dropout.cuh"
 #include "sm100_common.cuh"

@@ -33,6 +33,15 @@
 // is.  Otherwise P and dS are rounded to the type once (they are matrix operands); scores,
 // dP, statistics and all sums are fp32.
 //
+// fp16 has too few exponents for P and dS as they are: over 4096 keys a weight is near 2^-12,
+// and times a gradient of 2^-10 it would be a few multiples of 2^-24, the smallest step.  So
+// both go into their products times powers of two, which are taken out of the sums again.
+// P <= 1 is taken times 2^14.  |dS_ij| <= p_ij |do_i| (|v_j| + |o_i|) <= 2 |do_i| max|v|, and
+// dS is taken times the power of two that brings this bound to between 2^13 and 2^14: each
+// row's own in dQ, and for dK, where rows are added up, the one of the key head's largest
+// |do|.  x_norms_kernel finds these norms (fp16 alone; with it 5 x 333 queries of 8 heads of
+// 80 over 1021 keys take 91 us a training call, 83 without).
+//
 // A barrier that warps arrive on has one copy for each buffer, and the buffer is reused only
 // after its phase: with one for all, a warp that is a step ahead completes a phase that
 // another has not reached.
@@ -57,7 +66,22 @@ struct XBwdParams {
   int q_chunk;    // row tiles of a split; splits == 1: all of them
   int splits;
   float* part;    // [splits][2][batch][k_len][kv_heads][head_dim] (dv, dk * scale), with splits > 1
+  // fp16 (x_norms_kernel): |dout|^2 of each row [batch][heads][q_len], and of each key head [batch][kv_heads][2] the largest,
+  // and the largest |v|^2 of its kept keys, as the bits of a float
+  float* row_norm2;
+  unsigned int* max_norm2;
 };
+
+// fp16's powers of two (see above): P's, and the one for dS from the squares of the norms.
+template <typename T>
+constexpr bool kXScaled = std::is_same_v<T, __half>;
+constexpr int kXWeightExp = 14;
+__device__ __forceinline__ int x_ds_exp(float do2, float v2) {
+  const float bound = 2.0f * sqrtf(do2) * sqrtf(v2);
+  if (!(bound > 0.0f) || bound > 3.0e38f) return 0;  // no gradient, or no finite one
+  return max(-60, min(60, kXWeightExp - (static_cast<int>(__float_as_uint(bound) >> 23) - 126)));
+}
+__device__ __forceinline__ float x_exp2i(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 // Sum of the products of eight 16-bit values.
 template <typename T>
@@ -101,6 +125,47 @@ __device__ __forceinline__ void x_products_mn(uint32_t d, uint32_t operand, uint
       umma_f16_ts(d, w, b + k * 128, idesc, k > 0 ? 1u : accumulate);
       if (SPLIT) umma_f16_ts(d, w + 16, b + k * 128, idesc, 1u);
     }
+}
+
+// ============================================================================ norms (fp16)
+// A CTA takes kXNormRows rows of dO, and of V, of a (sequence, key head); 16 lanes a row, eight channels each.
+constexpr int kXNormRows = 128;
+template <typename T>
+__global__ void __launch_bounds__(256) x_norms_kernel(const XBwdParams p) {
+  __shared__ unsigned int most[2];
+  pdl_sync();
+  const XAttnParams& a = p.a;
+  const int lane = threadIdx.x & 15, first = threadIdx.x >> 4;
+  const int64_t q_rows = static_cast<int64_t>(a.q_len) * a.group, rows = q_rows + a.k_len;
+  const int64_t chunks = (rows + kXNormRows - 1) / kXNormRows, items = chunks * a.batch * a.kv_heads;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t head = item / chunks;  // of all sequences' key heads
+    const int b = static_cast<int>(head / a.kv_heads), hk = static_cast<int>(head % a.kv_heads);
+    const int count = x_key_count(a, x_raw_count(a, b));
+    if (threadIdx.x < 2) most[threadIdx.x] = 0;
+    __syncthreads();
+    for (int64_t r = item % chunks * kXNormRows + first; r < min(rows, (item % chunks + 1) * kXNormRows); r += 16) {
+      const bool is_q = r < q_rows;
+      const int token = static_cast<int>(is_q ? r / a.group : r - q_rows), h = hk * a.group + static_cast<int>(r % a.group);
+      const T* row = is_q ? static_cast<const T*>(a.dout) + b * a.sdo.batch + token * a.sdo.token + h * a.sdo.head
+                          : static_cast<const T*>(a.v) + b * a.sv.batch + token * a.sv.token + hk * a.sv.head;
+      const bool used = is_q || (token < count && x_key_kept(a, b, token));
+      float sum = 0.0f;
+      if (used && lane * 8 < a.head_dim) {
+        const uint4 w = *reinterpret_cast<const uint4*>(row + lane * 8);
+        sum = x_dot8<T>(w, w);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffu << (threadIdx.x & 16), sum, o);
+      if (lane == 0) {
+        if (is_q) p.row_norm2[(static_cast<int64_t>(b) * a.heads + h) * a.q_len + token] = sum;
+        atomicMax(most + (is_q ? 0 : 1), __float_as_uint(sum));  // (not negative: as bits in the same order, NaN above all)
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) atomicMax(p.max_norm2 + 2 * head + threadIdx.x, most[threadIdx.x]);
+    __syncthreads();
+  }
 }
 
 // ============================================================================ dQ
@@ -391,6 +456,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
     // item begins: the registers for it are not there, and items are longer.)
     uint4 o_row[4];
     float lse = -INFINITY;
+    float do2 = 0.0f, v2 = 0.0f;  // fp16: the squares of this row's |dO| and of its keys' largest |V|
     const auto fetch = [&](const XDqItems& items) {
       XDqItem t;
       const bool exists = items.ahead(t);
@@ -404,7 +470,12 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
           o_row[u] = live && c < a.head_dim ? *reinterpret_cast<const uint4*>(o + c) : make_uint4(0, 0, 0, 0);
         }
       }
-      lse = live ? a.lse[(static_cast<int64_t>(t.b) * a.heads + head) * a.q_len + token] : -INFINITY;
+      const int64_t r_index = (static_cast<int64_t>(t.b) * a.heads + head) * a.q_len + token;
+      lse = live ? a.lse[r_index] : -INFINITY;
+      if constexpr (kXScaled<T>) {
+        do2 = live ? p.row_norm2[r_index] : 0.0f;
+        v2 = live ? __uint_as_float(p.max_norm2[2 * (static_cast<int64_t>(t.b) * a.kv_heads + head / a.group) + 1]) : 0.0f;
+      }
     };
     uint32_t n_item = 0, g = 0;
     int stored = -1;  // Q stage whose gradient is on its way out
@@ -421,10 +492,12 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       uint32_t n;
       int b, hv, tile;
       bool dead;
+      float scale;  // fp16: of the sum
     };
     const auto hand_out = [&](const Done& w) {
       const uint32_t acc = w.n % Ly::kAccs, phase = w.n / Ly::kAccs;
       const int qs = w.n % Ly::kQStages;
+      const float f = kXScaled<T> ? w.scale : a.scale;
       uint8_t* stage = smem + 2 * qs * Ly::kTileBytes;
       release_stored();
       if (!wait(acc_full + acc, phase, kWaitAcc)) return false;
@@ -437,7 +510,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         uint32_t pk[8];
 #pragma unroll
         for (int k = 0; k < 16; k += 2)
-          pk[k >> 1] = w.dead ? 0u : XType<T>::pack2(__uint_as_float(o[k]) * a.scale, __uint_as_float(o[k + 1]) * a.scale);
+          pk[k >> 1] = w.dead ? 0u : XType<T>::pack2(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f);
         uint8_t* half = stage + (col >> 6) * 16384;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -489,6 +562,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       uint8_t* stage = smem + 2 * qs * Ly::kTileBytes;
       const bool dead = lse == -INFINITY;  // no such row, or no kept key
       const float neg_lse = dead ? -INFINITY : -lse * 1.4426950408889634f;
+      const int ds_exp = kXScaled<T> ? x_ds_exp(do2, v2) : 0;
       float neg_delta = 0.0f;
       float* parts = delta_part + n_item % Ly::kDeltas * (2 * kXTile);
       // (Half of the warps arrive and all wait.  An item of one key tile may let those that arrive go on to the next item's
@@ -519,6 +593,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         if (!wait(delta_here, n_item / Ly::kDeltas, kWaitDelta)) return false;
         neg_delta = parts[row] + parts[kXTile + row];
         if (SPLIT) neg_delta += parts[2 * kXTile + row] + parts[3 * kXTile + row];
+        if (SPLIT && kXScaled<T>) neg_delta *= x_exp2i(-ds_exp);  // (summed with the weights that dS is made from)
         if (dead) neg_delta = 0.0f;
         if (wq == 0) {
           stat[0] = neg_lse;
@@ -530,7 +605,8 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         ok = join_delta();
         if (!ok) break;
       }
-      const uint64_t nl2 = pair2(neg_lse, neg_lse);
+      const float nl = kXScaled<T> ? neg_lse + static_cast<float>(ds_exp) : neg_lse;
+      const uint64_t nl2 = pair2(nl, nl);
       for (int j = 0; j < t.tiles; ++j, ++g) {
         const uint32_t t_s = t_lane + kXDqS + (g & 1) * 128 + wq * 32;
         const bool some = wq < x_chunks(t.keys, j);  // the chunk holds keys
@@ -625,7 +701,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       }
       if (!ok) break;
       fetch(items);
-      const Done now{n_item, t.b, t.hv, t.tile, dead};
+      const Done now{n_item, t.b, t.hv, t.tile, dead, kXScaled<T> ? a.scale * x_exp2i(-ds_exp) : 0.0f};
       if (Ly::kAccs == 1 || any_done) ok = hand_out(Ly::kAccs == 1 ? now : done);
       done = now;
       any_done = true;
@@ -952,6 +1028,13 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
         }
         continue;
       }
+      int ds_exp = 0;
+      if constexpr (kXScaled<T>) {
+        const unsigned int* norm2 = p.max_norm2 + 2 * (static_cast<int64_t>(t.b) * a.kv_heads + t.hk);
+        ds_exp = x_ds_exp(__uint_as_float(norm2[0]), __uint_as_float(norm2[1]));
+      }
+      // from P times its power of two to dS times its own
+      const float f_ds = x_exp2i(ds_exp - kXWeightExp);
       for (int j = t.j0; j < t.j1 && ok; ++j, ++g) {
         const int steps = x_row_steps(a, j % p.row_tiles);
         for (int u = 0; u < steps; ++u, ++n) {
@@ -968,7 +1051,9 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
             tmem_read(t_s, s);
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
-              const float4 nl = neg_lse[k >> 2];
+              float4 nl = neg_lse[k >> 2];
+              if constexpr (kXScaled<T>)
+                nl = make_float4(nl.x + kXWeightExp, nl.y + kXWeightExp, nl.z + kXWeightExp, nl.w + kXWeightExp);
               float x0, x1, x2, x3;
               unpair2(fma2(pair2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c22, pair2(nl.x, nl.y)), x0, x1);
               unpair2(fma2(pair2(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])), c22, pair2(nl.z, nl.w)), x2, x3);
@@ -995,6 +1080,10 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
                            add2(pair2(__uint_as_float(dp[k + 2]), __uint_as_float(dp[k + 3])), pair2(nd.z, nd.w))),
                       pr[k + 2], pr[k + 3]);
             }
+            if constexpr (kXScaled<T>) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) pr[k] *= f_ds;
+            }
             x_store_operand<T, SPLIT>(t_dp, pr);
           }
           tmem_st_wait();
@@ -1014,7 +1103,7 @@ __global__ void __launch_bounds__(kXBwdThreads, 1)
       const bool single = SPLIT && __popc(w.x) + __popc(w.y) + __popc(w.z) + __popc(w.w) == 1;
       // dV goes out from V's tile, dK from K's
       uint8_t* stage = smem + (2 * ks + 1 - gp) * Ly::kTileBytes;
-      const float f = gp ? a.scale : 1.0f;
+      const float f = !kXScaled<T> ? (gp ? a.scale : 1.0f) : gp ? a.scale * x_exp2i(-ds_exp) : x_exp2i(-kXWeightExp);
       const bool zero = !kept || (gp && single);
 #pragma unroll
       for (int c = 0; c < HALVES; ++c) {
