@@ -70,6 +70,11 @@ void not_twice(const char* what) {
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// Nor have the operators a forward-mode derivative: a tangent would be lost, that is, taken for zero.
+void no_tangent(const char* what, const Tensor& t) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, ": there is no forward-mode derivative");
+}
+
 // ------------------------------------------------------------------ cross attention
 constexpr const char* kX = "cross attention";
 
@@ -272,6 +277,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
 
 Tensor cross_attention_autograd(const Tensor& q, const Tensor& k, const OptTensor& v, const OptTensor& key_lengths,
                                 const OptTensor& key_mask, std::optional<double> scale) {
+  for (const Tensor* t : {&q, &k, &or_undefined(v)}) no_tangent(kX, *t);
   if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(or_undefined(v))))
     return CrossAttention::apply(q, k, v, key_lengths, key_mask, scale_of(q, scale));
   static const auto op = typed_op<decltype(cross_attention_no_grad)>("fp8_b200::cross_attention");
@@ -367,6 +373,7 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
 // padding_idx: -1 for none (the caller has resolved one that counts from the end).
 Tensor embed_tokens_autograd(const Tensor& ids, const Tensor& weight, double scale, int64_t padding_idx,
                              at::ScalarType dtype) {
+  no_tangent(kE, weight);
   if (at::GradMode::is_enabled() && weight.requires_grad())
     return TokenEmbedding::apply(ids, weight, scale, padding_idx, dtype);
   static const auto op = typed_op<decltype(embedding_fwd)>("fp8_b200::embedding_fwd");
@@ -424,6 +431,8 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 
 Tensor dropout_autograd(const Tensor& x, const OptTensor& residual, double p, const Tensor& seed) {
+  no_tangent(kD, x);
+  no_tangent(kD, or_undefined(residual));
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(or_undefined(residual))))
     return Dropout::apply(x, residual, p, seed);
   static const auto op = typed_op<decltype(dropout_apply)>("fp8_b200::dropout_add");

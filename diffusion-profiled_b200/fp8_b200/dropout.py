@@ -5,7 +5,10 @@ row-major order) is kept by a rule on ``(seed, e)`` alone, the one the fused
 group norm's dropout draws from (include/fp8ops.h, ``fp8_dropout``), so the
 backward makes the mask again.  ``seed`` is an int64 device scalar, read when the
 kernel runs: a captured CUDA graph draws a new mask on each replay if the caller
-advances it.  The operator and its gradient are registered by csrc/torch_ops.cpp.
+advances it.  The operator and its gradient are registered by csrc/torch_ops.cpp;
+there is no second and no forward-mode derivative (both are refused).  Under
+``torch.vmap`` every slice is a call of its own, whose elements are counted from 0:
+with one seed all slices get one mask.
 """
 
 from __future__ import annotations
