@@ -305,19 +305,40 @@ class GraphedTrainStep:
     def step(self, images: torch.Tensor | None = None, t: torch.Tensor | None = None,
              eps: torch.Tensor | None = None, prompt_ids: torch.Tensor | None = None,
              prompt_lengths: torch.Tensor | None = None) -> None:
+        """``images``, ``t``, ``eps``: copied in where they are given; without them the last step's are used again.  A
+        UNet built with ``prompt_vocab`` takes ``prompt_ids`` (``[batch, prompt_tokens]``) with its images, and how many
+        of each prompt's tokens there are (``prompt_lengths [batch]``; all of them if None)."""
+        self._check_prompt(images, prompt_ids, prompt_lengths)
         if images is not None:
             self.static_batch.copy_(images, non_blocking=True)
         if t is not None:
             self.static_t.copy_(t, non_blocking=True)
         if eps is not None:
             self.static_eps.copy_(eps, non_blocking=True)
-        for static, given in zip(self.static_prompt, (prompt_ids, prompt_lengths)):
-            if given is not None:
-                static.copy_(given, non_blocking=True)
+        if prompt_ids is not None:
+            ids, lengths = self.static_prompt
+            ids.copy_(prompt_ids, non_blocking=True)
+            if prompt_lengths is None:
+                lengths.fill_(ids.shape[1])
+            else:
+                lengths.copy_(prompt_lengths, non_blocking=True)
         if self.graph is not None:
             self.graph.replay()
         else:
             self._body()
+
+    def _check_prompt(self, images, ids, lengths) -> None:
+        if not self.static_prompt:
+            if ids is not None or lengths is not None:
+                raise RuntimeError("train step: a prompt was given to a UNet that was built without prompt_vocab")
+            return
+        if ids is None:
+            if images is not None or lengths is not None:
+                raise RuntimeError("train step: images of a UNet with prompt_vocab need their prompt_ids")
+            return
+        for name, given, static in zip(("prompt_ids", "prompt_lengths"), (ids, lengths), self.static_prompt):
+            if given is not None and given.shape != static.shape:
+                raise RuntimeError(f"train step: {name} must be {list(static.shape)}, got {list(given.shape)}")
 
     def release(self) -> None:
         """Drop the graph (before tearing the process group down) and the hooks."""
