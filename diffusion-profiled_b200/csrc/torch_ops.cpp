@@ -22,6 +22,11 @@
 
 #include "fp8ops.h"
 
+#ifndef FP8_TORCH_MARK
+#error "FP8_TORCH_MARK: the torch this is built for (fp8_b200/build.py)"
+#endif
+extern "C" __attribute__((used, visibility("default"))) const char fp8_torch_mark[] = FP8_TORCH_MARK;
+
 namespace {
 
 using at::Tensor;

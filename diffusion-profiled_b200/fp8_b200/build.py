@@ -22,6 +22,7 @@ LIB_NAME = "libfp8ops.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 TORCH_LIB_PATH = PKG_DIR / "libfp8torch.so"
 TORCH_SRC = SRC_DIR / "torch_ops.cpp"
+TORCH_MARK = "fp8_b200 operators for torch "
 OBJ_DIR = PKG_DIR / "_build"
 
 NVCC_FLAGS = [
@@ -54,8 +55,17 @@ def headers() -> list[Path]:
     return sorted(SRC_DIR.glob("*.cuh")) + sorted(SRC_DIR.glob("*.h")) + [INCLUDE_DIR / "fp8ops.h"]
 
 
+def torch_library_fits(torch_version: str, path: Path | None = None) -> bool:
+    """Whether the library of torch operators is there and was built for this torch (it says so in a string of its own,
+    TORCH_MARK and the version; torch's C++ interface changes from version to version)."""
+    path = TORCH_LIB_PATH if path is None else path
+    return path.exists() and (TORCH_MARK + torch_version).encode() + b"\0" in path.read_bytes()
+
+
 def needs_rebuild() -> bool:
-    if not LIB_PATH.exists() or not TORCH_LIB_PATH.exists():
+    import torch
+
+    if not LIB_PATH.exists() or not torch_library_fits(torch.__version__):
         return True
     mtime = min(LIB_PATH.stat().st_mtime, TORCH_LIB_PATH.stat().st_mtime)
     return any(p.stat().st_mtime > mtime for p in sources())
@@ -75,7 +85,7 @@ def _compile_torch_ops(obj: Path, verbose: bool) -> None:
 
     cuda_include = Path(_nvcc()).resolve().parent.parent / "include"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-c", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f"-I{INCLUDE_DIR}", *(f"-isystem{p}" for p in (*include_paths(), cuda_include)), "-o", str(obj), str(TORCH_SRC)]
+           f'-DFP8_TORCH_MARK="{TORCH_MARK}{torch.__version__}"', f"-I{INCLUDE_DIR}", *(f"-isystem{p}" for p in (*include_paths(), cuda_include)), "-o", str(obj), str(TORCH_SRC)]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
@@ -95,6 +105,8 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     """Compile every csrc/*.cu (side by side) and link libfp8ops.so for sm_100a; returns its path.
 
     An object file in ``_build/`` is kept while it is newer than its source and every header."""
+    import torch
+
     if not force and not needs_rebuild():
         return LIB_PATH
     OBJ_DIR.mkdir(exist_ok=True)
@@ -106,9 +118,11 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
             jobs.append((src, obj))
     torch_obj = OBJ_DIR / (TORCH_SRC.stem + ".o")
     torch_newest = max(TORCH_SRC.stat().st_mtime, (INCLUDE_DIR / "fp8ops.h").stat().st_mtime)
+    keep_torch_obj = not force and torch_obj.exists() and torch_obj.stat().st_mtime > torch_newest \
+        and torch_library_fits(torch.__version__, torch_obj)
     with ThreadPoolExecutor() as pool:
         running = [pool.submit(_compile, src, obj, verbose) for src, obj in jobs]
-        if force or not torch_obj.exists() or torch_obj.stat().st_mtime <= torch_newest:
+        if not keep_torch_obj:
             running.append(pool.submit(_compile_torch_ops, torch_obj, verbose))
         for done in running:
             done.result()

@@ -18,7 +18,9 @@ from __future__ import annotations
 
 import torch
 
-from . import ops  # noqa: F401  (loads libfp8torch.so)
+from . import torch_ops
+
+torch_ops.load(required=True)
 
 MAX_HEAD_DIM = 128
 

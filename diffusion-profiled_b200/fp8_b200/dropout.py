@@ -15,7 +15,9 @@ from __future__ import annotations
 
 import torch
 
-from . import ops  # noqa: F401  (loads libfp8torch.so)
+from . import torch_ops
+
+torch_ops.load(required=True)
 
 
 def dropout_add(x: torch.Tensor, residual: torch.Tensor | None, p: float, seed: torch.Tensor) -> torch.Tensor:

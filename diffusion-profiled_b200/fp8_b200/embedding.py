@@ -10,7 +10,9 @@ from __future__ import annotations
 
 import torch
 
-from . import ops  # noqa: F401  (loads libfp8torch.so)
+from . import torch_ops
+
+torch_ops.load(required=True)
 
 
 def embed_tokens(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None,

@@ -5,8 +5,8 @@ launches the native kernels on torch's current stream and never synchronises,
 so the ops can be captured in CUDA graphs.  They are registered with
 ``torch.library.custom_op`` plus fake (meta) implementations so that
 ``torch.compile`` treats them as opaque nodes; the text-conditioning operators
-(cross attention, token embedding, dropout) are registered by ``libfp8torch.so``,
-which this module loads.
+(cross attention, token embedding, dropout) are registered by ``libfp8torch.so``
+(:mod:`fp8_b200.torch_ops`).
 
 Layouts: 4-D activations and conv weights are channels_last (physically NHWC /
 [Cout][3][3][Cin]); FP8 tensors are ``torch.float8_e4m3fn``; scales are fp32
@@ -21,13 +21,9 @@ from ctypes import c_int64, c_void_p
 import torch
 
 from . import _lib
-from .build import TORCH_LIB_PATH
+from . import torch_ops
 
-if not TORCH_LIB_PATH.exists():
-    raise RuntimeError(f"{TORCH_LIB_PATH} is missing: build it with fp8_b200.build.build_library() "
-                       "(or __graft_entry__.build()); there is no fallback implementation")
-_lib.load()  # libfp8ops.so, which the torch operators call
-torch.ops.load_library(str(TORCH_LIB_PATH))
+torch_ops.load(required=False)
 
 FP8_DTYPE = torch.float8_e4m3fn
 

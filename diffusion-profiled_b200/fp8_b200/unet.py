@@ -29,7 +29,6 @@ import torch.nn.functional as F
 
 from . import _lib, ops
 from .attention import attention_supported, fp8_attention
-from .conditioning import PromptAttention, PromptEncoder
 from .delayed import ConvFP8Delayed, GroupNormActConvFP8Delayed, quantize_conv_weights
 from .fp8_kernels import SUPPORTED_UNET_SHAPES, triton_conv2d_fp8
 from .resample import downsample_nearest, residual_join, upsample_cat, upsample_cat_pair
@@ -336,6 +335,8 @@ class Stage(nn.Module):
         )
         self.prompt_attns = None
         if attention and config.prompt_vocab > 0:
+            from .conditioning import PromptAttention  # (needs libfp8torch.so, as nothing else here does)
+
             self.prompt_attns = nn.ModuleList(
                 PromptAttention(widths[i + 1], config.prompt_width, config.n_heads, config.p_drop) for i in range(num_blocks)
             )
@@ -379,6 +380,8 @@ class UNet(nn.Module):
         )
         self.prompt = None
         if config.prompt_vocab > 0:
+            from .conditioning import PromptEncoder
+
             self.prompt = PromptEncoder(config.prompt_vocab, config.prompt_width, config.prompt_tokens,
                                         config.prompt_padding_idx, config.p_drop)
         self.time_embed = nn.Sequential(
