@@ -54,6 +54,14 @@ __device__ __forceinline__ Words8<T> load_words8(const T* p) {
   for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) v.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
   return v;
 }
+// The same of memory that the kernel may write too (not by the read-only path).
+template <typename T>
+__device__ __forceinline__ Words8<T> load_own_words8(const T* p) {
+  Words8<T> v;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) v.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  return v;
+}
 template <typename T>
 __device__ __forceinline__ void widen8(const Words8<T>& v, float (&f)[8]) {
   const T* t = reinterpret_cast<const T*>(&v);
@@ -72,7 +80,7 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
 
 constexpr int kDropoutThreads = 256;
 
-// VEC: the pointers are 16-byte aligned.
+// VEC: the pointers are 16-byte aligned.  y may be x or the residual: each value is read by the thread that writes it.
 template <typename T, bool VEC, bool RESIDUAL>
 __global__ void __launch_bounds__(kDropoutThreads) dropout_kernel(const DropoutParams p) {
   pdl_sync();
@@ -90,8 +98,8 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_kernel(const DropoutP
     for (int u = 0; u < kAtOnce; ++u) {
       const int64_t g = g0 + u * threads;
       if (g >= whole) continue;
-      xv[u] = load_words8(x + g * 8);
-      if (RESIDUAL) rv[u] = load_words8(res + g * 8);
+      xv[u] = load_own_words8(x + g * 8);
+      if (RESIDUAL) rv[u] = load_own_words8(res + g * 8);
     }
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {

@@ -600,7 +600,7 @@ int fp8_selftest_sort_timeout(uint64_t limit_ns);
  * the (e mod 4)-th 16 bits of splitmix64(*seed ^ (e / 4) * 0xD1B54A32D192ED03) are
  * at least p * 65536 rounded to an integer (the group norm's dropout draws from the
  * same generator).  The gradient of x is the same call on dy without a residual.
- * seed: device int64; 0 <= p <= 1.  y may be x. */
+ * seed: device int64; 0 <= p <= 1.  y may be x, or the residual. */
 int fp8_dropout(const void* x, const void* residual, void* y, int dtype, int64_t n, double p, const int64_t* seed,
                 fp8_stream_t stream);
 

@@ -147,6 +147,29 @@ def test_a_replayed_gradient_beside_many_calls(cuda):
     assert _lib.device_error() == 0
 
 
+@pytest.mark.parametrize("dtype,code", [(BF16, 0), (torch.float32, 1), (torch.float16, 2)])
+@pytest.mark.parametrize("n,offset", [(1 << 20, 0), (3_000_001, 0), (70_001, 1)])
+def test_dropout_in_place(cuda, n, offset, dtype, code):
+    """Over its input, and over its residual: the values of the call that writes elsewhere."""
+    from fp8_b200 import _lib
+    from fp8_b200.dropout import dropout, dropout_add
+
+    g = torch.Generator(device=cuda).manual_seed(n)
+    x, r = (torch.randn(n + offset, device=cuda, generator=g).to(dtype)[offset:] for _ in range(2))
+    seed = torch.tensor(5, device=cuda)
+    stream = torch.cuda.current_stream(cuda).cuda_stream
+    run = lambda x, r, y: _lib.load().fp8_dropout(x.data_ptr(), None if r is None else r.data_ptr(), y.data_ptr(),  # noqa: E731
+                                                  code, n, 0.3, seed.data_ptr(), stream)
+    alone, joined = dropout(x, 0.3, seed), dropout_add(x, r, 0.3, seed)
+    storage = torch.empty(n + offset, dtype=dtype, device=cuda)
+    y = storage[offset:]
+    for r_in, want in ((None, alone), (r, joined)):
+        y.copy_(x)
+        assert run(y, r_in, y) == 0 and torch.equal(y, want)
+    y.copy_(r)
+    assert run(x, y, y) == 0 and torch.equal(y, joined)
+
+
 def test_a_sort_that_gives_up_reads_nothing_and_leaves_nothing_behind(cuda):
     from fp8_b200 import _lib
 
