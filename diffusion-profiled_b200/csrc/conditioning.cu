@@ -51,6 +51,9 @@ int x_check(const fp8_cross_attention_args* a, bool backward) {
   FP8_REQUIRE(a->batch > 0 && a->q_len > 0 && a->k_len > 0 && a->heads > 0 && a->kv_heads > 0,
               FP8_ERR_INVALID_ARGUMENT, "cross attention: sizes must be positive (batch %d, q_len %d, k_len %d, heads %d, "
               "kv_heads %d)", a->batch, a->q_len, a->k_len, a->heads, a->kv_heads);
+  // (so that tile and key numbers rounded up stay 32-bit ones)
+  FP8_REQUIRE(a->q_len <= INT32_MAX - kXTile && a->k_len <= INT32_MAX - kXTile, FP8_ERR_UNSUPPORTED,
+              "cross attention: too long (q_len %d, k_len %d)", a->q_len, a->k_len);
   FP8_REQUIRE(a->heads % a->kv_heads == 0, FP8_ERR_INVALID_ARGUMENT,
               "cross attention: %d heads are not a multiple of %d key heads", a->heads, a->kv_heads);
   FP8_REQUIRE(a->head_dim >= 8 && a->head_dim <= 128 && a->head_dim % 8 == 0, FP8_ERR_UNSUPPORTED,
@@ -452,6 +455,7 @@ static int embed_check(const void* ids, int ids64, int64_t tokens, int64_t vocab
                        int out_dtype) {
   FP8_REQUIRE(tokens >= 0 && vocab > 0 && width > 0, FP8_ERR_INVALID_ARGUMENT,
               "embedding: bad sizes (tokens %lld, vocab %lld, width %d)", (long long)tokens, (long long)vocab, width);
+  FP8_REQUIRE(width <= INT32_MAX - 1024, FP8_ERR_UNSUPPORTED, "embedding: rows too wide (%d)", width);  // (as above)
   FP8_REQUIRE(known_dtype(weight_dtype) && known_dtype(out_dtype), FP8_ERR_UNSUPPORTED,
               "embedding: unknown dtype code %d / %d", weight_dtype, out_dtype);
   FP8_REQUIRE(tokens == 0 || (ids != nullptr && aligned(ids, ids64 ? 8 : 4)), FP8_ERR_INVALID_ARGUMENT,
