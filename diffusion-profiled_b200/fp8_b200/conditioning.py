@@ -37,7 +37,8 @@ class _Seeded(nn.Module):
 
 
 def _norm_bf16(x: torch.Tensor, norm: nn.LayerNorm) -> torch.Tensor:
-    return layer_norm_bf16(x, norm) if fused_layer_norm_supported(x, norm) else norm(x.float()).to(torch.bfloat16)
+    fused = x.numel() > 0 and fused_layer_norm_supported(x, norm)
+    return layer_norm_bf16(x, norm) if fused else norm(x.float()).to(torch.bfloat16)
 
 
 class PromptEncoder(_Seeded):
@@ -81,13 +82,15 @@ class PromptAttention(_Seeded):
 
     def forward(self, x: torch.Tensor, states: torch.Tensor, lengths: torch.Tensor | None = None) -> torch.Tensor:
         b, c, h, w = x.shape
+        if states.dim() != 3 or states.shape[0] != b:
+            raise RuntimeError(f"prompt attention: states must be [{b}, tokens, width], got {tuple(states.shape)}")
         d = c // self.nh
         tokens = x.flatten(2).transpose(1, 2).contiguous()  # [B, HW, C]: a view where x is channels-last
         linear_dtype = self.q.weight.dtype
         feed = lambda t: t if torch.is_autocast_enabled("cuda") else t.to(linear_dtype)  # noqa: E731
         q = self.q(feed(_norm_bf16(tokens, self.norm))).to(torch.bfloat16)
         kv = self.kv(feed(states)).to(torch.bfloat16)
-        o = cross_attention_packed(q.view(b, h * w, self.nh, d), kv.view(b, -1, 2, self.nh, d), lengths)
+        o = cross_attention_packed(q.view(b, h * w, self.nh, d), kv.view(b, states.shape[1], 2, self.nh, d), lengths)
         o = self.out(feed(o.flatten(2))).to(x.dtype)
         if self.training and self.p_drop > 0.0:
             y = dropout_add(o, tokens, self.p_drop, self._next_seed())
