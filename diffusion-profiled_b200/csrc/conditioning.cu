@@ -156,7 +156,7 @@ struct XPlan {
   int row_tiles, hv, n_tiles, splits, key_chunk;
   int64_t rows, items, slots;
   bool two_values;   // P in two values of the type: x_fwd_kernel's SPLIT
-  bool join_inside;  // x_join (with two_values only)
+  bool join_inside;  // x_join (with two_values only): the splits are a cluster
 };
 XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
   XPlan w{};
@@ -181,20 +181,21 @@ XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
                                                      (w.n_tiles + kXMaxSplits - 1) / kXMaxSplits));
     w.splits = (w.n_tiles + w.key_chunk - 1) / w.key_chunk;
   }
-  w.items = base * w.splits;
   w.two_values = w.n_tiles == 1 || few_rows;
-  w.join_inside = few_rows && w.splits > 1 && w.items <= w.slots;
+  // Joined by the launch itself where the splits fit a cluster of the portable sizes 2, 4 and 8 (the last ones may have no
+  // keys) and every CTA has one item: a CTA that goes on with other items would be held up.  (Joined at counters in
+  // memory, zeroed before the launch: 12.3 us for one query of 4 heads of 64 over 1,024 keys, 30.8 over 8,192, whose 64
+  // splits take 22.5 with a second launch; in a cluster 11.1.)
+  int cluster = 2;
+  while (cluster < w.splits) cluster *= 2;
+  w.join_inside = few_rows && w.splits > 1 && cluster <= 8 && base * cluster <= w.slots;
+  if (w.join_inside) w.splits = cluster;
+  w.items = base * w.splits;
   return w;
 }
-// The workspace: the splits' outputs, their log-sum-exps and, where the launch joins them, its counters.  (The counters
-// are the call's own, zeroed before its launch: neither another call nor a replay of a captured one can meet them, and a
-// launch that gave up leaves nothing behind.)
-size_t x_part_floats(const fp8_cross_attention_args* a, const XPlan& w) {
-  return w.splits == 1 ? 0 : static_cast<size_t>(w.splits) * w.rows * (a->head_dim + 1);
-}
-size_t x_join_counters(const XPlan& w) { return w.join_inside ? static_cast<size_t>(w.items / w.splits) : 0; }
+// The workspace: the splits' outputs and their log-sum-exps.
 size_t x_fwd_workspace(const fp8_cross_attention_args* a, const XPlan& w) {
-  return sizeof(float) * x_part_floats(a, w) + sizeof(unsigned int) * x_join_counters(w);
+  return w.splits == 1 ? 0 : sizeof(float) * static_cast<size_t>(w.splits) * w.rows * (a->head_dim + 1);
 }
 
 template <typename T, int HALVES>
@@ -203,7 +204,8 @@ int x_fwd_launch(const XFwdParams& f, const CUtensorMap (&maps)[4], bool two_val
   const auto kernel = two_values ? x_fwd_kernel<T, HALVES, true> : x_fwd_kernel<T, HALVES, false>;
   FP8_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ly::kSmemBytes));
   FP8_CUDA_TRY(launch_kernel(kernel, dim3(static_cast<unsigned>(std::min<int64_t>(f.items, slots))), dim3(Ly::kThreads),
-                             Ly::kSmemBytes, stream, 1, kTensorKernel, f, maps[0], maps[1], maps[2], maps[3]));
+                             Ly::kSmemBytes, stream, f.join ? f.splits : 1, kTensorKernel, f, maps[0], maps[1], maps[2],
+                             maps[3]));
   count_launches(1);
   return FP8_OK;
 }
@@ -222,10 +224,7 @@ int x_fwd(const fp8_cross_attention_args* args, const XAttnParams& a, const XPla
   f.rows = w.rows;
   f.items = static_cast<uint32_t>(w.items);
   if (int s = bind_context()) return s;
-  if (w.join_inside) {
-    f.join = reinterpret_cast<unsigned int*>(f.part_o + x_part_floats(args, w));
-    FP8_CUDA_TRY(cudaMemsetAsync(f.join, 0, sizeof(unsigned int) * x_join_counters(w), stream));
-  }
+  f.join = w.join_inside;
   CUtensorMap maps[4];
   const int dt = args->dtype;
   if (int s = x_map(&maps[0], a.q, dt, a.sq, a.batch, a.q_len, a.heads, a.head_dim, a.pack, a.tile_tokens)) return s;
@@ -429,8 +428,8 @@ EmbedPlan embed_plan(int64_t tokens, int64_t vocab, int width) {
     w.pos[i] = take(sizeof(uint32_t) * static_cast<size_t>(tokens));
   }
   w.counts = take(sizeof(uint32_t) * static_cast<size_t>(w.ctas) << w.bits);
-  // zeroed before the sort: the number of live keys, and the counter where its CTAs meet (the call's own, as the
-  // attention's)
+  // zeroed before the sort: the number of live keys, and the counter where its CTAs meet.  (The call's own: neither
+  // another call nor a replay of a captured one can meet there, and a launch that gave up leaves nothing behind.)
   w.live = take(sizeof(uint32_t));
   w.arrive = take(sizeof(uint32_t));
   w.present = take(sizeof(uint32_t) * static_cast<size_t>(vocab / 32 + 1));

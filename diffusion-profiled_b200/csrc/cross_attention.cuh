@@ -340,9 +340,7 @@ struct XFwdParams {
   float* part_lse;  // [splits][batch * heads * q_len], base-2 logarithm
   int64_t rows;     // batch * heads * q_len
   uint32_t items;   // (sequence, head group, row tile group, split)
-  // where the launch itself joins the splits (x_join): a counter for each (sequence, head group), zero when it starts;
-  // else null
-  unsigned int* join;
+  int join;         // the launch itself joins the splits, which are the CTAs of a cluster (x_join)
 };
 constexpr int kXMaxSplits = 128;  // four a lane
 
@@ -404,21 +402,14 @@ struct XItems {
 __device__ __forceinline__ int x_chunks(int keys, int j) { return (min(kXTile, keys - j * kXTile) + 31) >> 5; }
 __device__ __forceinline__ int x_chunks64(int keys, int u) { return (min(64, keys - u * 64) + 31) >> 5; }
 
-// This warp's rows of a split are written.  The warp that is the last of the splits to say so joins them, in the order
-// of the splits: o = sum_s 2^(lse_s - lse) o_s.  For calls of one warp's rows a (sequence, head group) and one item a
-// CTA, which wait for the host: zeroing the counters and joining here takes less of its time than a launch of
-// x_combine_kernel (one query over 1,024 keys: 12.3 us a call against 13.2).  Where a CTA goes on with other items, the
-// wait for the memory's answer, behind the copies under way, holds them up: 32 queries over 8,192 keys took 161 us, with
-// the second launch 93.
+// Joins the splits of one warp's rows, in their order: o = sum_s 2^(lse_s - lse) o_s.  For calls of few rows whose splits
+// of a (sequence, head group) make up a cluster of one item a CTA: its first CTA joins them when all have met at the
+// cluster's barrier, for which no memory is shared with other calls.  Such calls wait for the host, and this saves it a
+// launch of x_combine_kernel (one query over 1,024 keys: 11.1 us a call against 13.2).
 // r_index: this lane's row; o_at: where its output goes.
 template <typename T>
-__device__ __forceinline__ void x_join(const XFwdParams& p, uint32_t counter, bool live, int64_t r_index, int64_t o_at) {
+__device__ __forceinline__ void x_join(const XFwdParams& p, bool live, int64_t r_index, int64_t o_at) {
   const int lane = threadIdx.x & 31;
-  __syncwarp();  // the other lanes' writes come before this one's release
-  unsigned int before = 0;
-  if (lane == 0) before = atom_add_acq_rel_gpu_u32(p.join + counter, 1u);
-  if (__shfl_sync(~0u, before, 0) + 1 != static_cast<unsigned int>(p.splits)) return;
-  __syncwarp();  // and this one's acquire before what the others read (the shuffle orders no memory)
   const int head_dim = p.a.head_dim, rows = __popc(__ballot_sync(~0u, live));  // the first lanes
   // ---- lane = row: the sum of the splits' weights
   constexpr int kAtOnce = 8;
@@ -711,10 +702,6 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES>::kThreads, kXFwdCtasPerSm)
       // rows of this warp that exist: a warp without any keeps only the barriers
       const bool any_row = __any_sync(0xffffffffu, live);
       const int64_t o_at = t.b * a.so.batch + token * a.so.token + head * a.so.head;
-      const auto join = [&]() {
-        if constexpr (SPLIT)  // (calls of few rows)
-          if (p.join != nullptr && any_row) x_join<T>(p, static_cast<uint32_t>(t.b) * p.hv + t.hv, live, r_index, o_at);
-      };
       if (t.j0 >= t.j1) {  // no keys
         if (live) {
           if (p.splits > 1) {
@@ -725,7 +712,6 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES>::kThreads, kXFwdCtasPerSm)
             if (a.lse != nullptr) a.lse[r_index] = -INFINITY;
           }
         }
-        join();
         continue;
       }
       const int qs = n_item % Ly::kQStages;
@@ -878,7 +864,6 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES>::kThreads, kXFwdCtasPerSm)
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      join();
       stored = qs;
       ++n_item;
     }
@@ -889,6 +874,19 @@ __global__ void __launch_bounds__(XFwdLayout<HALVES>::kThreads, kXFwdCtasPerSm)
   if (warp == Ly::kWarps) {
     tc_fence_after();
     tmem_dealloc(tmem, Ly::kTmemCols);
+  }
+  if constexpr (SPLIT) {  // (calls of few rows)
+    if (p.join) {
+      __syncwarp();
+      cluster_sync();
+      if (cluster_ctarank() == 0 && warp == 0) {
+        const XCount at = x_count(blockIdx.x, p.row_tiles, p.splits, p.hv);
+        const int token = lane / a.pack, head = at.d2 * a.pack + lane % a.pack;
+        const bool live = lane < a.q_len * a.pack;
+        x_join<T>(p, live, (static_cast<int64_t>(at.d3) * a.heads + head) * a.q_len + token,
+                  at.d3 * a.so.batch + token * a.so.token + head * a.so.head);
+      }
+    }
   }
 }
 

@@ -1,8 +1,8 @@
 """GPU tests of what the conditioning operators share between calls: nothing.
 
-Where CTAs of a launch meet, they meet at counters of the call's own workspace, which the
-call zeroes: whatever the workspace held, whatever runs beside the call, and however often a
-captured call is replayed, the results are the same.
+Where CTAs of a launch meet, they meet at a cluster's barrier or at a counter of the call's own
+workspace, which the call zeroes: whatever the workspace held, whatever runs beside the call,
+and however often a captured call is replayed, the results are the same.
 """
 
 from __future__ import annotations
@@ -35,26 +35,32 @@ def _attention_args(q, k, v, o):
     return a
 
 
-def test_attention_joins_at_counters_of_its_workspace(cuda):
+@pytest.mark.parametrize("lk,splits", [(129, 2), (300, 4), (600, 8), (1000, 8), (1500, 12)])
+@pytest.mark.parametrize("lengths", ["all", "short"])
+def test_attention_needs_its_partial_results_alone(cuda, lk, splits, lengths):
+    """Up to 8 splits of 128 keys meet in a cluster, more are joined by a second launch; none at a counter in memory."""
     from fp8_b200 import _lib
 
     lib = _lib.load()
-    q, k, v = _single_queries(cuda, 3, 1000, 4, 2, 64)
+    q, k, v = _single_queries(cuda, 3, lk, 4, 2, 64)
     o = torch.empty_like(q)
     a = _attention_args(q, k, v, o)
-    splits = 8  # one of each 128 keys
-    partial = 4 * splits * 3 * 4 * (64 + 1)
+    count = None
+    if lengths == "short":  # splits without keys, and a sequence without any
+        count = torch.tensor([lk, 1, 0], dtype=torch.int32, device=cuda)
+        a.key_lengths = count.data_ptr()
     need = lib.fp8_cross_attention_workspace_bytes(ctypes.byref(a), 0)
-    assert need == partial + 4 * 3 * 2  # a counter for each sequence and key head
+    assert need == 4 * splits * 3 * 4 * (64 + 1)
     ws = torch.empty(need, dtype=torch.uint8, device=cuda)
     stream = torch.cuda.current_stream(cuda).cuda_stream
-    want = oracle.cross_attention(q, k, v)["o"]
+    want = oracle.cross_attention(q, k, v, None, count)["o"]
     for fill in (0, 255, 1):
         ws.fill_(fill)
         o.fill_(torch.nan)
         assert lib.fp8_cross_attention_fwd(ctypes.byref(a), ws.data_ptr(), need, stream) == 0, _lib.last_error()
         assert oracle.excess(o, *want) <= 1.0
     assert lib.fp8_cross_attention_fwd(ctypes.byref(a), ws.data_ptr(), need - 4, stream) != 0
+    assert _lib.device_error() == 0
 
 
 def test_a_replayed_attention_beside_many_calls(cuda):
