@@ -128,8 +128,9 @@ __device__ __forceinline__ void x_products_mn(uint32_t d, uint32_t operand, uint
 }
 
 // ============================================================================ norms (fp16)
-// A CTA takes kXNormRows rows of dO, and of V, of a (sequence, key head); 16 lanes a row, eight channels each.
-constexpr int kXNormRows = 128;
+// A CTA takes kXNormRows rows of dO, and of V, of a (sequence, key head) at a time; 16 lanes a row, eight channels each,
+// four rows' loads under way.
+constexpr int kXNormAtOnce = 4, kXNormRows = 16 * kXNormAtOnce;
 template <typename T>
 __global__ void __launch_bounds__(256) x_norms_kernel(const XBwdParams p) {
   __shared__ unsigned int most[2];
@@ -144,22 +145,28 @@ __global__ void __launch_bounds__(256) x_norms_kernel(const XBwdParams p) {
     const int count = x_key_count(a, x_raw_count(a, b));
     if (threadIdx.x < 2) most[threadIdx.x] = 0;
     __syncthreads();
-    for (int64_t r = item % chunks * kXNormRows + first; r < min(rows, (item % chunks + 1) * kXNormRows); r += 16) {
+    uint4 w[kXNormAtOnce];
+    int64_t row_of[kXNormAtOnce];  // of dO: where its norm goes; of V: -1; no such row: -2
+#pragma unroll
+    for (int u = 0; u < kXNormAtOnce; ++u) {
+      const int64_t r = item % chunks * kXNormRows + first + 16 * u;
       const bool is_q = r < q_rows;
       const int token = static_cast<int>(is_q ? r / a.group : r - q_rows), h = hk * a.group + static_cast<int>(r % a.group);
       const T* row = is_q ? static_cast<const T*>(a.dout) + b * a.sdo.batch + token * a.sdo.token + h * a.sdo.head
                           : static_cast<const T*>(a.v) + b * a.sv.batch + token * a.sv.token + hk * a.sv.head;
-      const bool used = is_q || (token < count && x_key_kept(a, b, token));
-      float sum = 0.0f;
-      if (used && lane * 8 < a.head_dim) {
-        const uint4 w = *reinterpret_cast<const uint4*>(row + lane * 8);
-        sum = x_dot8<T>(w, w);
-      }
+      const bool used = is_q || (r < rows && token < count && x_key_kept(a, b, token));
+      row_of[u] = is_q ? (static_cast<int64_t>(b) * a.heads + h) * a.q_len + token : used ? -1 : -2;
+      w[u] = make_uint4(0, 0, 0, 0);
+      if (used && lane * 8 < a.head_dim) w[u] = *reinterpret_cast<const uint4*>(row + lane * 8);
+    }
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffu << (threadIdx.x & 16), sum, o);
-      if (lane == 0) {
-        if (is_q) p.row_norm2[(static_cast<int64_t>(b) * a.heads + h) * a.q_len + token] = sum;
-        atomicMax(most + (is_q ? 0 : 1), __float_as_uint(sum));  // (not negative: as bits in the same order, NaN above all)
+    for (int u = 0; u < kXNormAtOnce; ++u) {
+      float sum = x_dot8<T>(w[u], w[u]);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);  // (within the row's 16 lanes)
+      if (lane == 0 && row_of[u] > -2) {
+        if (row_of[u] >= 0) p.row_norm2[row_of[u]] = sum;
+        atomicMax(most + (row_of[u] >= 0 ? 0 : 1), __float_as_uint(sum));  // (not negative: as bits in the same order, NaN above all)
       }
     }
     __syncthreads();
