@@ -30,19 +30,22 @@
 //   * keys that are not kept: their scores are replaced by -inf, and their rows of V are
 //     zeroed in shared memory before the product.
 // What bounds it: with many queries the softmax (an exponential a score, 16 a clock and
-// SM) and the products by turns: the 2 x 4096 x 4096 above takes 150 us now, 919 TFLOP/s,
-// 55 % of the measured peak, and 13 % of it is the last wave (512 row tiles on 296 CTAs);
+// SM) and the products by turns: the 2 x 4096 x 4096 above takes 135 us in a loop of its own,
+// 1,018 TFLOP/s, 61 % of the measured peak, and 150 among the gradient's launches; 13 % of it
+// is the last wave (512 row tiles on 296 CTAs);
 // with few keys the beginning and end of an item (3,000 of 8,000 cycles at 160 keys), which
 // the other CTA of the SM fills in part; with single queries the bytes of K and V and the
-// latency of a step (32 queries of 16 heads over 8192 keys of 4: 342 MB in 100 us a call,
-// 3.4 TB/s, the join's 5 us included; of these, 25 do not depend on the bytes).
+// latency of a step (32 queries of 16 heads over 8192 keys of 4: 342 MB in 96 us, 3.6 TB/s,
+// and 5 us for the join).
 // The sums and statistics are fp32; P is the one value rounded before a sum (it is a
 // matrix operand).  Over many keys that rounding averages out against the output's own.
 // Where the states are at most one key tile it would not, and the products are cheap; with
 // few rows a sequence the tensor cores idle.  There (SPLIT) P goes in as the sum of two
 // values of the type, P V = P_hi V + P_lo V: the output's error is that of its own rounding
 // (1.7e-3 of its norm in bf16, 2.3e-3 with P rounded once), for 8 % of the time of the 32
-// queries above (92 us before), none of one query's over 1,024 keys.
+// queries above (92 us before), none of one query's over 1,024 keys.  For whole tiles of
+// rows over several key tiles two values would cost 15 to 24 % (64 x 1024 queries over 256
+// keys 41.6 -> 48.0 us, 2 x 4096 x 4096 135 -> 167): there P is rounded once.
 //
 // Every mbarrier wait is bounded (mbar_wait); on a timeout the kernel records the error
 // code, skips the remaining work and frees its tensor memory.

@@ -4,8 +4,8 @@
 //   dW_v = scale * sum_{i : id_i = v} dy_i         (fp32; zero rows for tokens that do
 //                                                   not occur and for the padding token)
 //
-// An id outside [0, vocab) reads nothing: its output row is zero, it adds to no
-// gradient, and the device error word records kErrTokenRange.
+// An id outside [0, vocab) reads nothing: its output row is zero, the lookup records
+// kErrTokenRange in the device error word, and it adds to no gradient.
 //
 // Gradient of few tokens, one launch (embed_few_kernel): every token looks through all ids
 // for its row's others, and the first of a row sums them.  Of more tokens, three launches:

@@ -6,7 +6,9 @@ token ids into states (:func:`fp8_b200.embedding.embed_tokens`, dropout, layer n
 :class:`PromptAttention` reads them from a feature map's pixels
 (:func:`fp8_b200.cross_attention.cross_attention_packed`) and adds what it found onto
 the map with dropout (:func:`fp8_b200.dropout.dropout_add`).  They run on CUDA tensors
-only; the linears follow autocast, as the UNet's own do.
+only.  The projections are ``nn.Linear``, which follows autocast, as in the UNet's own
+attention blocks (its FP8 whitelist is of 3x3 convolutions); the sums with the position,
+and with the map where there is no dropout, are torch's.
 """
 
 from __future__ import annotations
