@@ -409,7 +409,7 @@ class UNet(nn.Module):
     def forward(self, x: torch.Tensor, t: torch.Tensor, prompt_ids: torch.Tensor | None = None,
                 prompt_lengths: torch.Tensor | None = None) -> torch.Tensor:
         cfg = self.config
-        if (prompt_ids is None) != (self.prompt is None):
+        if (prompt_ids is None) != (self.prompt is None) or (prompt_ids is None and prompt_lengths is not None):
             raise RuntimeError("the UNet takes prompt ids if and only if it was built with prompt_vocab > 0")
         if cfg.fp8_convs_enabled and cfg.fp8_scaling_type == "delayed" and cfg.device_scale_history:
             # process-wide mode, read by the history-updating launches of this step (forward and backward)

@@ -1,4 +1,5 @@
-"""Prompts at the edge of what the UNet's conditioning takes: of another batch than the images, and of no tokens at all."""
+"""Prompts at the edge of what the UNet's conditioning takes: of another batch than the images, of no tokens at all, and
+lengths without prompts."""
 
 from __future__ import annotations
 
@@ -6,6 +7,7 @@ import pytest
 import torch
 
 from fp8_b200.conditioning import PromptAttention, PromptEncoder
+from fp8_b200.unet import UNet, UNetConfig
 
 
 @pytest.mark.parametrize("shape", [(2, 10, 32), (1, 10, 32), (10, 32), (4, 1, 10, 32)])
@@ -14,6 +16,12 @@ def test_states_of_another_batch_are_refused(shape):
     attention, x = PromptAttention(64, 32, 1), torch.zeros(4, 64, 2, 2)
     with pytest.raises(RuntimeError, match=r"states must be \[4, tokens, width\]"):
         attention(x, torch.zeros(shape))
+
+
+def test_lengths_without_prompts_are_refused():
+    x, t = torch.zeros(1, 3, 32, 32), torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="prompt_vocab"):
+        UNet(UNetConfig())(x, t, prompt_lengths=torch.tensor([3]))
 
 
 @pytest.mark.gpu
