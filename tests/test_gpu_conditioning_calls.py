@@ -218,3 +218,35 @@ def test_an_id_outside_the_vocabulary_does_not_hide_a_time_out(cuda):
     assert _lib.device_error() == 202
     stray()
     assert _lib.device_error() == 201 and _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float16])
+@pytest.mark.parametrize("mode", [1, 2])
+def test_programmatic_launches_give_the_same(cuda, mode, dtype):
+    """Kernels that begin while the one before ends (fp8_set_pdl) wait for what it wrote, zeroed words included."""
+    from fp8_b200 import _lib
+    from fp8_b200.cross_attention import cross_attention
+    from fp8_b200.dropout import dropout_add
+    from fp8_b200.embedding import embed_tokens
+
+    g = torch.Generator(device=cuda).manual_seed(mode)
+    new = lambda *s: torch.randn(*s, device=cuda, generator=g).to(dtype)  # noqa: E731
+    q, k, v, w, r = (new(*s).requires_grad_(True) for s in ((3, 200, 4, 64), (3, 700, 2, 64), (3, 700, 2, 64), (500, 256),
+                                                           (3, 200, 256)))
+    ids = torch.randint(0, 500, (3, 1000), device=cuda, generator=g)
+    seed, dy, dx = torch.tensor(2, device=cuda), new(3, 200, 256), new(3, 1000, 256)
+
+    def step():
+        y = dropout_add(cross_attention(q, k, v).flatten(2), r, 0.2, seed)
+        x = embed_tokens(ids, w)
+        one = cross_attention(q[:, :1], k, v)
+        return (y.detach(), x.detach(), one.detach(), *torch.autograd.grad((y, x), (q, k, v, w, r), (dy, dx)))
+
+    want = step()
+    try:
+        _lib.set_pdl(mode)
+        for _ in range(20):
+            assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    finally:
+        _lib.set_pdl(0)
+    assert _lib.device_error() == 0
