@@ -171,7 +171,8 @@ XPlan x_plan(const fp8_cross_attention_args* a, int sm_count) {
   w.key_chunk = w.n_tiles;
   // A split writes its rows' partial outputs in fp32.  With a few rows a tile that is nothing, and pieces that are a
   // quarter of an even share even out sequences of different lengths (finer ones only make the join longer: 32 queries
-  // over 8192 keys, 88 us and the join at four pieces a CTA, the same at eight and twelve, 92 at sixteen).  With whole
+  // over 8192 keys, with their weights rounded once 88 us and the join at four pieces a CTA, the same at eight and
+  // twelve, 92 at sixteen).  With whole
   // tiles of rows the keys are split only to reach SMs that would have no work at all (5 x 333 queries of 8 heads over
   // 1021 keys, 110 row tiles: 28 us unsplit, 36 split for two CTAs an SM).
   const bool few_rows = w.row_tiles == 1 && a->q_len * pack <= 16;
